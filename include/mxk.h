@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define MXK_ABI_VERSION 11
+#define MXK_ABI_VERSION 12
 
 typedef enum {
   MXK_OK = 0,
@@ -423,6 +423,86 @@ int mxk_vector_quantize(const void* x, int x_type, int64_t rows, int64_t cols, i
  * out[r][c] = RN(codes[r][c] * s), s = scales[r] (axis = 1) or scales[c]. */
 int mxk_vector_dequantize(const int32_t* codes, const float* scales, int64_t rows, int64_t cols, int axis, float* out,
                           void* stream);
+
+/* ------------------------------------------------ microscaled 4-bit floats
+ * Rows of K values in KB = ceil(K/32) blocks of 32 E2M1 codes (two a byte, the
+ * lower half first; 16*KB bytes a row, codes past K are 0) and one E8M0 scale
+ * byte each (KB a row): value = grid(code) * 2^(scale-127), grid 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6 and their negatives (bit 3), scale 255: NaN.  No
+ * counterpart in the reference, whose blocks have float32 scales.
+ */
+
+/* codes/scales of x [rows][cols] (x_type, rows row_stride elements apart):
+ * scale = max(floor(log2 max|x|) - 2, -127) + 127 of the block, code = the
+ * nearest value of x * 2^(127-scale), ties to the even code, at most 6; a
+ * block with a NaN or an infinity has scale 255 and zero codes.  Codes 4-byte
+ * aligned; cols below 2^28. */
+int mxk_mxfp4_quantize(const void* x, int x_type, int64_t rows, int64_t cols, int64_t row_stride, void* codes,
+                       void* scales, void* stream);
+
+/* y [rows][cols] (y_type) = the values: exact in float32 and bfloat16 up to
+ * their largest value, rounded to nearest even in float16. */
+int mxk_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, int y_type, void* y,
+                         void* stream);
+
+/* y [M][N] (y_type) = a @ b^T (+ bias[N], float32), a [a_rows][K] and b
+ * [N][K] packed, exact products, float32 sums.
+ * Dense: offsets = order = NULL, a_rows = M.
+ * By expert: offsets int32 [experts+1] on the device; rows offsets[e] to
+ * offsets[e+1] of y are those of a times b[e] (b [experts][N][K], bias
+ * [experts][N]); rows from offsets[experts] on are zeros.  With order (int32
+ * [M]) row r reads row order[r]/top of a (none, as zeros, if order[r] < 0 or
+ * the row is past a_rows); without it a_rows = M.  Offsets are taken into
+ * [0, M].  Codes 16-byte aligned; at most 1000 experts. */
+int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, const void* b_codes,
+                     const void* b_scales, int64_t M, int64_t N, int64_t K, const float* bias, int y_type, void* y,
+                     const int32_t* offsets, int experts, const int32_t* order, int top, void* stream);
+
+/* da [M][K] (out_type) = dy [M][N] (dy_type) @ dequantize(b) [N][K]: the
+ * gradient of a, straight through its quantization.  dy is not rounded,
+ * sums are float32.  By expert as mxk_mxfp4_matmul: b [experts][N][K], rows
+ * past the last expert's zeros. */
+int mxk_mxfp4_grad_a(const void* dy, int dy_type, int64_t M, int64_t N, const void* b_codes, const void* b_scales,
+                     int64_t K, int out_type, void* da, const int32_t* offsets, int experts, void* stream);
+
+/* db [N][K] (out_type) = dy [M][N]^T @ dequantize(a) [M][K]: the gradient of
+ * b.  By expert: db [experts][N][K], each over its own rows (zeros for an
+ * expert without rows). */
+int mxk_mxfp4_grad_b(const void* dy, int dy_type, int64_t M, int64_t N, const void* a_codes, const void* a_scales,
+                     int64_t K, int out_type, void* db, const int32_t* offsets, int experts, void* stream);
+
+/* ------------------------------------------------ tokens to experts and back
+ * Pick i = t*top + j is token t's j-th choice.  All arrays int32 on the
+ * device; no counterpart in the reference.
+ */
+
+/* Workspace bytes mxk_expert_sort needs (0 if none). */
+size_t mxk_expert_sort_workspace(int64_t picks, int experts);
+
+/* Stable order of picks by expert id (id_bytes 4 or 8, signed):
+ * order[picks] = the pick at each place (-1 past the last in use),
+ * place[picks] = the place of each pick (-1: its id is outside
+ * [0, experts)), offsets[experts+1] = each expert's first place; the last is
+ * the number in use.  At most 1000 experts. */
+int mxk_expert_sort(const void* ids, int id_bytes, int64_t picks, int experts, int32_t* order, int32_t* place,
+                    int32_t* offsets, void* workspace, size_t workspace_nbytes, void* stream);
+
+/* out [rows][cols] = x[order[r]/top] (elements of 2 or 4 bytes, x rows
+ * row_stride elements apart), zeros where order[r] < 0. */
+int mxk_expert_gather(const void* x, int elem_bytes, int64_t tokens, int64_t cols, int64_t row_stride,
+                      const int32_t* order, int64_t rows, int top, void* out, void* stream);
+
+/* y [tokens][cols] = sum over j of gates[t][j] * h[place[t][j]] in float32
+ * by ascending j (gates NULL: ones); places outside [0, rows) add nothing. */
+int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* place, const float* gates,
+                       int64_t tokens, int top, int64_t cols, void* y, void* stream);
+
+/* Gradients of mxk_expert_combine: dh[place[t][j]] = gates[t][j] * dy[t],
+ * zeros in rows from *used (device int32) on; dgates[t][j] = <dy[t],
+ * h[place[t][j]]>, 0 without a place.  rows = tokens * top. */
+int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t rows, const int32_t* place,
+                            const float* gates, const int32_t* used, int64_t tokens, int top, int64_t cols, void* dh,
+                            float* dgates, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,8 +12,11 @@ tensors must be on a GPU.
 """
 from . import dtypes as _dtypes
 from .dtypes import get_mx_dtype, matmul_output_dtype, mx_dtype
+from .experts import (expert_combine, expert_gather, expert_linear, expert_plan, expert_sort,
+                      mxfp4_expert_mlp)
 from .io import load_quantized, save_quantized
 from .kv import kv_cache_quantizer
+from .microscale import mxfp4_linear, mxfp4_matmul, mxfp4_quantize, mxfp4_tensor
 from .nn import (install_module_to, mx_dynamic_linear, mx_layer_norm, mx_linear, mx_multihead_attention,
                  mx_transformer_encoder_layer, to_mx, uninstall_module_to)
 from .ops import HADAMARD_DEQUANT_MODE, _dequant, quantize, vector_dequantize, vector_quantize
@@ -30,4 +33,5 @@ __all__ = ["mx_dtype", "get_mx_dtype", "matmul_output_dtype", "mx_tensor", "quan
            "kv_cache_quantizer", "install_module_to", "uninstall_module_to", "save_quantized", "load_quantized",
            "dynamic_quantize", "fused_int8_linear", "mx_fused_ops", "mx_dynamic_linear", "_MXLinearAutograd",
            "_mx_linear_forward", "mx_layer_norm", "mx_multihead_attention", "mx_transformer_encoder_layer",
-           "vector_quantize", "vector_dequantize"]
+           "vector_quantize", "vector_dequantize", "mxfp4_tensor", "mxfp4_quantize", "mxfp4_matmul", "mxfp4_linear",
+           "expert_plan", "expert_sort", "expert_gather", "expert_linear", "expert_combine", "mxfp4_expert_mlp"]

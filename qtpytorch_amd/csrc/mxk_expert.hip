@@ -1,0 +1,471 @@
+// Tokens to experts and back, for gfx950: the order of picks by expert, the
+// copy of token rows in that order, their weighted sum and its gradients.
+//
+// P = tokens * top picks, pick i = t * top + j of token t.  The plan of a
+// routing is three int32 arrays:
+//   order[P]      pick at each sorted place (stable: by expert, then by
+//                 pick), -1 past the last pick that has an expert
+//   place[P]      where each pick went, -1 for one without an expert (an id
+//                 outside [0, E): another device's, or a padded token's)
+//   offsets[E+1]  first place of each expert; offsets[E] is the number in use
+// Every kernel here gathers: each output element is written by one thread in
+// a fixed order of additions, so results do not depend on timing.
+#include "mxk_mxfp4.h"
+
+namespace mxk {
+
+#define MXK_SORT_THREADS 1024
+#define MXK_SORT_WAVES (MXK_SORT_THREADS / 64)
+
+// expert of a pick, E for one without
+template <typename I>
+__device__ __forceinline__ uint32_t expert_of(I id, uint32_t E) {
+  return (uint64_t)(int64_t)id < (uint64_t)E ? (uint32_t)id : E;
+}
+
+// Counts of each expert in each chunk of picks: hist[chunk][E].
+template <typename I>
+__global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_count(const I* __restrict__ ids, uint32_t P, uint32_t E,
+                                                                   uint32_t chunk, int* __restrict__ hist) {
+  extern __shared__ int cnt[];  // [E + 1]
+  for (uint32_t e = threadIdx.x; e <= E; e += MXK_SORT_THREADS) cnt[e] = 0;
+  __syncthreads();
+  const uint32_t lo = blockIdx.x * chunk, hi = min(P, lo + chunk);
+  for (uint32_t i = lo + threadIdx.x; i < hi; i += MXK_SORT_THREADS) atomicAdd(&cnt[expert_of(ids[i], E)], 1);
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < E; e += MXK_SORT_THREADS) hist[(int64_t)blockIdx.x * E + e] = cnt[e];
+}
+
+// One chunk of picks to their places.  Bounded by latency (the ids are a few
+// hundred KB at most): each wave counts its own contiguous share in LDS, the
+// shares' first places follow from the counts of the chunks before (`hist`,
+// which a single chunk does not need) and of the waves before, and a wave
+// then places 64 picks at a time, ranked among the lanes with the same expert by
+// ballots over the bits of the expert's number.
+template <typename I>
+__global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __restrict__ ids, uint32_t P, uint32_t E,
+                                                                   uint32_t chunk, const int* __restrict__ hist,
+                                                                   int* __restrict__ order, int* __restrict__ place,
+                                                                   int* __restrict__ offsets) {
+  extern __shared__ int sh[];
+  int* start = sh;                                  // [waves][E + 1]: counts, then next places
+  int* sums = sh + MXK_SORT_WAVES * (E + 1);        // [waves]: scan over waves of experts
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  for (uint32_t k = tid; k < MXK_SORT_WAVES * (E + 1); k += MXK_SORT_THREADS) start[k] = 0;
+  __syncthreads();
+  const uint32_t share = (chunk / MXK_SORT_WAVES + 63u) & ~63u;  // a multiple of 64 per wave
+  const uint32_t c0 = blockIdx.x * chunk, c1 = min(P, c0 + chunk);
+  const uint32_t lo = min(c1, c0 + wave * share), hi = min(c1, lo + share);
+  int* mine = start + wave * (E + 1);
+  for (uint32_t i = lo + lane; i < hi; i += 64) atomicAdd(&mine[expert_of(ids[i], E)], 1);
+  __syncthreads();
+  // experts in groups of 1024, one per thread: totals, exclusive scan, first places
+  int base = 0;
+  for (uint32_t e0 = 0; e0 < E; e0 += MXK_SORT_THREADS) {
+    const uint32_t e = e0 + tid;
+    int before = 0, total = 0;
+    if (e < E) {
+      if (gridDim.x > 1) {
+        for (uint32_t c = 0; c < gridDim.x; ++c) {
+          const int n = hist[(int64_t)c * E + e];
+          total += n;
+          before += c < blockIdx.x ? n : 0;
+        }
+      } else {
+        for (int w = 0; w < MXK_SORT_WAVES; ++w) total += start[w * (E + 1) + e];
+      }
+    }
+    int scan = total;  // inclusive over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(scan, d);
+      if ((int)lane >= d) scan += up;
+    }
+    if (lane == 63) sums[wave] = scan;
+    __syncthreads();
+    int left = base;
+    for (uint32_t w = 0; w < MXK_SORT_WAVES; ++w) {
+      if (w < wave) left += sums[w];
+      base += sums[w];
+    }
+    if (e < E) {
+      const int first = left + scan - total;
+      if (blockIdx.x == 0) offsets[e] = first;
+      int next = first + before;
+      for (int w = 0; w < MXK_SORT_WAVES; ++w) {
+        const int n = start[w * (E + 1) + e];
+        start[w * (E + 1) + e] = next;
+        next += n;
+      }
+    }
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && tid == 0) offsets[E] = base;
+  // places past the last one in use
+  for (uint32_t i = c0 + tid; i < c1; i += MXK_SORT_THREADS)
+    if (i >= (uint32_t)base) order[i] = -1;
+  const int bits = 32 - __builtin_clz(E | 1u);  // of 0 .. E
+  for (uint32_t i0 = lo; i0 < hi; i0 += 64) {
+    const uint32_t i = i0 + lane;
+    const bool live = i < hi;
+    const uint32_t e = live ? expert_of(ids[i], E) : E;
+    uint64_t same = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((e >> b) & 1u);
+      same &= ((e >> b) & 1u) ? set : ~set;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1ull));
+    const bool picked = live && e < E;
+    int at = -1;
+    if (picked) at = mine[e] + rank;
+    // every lane has read its counter before the first of each expert moves it
+    __builtin_amdgcn_wave_barrier();
+    if (picked && rank == 0) mine[e] += __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+    if (live) place[i] = at;
+    if (picked) order[at] = (int)i;
+  }
+}
+
+// out[r] = x[order[r] / top], zeros where order[r] < 0: a copy, bound by
+// HBM's write rate (a token's row is read `top` times, from L2 after the
+// first).  Rows are copied in pieces of 16 bytes (any alignment; the last
+// piece of a row may be shorter), U pieces a thread with their loads issued first.
+template <int U>
+__global__ __launch_bounds__(256) void k_expert_gather(const uint8_t* __restrict__ x, int64_t x_stride,
+                                                       const int* __restrict__ order, DivU32 by_top, uint32_t tokens,
+                                                       uint32_t total, DivU32 by_pieces, uint32_t pieces, uint32_t row_bytes,
+                                                       uint8_t* __restrict__ out) {
+  const uint64_t first = (uint64_t)blockIdx.x * (256u * U) + threadIdx.x;
+  u32x4 v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint64_t i = first + 256u * u;
+    v[u] = u32x4{0u, 0u, 0u, 0u};
+    if (i < total) {
+      const uint32_t r = divu32((uint32_t)i, by_pieces), c = ((uint32_t)i - r * pieces) * 16u;
+      const int pick = order[r];
+      const uint32_t token = divu32((uint32_t)pick, by_top);
+      if (pick >= 0 && token < tokens) {
+        const uint8_t* p = x + (int64_t)token * x_stride + c;
+        if (c + 16u <= row_bytes) {
+          __builtin_memcpy(&v[u], p, 16);
+        } else {  // elements have an even number of bytes
+          uint16_t t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+          for (uint32_t k = 0; k < 8; ++k)
+            if (c + 2 * k < row_bytes) __builtin_memcpy(&t[k], p + 2 * k, 2);
+          __builtin_memcpy(&v[u], t, 16);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint64_t i = first + 256u * u;
+    if (i >= total) continue;
+    const uint32_t r = divu32((uint32_t)i, by_pieces), c = ((uint32_t)i - r * pieces) * 16u;
+    uint8_t* p = out + (int64_t)r * row_bytes + c;
+    if (c + 16u <= row_bytes) {
+      __builtin_memcpy(p, &v[u], 16);
+    } else {
+      uint16_t t[8];
+      __builtin_memcpy(t, &v[u], 16);
+      for (uint32_t k = 0; k < 8; ++k)
+        if (c + 2 * k < row_bytes) __builtin_memcpy(p + 2 * k, &t[k], 2);
+    }
+  }
+}
+
+// 8 elements at p (the first `live` where fewer are left) as float32
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int live, float (&v)[8]) {
+  FpWords<T, 8> w;
+  if (live >= 8) fp4_load(p, w);
+  else fp4_load_tail(p, live, w);
+  T t[8];
+  __builtin_memcpy(t, w.w, sizeof(t));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = ElemT<T>::cvt(t[e]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int live, const float (&v)[8]) {
+  T t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(v[e]);
+  if (live >= 8) {
+    __builtin_memcpy(p, t, sizeof(t));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < live) p[e] = t[e];
+  }
+}
+
+// y[t] = sum over j of gate[t, j] * h[place[t, j]] (gate = 1 where gates is
+// null), in float32 by ascending j, picks without an expert left out.  Bound
+// by HBM: one read of the rows in use, one write of the tokens.  A thread
+// holds 8 columns of a token and issues the loads of four picks at a time.
+template <typename T, bool GATED>
+__global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h, const int* __restrict__ place,
+                                                        const float* __restrict__ gates, int top, int rows,
+                                                        uint32_t total, DivU32 by_pieces, uint32_t pieces, int cols,
+                                                        T* __restrict__ y) {
+  const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+  if (i >= total) return;
+  const uint32_t t = divu32((uint32_t)i, by_pieces), c = 8u * ((uint32_t)i - t * pieces);
+  const int live = cols - (int)c;
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const int64_t p0 = (int64_t)t * top;
+  for (int j0 = 0; j0 < top; j0 += 4) {
+    float v[4][8], g[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = j0 + q < top ? place[p0 + j0 + q] : -1;
+      g[q] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[q][e] = 0.0f;
+      if (at >= 0 && at < rows) {
+        g[q] = GATED ? gates[p0 + j0 + q] : 1.0f;
+        load8(h + (int64_t)at * cols + c, live, v[q]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(g[q], v[q][e], acc[e]);
+    }
+  }
+  store8(y + (int64_t)t * cols + c, live, acc);
+}
+
+// Gradients of the weighted sum: dh[place[t, j]] = gate[t, j] * dy[t] and
+// dgate[t, j] = <dy[t], h[place[t, j]]>; zeros for rows past the last in
+// use and for picks without an expert.  Bound by HBM: dy is read once per
+// token and group of four picks, h read and dh written once.  W waves share a
+// token (4 where there are too few tokens to fill the card with one each); a
+// lane's share of the products is added in order of its columns, then over the
+// lanes of a wave and the waves of a token in a fixed order.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void k_expert_combine_grad(const T* __restrict__ dy, const T* __restrict__ h,
+                                                             const int* __restrict__ place,
+                                                             const float* __restrict__ gates,
+                                                             const int* __restrict__ used, int tokens, int top,
+                                                             int rows, int cols, T* __restrict__ dh, float* __restrict__ dg) {
+  __shared__ float part[4][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t t = (int64_t)blockIdx.x * (4 / W) + wave / W;
+  const int w = wave % W;
+  const bool live_t = t < tokens;  // the waves of a group share t, and with W = 4 so does the workgroup
+  const int64_t p0 = t * top;
+  const int n_used = *used;
+  const T* dyt = dy + t * cols;
+  for (int j0 = 0; j0 < top; j0 += 4) {
+    float dot[4] = {0, 0, 0, 0};
+    if (live_t) {
+      int at[4];
+      float g[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool in = j0 + q < top;
+        at[q] = in ? place[p0 + j0 + q] : -1;
+        if (at[q] >= rows) at[q] = -1;
+        g[q] = in ? gates[p0 + j0 + q] : 0.0f;
+      }
+      for (int c = (w * 64 + lane) * 8; c < cols; c += W * 512) {
+        const int live = cols - c;
+        float d[8], v[4][8];
+        load8(dyt + c, live, d);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (at[q] >= 0) load8(h + (int64_t)at[q] * cols + c, live, v[q]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (at[q] >= 0) {
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              dot[q] = __builtin_fmaf(d[e], v[q][e], dot[q]);
+              o[e] = g[q] * d[e];
+            }
+            store8(dh + (int64_t)at[q] * cols + c, live, o);
+          }
+          if (j0 + q < top && p0 + j0 + q >= n_used) {  // row number p0 + j0 + q is in no one's use
+            const float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            store8(dh + (p0 + j0 + q) * cols + c, live, z);
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1) dot[q] += __shfl_xor(dot[q], s);
+        if (at[q] < 0) dot[q] = 0.0f;
+      }
+    }
+    if constexpr (W == 1) {
+      if (live_t && lane == 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (j0 + q < top) dg[p0 + j0 + q] = dot[q];
+      }
+    } else {
+      if (lane == 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) part[wave][q] = dot[q];
+      }
+      __syncthreads();
+      if (live_t && threadIdx.x < 4 && j0 + (int)threadIdx.x < top) {
+        const int q = threadIdx.x;
+        dg[p0 + j0 + q] = (part[0][q] + part[1][q]) + (part[2][q] + part[3][q]);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Picks per chunk: one chunk (one launch) up to 2048; above it at most 128 chunks
+// of at least 2048 picks, whose counts every workgroup reads
+static int64_t sort_chunk(int64_t P) {
+  if (P <= 2048) return 2048;
+  const int64_t c = std::max<int64_t>(2048, ceil_div(P, 128));
+  return ceil_div(c, MXK_SORT_THREADS) * MXK_SORT_THREADS;
+}
+
+template <typename I>
+static int launch_sort(const I* ids, int64_t P, int E, int* order, int* place, int* offsets, int* hist,
+                       hipStream_t st) {
+  const int64_t chunk = sort_chunk(P), n = std::max<int64_t>(1, ceil_div(P, chunk));
+  if (n > 1)
+    hipLaunchKernelGGL((k_expert_count<I>), dim3((unsigned)n), dim3(MXK_SORT_THREADS), (E + 1) * sizeof(int), st, ids,
+                       (uint32_t)P, (uint32_t)E, (uint32_t)chunk, hist);
+  const size_t lds = ((size_t)MXK_SORT_WAVES * (E + 1) + MXK_SORT_WAVES) * sizeof(int);
+  hipLaunchKernelGGL((k_expert_place<I>), dim3((unsigned)n), dim3(MXK_SORT_THREADS), lds, st, ids, (uint32_t)P,
+                     (uint32_t)E, (uint32_t)chunk, hist, order, place, offsets);
+  return check_launch("expert_sort");
+}
+
+}  // namespace mxk
+
+using namespace mxk;
+
+extern "C" {
+
+size_t mxk_expert_sort_workspace(int64_t picks, int experts) {
+  if (picks <= 0 || experts <= 0) return 0;
+  const int64_t n = ceil_div(picks, sort_chunk(picks));
+  return n > 1 ? (size_t)n * experts * sizeof(int) : 0;
+}
+
+int mxk_expert_sort(const void* ids, int id_bytes, int64_t picks, int experts, int32_t* order, int32_t* place,
+                    int32_t* offsets, void* workspace, size_t workspace_nbytes, void* stream) {
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (picks < 0 || picks >= ((int64_t)1 << 31) - 65536) return fail(MXK_EINVAL, "expert_sort: 0 <= picks < 2^31 - 2^16");
+  // the waves' counters have to fit 64 KiB of LDS
+  if (experts < 1 || experts > 1000) return fail(MXK_EINVAL, "expert_sort: 1 to 1000 experts");
+  if (id_bytes != 4 && id_bytes != 8) return fail(MXK_EINVAL, "expert_sort: ids of 4 or 8 bytes");
+  if (!offsets || (picks > 0 && (!ids || !order || !place))) return fail(MXK_EINVAL, "expert_sort: null pointer");
+  const size_t need = mxk_expert_sort_workspace(picks, experts);
+  if (need > 0 && (!workspace || workspace_nbytes < need)) return fail(MXK_EINVAL, "expert_sort: workspace too small");
+  int* hist = reinterpret_cast<int*>(workspace);
+  if (id_bytes == 4)
+    return launch_sort(reinterpret_cast<const int32_t*>(ids), picks, experts, order, place, offsets, hist, st);
+  return launch_sort(reinterpret_cast<const int64_t*>(ids), picks, experts, order, place, offsets, hist, st);
+}
+
+int mxk_expert_gather(const void* x, int elem_bytes, int64_t tokens, int64_t cols, int64_t row_stride,
+                      const int32_t* order, int64_t rows, int top, void* out, void* stream) {
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (elem_bytes != 2 && elem_bytes != 4) return fail(MXK_EINVAL, "expert_gather: elements of 2 or 4 bytes");
+  if (tokens < 0 || cols < 0 || rows < 0 || top < 1 || row_stride < 0 || rows >= ((int64_t)1 << 31) ||
+      tokens >= ((int64_t)1 << 31) || cols >= ((int64_t)1 << 28) || rows > tokens * top)
+    return fail(MXK_EINVAL, "expert_gather: bad sizes (rows at most tokens * top, below 2^31; cols below 2^28)");
+  if (rows == 0 || cols == 0) return MXK_OK;
+  if (!x || !order || !out) return fail(MXK_EINVAL, "expert_gather: null pointer");
+  const int64_t row_bytes = cols * elem_bytes, pieces = ceil_div(row_bytes, 16);
+  const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 31) / pieces - 1);
+  const DivU32 bt = make_divu32((uint32_t)top), bp = make_divu32((uint32_t)pieces);
+  for (int64_t r0 = 0; r0 < rows; r0 += step) {
+    const uint32_t total = (uint32_t)(std::min(step, rows - r0) * pieces);
+    const uint8_t* xp = reinterpret_cast<const uint8_t*>(x);
+    uint8_t* op = reinterpret_cast<uint8_t*>(out) + r0 * row_bytes;
+    const bool big = total >= 256u * 4u * 1024u;
+    const dim3 grid((unsigned)ceil_div(total, big ? 1024 : 256));
+    if (big)
+      hipLaunchKernelGGL((k_expert_gather<4>), grid, dim3(256), 0, st, xp, row_stride * elem_bytes, order + r0, bt,
+                         (uint32_t)tokens, total, bp, (uint32_t)pieces, (uint32_t)row_bytes, op);
+    else
+      hipLaunchKernelGGL((k_expert_gather<1>), grid, dim3(256), 0, st, xp, row_stride * elem_bytes, order + r0, bt,
+                         (uint32_t)tokens, total, bp, (uint32_t)pieces, (uint32_t)row_bytes, op);
+  }
+  return check_launch("expert_gather");
+}
+
+int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* place, const float* gates,
+                       int64_t tokens, int top, int64_t cols, void* y, void* stream) {
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (tokens < 0 || top < 1 || cols < 0 || rows < 0 || rows >= ((int64_t)1 << 31) || tokens * top >= ((int64_t)1 << 31) || cols >= ((int64_t)1 << 28))
+    return fail(MXK_EINVAL, "expert_combine: bad sizes (tokens * top below 2^31, cols below 2^28)");
+  if (tokens == 0 || cols == 0) return MXK_OK;
+  if ((rows > 0 && !h) || !place || !y) return fail(MXK_EINVAL, "expert_combine: null pointer");
+  if (h_type != MXK_IN_F32 && h_type != MXK_IN_F16 && h_type != MXK_IN_BF16)
+    return fail(MXK_EINVAL, "expert_combine: unknown h_type");
+  const int64_t pieces = ceil_div(cols, 8), step = std::max<int64_t>(1, ((int64_t)1 << 31) / pieces - 1);
+  const DivU32 bp = make_divu32((uint32_t)pieces);
+  for (int64_t t0 = 0; t0 < tokens; t0 += step) {
+    const uint32_t total = (uint32_t)(std::min(step, tokens - t0) * pieces);
+    const dim3 grid((unsigned)ceil_div(total, 256));
+    const int* pl = place + t0 * top;
+    const float* gt = gates ? gates + t0 * top : nullptr;
+#define MXK_C(T)                                                                                                  \
+  do {                                                                                                            \
+    const T* hp = reinterpret_cast<const T*>(h);                                                                  \
+    T* yp = reinterpret_cast<T*>(y) + t0 * cols;                                                                  \
+    if (gt)                                                                                                       \
+      hipLaunchKernelGGL((k_expert_combine<T, true>), grid, dim3(256), 0, st, hp, pl, gt, top, (int)rows, total, bp, \
+                         (uint32_t)pieces, (int)cols, yp);                                                        \
+    else                                                                                                          \
+      hipLaunchKernelGGL((k_expert_combine<T, false>), grid, dim3(256), 0, st, hp, pl, gt, top, (int)rows, total, bp, \
+                         (uint32_t)pieces, (int)cols, yp);                                                        \
+  } while (0)
+    if (h_type == MXK_IN_F32) MXK_C(float);
+    else if (h_type == MXK_IN_F16) MXK_C(__half);
+    else MXK_C(hip_bfloat16);
+#undef MXK_C
+  }
+  return check_launch("expert_combine");
+}
+
+int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t rows, const int32_t* place,
+                            const float* gates, const int32_t* used, int64_t tokens, int top, int64_t cols, void* dh, float* dgates,
+                            void* stream) {
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (tokens < 0 || top < 1 || cols < 0 || rows < 0 || rows >= ((int64_t)1 << 31) || tokens * top >= ((int64_t)1 << 31) || cols >= ((int64_t)1 << 28))
+    return fail(MXK_EINVAL, "expert_combine_grad: bad sizes (tokens * top below 2^31, cols below 2^28)");
+  if (tokens == 0) return MXK_OK;
+  if (rows != tokens * top) return fail(MXK_EINVAL, "expert_combine_grad: rows must be tokens * top");
+  if (!place || !gates || !used || !dgates || (cols > 0 && (!dy || !h || !dh)))
+    return fail(MXK_EINVAL, "expert_combine_grad: null pointer");
+  if (h_type != MXK_IN_F32 && h_type != MXK_IN_F16 && h_type != MXK_IN_BF16)
+    return fail(MXK_EINVAL, "expert_combine_grad: unknown h_type");
+  // one wave a token where that fills the card (8 waves a CU), else four
+  const bool few = tokens < 8 * (int64_t)num_cus();
+#define MXK_G(T)                                                                                                    \
+  do {                                                                                                              \
+    const T* dp = reinterpret_cast<const T*>(dy);                                                                   \
+    const T* hp = reinterpret_cast<const T*>(h);                                                                    \
+    T* op = reinterpret_cast<T*>(dh);                                                                               \
+    if (few)                                                                                                        \
+      hipLaunchKernelGGL((k_expert_combine_grad<T, 4>), dim3((unsigned)tokens), dim3(256), 0, st, dp, hp, place,    \
+                         gates, used, (int)tokens, top, (int)rows, (int)cols, op, dgates);                                     \
+    else                                                                                                            \
+      hipLaunchKernelGGL((k_expert_combine_grad<T, 1>), dim3((unsigned)ceil_div(tokens, 4)), dim3(256), 0, st, dp,  \
+                         hp, place, gates, used, (int)tokens, top, (int)rows, (int)cols, op, dgates);                          \
+  } while (0)
+  if (h_type == MXK_IN_F32) MXK_G(float);
+  else if (h_type == MXK_IN_F16) MXK_G(__half);
+  else MXK_G(hip_bfloat16);
+#undef MXK_G
+  return check_launch("expert_combine_grad");
+}
+
+}  // extern "C"

@@ -1,0 +1,136 @@
+// Helpers of the microscaled 4-bit format (gfx950 only): blocks of 32 E2M1
+// codes along a row, one E8M0 scale byte each.
+//
+//   value = grid(code) * 2^(scale - 127), scale 255: NaN
+//   scale = max(floor(log2 max|x|) - 2, -127) + 127, code = the nearest grid
+//   value of x * 2^(127 - scale) (ties to the even code), at most 6
+//
+// Two codes a byte, the lower half first; a row holds KB = ceil(K / 32)
+// blocks, 16 * KB bytes and KB scale bytes, and its last block is padded
+// with zero codes.
+#pragma once
+
+#include "mxk_internal.h"
+
+namespace mxk {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2f __attribute__((ext_vector_type(2)));
+typedef float f32x4f __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+inline int64_t fp4_blocks(int64_t cols) { return (cols + 31) / 32; }
+
+// 2^(s - 127) as float32 (s = 0: the subnormal 2^-127; s = 255: NaN)
+__device__ __forceinline__ float e8m0_value(uint32_t s) {
+  const uint32_t b = max(s << 23, 0x00400000u);
+  return __uint_as_float(s == 255u ? 0x7FC00000u : b);
+}
+
+// N elements of type T as the dwords that hold them
+template <typename T, int N>
+struct FpWords {
+  static constexpr int NW = N * (int)sizeof(T) / 4;
+  uint32_t w[NW];
+};
+
+// N elements at p, which needs no more alignment than an element's: global
+// memory takes wide loads at any address (unaligned mode), at one
+// instruction per 16 bytes
+template <typename T, int N>
+__device__ __forceinline__ void fp4_load(const T* p, FpWords<T, N>& v) {
+  __builtin_memcpy(v.w, p, sizeof(v.w));
+}
+// the first `live` of them (the others read as +0), element by element
+template <typename T, int N>
+__device__ __forceinline__ void fp4_load_tail(const T* p, int live, FpWords<T, N>& v) {
+  T e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    uint32_t z = 0;
+    __builtin_memcpy(&e[i], &z, sizeof(T));
+    if (i < live) e[i] = p[i];
+  }
+  __builtin_memcpy(v.w, e, sizeof(v.w));
+}
+
+// Largest magnitude of the elements, as the bits of its float32 value (so
+// that NaN and infinity compare above every number).  16-bit types compare
+// as pairs of 16-bit integers.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+template <typename T, int N>
+__device__ __forceinline__ uint32_t fp4_amax_bits(const FpWords<T, N>& v) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t m = v.w[0] & 0x7FFFFFFFu;
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = max(m, v.w[i] & 0x7FFFFFFFu);
+    return m;
+  } else {
+    u16x2 m = __builtin_bit_cast(u16x2, v.w[0] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int i = 1; i < N / 2; ++i)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v.w[i] & 0x7FFF7FFFu));
+    const uint32_t h = max((uint32_t)m[0], (uint32_t)m[1]);
+    if constexpr (__is_same(T, __half))
+      return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)h));
+    else
+      return h << 16;
+  }
+}
+
+// Scale byte of a block from the bits of its largest magnitude: the exponent
+// field less 2 (E2M1's largest binade), at least 0; 255 for NaN and infinity
+__device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t amax_bits) {
+  const uint32_t e = amax_bits >> 23;
+  return e == 255u ? 255u : max(e, 2u) - 2u;
+}
+
+// Codes of the N elements (N / 8 dwords) for scale s = e8m0_value(byte): the
+// conversion divides by the power of two, rounds to the nearest even code
+// and saturates at 6 (checked against the grid's midpoints)
+template <typename T, int N>
+__device__ __forceinline__ void fp4_codes(const FpWords<T, N>& v, float s, uint32_t (&q)[N / 8]) {
+#pragma unroll
+  for (int d = 0; d < N / 8; ++d) {
+    uint32_t o = 0u;
+    if constexpr (sizeof(T) == 4) {
+      const float* f = reinterpret_cast<const float*>(v.w) + 8 * d;
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, f[0], f[1], s, 0);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, f[2], f[3], s, 1);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, f[4], f[5], s, 2);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, f[6], f[7], s, 3);
+    } else if constexpr (__is_same(T, __half)) {
+      const uint32_t* w = v.w + 4 * d;
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(f16x2, w[0]), s, 0);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(f16x2, w[1]), s, 1);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(f16x2, w[2]), s, 2);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(f16x2, w[3]), s, 3);
+    } else {
+      const uint32_t* w = v.w + 4 * d;
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(bf16x2, w[0]), s, 0);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(bf16x2, w[1]), s, 1);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(bf16x2, w[2]), s, 2);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(bf16x2, w[3]), s, 3);
+    }
+    q[d] = o;
+  }
+}
+
+// a float32 result as T, rounded to nearest even
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __builtin_bit_cast(__half, (_Float16)v);
+}
+template <>
+__device__ __forceinline__ hip_bfloat16 from_f32<hip_bfloat16>(float v) {
+  return __builtin_bit_cast(hip_bfloat16, (__bf16)v);
+}
+
+}  // namespace mxk

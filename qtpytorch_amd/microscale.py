@@ -1,0 +1,260 @@
+"""Microscaled 4-bit floating point: blocks of 32 E2M1 values along the last
+dimension, each block with one power-of-two scale (E8M0).
+
+A value is ``grid[code] * 2**(scale - 127)`` with the grid 0, 0.5, 1, 1.5, 2,
+3, 4, 6 and its negatives; the scale of a block is two binades below its
+largest magnitude, and a scale of 255 makes the block NaN (a block that held a NaN
+or an infinity).  gfx950 multiplies such operands as they are stored, at four
+times the bf16 rate, where the formats of ``mx_dtype`` (one float32 scale per
+block of any length) are decoded first.
+
+  mxfp4_quantize(x)                 -> mxfp4_tensor, rounded to nearest even
+  mxfp4_tensor.dequantize(dtype)    the values
+  mxfp4_matmul(a, b, bias)          a @ b.T of packed operands
+  mxfp4_linear(x, weight, bias)     float x, packed on the way; differentiable
+
+``mxfp4_linear`` passes gradients straight through the quantizer:
+``dx = dy @ dequantize(weight)`` and, for a float weight, ``dw = dy.T @
+dequantize(quantize(x))``, both with dy unrounded and sums in float32.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _lib as L
+
+Tensor = torch.Tensor
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+class mxfp4_tensor:
+    """Packed values of a [..., K] tensor: ``codes`` uint8 [..., 16 * KB] (two
+    a byte, the lower half first) and ``scales`` uint8 [..., KB], KB =
+    ceil(K / 32); codes past K are 0."""
+
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes: Tensor, scales: Tensor, shape):
+        shape = torch.Size(shape)
+        if len(shape) < 1:
+            raise ValueError("mxfp4_tensor: a tensor of at least one dimension")
+        kb = -(-shape[-1] // 32)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError(f"mxfp4_tensor: codes and scales are uint8, got {codes.dtype} and {scales.dtype}")
+        if codes.shape != (*shape[:-1], 16 * kb) or scales.shape != (*shape[:-1], kb):
+            raise ValueError(f"mxfp4_tensor: shape {tuple(shape)} has codes [..., {16 * kb}] and scales [..., {kb}], "
+                             f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if codes.device != scales.device:
+            raise L.MXKError(f"tensors on different devices: {codes.device} and {scales.device}")
+        self.codes = _aligned(codes.contiguous())
+        self.scales = scales.contiguous()
+        self.shape = shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def dim(self) -> int:
+        return len(self.shape)
+
+    def to(self, device) -> "mxfp4_tensor":
+        return mxfp4_tensor(self.codes.to(device), self.scales.to(device), self.shape)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> Tensor:
+        """The values as float32, float16 or bfloat16 (exact in float32 and
+        bfloat16 below their largest value; float16 rounds to nearest even)."""
+        dev = L.require_gpu(self.codes)
+        y = torch.empty(self.shape, dtype=dtype, device=dev)
+        if y.numel():
+            with L.on_device(dev):
+                rc = L.lib().mxk_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _rows(self.shape),
+                                                  self.shape[-1], L.elem_type(dtype), y.data_ptr(), L.stream_of(y))
+            L.check(rc, "mxfp4 dequantize")
+        return y
+
+    def __repr__(self):
+        return f"mxfp4_tensor(shape={tuple(self.shape)}, device={self.device})"
+
+
+def _aligned(codes: Tensor) -> Tensor:
+    """Codes on a 16-byte boundary, as the products read them (rows are 16-byte multiples)."""
+    return codes if codes.data_ptr() % 16 == 0 else codes.clone()
+
+
+def _rows(shape) -> int:
+    return math.prod(shape[:-1])
+
+
+def mxfp4_quantize(x: Tensor) -> mxfp4_tensor:
+    """Pack a [..., K] tensor in blocks of 32 along its last dimension.
+
+    Per block: scale byte = max(exponent of the largest magnitude - 2, -127) +
+    127, code = the nearest grid value of x / 2**(scale - 127), ties to the
+    even code, magnitudes above 6 to 6."""
+    if x.dim() < 1:
+        raise ValueError("mxfp4_quantize: a tensor of at least one dimension")
+    dev = L.require_gpu(x)
+    x = x.detach()
+    if x.dtype not in _FLOATS:
+        x = x.float()
+    shape = x.shape
+    cols = shape[-1]
+    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
+        ld = x.stride(0)  # rows may lie apart
+    else:
+        x = x.contiguous()
+        ld = cols
+    kb = -(-cols // 32)
+    codes = torch.empty(*shape[:-1], 16 * kb, dtype=torch.uint8, device=dev)
+    scales = torch.empty(*shape[:-1], kb, dtype=torch.uint8, device=dev)
+    if x.numel():
+        with L.on_device(dev):
+            rc = L.lib().mxk_mxfp4_quantize(x.data_ptr(), L.elem_type(x.dtype), _rows(shape), cols, ld,
+                                            codes.data_ptr(), scales.data_ptr(), L.stream_of(x))
+        L.check(rc, f"mxfp4_quantize({tuple(shape)})")
+    return mxfp4_tensor(codes, scales, shape)
+
+
+def _bias_f32(bias: Optional[Tensor], shape: Tuple[int, ...]) -> Optional[Tensor]:
+    if bias is None:
+        return None
+    if tuple(bias.shape) != shape:
+        raise ValueError(f"bias of shape {shape} expected, got {tuple(bias.shape)}")
+    return bias.detach().float().contiguous()
+
+
+def _product(a: mxfp4_tensor, b: mxfp4_tensor, rows: int, N: int, bias: Optional[Tensor], out: Tensor,
+             offsets: Optional[Tensor] = None, order: Optional[Tensor] = None, top: int = 1) -> Tensor:
+    """out [rows, N] = a @ b.T (+ bias), by expert where offsets are given."""
+    dev = L.require_gpu(a.codes, b.codes, bias, offsets, order)
+    with L.on_device(dev):
+        rc = L.lib().mxk_mxfp4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), _rows(a.shape), b.codes.data_ptr(),
+                                      b.scales.data_ptr(), rows, N, b.shape[-1], L.ptr(bias),
+                                      L.elem_type(out.dtype), out.data_ptr(), L.ptr(offsets),
+                                      0 if offsets is None else offsets.numel() - 1, L.ptr(order), top,
+                                      L.stream_of(out))
+    L.check(rc, f"mxfp4 product({rows}x{b.shape[-1]} by {N})")
+    return out
+
+
+def mxfp4_matmul(a: mxfp4_tensor, b: mxfp4_tensor, bias: Optional[Tensor] = None,
+                 out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """a [..., K] @ b [N, K].T (+ bias [N]) of packed operands, [..., N].
+    Products are exact, sums in float32, rounded once to out_dtype."""
+    if not isinstance(a, mxfp4_tensor) or not isinstance(b, mxfp4_tensor):
+        raise TypeError("mxfp4_matmul: two mxfp4_tensors (mxfp4_quantize packs a float tensor)")
+    if b.dim() != 2 or a.shape[-1] != b.shape[1]:
+        raise ValueError(f"mxfp4_matmul: [..., K] and [N, K] expected, got {tuple(a.shape)} and {tuple(b.shape)}")
+    out = torch.empty(*a.shape[:-1], b.shape[0], dtype=out_dtype, device=a.device)
+    return _product(a, b, _rows(a.shape), b.shape[0], _bias_f32(bias, (b.shape[0],)), out)
+
+
+def _grad_a(dy: Tensor, b: mxfp4_tensor, dtype: torch.dtype, offsets: Optional[Tensor] = None) -> Tensor:
+    """dy [M, N] @ dequantize(b) [N, K] (b [E, N, K] by expert), [M, K]."""
+    dev = L.require_gpu(dy, b.codes, offsets)
+    M, N = dy.shape
+    K = b.shape[-1]
+    out = torch.empty(M, K, dtype=dtype, device=dev)
+    with L.on_device(dev):
+        rc = L.lib().mxk_mxfp4_grad_a(dy.data_ptr(), L.elem_type(dy.dtype), M, N, b.codes.data_ptr(),
+                                      b.scales.data_ptr(), K, L.elem_type(dtype), out.data_ptr(), L.ptr(offsets),
+                                      0 if offsets is None else offsets.numel() - 1, L.stream_of(out))
+    L.check(rc, f"mxfp4 gradient of a({M}x{N} by {K})")
+    return out
+
+
+def _grad_b(dy: Tensor, a: mxfp4_tensor, dtype: torch.dtype, offsets: Optional[Tensor] = None) -> Tensor:
+    """dy [M, N].T @ dequantize(a) [M, K], [N, K] ([E, N, K] by expert)."""
+    dev = L.require_gpu(dy, a.codes, offsets)
+    M, N = dy.shape
+    K = a.shape[-1]
+    E = 0 if offsets is None else offsets.numel() - 1
+    out = torch.empty((E, N, K) if E else (N, K), dtype=dtype, device=dev)
+    with L.on_device(dev):
+        rc = L.lib().mxk_mxfp4_grad_b(dy.data_ptr(), L.elem_type(dy.dtype), M, N, a.codes.data_ptr(),
+                                      a.scales.data_ptr(), K, L.elem_type(dtype), out.data_ptr(), L.ptr(offsets), E,
+                                      L.stream_of(out))
+    L.check(rc, f"mxfp4 gradient of b({M}x{N} by {K})")
+    return out
+
+
+def _grad_bias(dy: Tensor, dtype: torch.dtype, offsets: Optional[Tensor] = None) -> Tensor:
+    """Column sums of dy, per expert where offsets are given: the gradient of b
+    against one column of ones."""
+    codes = torch.zeros(dy.shape[0], 16, dtype=torch.uint8, device=dy.device)
+    codes[:, 0] = 2  # the code of 1.0
+    ones = mxfp4_tensor(codes, torch.full((dy.shape[0], 1), 127, dtype=torch.uint8, device=dy.device),
+                        (dy.shape[0], 1))
+    return _grad_b(dy, ones, dtype, offsets).squeeze(-1)
+
+
+def _pack_weight(weight: Union[Tensor, mxfp4_tensor]) -> mxfp4_tensor:
+    return weight if isinstance(weight, mxfp4_tensor) else mxfp4_quantize(weight)
+
+
+class _MXFP4Linear(torch.autograd.Function):
+    """mxfp4_linear over [M, K] rows; `packed` is the weight where it is held
+    packed (weight is then None)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, packed):
+        b = packed if packed is not None else mxfp4_quantize(weight)
+        a = mxfp4_quantize(x)
+        out = torch.empty(x.shape[0], b.shape[0], dtype=x.dtype, device=x.device)
+        _product(a, b, x.shape[0], b.shape[0], _bias_f32(bias, (b.shape[0],)), out)
+        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        kept = ((b.codes, b.scales) if need_x else (None, None)) + ((a.codes, a.scales) if need_w else (None, None))
+        ctx.save_for_backward(*kept)
+        ctx.sizes = (a.shape, b.shape, x.dtype, None if weight is None else weight.dtype,
+                     None if bias is None else bias.dtype)
+        return out
+
+    @staticmethod
+    def backward(ctx, dy):
+        bc, bs, ac, as_ = ctx.saved_tensors
+        a_shape, b_shape, x_dtype, w_dtype, bias_dtype = ctx.sizes
+        dy = dy.contiguous()
+        dx = _grad_a(dy, mxfp4_tensor(bc, bs, b_shape), x_dtype) if ctx.needs_input_grad[0] else None
+        dw = _grad_b(dy, mxfp4_tensor(ac, as_, a_shape), w_dtype) if ctx.needs_input_grad[1] else None
+        db = _grad_bias(dy, bias_dtype) if ctx.needs_input_grad[2] else None
+        return dx, dw, db, None
+
+
+def _check_linear(name: str, x: Tensor, weight, dims: int) -> None:
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"{name}: x is float32, float16 or bfloat16, got {x.dtype}")
+    if not isinstance(weight, mxfp4_tensor) and weight.dtype not in _FLOATS:
+        raise TypeError(f"{name}: the weight is an mxfp4_tensor or a float tensor, got {weight.dtype}")
+    if weight.dim() != dims or x.dim() < 1 or x.shape[-1] != weight.shape[-1]:
+        want = "[N, K]" if dims == 2 else "[E, N, K]"
+        raise ValueError(f"{name}: x [..., K] and a weight {want} expected, got {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)}")
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in ts)
+
+
+def mxfp4_linear(x: Tensor, weight: Union[Tensor, mxfp4_tensor], bias: Optional[Tensor] = None) -> Tensor:
+    """x [..., K] packed to 4 bits, times weight [N, K].T (+ bias [N]), as x's
+    dtype.  weight: an mxfp4_tensor (held packed, no gradient) or a float
+    tensor, packed in the call and differentiable."""
+    _check_linear("mxfp4_linear", x, weight, 2)
+    N, K = weight.shape
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if _wants_grad(x, weight, bias):
+        held = isinstance(weight, mxfp4_tensor)
+        y = _MXFP4Linear.apply(x2, None if held else weight, bias, weight if held else None)
+    else:
+        b = _pack_weight(weight)
+        y = torch.empty(x2.shape[0], N, dtype=x.dtype, device=x.device)
+        _product(mxfp4_quantize(x2), b, x2.shape[0], N, _bias_f32(bias, (N,)), y)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
