@@ -445,6 +445,10 @@ int mxk_mxfp4_quantize(const void* x, int x_type, int64_t rows, int64_t cols, in
 int mxk_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, int y_type, void* y,
                          void* stream);
 
+/* Workspace bytes mxk_mxfp4_matmul needs (0 if none); experts = 0 for a dense
+ * product, picked = 1 with an order. */
+size_t mxk_mxfp4_matmul_workspace(int64_t a_rows, int64_t M, int64_t N, int64_t K, int experts, int picked);
+
 /* y [M][N] (y_type) = a @ b^T (+ bias[N], float32), a [a_rows][K] and b
  * [N][K] packed, exact products, float32 sums.
  * Dense: offsets = order = NULL, a_rows = M.
@@ -456,7 +460,8 @@ int mxk_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, in
  * [0, M].  Codes 16-byte aligned; at most 1000 experts. */
 int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, const void* b_codes,
                      const void* b_scales, int64_t M, int64_t N, int64_t K, const float* bias, int y_type, void* y,
-                     const int32_t* offsets, int experts, const int32_t* order, int top, void* stream);
+                     const int32_t* offsets, int experts, const int32_t* order, int top, void* workspace,
+                     size_t workspace_nbytes, void* stream);
 
 /* da [M][K] (out_type) = dy [M][N] (dy_type) @ dequantize(b) [N][K]: the
  * gradient of a, straight through its quantization.  dy is not rounded,

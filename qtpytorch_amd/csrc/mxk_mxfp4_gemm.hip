@@ -33,24 +33,40 @@ struct Segment {
   int64_t lo, hi;
 };
 template <int BM>
-__device__ __forceinline__ Segment find_segment(int64_t s, const int* offsets, int E, int64_t M) {
-  Segment g;
-  int64_t lo = 0;
-  for (int e = 0; e <= E; ++e) {
-    int64_t hi = e < E ? (int64_t)offsets[e + 1] : M;
-    hi = hi < lo ? lo : (hi > M ? M : hi);
-    const int64_t tiles = (hi - lo + BM - 1) / BM;
-    if (s < tiles) {
-      g.e = e;
-      g.lo = lo + s * BM;
-      g.hi = hi < g.lo + BM ? hi : g.lo + BM;
+__device__ __forceinline__ Segment find_segment(int64_t slot, const int* offsets, int E, int64_t M) {
+  // one segment per lane, 64 at a time: tiles of the segments before by a scan
+  const int lane = threadIdx.x & 63;
+  Segment g = {E + 1, 0, 0};
+  int64_t before = 0;
+  for (int e0 = 0; e0 <= E; e0 += 64) {
+    const int e = e0 + lane;
+    int64_t lo = 0, hi = 0;
+    if (e <= E) {
+      lo = e == 0 ? 0 : (int64_t)offsets[e];
+      hi = e == E ? M : (int64_t)offsets[e + 1];
+      lo = lo < 0 ? 0 : (lo > M ? M : lo);
+      hi = hi < lo ? lo : (hi > M ? M : hi);
+    }
+    const int tiles = (int)((hi - lo + BM - 1) / BM);
+    int upto = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(upto, d);
+      if (lane >= d) upto += v;
+    }
+    const int64_t at = slot - before;
+    const uint64_t here = __ballot(at >= upto - tiles && at < upto);
+    if (here) {
+      const int src = __builtin_ctzll(here);
+      const int first = __shfl(upto - tiles, src);
+      const int64_t slo = __shfl((int)lo, src), shi = __shfl((int)hi, src);
+      g.e = __builtin_amdgcn_readfirstlane(e0 + src);
+      g.lo = __builtin_amdgcn_readfirstlane((int)(slo + (at - first) * BM));
+      g.hi = __builtin_amdgcn_readfirstlane((int)(shi < slo + (at - first + 1) * BM ? shi : slo + (at - first + 1) * BM));
       return g;
     }
-    s -= tiles;
-    lo = hi;
+    before += __shfl(upto, 63);
   }
-  g.e = E + 1;
-  g.lo = g.hi = 0;
   return g;
 }
 // Slots that cover every case of M rows in E segments and the rows without an
@@ -149,19 +165,434 @@ __global__ __launch_bounds__(256) void k_fp4_gemm(Fp4Gemm p) {
   }
 }
 
-static int launch_gemm(const Fp4Gemm& p, int y_type, hipStream_t st) {
+
+// ---------------------------------------------------------------- tiles through LDS
+// Scale bytes in the order in which the tile kernel's stages read them:
+// out[kt][row][8], kt = stages of 8 blocks (256 values of K), zeros past KB,
+// for the rows of the product (picked by `order` where there is one) and those of b.  One
+// launch for both operands: 17/16 of a byte moved per 32 values.
+__global__ __launch_bounds__(256) void k_fp4_stage_scales(Fp4Gemm p, int64_t b_rows, int64_t a_blocks,
+                                                          uint8_t* __restrict__ ta, uint8_t* __restrict__ tb) {
+  const bool of_a = (int64_t)blockIdx.x < a_blocks;
+  const int64_t rows = of_a ? p.M : b_rows;
+  const int64_t r = (of_a ? (int64_t)blockIdx.x : (int64_t)blockIdx.x - a_blocks) * 32 + (threadIdx.x >> 3);
+  if (r >= rows) return;
+  const int64_t src = of_a ? source_row(p, r) : r;
+  const uint8_t* s = (of_a ? p.as : p.bs) + (src < 0 ? 0 : src) * p.KB;
+  uint8_t* out = of_a ? ta : tb;
+  for (int64_t k = 8 * (threadIdx.x & 7); k < p.KB; k += 64) {
+    uint64_t v = 0;
+    if (src >= 0) {
+      if (k + 8 <= p.KB) {
+        __builtin_memcpy(&v, s + k, 8);
+      } else {
+        for (int i = 0; i < 8; ++i)
+          if (k + i < p.KB) v |= (uint64_t)s[k + i] << (8 * i);
+      }
+    }
+    *reinterpret_cast<uint64_t*>(out + ((k >> 3) * rows + r) * 8) = v;
+  }
+}
+
+// Raw buffer resource over [p, p + bytes), wave-uniform: loads past the end return 0
+__device__ __forceinline__ i32x4 buffer_words(const void* p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+               __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xFFFF),
+               __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+// 16 bytes per lane from a buffer into LDS at `lds` + 16 * lane.  In
+// assembly, so that the compiler does not order the tile's LDS reads behind
+// loads of the other buffer; the kernel waits for them itself (wait_loads).
+__device__ __forceinline__ void load_to_lds(i32x4 r, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(off), "s"(r)
+               : "memory");
+}
+// The scales of R rows, 8 bytes each, by one instruction of the wave
+template <int R>
+__device__ __forceinline__ void load_scales_to_lds(i32x4 r, int lane, uint32_t lds) {
+  if constexpr (R == 128) {
+    load_to_lds(r, 16u * lane, lds);
+  } else {
+    static_assert(R == 64, "16 or 8 bytes per lane");
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds\n\t"
+                 "s_mov_b32 m0, %3\n\tbuffer_load_dword %4, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(4u * lane), "s"(r), "s"(lds + 256u), "v"(4u * lane + 256u)
+                 : "memory");
+  }
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"(N) : "memory");
+}
+
+// wait_loads<N> where `counted`, else wait_loads<0>; the choice is made inside
+// the assembly, which keeps the compiler from doubling the loop around it
+template <int N>
+__device__ __forceinline__ void wait_loads_if(uint32_t counted) {
+  asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 1f\n\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_branch 2f\n"
+               "1:\ts_waitcnt vmcnt(0) lgkmcnt(0)\n2:"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(counted)), "i"(N)
+               : "memory", "scc");
+}
+
+// Tile t of a grid of tm x tn, taken so that the workgroups of one XCD
+// (blockIdx % 8) are consecutive tiles of an order that walks 8 rows of tiles
+// down before it goes right: the 32 tiles an XCD holds at once share 8 row
+// and 4 column panels in its L2.
+__device__ __forceinline__ void place_tile(uint32_t id, uint32_t tm, uint32_t tn, uint32_t& m, uint32_t& n) {
+  const uint32_t total = tm * tn, xcd = id & 7u, local = id >> 3;
+  const uint32_t per = total >> 3, rest = total & 7u;
+  const uint32_t t = xcd * per + min(xcd, rest) + local;
+  const uint32_t group = t / (8u * tn), in = t - group * 8u * tn;
+  const uint32_t high = min(8u, tm - group * 8u);
+  n = in / high;
+  m = group * 8u + (in - n * high);
+}
+
+#define MXK_FAR_ROW 0x80000000u   // offset of a row that is not there: past every buffer (at most 2^30 bytes)
+#define MXK_FAR_BLOCK 0x40000000u // added for blocks past KB
+
+// Tiles of (2 * 32 * F)^2, four waves of F x F fragments of 32 x 32, stages
+// of 256 values of K (128 bytes a row) in two LDS buffers.
+//
+// v_mfma_scale_f32_32x32x64_f8f6f4: lane l holds row l % 32 and one of the two
+// blocks of a step; the four steps of a stage give lane half h the blocks
+// 4h .. 4h+3, so one dword per row holds its four scale bytes and a step
+// selects its byte.  (Any order of K is right as long as both operands share it.)
+//
+// LDS rows are 128 bytes: 16-byte chunk c of row r sits at c ^ (r & 7), so
+// that 8 lanes of consecutive rows read all banks once.  The loads write LDS
+// in lane order, so the lane picks the chunk that belongs at its place.
+//
+// The barrier of a stage sits before its last step: by then the next stage
+// has landed and this stage's last fragments are in registers, so the loads of the
+// stage after next go into the buffer just read, and the next stage's first
+// fragments are read while the last step multiplies.
+template <typename T, int F, bool EXPERT>
+__global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8_t* __restrict__ ta,
+                                                          const uint8_t* __restrict__ tb, int64_t b_rows, uint32_t tm,
+                                                          uint32_t tn) {
+  constexpr int B = 64 * F;                 // rows of a tile
+  constexpr int OP = B * 128, SC = B * 8;   // bytes of an operand's stage and of its scales
+  constexpr int BUF = 2 * OP, SBUF = 2 * SC;
+  constexpr int LI = B / 32;                // load instructions per wave, operand and stage
+  constexpr int NW = 32 * F;                // columns of a wave
+  constexpr int CB = F == 4 ? 128 : 64;     // bytes of a row that the result passes through LDS at once
+  constexpr int CH = CB / 16, CC = CB / (int)sizeof(T), PASS = NW / CC;
+  constexpr int STORES = F * PASS * 32 * CH / 64;  // store instructions per wave and tile
+  __shared__ __align__(16) uint8_t lds[2 * BUF + 2 * SBUF + 4 * 32 * CB];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r32 = lane & 31, h = lane >> 5;
+  T* y = reinterpret_cast<T*>(p.y);
+  const uint32_t row_bytes = (uint32_t)p.KB * 16u;
+  const uint32_t KB = (uint32_t)p.KB, stages = (KB + 7u) >> 3;
+  const bool picked = EXPERT && p.order != nullptr;
+  // whole 16-byte pieces of y: stores by buffer, as many for every tile
+  const bool whole = p.N * (int)sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
+
+  // the tile that is being loaded, and the one whose result is due
+  int64_t lo = 0, hi = 0, n0 = 0;
+  int e = 0;
+  i32x4 ra, rb;
+  // loads of this wave: rows (wave * LI + i) * 8 + lane / 8 of either operand
+  const int lr = lane >> 3, chunk = (lane & 7) ^ lr;
+  const uint32_t off0 = (uint32_t)(wave * LI * 8 + lr) * row_bytes, step8 = 8u * row_bytes;
+  uint32_t off_a[EXPERT ? LI : 1];  // by expert: of any rows
+
+  // the next tile from `id` on that has products (rows without an expert are
+  // written here): true, or false at the end
+  auto next_tile = [&](uint32_t& id) -> bool {
+    for (; id < tm * tn; id += gridDim.x) {
+      uint32_t mt, nt;
+      place_tile(id, tm, tn, mt, nt);
+      lo = (int64_t)mt * B;
+      hi = p.M < lo + B ? p.M : lo + B;
+      n0 = (int64_t)nt * B;
+      if (EXPERT) {
+        const Segment s = find_segment<B>(mt, p.offsets, p.E, p.M);
+        e = s.e;
+        lo = s.lo;
+        hi = s.hi;
+        if (e > p.E) continue;
+        if (e == p.E) {
+          const int64_t w = p.N - n0 < B ? p.N - n0 : B;
+          for (int64_t r = lo + wave; r < hi; r += 4)
+            for (int64_t c = lane; c < w; c += 64) y[r * p.N + n0 + c] = from_f32<T>(0.0f);
+          continue;
+        }
+      }
+      const int64_t rows_b = p.N - n0 < B ? p.N - n0 : B;
+      const uint8_t* a0 = picked ? p.a : p.a + lo * (int64_t)row_bytes;
+      const int64_t rows_a = picked ? p.a_rows : (p.M - lo < B ? p.M - lo : B);
+      ra = buffer_words(a0, (uint32_t)(rows_a * row_bytes));
+      rb = buffer_words(p.b + ((int64_t)e * p.N + n0) * row_bytes, (uint32_t)(rows_b * row_bytes));
+      if constexpr (EXPERT) {
+#pragma unroll
+        for (int i = 0; i < LI; ++i) {
+          const int64_t r = lo + (wave * LI + i) * 8 + lr;
+          const int64_t src = r < hi ? (picked ? source_row(p, r) : r - lo) : -1;
+          off_a[i] = src >= 0 ? (uint32_t)src * row_bytes : MXK_FAR_ROW;
+        }
+      }
+      return true;
+    }
+    return false;
+  };
+  // part q of F of the loads of stage t
+  auto issue = [&](uint32_t t, uint32_t buf, int q) {
+    const uint32_t blk = 8u * t + chunk;
+    const uint32_t ok = blk < KB ? blk * 16u : MXK_FAR_BLOCK;
+#pragma unroll
+    for (int i = q * LI / F; i < (q + 1) * LI / F; ++i) {
+      const uint32_t off = off0 + i * step8 + ok;
+      load_to_lds(ra, EXPERT ? off_a[EXPERT ? i : 0] + ok : off, buf * BUF + (wave * LI + i) * 1024u);
+      load_to_lds(rb, off, buf * BUF + OP + (wave * LI + i) * 1024u);
+    }
+    // scales: planes of [rows][8] bytes, B / 128 kilobytes an operand; waves 0, 1
+    // take a's, 2, 3 b's (F = 2: each wave half a kilobyte, the upper lanes nothing)
+    if (q == 0) {
+      constexpr int R = B / 2;  // rows per wave
+      const bool of_b = wave >= 2;
+      const int64_t rows = of_b ? b_rows : p.M;
+      const int64_t first = (of_b ? (int64_t)e * p.N + n0 : lo) + R * (wave & 1);
+      // past the last row: bytes of the next plane or of the kilobytes kept after the
+      // last, for rows whose codes are zeros or whose results are not stored
+      const i32x4 rs = buffer_words((of_b ? tb : ta) + ((int64_t)t * rows + first) * 8, t < stages ? R * 8u : 0u);
+      load_scales_to_lds<R>(rs, lane, 2u * BUF + buf * SBUF + (of_b ? SC : 0) + R * 8u * (wave & 1));
+    }
+  };
+
+  // fragment reads: rows of this wave's half of a (wave / 2) and of b (wave % 2)
+  const uint32_t rd_a = (uint32_t)((wave >> 1) * 32 * F + r32) * 128u;
+  const uint32_t rd_b = OP + (uint32_t)((wave & 1) * 32 * F + r32) * 128u;
+  uint32_t at[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) at[s] = (uint32_t)((4 * h + s) ^ (lane & 7)) * 16u;
+  const uint32_t rs_a = 2 * BUF + ((wave >> 1) * 32 * F + r32) * 8 + 4 * h;
+  const uint32_t rs_b = 2 * BUF + SC + ((wave & 1) * 32 * F + r32) * 8 + 4 * h;
+
+  f32x16 acc[F][F];  // [b fragment][a fragment]: rows of the result are n
+  i32x4 fa[2][F], fb[2][F];
+  int sa[2][F], sb[2][F];
+  auto read_frag = [&](uint32_t buf, int s, int i, i32x4 (&xa)[F], i32x4 (&xb)[F]) {
+    xa[i] = *reinterpret_cast<const i32x4*>(lds + buf * BUF + rd_a + at[s] + i * 4096);
+    xb[i] = *reinterpret_cast<const i32x4*>(lds + buf * BUF + rd_b + at[s] + i * 4096);
+  };
+  auto read_scale = [&](uint32_t buf, int i, int (&xa)[F], int (&xb)[F]) {
+    xa[i] = *reinterpret_cast<const int*>(lds + buf * SBUF + rs_a + i * 256);
+    xb[i] = *reinterpret_cast<const int*>(lds + buf * SBUF + rs_b + i * 256);
+  };
+  // One step: a row of F MFMAs at a time, after what `between` issues for it
+#define MXK_STEP(SEL, XA, XB, BETWEEN)                                                                       \
+  _Pragma("unroll") for (int i = 0; i < F; ++i) {                                                           \
+    BETWEEN;                                                                                                \
+    __builtin_amdgcn_sched_barrier(0);                                                                      \
+    _Pragma("unroll") for (int j = 0; j < F; ++j) {                                                         \
+      const i32x8 va = {XA[j][0], XA[j][1], XA[j][2], XA[j][3], 0, 0, 0, 0};                                \
+      const i32x8 vb = {XB[i][0], XB[i][1], XB[i][2], XB[i][3], 0, 0, 0, 0};                                \
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vb, va, acc[i][j], 4, 4, SEL, sb[0][i],   \
+                                                                  SEL, sa[0][j]);                           \
+    }                                                                                                       \
+    __builtin_amdgcn_sched_barrier(0);                                                                      \
+  }
+
+  constexpr int LOADS = 2 * LI + (F == 4 ? 1 : 2);  // per wave and stage
+  uint32_t id = blockIdx.x;
+  if (!next_tile(id)) return;
+#pragma unroll
+  for (int q = 0; q < F; ++q) issue(0, 0, q);
+#pragma unroll
+  for (int q = 0; q < F; ++q) issue(1, 1, q);
+  // stores of the tile before, issued after this tile's first loads: memory
+  // operations of a wave complete in order, so those loads are waited for
+  // without them
+  constexpr bool COUNTED = STORES + LOADS <= 63;  // as the wait's field has room for
+  uint32_t stores_due = 0;
+  for (;;) {
+    // sums start from the bias, which every row of a fragment shares
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      float b[16];
+#pragma unroll
+      for (int q = 0; q < 16; ++q) b[q] = 0.0f;
+      if (p.bias) {
+        const int64_t n = n0 + (wave & 1) * NW + 32 * i + 4 * h;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const int64_t at = n + 8 * (q >> 2) + (q & 3);
+          b[q] = p.bias[(int64_t)e * p.N + (at < p.N ? at : p.N - 1)];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < F; ++j)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) acc[i][j][q] = b[q];
+    }
+    if (COUNTED && stores_due) wait_loads<(COUNTED ? STORES : 0) + LOADS>();
+    else wait_loads<LOADS>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      read_scale(0, i, sa[0], sb[0]);
+      read_frag(0, 0, i, fa[0], fb[0]);
+    }
+    // past the last stage the loads bring zeros and the reads are not used
+    uint32_t buf = 0;
+    for (uint32_t t = 0; t < stages; ++t) {
+      MXK_STEP(0, fa[0], fb[0], read_frag(buf, 1, i, fa[1], fb[1]))
+      MXK_STEP(1, fa[1], fb[1], read_frag(buf, 2, i, fa[0], fb[0]))
+      MXK_STEP(2, fa[0], fb[0], read_frag(buf, 3, i, fa[1], fb[1]))
+      if constexpr (COUNTED) {
+        wait_loads_if<STORES>(t == 0 ? stores_due : 0u);
+      } else {
+        wait_loads<0>();
+      }
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      buf ^= 1u;
+      MXK_STEP(3, fa[1], fb[1], {
+        read_scale(buf, i, sa[1], sb[1]);
+        read_frag(buf, 0, i, fa[0], fb[0]);
+        issue(t + 2, buf ^ 1u, i);
+      })
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        sa[0][i] = sa[1][i];
+        sb[0][i] = sb[1][i];
+      }
+    }
+    wait_loads<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+
+    // the next tile's first two stages are under way while this one's result leaves
+    const int64_t m0 = lo, m1 = hi, c0 = n0;
+    id += gridDim.x;
+    const bool more = next_tile(id);
+    if (more) {
+#pragma unroll
+      for (int q = 0; q < F; ++q) issue(0, 0, q);
+#pragma unroll
+      for (int q = 0; q < F; ++q) issue(1, 1, q);
+    }
+
+    // The result through LDS, 32 rows of m and CB bytes of n at a time and
+    // wave: a lane holds four consecutive n of one m; whole 64- or 128-byte
+    // pieces of rows leave in 16-byte stores.
+    uint8_t* mine = lds + 2 * BUF + 2 * SBUF + wave * 32 * CB;
+    const int64_t nw = c0 + (wave & 1) * NW, mw = m0 + (wave >> 1) * NW;
+    // the sums stay where they are until here: read earlier, they would push the loads' addresses into scratch
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+      for (int j = 0; j < F; ++j) asm volatile("" : "+a"(acc[i][j]));
+    // a buffer over this wave's rows; its offsets stay below 2^31 (N checked on the host)
+    const int64_t left = m1 - mw;
+    const uint32_t pitch = (uint32_t)p.N * (uint32_t)sizeof(T);
+    const __amdgpu_buffer_rsrc_t ry =
+        make_rsrc(y + mw * p.N, left <= 0 ? 0u : (uint32_t)(left < NW ? left : NW) * pitch);
+    uint32_t el = (uint32_t)lane;
+    asm volatile("" : "+v"(el));  // the addresses below are not worth registers during the products
+    const uint32_t col = (uint32_t)nw * (uint32_t)sizeof(T) + (el % CH) * 16u, out0 = (el / CH) * pitch + col;
+    uint8_t* put = mine + (el & 31u) * CB;
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+#pragma unroll
+      for (int s = 0; s < PASS; ++s) {
+#pragma unroll
+        for (int u = 0; u < CC / 8; ++u) {
+          const int iq = s * (CC / 8) + u, i = iq >> 2, q = iq & 3;
+          T t[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) t[k] = from_f32<T>(acc[i][j][4 * q + k]);
+          const uint32_t byte = (8 * u + 4 * (el >> 5)) * (uint32_t)sizeof(T);
+          uint8_t* d = put + (((byte >> 4) ^ (el & (CH - 1))) << 4) + (byte & 15);
+          __builtin_memcpy(__builtin_assume_aligned(d, 4 * sizeof(T)), t, sizeof(t));
+        }
+        __builtin_amdgcn_wave_barrier();
+        u32x4 v[CH / 2];
+#pragma unroll
+        for (int k = 0; k < CH / 2; ++k) {
+          const uint32_t row = k * (64 / CH) + el / CH, ch = el % CH;
+          v[k] = *reinterpret_cast<const u32x4*>(mine + row * CB + ((ch ^ (row & (CH - 1))) << 4));
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < CH / 2; ++k) {
+          if (whole) {
+            const uint32_t o = col + s * CB < pitch ? out0 + (32 * j + k * (64 / CH)) * pitch + s * CB : 0x80000000u;
+            __builtin_amdgcn_raw_buffer_store_b128(v[k], ry, (int)o, 0, 0);
+          } else if (const uint32_t row = 32 * j + k * (64 / CH) + el / CH; mw + row < m1) {
+            const int64_t n = nw + s * CC + (el % CH) * (16 / sizeof(T));
+            T t[16 / sizeof(T)];
+            __builtin_memcpy(t, &v[k], 16);
+#pragma unroll
+            for (int q = 0; q < 16 / (int)sizeof(T); ++q)
+              if (n + q < p.N) y[(mw + row) * p.N + n + q] = t[q];
+          }
+        }
+      }
+    if (!more) return;
+    stores_due = whole ? 1u : 0u;
+  }
+#undef MXK_STEP
+}
+
+// Bytes of the scales of `rows` rows in stage order, with room for the last tile's reads past the end
+static int64_t stage_bytes(int64_t rows, int64_t KB) { return ceil_div(KB, 8) * rows * 8 + 4096; }
+
+// Fragments a side of the tile kernel's waves for a problem, 0: the plain kernel
+static int tile_of(const Fp4Gemm& p) {
+  const int64_t row_bytes = p.KB * 16;
+  if (p.KB == 0 || p.M < 64 || p.N < 64 || row_bytes > (1 << 22)) return 0;
+  if (p.order && p.a_rows * row_bytes > ((int64_t)1 << 30)) return 0;
+  if (p.N >= ((int64_t)1 << 21)) return 0;  // 256 rows of 4-byte results within 2^31 bytes
+  const int64_t m4 = p.offsets ? segment_slots(p.M, p.E, 256) : ceil_div(p.M, 256);
+  if (p.offsets && p.M < 64 * (int64_t)p.E) return 0;
+  return m4 * ceil_div(p.N, 256) >= 192 ? 4 : 2;
+}
+
+static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_bytes, hipStream_t st) {
   const bool ex = p.offsets != nullptr;
-  const int64_t slots = ex ? segment_slots(p.M, p.E, 64) : ceil_div(p.M, 64);
-  const int64_t n = slots * ceil_div(p.N, 64);
+  const int F = tile_of(p);
+  const int64_t B = F ? 64 * F : 64;
+  const int64_t slots = ex ? segment_slots(p.M, p.E, (int)B) : ceil_div(p.M, B);
+  const int64_t tn = ceil_div(p.N, B), n = slots * tn;
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many tiles");
-#define MXK_L(T)                                                                                         \
-  do {                                                                                                   \
-    if (ex) hipLaunchKernelGGL((k_fp4_gemm<T, true>), dim3((unsigned)n), dim3(256), 0, st, p);           \
-    else hipLaunchKernelGGL((k_fp4_gemm<T, false>), dim3((unsigned)n), dim3(256), 0, st, p);             \
+  const int64_t b_rows = ex ? p.E * p.N : p.N, na = stage_bytes(p.M, p.KB), nb = stage_bytes(b_rows, p.KB);
+  if (F && (!ws || ws_bytes < (size_t)(na + nb))) return fail(MXK_EINVAL, "mxfp4 product: workspace too small");
+  if (F) {
+    const int64_t ga = ceil_div(p.M, 32), gb = ceil_div(b_rows, 32);
+    if (ga + gb >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many rows");
+    hipLaunchKernelGGL(k_fp4_stage_scales, dim3((unsigned)(ga + gb)), dim3(256), 0, st, p, b_rows, ga, ws, ws + na);
+  }
+  const int64_t cus = (num_cus() + 7) & ~7;  // a multiple of the XCDs: a workgroup's tiles stay on its own
+#define MXK_L(T, EX)                                                                                              \
+  do {                                                                                                            \
+    if (F == 4)                                                                                                   \
+      hipLaunchKernelGGL((k_fp4_gemm_tile<T, 4, EX>), dim3((unsigned)std::min(n, cus)), dim3(256), 0, st, p, ws, ws + na,       \
+                         b_rows, (uint32_t)slots, (uint32_t)tn);                                                  \
+    else if (F == 2)                                                                                              \
+      hipLaunchKernelGGL((k_fp4_gemm_tile<T, 2, EX>), dim3((unsigned)std::min(n, 2 * cus)), dim3(256), 0, st, p, ws, ws + na,       \
+                         b_rows, (uint32_t)slots, (uint32_t)tn);                                                  \
+    else                                                                                                          \
+      hipLaunchKernelGGL((k_fp4_gemm<T, EX>), dim3((unsigned)n), dim3(256), 0, st, p);                           \
   } while (0)
-  if (y_type == MXK_IN_F32) MXK_L(float);
-  else if (y_type == MXK_IN_F16) MXK_L(__half);
-  else MXK_L(hip_bfloat16);
+#define MXK_T(T)                \
+  do {                          \
+    if (ex) MXK_L(T, true);     \
+    else MXK_L(T, false);       \
+  } while (0)
+  if (y_type == MXK_IN_F32) MXK_T(float);
+  else if (y_type == MXK_IN_F16) MXK_T(__half);
+  else MXK_T(hip_bfloat16);
+#undef MXK_T
 #undef MXK_L
   return check_launch("mxfp4 product");
 }
@@ -172,9 +603,25 @@ using namespace mxk;
 
 extern "C" {
 
+size_t mxk_mxfp4_matmul_workspace(int64_t a_rows, int64_t M, int64_t N, int64_t K, int experts, int picked) {
+  if (a_rows < 0 || M <= 0 || N <= 0 || K <= 0 || experts < 0) return 0;
+  Fp4Gemm p = {};
+  static const int some = 0;
+  p.a_rows = a_rows;
+  p.M = M;
+  p.N = N;
+  p.KB = fp4_blocks(K);
+  p.offsets = experts > 0 ? &some : nullptr;
+  p.order = picked ? &some : nullptr;
+  p.E = experts;
+  if (!tile_of(p)) return 0;
+  return (size_t)(stage_bytes(M, p.KB) + stage_bytes(experts > 0 ? experts * N : N, p.KB));
+}
+
 int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, const void* b_codes,
                      const void* b_scales, int64_t M, int64_t N, int64_t K, const float* bias, int y_type, void* y,
-                     const int32_t* offsets, int experts, const int32_t* order, int top, void* stream) {
+                     const int32_t* offsets, int experts, const int32_t* order, int top, void* workspace,
+                     size_t workspace_nbytes, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (a_rows < 0 || M < 0 || N < 0 || K < 0) return fail(MXK_EINVAL, "mxfp4_matmul: negative size");
   if (M >= ((int64_t)1 << 31) || N >= ((int64_t)1 << 31) || K >= ((int64_t)1 << 28) || a_rows >= ((int64_t)1 << 31))
@@ -204,7 +651,7 @@ int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, 
   p.E = experts;
   p.order = order;
   p.top = make_divu32((uint32_t)(top < 1 ? 1 : top));
-  return launch_gemm(p, y_type, st);
+  return launch_gemm(p, y_type, reinterpret_cast<uint8_t*>(workspace), workspace_nbytes, st);
 }
 
 }  // extern "C"

@@ -135,13 +135,17 @@ def _product(a: mxfp4_tensor, b: mxfp4_tensor, rows: int, N: int, bias: Optional
              offsets: Optional[Tensor] = None, order: Optional[Tensor] = None, top: int = 1) -> Tensor:
     """out [rows, N] = a @ b.T (+ bias), by expert where offsets are given."""
     dev = L.require_gpu(a.codes, b.codes, bias, offsets, order)
+    lib = L.lib()
+    a_rows, K = _rows(a.shape), b.shape[-1]
+    E = 0 if offsets is None else offsets.numel() - 1
+    nbytes = lib.mxk_mxfp4_matmul_workspace(a_rows, rows, N, K, E, order is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with L.on_device(dev):
-        rc = L.lib().mxk_mxfp4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), _rows(a.shape), b.codes.data_ptr(),
-                                      b.scales.data_ptr(), rows, N, b.shape[-1], L.ptr(bias),
-                                      L.elem_type(out.dtype), out.data_ptr(), L.ptr(offsets),
-                                      0 if offsets is None else offsets.numel() - 1, L.ptr(order), top,
-                                      L.stream_of(out))
-    L.check(rc, f"mxfp4 product({rows}x{b.shape[-1]} by {N})")
+        rc = lib.mxk_mxfp4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), a_rows, b.codes.data_ptr(),
+                                  b.scales.data_ptr(), rows, N, K, L.ptr(bias), L.elem_type(out.dtype),
+                                  out.data_ptr(), L.ptr(offsets), E, L.ptr(order), top, L.ptr(ws), nbytes,
+                                  L.stream_of(out))
+    L.check(rc, f"mxfp4 product({rows}x{K} by {N})")
     return out
 
 
