@@ -463,18 +463,24 @@ int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, 
                      const int32_t* offsets, int experts, const int32_t* order, int top, void* workspace,
                      size_t workspace_nbytes, void* stream);
 
+/* Workspace bytes (16-byte aligned) the two gradients below need: 0 for
+ * bf16 dy whose rows start on 16 bytes, else its bf16 terms. */
+size_t mxk_mxfp4_grad_workspace(const void* dy, int dy_type, int64_t M, int64_t N);
+
 /* da [M][K] (out_type) = dy [M][N] (dy_type) @ dequantize(b) [N][K]: the
  * gradient of a, straight through its quantization.  dy is not rounded,
- * sums are float32.  By expert as mxk_mxfp4_matmul: b [experts][N][K], rows
+ * sums are float32.  N below 2^22, K below 2^26.  By expert as mxk_mxfp4_matmul: b [experts][N][K], rows
  * past the last expert's zeros. */
 int mxk_mxfp4_grad_a(const void* dy, int dy_type, int64_t M, int64_t N, const void* b_codes, const void* b_scales,
-                     int64_t K, int out_type, void* da, const int32_t* offsets, int experts, void* stream);
+                     int64_t K, int out_type, void* da, const int32_t* offsets, int experts, void* workspace,
+                     size_t workspace_nbytes, void* stream);
 
 /* db [N][K] (out_type) = dy [M][N]^T @ dequantize(a) [M][K]: the gradient of
  * b.  By expert: db [experts][N][K], each over its own rows (zeros for an
  * expert without rows). */
 int mxk_mxfp4_grad_b(const void* dy, int dy_type, int64_t M, int64_t N, const void* a_codes, const void* a_scales,
-                     int64_t K, int out_type, void* db, const int32_t* offsets, int experts, void* stream);
+                     int64_t K, int out_type, void* db, const int32_t* offsets, int experts, void* workspace,
+                     size_t workspace_nbytes, void* stream);
 
 /* ------------------------------------------------ tokens to experts and back
  * Pick i = t*top + j is token t's j-th choice.  All arrays int32 on the

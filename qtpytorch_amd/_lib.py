@@ -83,8 +83,11 @@ SIGNATURES = {
     "mxk_mxfp4_matmul": (c_int, [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_int,
                                  c_vp, c_int, c_vp, c_sz, c_vp]),
     "mxk_mxfp4_matmul_workspace": (c_sz, [c_i64, c_i64, c_i64, c_i64, c_int, c_int]),
-    "mxk_mxfp4_grad_a": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_vp]),
-    "mxk_mxfp4_grad_b": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_vp]),
+    "mxk_mxfp4_grad_a": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_vp,
+                                 c_sz, c_vp]),
+    "mxk_mxfp4_grad_b": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_vp, c_sz,
+                                 c_vp]),
+    "mxk_mxfp4_grad_workspace": (c_sz, [c_vp, c_int, c_i64, c_i64]),
     "mxk_expert_sort_workspace": (c_sz, [c_i64, c_int]),
     "mxk_expert_sort": (c_int, [c_vp, c_int, c_i64, c_int, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "mxk_expert_gather": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_int, c_vp, c_vp]),

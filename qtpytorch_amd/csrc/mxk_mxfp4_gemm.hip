@@ -25,56 +25,6 @@ struct Fp4Gemm {
   DivU32 top;
 };
 
-// Slot s of the tiles of BM rows of all segments (the experts', then the rows
-// without one): its segment and rows.  Offsets are brought into [0, M], so
-// that no row outside the product is named whatever they hold.
-struct Segment {
-  int e;  // E: rows without an expert; E + 1: no tile
-  int64_t lo, hi;
-};
-template <int BM>
-__device__ __forceinline__ Segment find_segment(int64_t slot, const int* offsets, int E, int64_t M) {
-  // one segment per lane, 64 at a time: tiles of the segments before by a scan
-  const int lane = threadIdx.x & 63;
-  Segment g = {E + 1, 0, 0};
-  int64_t before = 0;
-  for (int e0 = 0; e0 <= E; e0 += 64) {
-    const int e = e0 + lane;
-    int64_t lo = 0, hi = 0;
-    if (e <= E) {
-      lo = e == 0 ? 0 : (int64_t)offsets[e];
-      hi = e == E ? M : (int64_t)offsets[e + 1];
-      lo = lo < 0 ? 0 : (lo > M ? M : lo);
-      hi = hi < lo ? lo : (hi > M ? M : hi);
-    }
-    const int tiles = (int)((hi - lo + BM - 1) / BM);
-    int upto = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(upto, d);
-      if (lane >= d) upto += v;
-    }
-    const int64_t at = slot - before;
-    const uint64_t here = __ballot(at >= upto - tiles && at < upto);
-    if (here) {
-      const int src = __builtin_ctzll(here);
-      const int first = __shfl(upto - tiles, src);
-      const int64_t slo = __shfl((int)lo, src), shi = __shfl((int)hi, src);
-      g.e = __builtin_amdgcn_readfirstlane(e0 + src);
-      g.lo = __builtin_amdgcn_readfirstlane((int)(slo + (at - first) * BM));
-      g.hi = __builtin_amdgcn_readfirstlane((int)(shi < slo + (at - first + 1) * BM ? shi : slo + (at - first + 1) * BM));
-      return g;
-    }
-    before += __shfl(upto, 63);
-  }
-  return g;
-}
-// Slots that cover every case of M rows in E segments and the rows without an
-// expert: each segment wastes less than a tile, and no tile is empty
-static int64_t segment_slots(int64_t M, int E, int BM) {
-  return std::min<int64_t>(M, (M + (int64_t)(E + 1) * (BM - 1)) / BM);
-}
-
 // Row of a that row r of the product reads, -1: none
 __device__ __forceinline__ int64_t source_row(const Fp4Gemm& p, int64_t r) {
   if (!p.order) return r < p.a_rows ? r : -1;
@@ -238,20 +188,6 @@ __device__ __forceinline__ void wait_loads_if(uint32_t counted) {
                :
                : "s"(__builtin_amdgcn_readfirstlane(counted)), "i"(N)
                : "memory", "scc");
-}
-
-// Tile t of a grid of tm x tn, taken so that the workgroups of one XCD
-// (blockIdx % 8) are consecutive tiles of an order that walks 8 rows of tiles
-// down before it goes right: the 32 tiles an XCD holds at once share 8 row
-// and 4 column panels in its L2.
-__device__ __forceinline__ void place_tile(uint32_t id, uint32_t tm, uint32_t tn, uint32_t& m, uint32_t& n) {
-  const uint32_t total = tm * tn, xcd = id & 7u, local = id >> 3;
-  const uint32_t per = total >> 3, rest = total & 7u;
-  const uint32_t t = xcd * per + min(xcd, rest) + local;
-  const uint32_t group = t / (8u * tn), in = t - group * 8u * tn;
-  const uint32_t high = min(8u, tm - group * 8u);
-  n = in / high;
-  m = group * 8u + (in - n * high);
 }
 
 #define MXK_FAR_ROW 0x80000000u   // offset of a row that is not there: past every buffer (at most 2^30 bytes)

@@ -161,33 +161,33 @@ def mxfp4_matmul(a: mxfp4_tensor, b: mxfp4_tensor, bias: Optional[Tensor] = None
     return _product(a, b, _rows(a.shape), b.shape[0], _bias_f32(bias, (b.shape[0],)), out)
 
 
+def _grad(entry: str, dy: Tensor, q: mxfp4_tensor, out: Tensor, offsets: Optional[Tensor]) -> Tensor:
+    dev = L.require_gpu(dy, q.codes, offsets)
+    lib = L.lib()
+    M, N = dy.shape
+    K = q.shape[-1]
+    kind = L.elem_type(dy.dtype)
+    nbytes = lib.mxk_mxfp4_grad_workspace(dy.data_ptr(), kind, M, N)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with L.on_device(dev):
+        rc = getattr(lib, entry)(dy.data_ptr(), kind, M, N, q.codes.data_ptr(), q.scales.data_ptr(), K,
+                                 L.elem_type(out.dtype), out.data_ptr(), L.ptr(offsets),
+                                 0 if offsets is None else offsets.numel() - 1, L.ptr(ws), nbytes, L.stream_of(out))
+    L.check(rc, f"{entry[4:]}({M}x{N} by {K})")
+    return out
+
+
 def _grad_a(dy: Tensor, b: mxfp4_tensor, dtype: torch.dtype, offsets: Optional[Tensor] = None) -> Tensor:
     """dy [M, N] @ dequantize(b) [N, K] (b [E, N, K] by expert), [M, K]."""
-    dev = L.require_gpu(dy, b.codes, offsets)
-    M, N = dy.shape
-    K = b.shape[-1]
-    out = torch.empty(M, K, dtype=dtype, device=dev)
-    with L.on_device(dev):
-        rc = L.lib().mxk_mxfp4_grad_a(dy.data_ptr(), L.elem_type(dy.dtype), M, N, b.codes.data_ptr(),
-                                      b.scales.data_ptr(), K, L.elem_type(dtype), out.data_ptr(), L.ptr(offsets),
-                                      0 if offsets is None else offsets.numel() - 1, L.stream_of(out))
-    L.check(rc, f"mxfp4 gradient of a({M}x{N} by {K})")
-    return out
+    out = torch.empty(dy.shape[0], b.shape[-1], dtype=dtype, device=dy.device)
+    return _grad("mxk_mxfp4_grad_a", dy, b, out, offsets)
 
 
 def _grad_b(dy: Tensor, a: mxfp4_tensor, dtype: torch.dtype, offsets: Optional[Tensor] = None) -> Tensor:
     """dy [M, N].T @ dequantize(a) [M, K], [N, K] ([E, N, K] by expert)."""
-    dev = L.require_gpu(dy, a.codes, offsets)
-    M, N = dy.shape
-    K = a.shape[-1]
-    E = 0 if offsets is None else offsets.numel() - 1
-    out = torch.empty((E, N, K) if E else (N, K), dtype=dtype, device=dev)
-    with L.on_device(dev):
-        rc = L.lib().mxk_mxfp4_grad_b(dy.data_ptr(), L.elem_type(dy.dtype), M, N, a.codes.data_ptr(),
-                                      a.scales.data_ptr(), K, L.elem_type(dtype), out.data_ptr(), L.ptr(offsets), E,
-                                      L.stream_of(out))
-    L.check(rc, f"mxfp4 gradient of b({M}x{N} by {K})")
-    return out
+    shape = (dy.shape[1], a.shape[-1])
+    out = torch.empty(shape if offsets is None else (offsets.numel() - 1, *shape), dtype=dtype, device=dy.device)
+    return _grad("mxk_mxfp4_grad_b", dy, a, out, offsets)
 
 
 def _grad_bias(dy: Tensor, dtype: torch.dtype, offsets: Optional[Tensor] = None) -> Tensor:
