@@ -463,6 +463,18 @@ int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, 
                      const int32_t* offsets, int experts, const int32_t* order, int top, void* workspace,
                      size_t workspace_nbytes, void* stream);
 
+/* Workspace bytes (16-byte aligned) mxk_mxfp4_linear needs (0 if none). */
+size_t mxk_mxfp4_linear_workspace(int x_type, int64_t x_rows, int64_t x_stride, int64_t M, int64_t N, int64_t K,
+                                  int experts, int picked);
+
+/* mxk_mxfp4_quantize of x [x_rows][K] (x_type, rows x_stride >= K elements
+ * apart), then mxk_mxfp4_matmul, y of x_type.  Products of at most 16 rows (by
+ * expert: on average) pack x inside the product's kernel. */
+int mxk_mxfp4_linear(const void* x, int x_type, int64_t x_rows, int64_t x_stride, const void* b_codes,
+                     const void* b_scales, int64_t M, int64_t N, int64_t K, const float* bias, void* y,
+                     const int32_t* offsets, int experts, const int32_t* order, int top, void* workspace,
+                     size_t workspace_nbytes, void* stream);
+
 /* Workspace bytes (16-byte aligned) the two gradients below need: 0 for
  * bf16 dy whose rows start on 16 bytes, else its bf16 terms. */
 size_t mxk_mxfp4_grad_workspace(const void* dy, int dy_type, int64_t M, int64_t N);

@@ -83,6 +83,9 @@ SIGNATURES = {
     "mxk_mxfp4_matmul": (c_int, [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_int,
                                  c_vp, c_int, c_vp, c_sz, c_vp]),
     "mxk_mxfp4_matmul_workspace": (c_sz, [c_i64, c_i64, c_i64, c_i64, c_int, c_int]),
+    "mxk_mxfp4_linear_workspace": (c_sz, [c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_int]),
+    "mxk_mxfp4_linear": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_int,
+                                 c_vp, c_int, c_vp, c_sz, c_vp]),
     "mxk_mxfp4_grad_a": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_vp,
                                  c_sz, c_vp]),
     "mxk_mxfp4_grad_b": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_vp, c_sz,

@@ -23,6 +23,9 @@ struct Fp4Gemm {
   int E;
   const int* order;          // by expert: [M] or null
   DivU32 top;
+  const void* x;             // float rows in place of a (k_fp4_few), x_stride elements apart
+  int64_t x_stride;
+  int K;
 };
 
 // Row of a that row r of the product reads, -1: none
@@ -480,22 +483,300 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
 #undef MXK_STEP
 }
 
+// ---------------------------------------------------------------- few rows
+// 16 * MT rows of a by 16 * NT rows of b per workgroup, K shared out over its
+// waves in chunks of 512 and the waves' sums added through LDS in their order.
+//
+// Bound by HBM (17/32 byte per weight, each read once).  A wave requests its
+// chunk of b, 256 bytes a row, straight into LDS of its own, in whole lines
+// (lanes of an MFMA operand lie in different rows: read in that order, each
+// lane's 16 bytes would be a request by itself, 64 a wave instruction), then
+// reads it as v_mfma_scale_f32_16x16x128 wants it: lane l row l % 16, block 4
+// s + l / 16 of step s.  16-byte chunk c of row r sits at c ^ r.
+//
+// Float rows of x (MT = 1) are packed while b is on its way: the loads of x
+// come first, 16 lanes to 128 elements of a row; a block's largest magnitude
+// is shared by 4 lanes, and codes and scale bytes change lanes through a
+// kilobyte of LDS.
+template <typename X> struct IsPacked { static constexpr bool V = false; };
+template <> struct IsPacked<uint8_t> { static constexpr bool V = true; };
+
+template <typename X, typename T, int MT, int NT, bool EXPERT>
+__global__ __launch_bounds__(1024) void k_fp4_few(Fp4Gemm p) {
+  constexpr bool PACKED = IsPacked<X>::V;
+  constexpr int OWN = NT * 4096 + (PACKED ? 0 : 1088);  // bytes of LDS of a wave
+  extern __shared__ __align__(16) uint8_t few_lds[];    // then the sums: [waves][MT * NT][64][4] floats
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int64_t tiles_n = (p.N + 16 * NT - 1) / (16 * NT);
+  const int64_t slot = blockIdx.x / tiles_n, n0 = (blockIdx.x - slot * tiles_n) * (16 * NT);
+  int64_t lo = slot * 16 * MT, hi = p.M < lo + 16 * MT ? p.M : lo + 16 * MT;
+  int e = 0;
+  if (EXPERT) {
+    const Segment sg = find_segment<16 * MT>(slot, p.offsets, p.E, p.M);
+    e = sg.e;
+    lo = sg.lo;
+    hi = sg.hi;
+    if (e > p.E) return;
+  }
+  T* y = reinterpret_cast<T*>(p.y);
+  if (EXPERT && e == p.E) {
+    for (int i = threadIdx.x; i < (int)(hi - lo) * 16 * NT; i += blockDim.x) {
+      const int64_t n = n0 + i % (16 * NT);
+      if (n < p.N) y[(lo + i / (16 * NT)) * p.N + n] = from_f32<T>(0.0f);
+    }
+    return;
+  }
+  const int KB = (int)p.KB, chunks = (KB + 15) >> 4;
+  const uint32_t row_bytes = (uint32_t)KB * 16u;
+  const int64_t rows_b = p.N - n0 < 16 * NT ? p.N - n0 : 16 * NT;
+  const i32x4 rb = buffer_words(p.b + ((int64_t)e * p.N + n0) * row_bytes, (uint32_t)rows_b * row_bytes);
+  const uint8_t* bsp[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int64_t n = n0 + 16 * i + r;
+    bsp[i] = p.bs + ((int64_t)e * p.N + (n < p.N ? n : p.N - 1)) * KB;  // columns past N are not stored
+  }
+  uint8_t* own = few_lds + wave * OWN;
+  const uint32_t own_at = (uint32_t)(wave * OWN);
+  // rows of b into LDS: 4 rows an instruction; row 4 k + lane / 16 has its chunk (lane % 16) ^ row at lane % 16
+  auto fetch_b = [&](int chunk) {
+#pragma unroll
+    for (int k = 0; k < 4 * NT; ++k) {
+      const int row = 4 * k + g, c = r ^ (row & 15);
+      const uint32_t blk = 16u * chunk + c;
+      load_to_lds(rb, (uint32_t)row * row_bytes + (blk < (uint32_t)KB ? blk * 16u : MXK_FAR_BLOCK), own_at + 1024u * k);
+    }
+  };
+  // the four scale bytes of a lane's blocks in a chunk, byte s that of step s
+  auto scales4 = [&](const uint8_t* row, int chunk) -> uint32_t {
+    uint32_t v = 0;
+    if (16 * chunk + 16 <= KB) {
+      uint32_t w[4];
+      __builtin_memcpy(w, row + 16 * chunk, 16);
+      const uint32_t sel = 0x0C0C0000u | (uint32_t)((4 + g) << 8) | (uint32_t)g;
+      v = __builtin_amdgcn_perm(w[1], w[0], sel) | (__builtin_amdgcn_perm(w[3], w[2], sel) << 16);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (16 * chunk + 4 * s + g < KB) v |= (uint32_t)row[16 * chunk + 4 * s + g] << (8 * s);
+    }
+    return v;
+  };
+  f32x4f acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4f{0, 0, 0, 0};
+  // one step of the products: codes and scales of rows of a against the tiles of b
+#define MXK_FEW(S, I, XC, XS)                                                                                        \
+  _Pragma("unroll") for (int j = 0; j < NT; ++j) {                                                                  \
+    const i32x4 w = *reinterpret_cast<const i32x4*>(own + (16 * j + r) * 256 + (((4 * S + g) ^ r) << 4));           \
+    const i32x8 va = {(int)XC[0], (int)XC[1], (int)XC[2], (int)XC[3], 0, 0, 0, 0};                                  \
+    const i32x8 vb = {w[0], w[1], w[2], w[3], 0, 0, 0, 0};                                                          \
+    acc[I][j] =                                                                                                     \
+        __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb, va, acc[I][j], 4, 4, S, (int)bsc[j], S, (int)XS);      \
+  }
+  if constexpr (PACKED) {
+    const uint8_t *ap[MT], *asp[MT];
+    bool al[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = lo + 16 * i + r;
+      const int64_t src = m < hi ? source_row(p, m) : -1;
+      al[i] = src >= 0;
+      ap[i] = p.a + (al[i] ? src : 0) * p.KB * 16;
+      asp[i] = p.as + (al[i] ? src : 0) * p.KB;
+    }
+    for (int chunk = wave; chunk < chunks; chunk += waves) {
+      if (chunk != wave) wait_loads<0>();  // this chunk's place has been read
+      fetch_b(chunk);
+      uint32_t bsc[NT], xs[MT];
+      u32x4 xc[MT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) bsc[i] = scales4(bsp[i], chunk);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        xs[i] = 0;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) xc[i][s] = u32x4{0u, 0u, 0u, 0u};
+        if (al[i]) {
+          xs[i] = scales4(asp[i], chunk);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const int blk = 16 * chunk + 4 * s + g;
+            if (blk < KB) xc[i][s] = *reinterpret_cast<const u32x4*>(ap[i] + (int64_t)blk * 16);
+          }
+        }
+      }
+      wait_loads<0>();
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        MXK_FEW(0, i, xc[i][0], xs[i])
+        MXK_FEW(1, i, xc[i][1], xs[i])
+        MXK_FEW(2, i, xc[i][2], xs[i])
+        MXK_FEW(3, i, xc[i][3], xs[i])
+      }
+    }
+  } else {
+    static_assert(MT == 1, "float rows: one tile");
+    // rows 4 k + g of x, k = 0 .. 3, as a buffer (the host keeps x below 2^31
+    // bytes): a row that is not there lies past its end and reads as zeros
+    const __amdgpu_buffer_rsrc_t rx =
+        make_rsrc(p.x, (uint32_t)(((p.a_rows - 1) * p.x_stride + p.K) * (int)sizeof(X)));
+    uint32_t x_off[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t m = lo + 4 * k + g;
+      const int64_t src = m < hi ? source_row(p, m) : -1;
+      x_off[k] = src >= 0 ? (uint32_t)(src * p.x_stride * (int)sizeof(X)) : MXK_FAR_ROW;
+    }
+    constexpr int W = (int)sizeof(X) * 2 / 4;  // 16-byte loads of 8 elements
+    constexpr int AT = sizeof(X) == 4 ? 2 : 4; // steps whose elements are in registers at once
+    uint8_t* xch = own + NT * 4096;            // codes of a step [16 rows][64 bytes], then their scales [16][4]
+    for (int chunk = wave; chunk < chunks; chunk += waves) {
+      if (chunk != wave) wait_loads<0>();
+      uint32_t bsc[NT], xs = 0;
+      u32x4 xc[4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) bsc[i] = scales4(bsp[i], chunk);
+#pragma unroll
+      for (int s0 = 0; s0 < 4; s0 += AT) {
+        FpWords<X, 8> v[AT][4];  // of step s0 + t, rows 4 k + g: elements 8 r .. 8 r + 7 of its 128
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+          for (int t = 0; t < AT; ++t)
+#pragma unroll
+            for (int q = 0; q < W; ++q) {
+              const u32x4 w4 = buf_load_b128(
+                  rx, x_off[k] + (uint32_t)(512 * chunk + 128 * (s0 + t) + 8 * r) * (uint32_t)sizeof(X) + 16u * q, 0);
+              __builtin_memcpy(&v[t][k].w[4 * q], &w4, 16);
+            }
+        }
+        if (s0 + AT >= 4) {
+          // x and the scales have arrived (the compiler keeps count of this
+          // wait); b is requested now and travels while x is packed
+          __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+          fetch_b(chunk);
+        }
+        if (512 * chunk + 512 > p.K) {  // the elements past the end of a row are the next one's: whole dwords of zeros
+#pragma unroll
+          for (int t = 0; t < AT; ++t)
+#pragma unroll
+            for (int q = 0; q < 4 * W; ++q) {
+              const bool in = 512 * chunk + 128 * (s0 + t) + 8 * r + q * 4 / (int)sizeof(X) < p.K;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[t][k].w[q] = in ? v[t][k].w[q] : 0u;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < AT; ++t) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t byte = fp4_scale_byte(group_max_u<4>(fp4_amax_bits(v[t][k])));
+            uint32_t q[1];
+            fp4_codes(v[t][k], e8m0_value(byte), q);
+            const int row = 4 * k + g;
+            *reinterpret_cast<uint32_t*>(xch + row * 64 + (((r >> 2) ^ (row & 3)) << 4) + 4 * (r & 3)) =
+                byte == 255u ? 0u : q[0];
+            xch[1024 + row * 4 + (r >> 2)] = (uint8_t)byte;  // the same from the block's four lanes
+          }
+          __builtin_amdgcn_wave_barrier();
+          xc[s0 + t] = *reinterpret_cast<const u32x4*>(xch + r * 64 + ((g ^ (r & 3)) << 4));
+          xs |= (uint32_t)xch[1024 + r * 4 + g] << (8 * (s0 + t));
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+      wait_loads<0>();
+      MXK_FEW(0, 0, xc[0], xs)
+      MXK_FEW(1, 0, xc[1], xs)
+      MXK_FEW(2, 0, xc[2], xs)
+      MXK_FEW(3, 0, xc[3], xs)
+    }
+  }
+#undef MXK_FEW
+  __syncthreads();  // every wave has read its rows of b: the sums take their place
+  float* part = reinterpret_cast<float*>(few_lds);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      *reinterpret_cast<f32x4f*>(&part[(((wave * MT + i) * NT + j) * 64 + lane) * 4]) = acc[i][j];
+  __syncthreads();
+  for (int o = threadIdx.x; o < MT * NT * 256; o += blockDim.x) {
+    const int nl = o % (16 * NT), ml = o / (16 * NT);
+    const int64_t m = lo + ml, n = n0 + nl;
+    if (m >= hi || n >= p.N) continue;
+    const int at = (((ml >> 4) * NT + (nl >> 4)) * 64 + ((nl & 15) >> 2) * 16 + (ml & 15)) * 4 + (nl & 3);
+    float v = p.bias ? p.bias[(int64_t)e * p.N + n] : 0.0f;
+    for (int w = 0; w < waves; ++w) v += part[w * MT * NT * 256 + at];
+    y[m * p.N + n] = from_f32<T>(v);
+  }
+}
+
 // Bytes of the scales of `rows` rows in stage order, with room for the last tile's reads past the end
 static int64_t stage_bytes(int64_t rows, int64_t KB) { return ceil_div(KB, 8) * rows * 8 + 4096; }
+
+// Tiles of 16 rows of k_fp4_few for a problem (0: another kernel): the rows
+// of a dense product, the rows an expert has on average
+static int few_of(const Fp4Gemm& p) {
+  if (p.KB == 0 || p.KB > (1 << 18)) return 0;  // 32 rows of b in a buffer of at most 2^30 bytes
+  const int64_t rows = p.offsets ? ceil_div(p.M, p.E) : p.M;
+  return rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 ? 4 : 0));
+}
 
 // Fragments a side of the tile kernel's waves for a problem, 0: the plain kernel
 static int tile_of(const Fp4Gemm& p) {
   const int64_t row_bytes = p.KB * 16;
-  if (p.KB == 0 || p.M < 64 || p.N < 64 || row_bytes > (1 << 22)) return 0;
+  if (p.KB == 0 || few_of(p) || p.N < 64 || row_bytes > (1 << 22)) return 0;
   if (p.order && p.a_rows * row_bytes > ((int64_t)1 << 30)) return 0;
   if (p.N >= ((int64_t)1 << 21)) return 0;  // 256 rows of 4-byte results within 2^31 bytes
   const int64_t m4 = p.offsets ? segment_slots(p.M, p.E, 256) : ceil_div(p.M, 256);
-  if (p.offsets && p.M < 64 * (int64_t)p.E) return 0;
   return m4 * ceil_div(p.N, 256) >= 192 ? 4 : 2;
+}
+
+// Whether the kernel of few rows packs float x itself: 16 rows at most, whole
+// dwords a row, in a buffer of less than 2^31 bytes
+static bool packs_inside(const Fp4Gemm& p, int64_t x_stride, int x_type, int64_t K) {
+  const int64_t size = x_type == MXK_IN_F32 ? 4 : 2;
+  return few_of(p) == 1 && p.a_rows > 0 && K * size % 4 == 0 &&
+         p.a_rows * std::max(x_stride, p.KB * 32) < ((int64_t)1 << 31) / size;
+}
+
+template <typename X, typename T, int MT, int NT>
+static int launch_few_t(const Fp4Gemm& p, hipStream_t st) {
+  const bool ex = p.offsets != nullptr;
+  const int64_t n = (ex ? segment_slots(p.M, p.E, 16 * MT) : ceil_div(p.M, 16 * MT)) * ceil_div(p.N, 16 * NT);
+  if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many tiles");
+  const int waves = (int)std::min<int64_t>(16, ceil_div(p.KB, 16));
+  const size_t own = NT * 4096 + (IsPacked<X>::V ? 0 : 1088), sums = MT * NT * 1024;
+  const size_t lds = waves * std::max(own, sums);
+  if (ex) hipLaunchKernelGGL((k_fp4_few<X, T, MT, NT, true>), dim3((unsigned)n), dim3(64 * waves), lds, st, p);
+  else hipLaunchKernelGGL((k_fp4_few<X, T, MT, NT, false>), dim3((unsigned)n), dim3(64 * waves), lds, st, p);
+  return check_launch("mxfp4 product of few rows");
+}
+template <typename X, typename T, int MT>
+static int launch_few_n(const Fp4Gemm& p, hipStream_t st) {
+  // two tiles of columns share a's rows where that still leaves a workgroup per CU
+  const int64_t slots = p.offsets ? segment_slots(p.M, p.E, 16 * MT) : ceil_div(p.M, 16 * MT);
+  if (slots * ceil_div(p.N, 32) >= num_cus()) return launch_few_t<X, T, MT, 2>(p, st);
+  return launch_few_t<X, T, MT, 1>(p, st);
+}
+template <typename T>
+static int launch_few_packed(const Fp4Gemm& p, int mt, hipStream_t st) {
+  if (mt == 1) return launch_few_n<uint8_t, T, 1>(p, st);
+  if (mt == 2) return launch_few_n<uint8_t, T, 2>(p, st);
+  return launch_few_n<uint8_t, T, 4>(p, st);
 }
 
 static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_bytes, hipStream_t st) {
   const bool ex = p.offsets != nullptr;
+  if (const int mt = few_of(p)) {
+    if (y_type == MXK_IN_F32) return launch_few_packed<float>(p, mt, st);
+    if (y_type == MXK_IN_F16) return launch_few_packed<__half>(p, mt, st);
+    return launch_few_packed<hip_bfloat16>(p, mt, st);
+  }
   const int F = tile_of(p);
   const int64_t B = F ? 64 * F : 64;
   const int64_t slots = ex ? segment_slots(p.M, p.E, (int)B) : ceil_div(p.M, B);
@@ -533,16 +814,10 @@ static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_byte
   return check_launch("mxfp4 product");
 }
 
-}  // namespace mxk
-
-using namespace mxk;
-
-extern "C" {
-
-size_t mxk_mxfp4_matmul_workspace(int64_t a_rows, int64_t M, int64_t N, int64_t K, int experts, int picked) {
-  if (a_rows < 0 || M <= 0 || N <= 0 || K <= 0 || experts < 0) return 0;
-  Fp4Gemm p = {};
+// Sizes of a problem whose tensors are not known yet
+static bool sizes(Fp4Gemm& p, int64_t a_rows, int64_t M, int64_t N, int64_t K, int experts, int picked) {
   static const int some = 0;
+  if (a_rows < 0 || M <= 0 || N <= 0 || K <= 0 || experts < 0) return false;
   p.a_rows = a_rows;
   p.M = M;
   p.N = N;
@@ -550,33 +825,30 @@ size_t mxk_mxfp4_matmul_workspace(int64_t a_rows, int64_t M, int64_t N, int64_t 
   p.offsets = experts > 0 ? &some : nullptr;
   p.order = picked ? &some : nullptr;
   p.E = experts;
-  if (!tile_of(p)) return 0;
-  return (size_t)(stage_bytes(M, p.KB) + stage_bytes(experts > 0 ? experts * N : N, p.KB));
+  return true;
 }
+static int64_t packed_bytes(int64_t rows, int64_t KB) { return ceil_div(rows * KB * 17, 16) * 16; }
 
-int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, const void* b_codes,
-                     const void* b_scales, int64_t M, int64_t N, int64_t K, const float* bias, int y_type, void* y,
-                     const int32_t* offsets, int experts, const int32_t* order, int top, void* workspace,
-                     size_t workspace_nbytes, void* stream) {
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (a_rows < 0 || M < 0 || N < 0 || K < 0) return fail(MXK_EINVAL, "mxfp4_matmul: negative size");
+static int describe(Fp4Gemm& p, const char* what, const void* a, const void* as, int64_t a_rows, const void* b,
+                    const void* bs, int64_t M, int64_t N, int64_t K, const float* bias, int y_type, void* y,
+                    const int32_t* offsets, int experts, const int32_t* order, int top) {
+  const std::string w = std::string(what) + ": ";
+  if (a_rows < 0 || M < 0 || N < 0 || K < 0) return fail(MXK_EINVAL, w + "negative size");
   if (M >= ((int64_t)1 << 31) || N >= ((int64_t)1 << 31) || K >= ((int64_t)1 << 28) || a_rows >= ((int64_t)1 << 31))
-    return fail(MXK_EINVAL, "mxfp4_matmul: rows below 2^31, K below 2^28");
-  if (y_type != MXK_IN_F32 && y_type != MXK_IN_F16 && y_type != MXK_IN_BF16)
-    return fail(MXK_EINVAL, "mxfp4_matmul: unknown y_type");
+    return fail(MXK_EINVAL, w + "rows below 2^31, K below 2^28");
+  if (y_type != MXK_IN_F32 && y_type != MXK_IN_F16 && y_type != MXK_IN_BF16) return fail(MXK_EINVAL, w + "unknown type");
   if (offsets ? (experts < 1 || experts > 1000) : (order != nullptr || a_rows != M))
-    return fail(MXK_EINVAL, "mxfp4_matmul: 1 to 1000 experts with offsets; without them no order and a_rows = M");
+    return fail(MXK_EINVAL, w + "1 to 1000 experts with offsets; without them no order and as many rows as results");
   if (order ? (top < 1) : (offsets && a_rows != M))
-    return fail(MXK_EINVAL, "mxfp4_matmul: top at least 1 with an order, a_rows = M without one");
+    return fail(MXK_EINVAL, w + "top at least 1 with an order, as many rows as results without one");
   if (M == 0 || N == 0) return MXK_OK;
-  if (!y || (K > 0 && (!b_codes || !b_scales || (a_rows > 0 && (!a_codes || !a_scales)))))
-    return fail(MXK_EINVAL, "mxfp4_matmul: null pointer");
-  if (!aligned16(a_codes) || !aligned16(b_codes)) return fail(MXK_EINVAL, "mxfp4_matmul: codes must be 16-byte aligned");
-  Fp4Gemm p;
-  p.a = reinterpret_cast<const uint8_t*>(a_codes);
-  p.as = reinterpret_cast<const uint8_t*>(a_scales);
-  p.b = reinterpret_cast<const uint8_t*>(b_codes);
-  p.bs = reinterpret_cast<const uint8_t*>(b_scales);
+  if (!y || (K > 0 && (!b || !bs || (a_rows > 0 && (!a || !as))))) return fail(MXK_EINVAL, w + "null pointer");
+  if (!aligned16(b)) return fail(MXK_EINVAL, w + "codes must be 16-byte aligned");
+  p = {};
+  p.a = reinterpret_cast<const uint8_t*>(a);
+  p.as = reinterpret_cast<const uint8_t*>(as);
+  p.b = reinterpret_cast<const uint8_t*>(b);
+  p.bs = reinterpret_cast<const uint8_t*>(bs);
   p.a_rows = a_rows;
   p.M = M;
   p.N = N;
@@ -587,7 +859,68 @@ int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, 
   p.E = experts;
   p.order = order;
   p.top = make_divu32((uint32_t)(top < 1 ? 1 : top));
-  return launch_gemm(p, y_type, reinterpret_cast<uint8_t*>(workspace), workspace_nbytes, st);
+  return MXK_OK;
+}
+
+}  // namespace mxk
+
+using namespace mxk;
+
+extern "C" {
+
+size_t mxk_mxfp4_matmul_workspace(int64_t a_rows, int64_t M, int64_t N, int64_t K, int experts, int picked) {
+  Fp4Gemm p = {};
+  if (!sizes(p, a_rows, M, N, K, experts, picked) || !tile_of(p)) return 0;
+  return (size_t)(stage_bytes(M, p.KB) + stage_bytes(experts > 0 ? experts * N : N, p.KB));
+}
+
+int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, const void* b_codes,
+                     const void* b_scales, int64_t M, int64_t N, int64_t K, const float* bias, int y_type, void* y,
+                     const int32_t* offsets, int experts, const int32_t* order, int top, void* workspace,
+                     size_t workspace_nbytes, void* stream) {
+  Fp4Gemm p;
+  const int rc = describe(p, "mxfp4_matmul", a_codes, a_scales, a_rows, b_codes, b_scales, M, N, K, bias, y_type, y,
+                          offsets, experts, order, top);
+  if (rc != MXK_OK || M == 0 || N == 0) return rc;
+  if (!aligned16(a_codes)) return fail(MXK_EINVAL, "mxfp4_matmul: codes must be 16-byte aligned");
+  return launch_gemm(p, y_type, reinterpret_cast<uint8_t*>(workspace), workspace_nbytes,
+                     reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t mxk_mxfp4_linear_workspace(int x_type, int64_t x_rows, int64_t x_stride, int64_t M, int64_t N, int64_t K, int experts, int picked) {
+  Fp4Gemm p = {};
+  if (!sizes(p, x_rows, M, N, K, experts, picked) || packs_inside(p, x_stride, x_type, K)) return 0;
+  return (size_t)packed_bytes(x_rows, p.KB) + mxk_mxfp4_matmul_workspace(x_rows, M, N, K, experts, picked);
+}
+
+int mxk_mxfp4_linear(const void* x, int x_type, int64_t x_rows, int64_t x_stride, const void* b_codes,
+                     const void* b_scales, int64_t M, int64_t N, int64_t K, const float* bias, void* y,
+                     const int32_t* offsets, int experts, const int32_t* order, int top, void* workspace,
+                     size_t workspace_nbytes, void* stream) {
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  Fp4Gemm p;
+  int rc = describe(p, "mxfp4_linear", x, x, x_rows, b_codes, b_scales, M, N, K, bias, x_type, y, offsets, experts,
+                    order, top);
+  if (rc != MXK_OK || M == 0 || N == 0) return rc;
+  if (x_stride < K) return fail(MXK_EINVAL, "mxfp4_linear: x_stride below K");
+  if (packs_inside(p, x_stride, x_type, K)) {
+    p.x = x;
+    p.x_stride = x_stride;
+    p.K = (int)K;
+    if (x_type == MXK_IN_F32) return launch_few_n<float, float, 1>(p, st);
+    if (x_type == MXK_IN_F16) return launch_few_n<__half, __half, 1>(p, st);
+    return launch_few_n<hip_bfloat16, hip_bfloat16, 1>(p, st);
+  }
+  const size_t own = (size_t)packed_bytes(x_rows, p.KB);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  if (own > 0 && (!ws || !aligned16(ws) || workspace_nbytes < own))
+    return fail(MXK_EINVAL, "mxfp4_linear: workspace too small or not 16-byte aligned");
+  uint8_t* scales = ws + x_rows * p.KB * 16;
+  rc = mxk_mxfp4_quantize(x, x_type, x_rows, K, x_stride, ws, scales, stream);
+  if (rc != MXK_OK) return rc;
+  p.a = ws;
+  p.as = scales;
+  return launch_gemm(p, x_type, ws + own, workspace_nbytes - own, st);
 }
 
 }  // extern "C"

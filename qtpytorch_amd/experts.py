@@ -19,8 +19,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .microscale import (_bias_f32, _check_linear, _grad_a, _grad_b, _grad_bias, _pack_weight, _product,
-                         _wants_grad, mxfp4_quantize, mxfp4_tensor)
+from .microscale import (_bias_f32, _check_linear, _grad_a, _grad_b, _grad_bias, _linear, _pack_weight, _product,
+                         _row_major, _wants_grad, mxfp4_quantize, mxfp4_tensor)
 
 Tensor = torch.Tensor
 
@@ -85,8 +85,7 @@ def _float_rows(name: str, x: Tensor, rows: int, what: str) -> None:
 
 def _gather(x: Tensor, plan: expert_plan) -> Tensor:
     dev = L.require_gpu(x, *plan)
-    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
-        x = x.contiguous()
+    x = _row_major(x)
     tokens, top = plan.place.shape
     out = torch.empty(tokens * top, x.shape[1], dtype=x.dtype, device=dev)
     with L.on_device(dev):
@@ -233,7 +232,9 @@ def expert_linear(x: Tensor, weight: Union[Tensor, mxfp4_tensor], plan: expert_p
     if _wants_grad(x, weight, bias):
         held = isinstance(weight, mxfp4_tensor)
         return _ExpertLinear.apply(x, None if held else weight, bias, weight if held else None, plan, gather)
-    return _expert_product(mxfp4_quantize(x), _pack_weight(weight), plan, bias, gather, x.dtype)
+    b = _pack_weight(weight)
+    return _linear(x, b, tokens * top, _bias_f32(bias, tuple(b.shape[:2])), plan.offsets,
+                   plan.order if gather else None, top)
 
 
 class mxfp4_expert_mlp(nn.Module):

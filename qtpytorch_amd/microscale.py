@@ -107,11 +107,8 @@ def mxfp4_quantize(x: Tensor) -> mxfp4_tensor:
         x = x.float()
     shape = x.shape
     cols = shape[-1]
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
-        ld = x.stride(0)  # rows may lie apart
-    else:
-        x = x.contiguous()
-        ld = cols
+    x = _row_major(x) if x.dim() == 2 else x.contiguous()
+    ld = max(x.stride(0), cols) if x.dim() == 2 else cols
     kb = -(-cols // 32)
     codes = torch.empty(*shape[:-1], 16 * kb, dtype=torch.uint8, device=dev)
     scales = torch.empty(*shape[:-1], kb, dtype=torch.uint8, device=dev)
@@ -147,6 +144,31 @@ def _product(a: mxfp4_tensor, b: mxfp4_tensor, rows: int, N: int, bias: Optional
                                   L.stream_of(out))
     L.check(rc, f"mxfp4 product({rows}x{K} by {N})")
     return out
+
+
+def _row_major(x: Tensor) -> Tensor:
+    """x [rows, cols] itself if its rows are contiguous (they may lie apart), else a copy."""
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+
+
+def _linear(x: Tensor, b: mxfp4_tensor, rows: int, bias: Optional[Tensor], offsets: Optional[Tensor] = None,
+            order: Optional[Tensor] = None, top: int = 1) -> Tensor:
+    """Float rows x [*, K] packed and multiplied in one call, [rows, N] of x's dtype."""
+    dev = L.require_gpu(x, b.codes, bias, offsets, order)
+    lib = L.lib()
+    x = _row_major(x.detach())
+    N, K = b.shape[-2:]
+    E = 0 if offsets is None else offsets.numel() - 1
+    y = torch.empty(rows, N, dtype=x.dtype, device=dev)
+    kind, stride = L.elem_type(x.dtype), max(x.stride(0), K)
+    nbytes = lib.mxk_mxfp4_linear_workspace(kind, x.shape[0], stride, rows, N, K, E, order is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with L.on_device(dev):
+        rc = lib.mxk_mxfp4_linear(x.data_ptr(), kind, x.shape[0], stride, b.codes.data_ptr(),
+                                   b.scales.data_ptr(), rows, N, K, L.ptr(bias), y.data_ptr(),
+                                  L.ptr(offsets), E, L.ptr(order), top, L.ptr(ws), nbytes, L.stream_of(y))
+    L.check(rc, f"mxfp4 linear({rows}x{K} by {N})")
+    return y
 
 
 def mxfp4_matmul(a: mxfp4_tensor, b: mxfp4_tensor, bias: Optional[Tensor] = None,
@@ -258,7 +280,5 @@ def mxfp4_linear(x: Tensor, weight: Union[Tensor, mxfp4_tensor], bias: Optional[
         held = isinstance(weight, mxfp4_tensor)
         y = _MXFP4Linear.apply(x2, None if held else weight, bias, weight if held else None)
     else:
-        b = _pack_weight(weight)
-        y = torch.empty(x2.shape[0], N, dtype=x.dtype, device=x.device)
-        _product(mxfp4_quantize(x2), b, x2.shape[0], N, _bias_f32(bias, (N,)), y)
+        y = _linear(x2, _pack_weight(weight), x2.shape[0], _bias_f32(bias, (N,)))
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
