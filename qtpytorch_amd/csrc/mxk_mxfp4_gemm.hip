@@ -215,7 +215,7 @@ __device__ __forceinline__ void wait_loads_if(uint32_t counted) {
 template <typename T, int F, bool EXPERT>
 __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8_t* __restrict__ ta,
                                                           const uint8_t* __restrict__ tb, int64_t b_rows, uint32_t tm,
-                                                          uint32_t tn) {
+                                                          uint32_t tn, uint32_t splits) {
   constexpr int B = 64 * F;                 // rows of a tile
   constexpr int OP = B * 128, SC = B * 8;   // bytes of an operand's stage and of its scales
   constexpr int BUF = 2 * OP, SBUF = 2 * SC;
@@ -230,6 +230,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
   T* y = reinterpret_cast<T*>(p.y);
   const uint32_t row_bytes = (uint32_t)p.KB * 16u;
   const uint32_t KB = (uint32_t)p.KB, stages = (KB + 7u) >> 3;
+  uint32_t from = 0, to = stages;  // of the tile being loaded
   const bool picked = EXPERT && p.order != nullptr;
   // whole 16-byte pieces of y: stores by buffer, as many for every tile
   const bool whole = p.N * (int)sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
@@ -246,9 +247,16 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
   // the next tile from `id` on that has products (rows without an expert are
   // written here): true, or false at the end
   auto next_tile = [&](uint32_t& id) -> bool {
-    for (; id < tm * tn; id += gridDim.x) {
+    for (; id < tm * tn * splits; id += gridDim.x) {
       uint32_t mt, nt;
-      place_tile(id, tm, tn, mt, nt);
+      place_tile(id, tm, tn * splits, mt, nt);
+      if (!EXPERT && splits > 1) {
+        const uint32_t part = nt % splits;
+        nt /= splits;
+        from = part * stages / splits;
+        to = (part + 1u) * stages / splits;
+        y = reinterpret_cast<T*>(p.y) + (int64_t)part * p.M * p.N;
+      }
       lo = (int64_t)mt * B;
       hi = p.M < lo + B ? p.M : lo + B;
       n0 = (int64_t)nt * B;
@@ -285,7 +293,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
   // part q of F of the loads of stage t
   auto issue = [&](uint32_t t, uint32_t buf, int q) {
     const uint32_t blk = 8u * t + chunk;
-    const uint32_t ok = blk < KB ? blk * 16u : MXK_FAR_BLOCK;
+    const uint32_t ok = blk < KB && t < to ? blk * 16u : MXK_FAR_BLOCK;
 #pragma unroll
     for (int i = q * LI / F; i < (q + 1) * LI / F; ++i) {
       const uint32_t off = off0 + i * step8 + ok;
@@ -301,7 +309,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
       const int64_t first = (of_b ? (int64_t)e * p.N + n0 : lo) + R * (wave & 1);
       // past the last row: bytes of the next plane or of the kilobytes kept after the
       // last, for rows whose codes are zeros or whose results are not stored
-      const i32x4 rs = buffer_words((of_b ? tb : ta) + ((int64_t)t * rows + first) * 8, t < stages ? R * 8u : 0u);
+      const i32x4 rs = buffer_words((of_b ? tb : ta) + ((int64_t)t * rows + first) * 8, t < to ? R * 8u : 0u);
       load_scales_to_lds<R>(rs, lane, 2u * BUF + buf * SBUF + (of_b ? SC : 0) + R * 8u * (wave & 1));
     }
   };
@@ -344,9 +352,9 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
   uint32_t id = blockIdx.x;
   if (!next_tile(id)) return;
 #pragma unroll
-  for (int q = 0; q < F; ++q) issue(0, 0, q);
+  for (int q = 0; q < F; ++q) issue(from, 0, q);
 #pragma unroll
-  for (int q = 0; q < F; ++q) issue(1, 1, q);
+  for (int q = 0; q < F; ++q) issue(from + 1, 1, q);
   // stores of the tile before, issued after this tile's first loads: memory
   // operations of a wave complete in order, so those loads are waited for
   // without them
@@ -383,12 +391,12 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
     }
     // past the last stage the loads bring zeros and the reads are not used
     uint32_t buf = 0;
-    for (uint32_t t = 0; t < stages; ++t) {
+    for (uint32_t t = from; t < to; ++t) {
       MXK_STEP(0, fa[0], fb[0], read_frag(buf, 1, i, fa[1], fb[1]))
       MXK_STEP(1, fa[1], fb[1], read_frag(buf, 2, i, fa[0], fb[0]))
       MXK_STEP(2, fa[0], fb[0], read_frag(buf, 3, i, fa[1], fb[1]))
       if constexpr (COUNTED) {
-        wait_loads_if<STORES>(t == 0 ? stores_due : 0u);
+        wait_loads_if<STORES>(t == from ? stores_due : 0u);
       } else {
         wait_loads<0>();
       }
@@ -412,13 +420,14 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
 
     // the next tile's first two stages are under way while this one's result leaves
     const int64_t m0 = lo, m1 = hi, c0 = n0;
+    T* const y0 = y;
     id += gridDim.x;
     const bool more = next_tile(id);
     if (more) {
 #pragma unroll
-      for (int q = 0; q < F; ++q) issue(0, 0, q);
+      for (int q = 0; q < F; ++q) issue(from, 0, q);
 #pragma unroll
-      for (int q = 0; q < F; ++q) issue(1, 1, q);
+      for (int q = 0; q < F; ++q) issue(from + 1, 1, q);
     }
 
     // The result through LDS, 32 rows of m and CB bytes of n at a time and
@@ -435,7 +444,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
     const int64_t left = m1 - mw;
     const uint32_t pitch = (uint32_t)p.N * (uint32_t)sizeof(T);
     const __amdgpu_buffer_rsrc_t ry =
-        make_rsrc(y + mw * p.N, left <= 0 ? 0u : (uint32_t)(left < NW ? left : NW) * pitch);
+        make_rsrc(y0 + mw * p.N, left <= 0 ? 0u : (uint32_t)(left < NW ? left : NW) * pitch);
     uint32_t el = (uint32_t)lane;
     asm volatile("" : "+v"(el));  // the addresses below are not worth registers during the products
     const uint32_t col = (uint32_t)nw * (uint32_t)sizeof(T) + (el % CH) * 16u, out0 = (el / CH) * pitch + col;
@@ -473,7 +482,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
             __builtin_memcpy(t, &v[k], 16);
 #pragma unroll
             for (int q = 0; q < 16 / (int)sizeof(T); ++q)
-              if (n + q < p.N) y[(mw + row) * p.N + n + q] = t[q];
+              if (n + q < p.N) y0[(mw + row) * p.N + n + q] = t[q];
           }
         }
       }
@@ -484,28 +493,31 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
 }
 
 // ---------------------------------------------------------------- few rows
-// 16 * MT rows of a by 16 * NT rows of b per workgroup, K shared out over its
-// waves in chunks of 512 and the waves' sums added through LDS in their order.
+// 16 * MT rows of a by NT tiles of 16 rows of b per workgroup, K shared out
+// over its waves in chunks of 512 and the waves' sums added through LDS in
+// their order.
 //
 // Bound by HBM (17/32 byte per weight, each read once).  A wave requests its
-// chunk of b, 256 bytes a row, straight into LDS of its own, in whole lines
-// (lanes of an MFMA operand lie in different rows: read in that order, each
-// lane's 16 bytes would be a request by itself, 64 a wave instruction), then
-// reads it as v_mfma_scale_f32_16x16x128 wants it: lane l row l % 16, block 4
-// s + l / 16 of step s.  16-byte chunk c of row r sits at c ^ r.
+// chunk of a tile of b, 256 bytes a row, straight into LDS of its own, in
+// whole lines (lanes of an MFMA operand lie in different rows: read in that
+// order, each lane's 16 bytes would be a request by itself, 64 a wave
+// instruction), then reads it as v_mfma_scale_f32_16x16x128 wants it: lane l
+// row l % 16, block 4 s + l / 16 of step s.  16-byte chunk c of row r sits at
+// c ^ r.  The next tile is on its way while one is multiplied.
 //
-// Float rows of x (MT = 1) are packed while b is on its way: the loads of x
-// come first, 16 lanes to 128 elements of a row; a block's largest magnitude
-// is shared by 4 lanes, and codes and scale bytes change lanes through a
-// kilobyte of LDS.
+// Float rows of x (MT = 1) are packed while the first tiles of b travel: the
+// loads of x come first, 4 lanes to a block and 4 registers to 4 rows; the
+// lanes share the block's largest magnitude, and a 4 x 4 transpose between
+// those lanes and registers (8 VALU) leaves each lane with one whole block of
+// its own row.
 template <typename X> struct IsPacked { static constexpr bool V = false; };
 template <> struct IsPacked<uint8_t> { static constexpr bool V = true; };
 
 template <typename X, typename T, int MT, int NT, bool EXPERT>
 __global__ __launch_bounds__(1024) void k_fp4_few(Fp4Gemm p) {
   constexpr bool PACKED = IsPacked<X>::V;
-  constexpr int OWN = NT * 4096 + (PACKED ? 0 : 1088);  // bytes of LDS of a wave
-  extern __shared__ __align__(16) uint8_t few_lds[];    // then the sums: [waves][MT * NT][64][4] floats
+  constexpr int OWN = NT > 1 ? 8192 : 4096;           // bytes of LDS of a wave: two tiles, or the only one
+  extern __shared__ __align__(16) uint8_t few_lds[];  // then the sums: [waves][MT * NT][64][4] floats
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, g = lane >> 4;
   const int64_t tiles_n = (p.N + 16 * NT - 1) / (16 * NT);
@@ -530,53 +542,86 @@ __global__ __launch_bounds__(1024) void k_fp4_few(Fp4Gemm p) {
   const int KB = (int)p.KB, chunks = (KB + 15) >> 4;
   const uint32_t row_bytes = (uint32_t)KB * 16u;
   const int64_t rows_b = p.N - n0 < 16 * NT ? p.N - n0 : 16 * NT;
-  const i32x4 rb = buffer_words(p.b + ((int64_t)e * p.N + n0) * row_bytes, (uint32_t)rows_b * row_bytes);
-  const uint8_t* bsp[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int64_t n = n0 + 16 * i + r;
-    bsp[i] = p.bs + ((int64_t)e * p.N + (n < p.N ? n : p.N - 1)) * KB;  // columns past N are not stored
-  }
+  const __amdgpu_buffer_rsrc_t rb =
+      make_rsrc(p.b + ((int64_t)e * p.N + n0) * row_bytes, (uint32_t)rows_b * row_bytes);
   uint8_t* own = few_lds + wave * OWN;
-  const uint32_t own_at = (uint32_t)(wave * OWN);
-  // rows of b into LDS: 4 rows an instruction; row 4 k + lane / 16 has its chunk (lane % 16) ^ row at lane % 16
-  auto fetch_b = [&](int chunk) {
+  // tile i of b into LDS: 4 rows an instruction; row 4 k + lane / 16 has its chunk (lane % 16) ^ row at lane % 16
+  auto fetch_b = [&](int chunk, int i) {
 #pragma unroll
-    for (int k = 0; k < 4 * NT; ++k) {
-      const int row = 4 * k + g, c = r ^ (row & 15);
+    for (int k = 0; k < 4; ++k) {
+      const int row = 4 * k + g, c = r ^ row;
       const uint32_t blk = 16u * chunk + c;
-      load_to_lds(rb, (uint32_t)row * row_bytes + (blk < (uint32_t)KB ? blk * 16u : MXK_FAR_BLOCK), own_at + 1024u * k);
+      const uint32_t off = (uint32_t)(16 * i + row) * row_bytes + (blk < (uint32_t)KB ? blk * 16u : MXK_FAR_BLOCK);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rb, (__attribute__((address_space(3))) void*)(own + 4096 * (i & 1) + 1024 * k), 16, (int)off, 0, 0, 2);
     }
   };
-  // the four scale bytes of a lane's blocks in a chunk, byte s that of step s
-  auto scales4 = [&](const uint8_t* row, int chunk) -> uint32_t {
-    uint32_t v = 0;
+  // a row's 16 scale bytes of a chunk; of them this lane's four, byte s that of step s
+  auto load_scales = [&](const uint8_t* row, int chunk, uint32_t (&w)[4]) {
     if (16 * chunk + 16 <= KB) {
-      uint32_t w[4];
       __builtin_memcpy(w, row + 16 * chunk, 16);
-      const uint32_t sel = 0x0C0C0000u | (uint32_t)((4 + g) << 8) | (uint32_t)g;
-      v = __builtin_amdgcn_perm(w[1], w[0], sel) | (__builtin_amdgcn_perm(w[3], w[2], sel) << 16);
     } else {
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (16 * chunk + 4 * s + g < KB) v |= (uint32_t)row[16 * chunk + 4 * s + g] << (8 * s);
+      for (int s = 0; s < 4; ++s) {
+        w[s] = 0;
+        if (16 * chunk + 4 * s + g < KB) w[s] = (uint32_t)row[16 * chunk + 4 * s + g] << (8 * g);
+      }
     }
-    return v;
+  };
+  auto pick_scales = [&](const uint32_t (&w)[4]) -> uint32_t {
+    const uint32_t sel = 0x0C0C0000u | (uint32_t)((4 + g) << 8) | (uint32_t)g;
+    return __builtin_amdgcn_perm(w[1], w[0], sel) | (__builtin_amdgcn_perm(w[3], w[2], sel) << 16);
   };
   f32x4f acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4f{0, 0, 0, 0};
-  // one step of the products: codes and scales of rows of a against the tiles of b
-#define MXK_FEW(S, I, XC, XS)                                                                                        \
-  _Pragma("unroll") for (int j = 0; j < NT; ++j) {                                                                  \
-    const i32x4 w = *reinterpret_cast<const i32x4*>(own + (16 * j + r) * 256 + (((4 * S + g) ^ r) << 4));           \
-    const i32x8 va = {(int)XC[0], (int)XC[1], (int)XC[2], (int)XC[3], 0, 0, 0, 0};                                  \
-    const i32x8 vb = {w[0], w[1], w[2], w[3], 0, 0, 0, 0};                                                          \
-    acc[I][j] =                                                                                                     \
-        __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb, va, acc[I][j], 4, 4, S, (int)bsc[j], S, (int)XS);      \
+  // this lane's row of scales of tile i (columns past N are not stored)
+  auto scales_of = [&](int i) -> const uint8_t* {
+    const int64_t n = n0 + 16 * i + r;
+    return p.bs + ((int64_t)e * p.N + (n < p.N ? n : p.N - 1)) * KB;
+  };
+  uint32_t bw[2][4];
+  // requests of a tile: 4 loads into LDS and, in whole chunks, one of scales
+  auto request = [&](int chunk, int i) {
+    fetch_b(chunk, i);
+    load_scales(scales_of(i), chunk, bw[i & 1]);
+  };
+  // the products of a chunk, once its first two tiles are requested
+  auto multiply = [&](int chunk, const u32x4 (&xc)[MT][4], const uint32_t (&xs)[MT]) {
+    const bool full = 16 * chunk + 16 <= KB;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      // tile i is in LDS when only tile i + 1's requests are due (the
+      // compiler does not know of that dependence)
+      if (i + 1 < NT && full) wait_loads<5>();
+      else wait_loads<0>();
+      const uint8_t* tile = own + 4096 * (i & 1) + r * 256;
+      const int sb = (int)pick_scales(bw[i & 1]);
+      i32x8 vb[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const i32x4 w = *reinterpret_cast<const i32x4*>(tile + (((4 * s + g) ^ r) << 4));
+        vb[s] = i32x8{w[0], w[1], w[2], w[3], 0, 0, 0, 0};
+      }
+#define MXK_FEW(S)                                                                                               \
+  _Pragma("unroll") for (int m = 0; m < MT; ++m) {                                                              \
+    const i32x8 va = {(int)xc[m][S][0], (int)xc[m][S][1], (int)xc[m][S][2], (int)xc[m][S][3], 0, 0, 0, 0};      \
+    acc[m][i] =                                                                                                 \
+        __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb[S], va, acc[m][i], 4, 4, S, sb, S, (int)xs[m]);     \
   }
+      MXK_FEW(0)
+      MXK_FEW(1)
+      MXK_FEW(2)
+      MXK_FEW(3)
+#undef MXK_FEW
+      if (i + 2 < NT) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // tile i has been read
+        request(chunk, i + 2);
+      }
+    }
+  };
   if constexpr (PACKED) {
     const uint8_t *ap[MT], *asp[MT];
     bool al[MT];
@@ -589,19 +634,18 @@ __global__ __launch_bounds__(1024) void k_fp4_few(Fp4Gemm p) {
       asp[i] = p.as + (al[i] ? src : 0) * p.KB;
     }
     for (int chunk = wave; chunk < chunks; chunk += waves) {
-      if (chunk != wave) wait_loads<0>();  // this chunk's place has been read
-      fetch_b(chunk);
-      uint32_t bsc[NT], xs[MT];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the chunk before has been read
+      uint32_t xs[MT], xw[MT][4];
       u32x4 xc[MT][4];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) bsc[i] = scales4(bsp[i], chunk);
-#pragma unroll
       for (int i = 0; i < MT; ++i) {
-        xs[i] = 0;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) xc[i][s] = u32x4{0u, 0u, 0u, 0u};
+        for (int s = 0; s < 4; ++s) {
+          xw[i][s] = 0;
+          xc[i][s] = u32x4{0u, 0u, 0u, 0u};
+        }
         if (al[i]) {
-          xs[i] = scales4(asp[i], chunk);
+          load_scales(asp[i], chunk, xw[i]);
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const int blk = 16 * chunk + 4 * s + g;
@@ -609,93 +653,92 @@ __global__ __launch_bounds__(1024) void k_fp4_few(Fp4Gemm p) {
           }
         }
       }
-      wait_loads<0>();
+      request(chunk, 0);
+      if (NT > 1) request(chunk, 1);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        MXK_FEW(0, i, xc[i][0], xs[i])
-        MXK_FEW(1, i, xc[i][1], xs[i])
-        MXK_FEW(2, i, xc[i][2], xs[i])
-        MXK_FEW(3, i, xc[i][3], xs[i])
-      }
+      for (int i = 0; i < MT; ++i) xs[i] = pick_scales(xw[i]);
+      multiply(chunk, xc, xs);
     }
   } else {
     static_assert(MT == 1, "float rows: one tile");
-    // rows 4 k + g of x, k = 0 .. 3, as a buffer (the host keeps x below 2^31
-    // bytes): a row that is not there lies past its end and reads as zeros
+    // rows 4 (lane / 4 % 4) + k of x, k = 0 .. 3, as a buffer (the host keeps x below
+    // 2^31 bytes): a row that is not there lies past its end and reads as zeros
     const __amdgpu_buffer_rsrc_t rx =
         make_rsrc(p.x, (uint32_t)(((p.a_rows - 1) * p.x_stride + p.K) * (int)sizeof(X)));
     uint32_t x_off[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int64_t m = lo + 4 * k + g;
+      const int64_t m = lo + (r & 12) + k;
       const int64_t src = m < hi ? source_row(p, m) : -1;
       x_off[k] = src >= 0 ? (uint32_t)(src * p.x_stride * (int)sizeof(X)) : MXK_FAR_ROW;
     }
     constexpr int W = (int)sizeof(X) * 2 / 4;  // 16-byte loads of 8 elements
-    constexpr int AT = sizeof(X) == 4 ? 2 : 4; // steps whose elements are in registers at once
-    uint8_t* xch = own + NT * 4096;            // codes of a step [16 rows][64 bytes], then their scales [16][4]
+    constexpr int AT = sizeof(X) == 4 ? 1 : 4; // steps whose elements are in registers at once
+    const bool odd = lane & 1, high = lane & 2;
     for (int chunk = wave; chunk < chunks; chunk += waves) {
-      if (chunk != wave) wait_loads<0>();
-      uint32_t bsc[NT], xs = 0;
-      u32x4 xc[4];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) bsc[i] = scales4(bsp[i], chunk);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      uint32_t xs[1] = {0};
+      u32x4 xc[1][4];
 #pragma unroll
       for (int s0 = 0; s0 < 4; s0 += AT) {
-        FpWords<X, 8> v[AT][4];  // of step s0 + t, rows 4 k + g: elements 8 r .. 8 r + 7 of its 128
+        FpWords<X, 8> v[AT][4];  // of step s0 + t, row (r & 12) + k: elements 8 (r & 3) .. + 7 of block g
+        const int c0 = 512 * chunk + 128 * s0 + 32 * g + 8 * (r & 3);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int t = 0; t < AT; ++t)
 #pragma unroll
-          for (int t = 0; t < AT; ++t)
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
             for (int q = 0; q < W; ++q) {
-              const u32x4 w4 = buf_load_b128(
-                  rx, x_off[k] + (uint32_t)(512 * chunk + 128 * (s0 + t) + 8 * r) * (uint32_t)sizeof(X) + 16u * q, 0);
+              const u32x4 w4 = buf_load_b128(rx, x_off[k] + (uint32_t)(c0 + 128 * t) * (uint32_t)sizeof(X) + 16u * q, 0);
               __builtin_memcpy(&v[t][k].w[4 * q], &w4, 16);
             }
-        }
-        if (s0 + AT >= 4) {
-          // x and the scales have arrived (the compiler keeps count of this
-          // wait); b is requested now and travels while x is packed
-          __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-          fetch_b(chunk);
+        if (s0 + AT >= 4) {  // behind the last loads of x, which are waited for alone
+          __builtin_amdgcn_sched_barrier(0);
+          request(chunk, 0);
+          if (NT > 1) request(chunk, 1);
+          __builtin_amdgcn_sched_barrier(0);
         }
         if (512 * chunk + 512 > p.K) {  // the elements past the end of a row are the next one's: whole dwords of zeros
 #pragma unroll
           for (int t = 0; t < AT; ++t)
 #pragma unroll
             for (int q = 0; q < 4 * W; ++q) {
-              const bool in = 512 * chunk + 128 * (s0 + t) + 8 * r + q * 4 / (int)sizeof(X) < p.K;
+              const bool in = c0 + 128 * t + q * 4 / (int)sizeof(X) < p.K;
 #pragma unroll
               for (int k = 0; k < 4; ++k) v[t][k].w[q] = in ? v[t][k].w[q] : 0u;
             }
         }
 #pragma unroll
         for (int t = 0; t < AT; ++t) {
+          uint32_t a[4], byte[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t byte = fp4_scale_byte(group_max_u<4>(fp4_amax_bits(v[t][k])));
+            byte[k] = fp4_scale_byte(group_max_u<4>(fp4_amax_bits(v[t][k])));
             uint32_t q[1];
-            fp4_codes(v[t][k], e8m0_value(byte), q);
-            const int row = 4 * k + g;
-            *reinterpret_cast<uint32_t*>(xch + row * 64 + (((r >> 2) ^ (row & 3)) << 4) + 4 * (r & 3)) =
-                byte == 255u ? 0u : q[0];
-            xch[1024 + row * 4 + (r >> 2)] = (uint8_t)byte;  // the same from the block's four lanes
+            fp4_codes(v[t][k], e8m0_value(byte[k]), q);
+            a[k] = byte[k] == 255u ? 0u : q[0];
           }
-          __builtin_amdgcn_wave_barrier();
-          xc[s0 + t] = *reinterpret_cast<const u32x4*>(xch + r * 64 + ((g ^ (r & 3)) << 4));
-          xs |= (uint32_t)xch[1024 + r * 4 + g] << (8 * (s0 + t));
-          __builtin_amdgcn_wave_barrier();
+          // out[d] of lane k = a[k] of lane d (lanes of four), one bit of the two at a time
+#define MXK_SWAP(A, B, CTRL, UP)                                                        \
+  {                                                                                     \
+    const uint32_t x = (uint32_t)__builtin_amdgcn_mov_dpp((int)B, CTRL, 0xF, 0xF, true); \
+    const uint32_t z = (uint32_t)__builtin_amdgcn_mov_dpp((int)A, CTRL, 0xF, 0xF, true); \
+    A = UP ? x : A;                                                                     \
+    B = UP ? B : z;                                                                     \
+  }
+          MXK_SWAP(a[0], a[1], 0xB1, odd)
+          MXK_SWAP(a[2], a[3], 0xB1, odd)
+          MXK_SWAP(a[0], a[2], 0x4E, high)
+          MXK_SWAP(a[1], a[3], 0x4E, high)
+#undef MXK_SWAP
+          xc[0][s0 + t] = u32x4{a[0], a[1], a[2], a[3]};
+          const uint32_t mine = high ? (odd ? byte[3] : byte[2]) : (odd ? byte[1] : byte[0]);
+          xs[0] |= mine << (8 * (s0 + t));
         }
       }
-      wait_loads<0>();
-      MXK_FEW(0, 0, xc[0], xs)
-      MXK_FEW(1, 0, xc[1], xs)
-      MXK_FEW(2, 0, xc[2], xs)
-      MXK_FEW(3, 0, xc[3], xs)
+      multiply(chunk, xc, xs);
     }
   }
-#undef MXK_FEW
   __syncthreads();  // every wave has read its rows of b: the sums take their place
   float* part = reinterpret_cast<float*>(few_lds);
 #pragma unroll
@@ -715,6 +758,49 @@ __global__ __launch_bounds__(1024) void k_fp4_few(Fp4Gemm p) {
   }
 }
 
+// y = bias + the sum of the parts of K, in their order, four values a thread;
+// eight parts are requested at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void k_fp4_join(const float* __restrict__ parts, int splits, int64_t total, int64_t N,
+                                                  const float* __restrict__ bias, T* __restrict__ y) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= total) return;
+  float v[4] = {0, 0, 0, 0};
+  if (bias) {
+    uint32_t n = (uint32_t)(i % N);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = bias[n];
+      n = n + 1 == (uint32_t)N ? 0u : n + 1;
+    }
+  }
+  if (i + 4 <= total) {
+    for (int s0 = 0; s0 < splits; s0 += 8) {
+      float w[8][4];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[s][k] = 0.0f;
+        if (s0 + s < splits) __builtin_memcpy(w[s], parts + (s0 + s) * total + i, 16);
+      }
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += w[s][k];
+    }
+    T t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = from_f32<T>(v[k]);
+    __builtin_memcpy(y + i, t, sizeof(t));
+  } else {
+    for (int k = 0; i + k < total; ++k) {
+      float w = v[k];
+      for (int s = 0; s < splits; ++s) w += parts[s * total + i + k];
+      y[i + k] = from_f32<T>(w);
+    }
+  }
+}
+
 // Bytes of the scales of `rows` rows in stage order, with room for the last tile's reads past the end
 static int64_t stage_bytes(int64_t rows, int64_t KB) { return ceil_div(KB, 8) * rows * 8 + 4096; }
 
@@ -723,24 +809,48 @@ static int64_t stage_bytes(int64_t rows, int64_t KB) { return ceil_div(KB, 8) * 
 static int few_of(const Fp4Gemm& p) {
   if (p.KB == 0 || p.KB > (1 << 18)) return 0;  // 32 rows of b in a buffer of at most 2^30 bytes
   const int64_t rows = p.offsets ? ceil_div(p.M, p.E) : p.M;
-  return rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 ? 4 : 0));
+  return rows <= 16 ? 1 : (rows <= 32 ? 2 : 0);
 }
 
-// Fragments a side of the tile kernel's waves for a problem, 0: the plain kernel
-static int tile_of(const Fp4Gemm& p) {
+// The tile kernel's shape for a problem: fragments a side of its waves (0:
+// the plain kernel) and parts of K
+struct Shape {
+  int F, splits;
+};
+static Shape tile_of(const Fp4Gemm& p) {
   const int64_t row_bytes = p.KB * 16;
-  if (p.KB == 0 || few_of(p) || p.N < 64 || row_bytes > (1 << 22)) return 0;
-  if (p.order && p.a_rows * row_bytes > ((int64_t)1 << 30)) return 0;
-  if (p.N >= ((int64_t)1 << 21)) return 0;  // 256 rows of 4-byte results within 2^31 bytes
-  const int64_t m4 = p.offsets ? segment_slots(p.M, p.E, 256) : ceil_div(p.M, 256);
-  return m4 * ceil_div(p.N, 256) >= 192 ? 4 : 2;
+  if (p.KB == 0 || few_of(p) || p.N < 64 || row_bytes > (1 << 22)) return {0, 1};
+  if (p.order && p.a_rows * row_bytes > ((int64_t)1 << 30)) return {0, 1};
+  if (p.N >= ((int64_t)1 << 21)) return {0, 1};  // 256 rows of 4-byte results within 2^31 bytes
+  auto tiles = [&](int B) { return (p.offsets ? segment_slots(p.M, p.E, B) : ceil_div(p.M, B)) * ceil_div(p.N, B); };
+  // large tiles where they occupy most CUs (2048x8192x8192, 256 of them: 76 us
+  // against 92; 1024x8192x8192, 128: 61 against 48)
+  if (tiles(256) >= 192) return {4, 1};
+  if (p.offsets) return {2, 1};
+  // K in parts where tiles leave CUs idle and the stages saved, some 0.45 us
+  // each, outweigh a launch and the parts' way through memory (128x8192x8192
+  // in 4: 23 us against 30; 256x4096x4096 in 4: 22 against 16)
+  const int64_t stages = ceil_div(p.KB, 8), n = tiles(128);
+  const int64_t parts = std::min<int64_t>({num_cus() / n, stages / 4, 16});
+  if (parts < 2) return {2, 1};
+  const double saved = 0.45 * (double)(stages - stages / parts), cost = 3.0 + (double)(parts * p.M * p.N) * 1.6e-6;
+  return {2, saved > cost ? (int)parts : 1};
+}
+static int64_t tile_bytes(const Fp4Gemm& p, const Shape& t) {
+  const int64_t rows = p.offsets ? p.E * p.N : p.N;
+  return stage_bytes(p.M, p.KB) + stage_bytes(rows, p.KB) + (t.splits > 1 ? t.splits * p.M * p.N * 4 : 0);
 }
 
-// Whether the kernel of few rows packs float x itself: 16 rows at most, whole
-// dwords a row, in a buffer of less than 2^31 bytes
+// Whether the kernel of few rows packs float x itself: a dense product of at
+// most 16 rows and one chunk of K per wave, whole dwords a row, x a buffer of
+// less than 2^31 bytes.  The GPU takes as long either way (16x8192x8192 13.6
+// us, 1x4096x4096 6.3 against 5.9), the call 3 us less with one launch and no
+// workspace.  By expert, where many workgroups would each pack mostly rows
+// that are not there, packing first is faster: 8 tokens to 4 of 32 experts of
+// 4096x4096 44 us against 29 and 2.5 for packing.
 static bool packs_inside(const Fp4Gemm& p, int64_t x_stride, int x_type, int64_t K) {
   const int64_t size = x_type == MXK_IN_F32 ? 4 : 2;
-  return few_of(p) == 1 && p.a_rows > 0 && K * size % 4 == 0 &&
+  return !p.offsets && few_of(p) == 1 && p.KB <= 256 && K * size % 4 == 0 &&
          p.a_rows * std::max(x_stride, p.KB * 32) < ((int64_t)1 << 31) / size;
 }
 
@@ -750,24 +860,34 @@ static int launch_few_t(const Fp4Gemm& p, hipStream_t st) {
   const int64_t n = (ex ? segment_slots(p.M, p.E, 16 * MT) : ceil_div(p.M, 16 * MT)) * ceil_div(p.N, 16 * NT);
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many tiles");
   const int waves = (int)std::min<int64_t>(16, ceil_div(p.KB, 16));
-  const size_t own = NT * 4096 + (IsPacked<X>::V ? 0 : 1088), sums = MT * NT * 1024;
+  const size_t own = NT > 1 ? 8192 : 4096, sums = MT * NT * 1024;
   const size_t lds = waves * std::max(own, sums);
-  if (ex) hipLaunchKernelGGL((k_fp4_few<X, T, MT, NT, true>), dim3((unsigned)n), dim3(64 * waves), lds, st, p);
-  else hipLaunchKernelGGL((k_fp4_few<X, T, MT, NT, false>), dim3((unsigned)n), dim3(64 * waves), lds, st, p);
+  if constexpr (IsPacked<X>::V) {
+    if (ex) {
+      hipLaunchKernelGGL((k_fp4_few<X, T, MT, NT, true>), dim3((unsigned)n), dim3(64 * waves), lds, st, p);
+      return check_launch("mxfp4 product of few rows by expert");
+    }
+  }
+  hipLaunchKernelGGL((k_fp4_few<X, T, MT, NT, false>), dim3((unsigned)n), dim3(64 * waves), lds, st, p);
   return check_launch("mxfp4 product of few rows");
 }
 template <typename X, typename T, int MT>
 static int launch_few_n(const Fp4Gemm& p, hipStream_t st) {
-  // two tiles of columns share a's rows where that still leaves a workgroup per CU
-  const int64_t slots = p.offsets ? segment_slots(p.M, p.E, 16 * MT) : ceil_div(p.M, 16 * MT);
-  if (slots * ceil_div(p.N, 32) >= num_cus()) return launch_few_t<X, T, MT, 2>(p, st);
+  // tiles of b per workgroup: as many as leave each CU a workgroup (by expert
+  // four, since how many experts have rows is not known here), and as the
+  // registers hold (four only for one packed tile of rows)
+  const int64_t tiles = ceil_div(p.N, 16) * (p.offsets ? std::min<int64_t>(p.M, p.E) : 1);
+  const int64_t per = tiles / (num_cus() * (p.offsets ? 4 : 1));
+  if constexpr (IsPacked<X>::V && MT == 1)
+    if (per >= 4) return launch_few_t<X, T, MT, 4>(p, st);
+  if constexpr (IsPacked<X>::V || sizeof(X) == 2)
+    if (per >= 2) return launch_few_t<X, T, MT, 2>(p, st);
   return launch_few_t<X, T, MT, 1>(p, st);
 }
 template <typename T>
 static int launch_few_packed(const Fp4Gemm& p, int mt, hipStream_t st) {
   if (mt == 1) return launch_few_n<uint8_t, T, 1>(p, st);
-  if (mt == 2) return launch_few_n<uint8_t, T, 2>(p, st);
-  return launch_few_n<uint8_t, T, 4>(p, st);
+  return launch_few_n<uint8_t, T, 2>(p, st);
 }
 
 static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_bytes, hipStream_t st) {
@@ -777,40 +897,59 @@ static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_byte
     if (y_type == MXK_IN_F16) return launch_few_packed<__half>(p, mt, st);
     return launch_few_packed<hip_bfloat16>(p, mt, st);
   }
-  const int F = tile_of(p);
-  const int64_t B = F ? 64 * F : 64;
+  const Shape t = tile_of(p);
+  const int64_t B = t.F ? 64 * t.F : 64;
   const int64_t slots = ex ? segment_slots(p.M, p.E, (int)B) : ceil_div(p.M, B);
-  const int64_t tn = ceil_div(p.N, B), n = slots * tn;
+  const int64_t tn = ceil_div(p.N, B), n = slots * tn * t.splits;
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many tiles");
   const int64_t b_rows = ex ? p.E * p.N : p.N, na = stage_bytes(p.M, p.KB), nb = stage_bytes(b_rows, p.KB);
-  if (F && (!ws || ws_bytes < (size_t)(na + nb))) return fail(MXK_EINVAL, "mxfp4 product: workspace too small");
-  if (F) {
+  if (t.F) {
+    if (!ws || !aligned16(ws) || ws_bytes < (size_t)tile_bytes(p, t))
+      return fail(MXK_EINVAL, "mxfp4 product: workspace too small or not 16-byte aligned");
     const int64_t ga = ceil_div(p.M, 32), gb = ceil_div(b_rows, 32);
     if (ga + gb >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many rows");
     hipLaunchKernelGGL(k_fp4_stage_scales, dim3((unsigned)(ga + gb)), dim3(256), 0, st, p, b_rows, ga, ws, ws + na);
   }
   const int64_t cus = (num_cus() + 7) & ~7;  // a multiple of the XCDs: a workgroup's tiles stay on its own
-#define MXK_L(T, EX)                                                                                              \
-  do {                                                                                                            \
-    if (F == 4)                                                                                                   \
-      hipLaunchKernelGGL((k_fp4_gemm_tile<T, 4, EX>), dim3((unsigned)std::min(n, cus)), dim3(256), 0, st, p, ws, ws + na,       \
-                         b_rows, (uint32_t)slots, (uint32_t)tn);                                                  \
-    else if (F == 2)                                                                                              \
-      hipLaunchKernelGGL((k_fp4_gemm_tile<T, 2, EX>), dim3((unsigned)std::min(n, 2 * cus)), dim3(256), 0, st, p, ws, ws + na,       \
-                         b_rows, (uint32_t)slots, (uint32_t)tn);                                                  \
-    else                                                                                                          \
-      hipLaunchKernelGGL((k_fp4_gemm<T, EX>), dim3((unsigned)n), dim3(256), 0, st, p);                           \
+#define MXK_TILE(T, F, EX, P)                                                                                        \
+  hipLaunchKernelGGL((k_fp4_gemm_tile<T, F, EX>), dim3((unsigned)std::min<int64_t>(n, (F == 4 ? 1 : 2) * cus)),      \
+                     dim3(256), 0, st, P, ws, ws + na, b_rows, (uint32_t)slots, (uint32_t)tn, (uint32_t)t.splits)
+#define MXK_L(T, EX)                                                                                     \
+  do {                                                                                                   \
+    if (t.F == 4) MXK_TILE(T, 4, EX, p);                                                                 \
+    else if (t.F == 2) MXK_TILE(T, 2, EX, p);                                                            \
+    else hipLaunchKernelGGL((k_fp4_gemm<T, EX>), dim3((unsigned)n), dim3(256), 0, st, p);                \
   } while (0)
 #define MXK_T(T)                \
   do {                          \
     if (ex) MXK_L(T, true);     \
     else MXK_L(T, false);       \
   } while (0)
-  if (y_type == MXK_IN_F32) MXK_T(float);
-  else if (y_type == MXK_IN_F16) MXK_T(__half);
-  else MXK_T(hip_bfloat16);
+  if (t.splits > 1) {
+    float* parts = reinterpret_cast<float*>(ws + na + nb);
+    Fp4Gemm q = p;
+    q.y = parts;
+    q.bias = nullptr;
+    MXK_TILE(float, 2, false, q);
+    const int64_t total = p.M * p.N;
+    const dim3 grid((unsigned)ceil_div(total, 1024));
+#define MXK_J(T)                                                                                                    \
+  hipLaunchKernelGGL((k_fp4_join<T>), grid, dim3(256), 0, st, parts, t.splits, total, p.N, p.bias,                  \
+                     reinterpret_cast<T*>(p.y))
+    if (y_type == MXK_IN_F32) MXK_J(float);
+    else if (y_type == MXK_IN_F16) MXK_J(__half);
+    else MXK_J(hip_bfloat16);
+#undef MXK_J
+  } else if (y_type == MXK_IN_F32) {
+    MXK_T(float);
+  } else if (y_type == MXK_IN_F16) {
+    MXK_T(__half);
+  } else {
+    MXK_T(hip_bfloat16);
+  }
 #undef MXK_T
 #undef MXK_L
+#undef MXK_TILE
   return check_launch("mxfp4 product");
 }
 
@@ -870,8 +1009,9 @@ extern "C" {
 
 size_t mxk_mxfp4_matmul_workspace(int64_t a_rows, int64_t M, int64_t N, int64_t K, int experts, int picked) {
   Fp4Gemm p = {};
-  if (!sizes(p, a_rows, M, N, K, experts, picked) || !tile_of(p)) return 0;
-  return (size_t)(stage_bytes(M, p.KB) + stage_bytes(experts > 0 ? experts * N : N, p.KB));
+  if (!sizes(p, a_rows, M, N, K, experts, picked)) return 0;
+  const Shape t = tile_of(p);
+  return t.F ? (size_t)tile_bytes(p, t) : 0;
 }
 
 int mxk_mxfp4_matmul(const void* a_codes, const void* a_scales, int64_t a_rows, const void* b_codes,
