@@ -54,8 +54,8 @@ __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __re
   for (uint32_t k = tid; k < MXK_SORT_WAVES * (E + 1); k += MXK_SORT_THREADS) start[k] = 0;
   __syncthreads();
   const uint32_t share = (chunk / MXK_SORT_WAVES + 63u) & ~63u;  // a multiple of 64 per wave
-  const uint32_t c0 = blockIdx.x * chunk, c1 = min(P, c0 + chunk);
-  const uint32_t lo = min(c1, c0 + wave * share), hi = min(c1, lo + share);
+  const uint32_t first = blockIdx.x * chunk, last = min(P, first + chunk);
+  const uint32_t lo = min(last, first + wave * share), hi = min(last, lo + share);
   int* mine = start + wave * (E + 1);
   for (uint32_t i = lo + lane; i < hi; i += 64) atomicAdd(&mine[expert_of(ids[i], E)], 1);
   __syncthreads();
@@ -66,10 +66,15 @@ __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __re
     int before = 0, total = 0;
     if (e < E) {
       if (gridDim.x > 1) {
-        for (uint32_t c = 0; c < gridDim.x; ++c) {
-          const int n = hist[(int64_t)c * E + e];
-          total += n;
-          before += c < blockIdx.x ? n : 0;
+        for (uint32_t c0 = 0; c0 < gridDim.x; c0 += 16) {  // sixteen chunks' counts at a time
+          int n[16];
+#pragma unroll
+          for (uint32_t k = 0; k < 16; ++k) n[k] = c0 + k < gridDim.x ? hist[(int64_t)(c0 + k) * E + e] : 0;
+#pragma unroll
+          for (uint32_t k = 0; k < 16; ++k) {
+            total += n[k];
+            before += c0 + k < blockIdx.x ? n[k] : 0;
+          }
         }
       } else {
         for (int w = 0; w < MXK_SORT_WAVES; ++w) total += start[w * (E + 1) + e];
@@ -89,9 +94,9 @@ __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __re
       base += sums[w];
     }
     if (e < E) {
-      const int first = left + scan - total;
-      if (blockIdx.x == 0) offsets[e] = first;
-      int next = first + before;
+      const int at = left + scan - total;
+      if (blockIdx.x == 0) offsets[e] = at;
+      int next = at + before;
       for (int w = 0; w < MXK_SORT_WAVES; ++w) {
         const int n = start[w * (E + 1) + e];
         start[w * (E + 1) + e] = next;
@@ -102,7 +107,7 @@ __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __re
   }
   if (blockIdx.x == 0 && tid == 0) offsets[E] = base;
   // places past the last one in use
-  for (uint32_t i = c0 + tid; i < c1; i += MXK_SORT_THREADS)
+  for (uint32_t i = first + tid; i < last; i += MXK_SORT_THREADS)
     if (i >= (uint32_t)base) order[i] = -1;
   const int bits = 32 - __builtin_clz(E | 1u);  // of 0 .. E
   for (uint32_t i0 = lo; i0 < hi; i0 += 64) {
@@ -128,27 +133,35 @@ __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __re
 }
 
 // out[r] = x[order[r] / top], zeros where order[r] < 0: a copy, bound by
-// HBM's write rate (a token's row is read `top` times, from L2 after the
-// first).  Rows are copied in pieces of 16 bytes (any alignment; the last
-// piece of a row may be shorter), U pieces a thread with their loads issued first.
-template <int U>
+// HBM's write rate (a token's row is read `top` times, from the caches after
+// the first).  Rows are copied in pieces of 16 bytes, U pieces a thread with
+// their loads issued first.  WHOLE: rows of whole aligned pieces, written past
+// the caches; else any alignment, and the last piece of a row may be shorter.
+template <int U, bool WHOLE>
 __global__ __launch_bounds__(256) void k_expert_gather(const uint8_t* __restrict__ x, int64_t x_stride,
                                                        const int* __restrict__ order, DivU32 by_top, uint32_t tokens,
                                                        uint32_t total, DivU32 by_pieces, uint32_t pieces, uint32_t row_bytes,
-                                                       uint8_t* __restrict__ out) {
-  const uint64_t first = (uint64_t)blockIdx.x * (256u * U) + threadIdx.x;
+                                                       uint32_t slices, uint8_t* __restrict__ out) {
+  // slices = 8: workgroup b, on XCD b % 8, copies that eighth of the columns
+  // (pieces and total are a slice's), so that an XCD's L2 sees an eighth of each
+  // token; slices = 1: whole rows
+  const uint32_t slice = slices > 1 ? blockIdx.x & 7u : 0u, block = slices > 1 ? blockIdx.x >> 3 : blockIdx.x;
+  const uint32_t c0 = slice * pieces * 16u;
+  const uint64_t first = (uint64_t)block * (256u * U) + threadIdx.x;
   u32x4 v[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint64_t i = first + 256u * u;
     v[u] = u32x4{0u, 0u, 0u, 0u};
     if (i < total) {
-      const uint32_t r = divu32((uint32_t)i, by_pieces), c = ((uint32_t)i - r * pieces) * 16u;
+      const uint32_t r = divu32((uint32_t)i, by_pieces), c = c0 + ((uint32_t)i - r * pieces) * 16u;
       const int pick = order[r];
       const uint32_t token = divu32((uint32_t)pick, by_top);
       if (pick >= 0 && token < tokens) {
         const uint8_t* p = x + (int64_t)token * x_stride + c;
-        if (c + 16u <= row_bytes) {
+        if (WHOLE) {
+          v[u] = *reinterpret_cast<const u32x4*>(p);
+        } else if (c + 16u <= row_bytes) {
           __builtin_memcpy(&v[u], p, 16);
         } else {  // elements have an even number of bytes
           uint16_t t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -163,9 +176,11 @@ __global__ __launch_bounds__(256) void k_expert_gather(const uint8_t* __restrict
   for (int u = 0; u < U; ++u) {
     const uint64_t i = first + 256u * u;
     if (i >= total) continue;
-    const uint32_t r = divu32((uint32_t)i, by_pieces), c = ((uint32_t)i - r * pieces) * 16u;
+    const uint32_t r = divu32((uint32_t)i, by_pieces), c = c0 + ((uint32_t)i - r * pieces) * 16u;
     uint8_t* p = out + (int64_t)r * row_bytes + c;
-    if (c + 16u <= row_bytes) {
+    if (WHOLE) {
+      __builtin_nontemporal_store(v[u], reinterpret_cast<u32x4*>(p));
+    } else if (c + 16u <= row_bytes) {
       __builtin_memcpy(p, &v[u], 16);
     } else {
       uint16_t t[8];
@@ -201,11 +216,34 @@ __device__ __forceinline__ void store8(T* p, int live, const float (&v)[8]) {
   }
 }
 
+// 8 elements on 16 bytes that are read once, or written past the caches
+template <typename T>
+__device__ __forceinline__ void load8_nt(const T* p, FpWords<T, 8>& v) {
+#pragma unroll
+  for (int k = 0; k < FpWords<T, 8>::NW / 4; ++k) {
+    const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + k);
+    __builtin_memcpy(&v.w[4 * k], &w, 16);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8_nt(T* p, const float (&v)[8]) {
+  T t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(v[e]);
+  u32x4 w[sizeof(t) / 16];
+  __builtin_memcpy(w, t, sizeof(t));
+#pragma unroll
+  for (int k = 0; k < (int)sizeof(t) / 16; ++k) __builtin_nontemporal_store(w[k], reinterpret_cast<u32x4*>(p) + k);
+}
+
 // y[t] = sum over j of gate[t, j] * h[place[t, j]] (gate = 1 where gates is
 // null), in float32 by ascending j, picks without an expert left out.  Bound
 // by HBM: one read of the rows in use, one write of the tokens.  A thread
-// holds 8 columns of a token and issues the loads of four picks at a time.
-template <typename T, bool GATED>
+// holds 8 columns of a token and requests the rows of Q picks at a time: a
+// pick without an expert reads row 0 in place of a branch, and its values are
+// replaced by zeros.
+// WHOLE: columns in whole groups of 8 on 16 bytes.
+template <typename T, bool GATED, int Q, bool WHOLE>
 __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h, const int* __restrict__ place,
                                                         const float* __restrict__ gates, int top, int rows,
                                                         uint32_t total, DivU32 by_pieces, uint32_t pieces, int cols,
@@ -213,26 +251,34 @@ __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h,
   const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
   if (i >= total) return;
   const uint32_t t = divu32((uint32_t)i, by_pieces), c = 8u * ((uint32_t)i - t * pieces);
-  const int live = cols - (int)c;
+  const int live = WHOLE ? 8 : cols - (int)c;
   float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   const int64_t p0 = (int64_t)t * top;
-  for (int j0 = 0; j0 < top; j0 += 4) {
-    float v[4][8], g[4];
+  if (rows > 0) {
+    for (int j0 = 0; j0 < top; j0 += Q) {
+      FpWords<T, 8> v[Q];
+      float g[Q];
+      bool ok[Q];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = j0 + q < top ? place[p0 + j0 + q] : -1;
-      g[q] = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[q][e] = 0.0f;
-      if (at >= 0 && at < rows) {
-        g[q] = GATED ? gates[p0 + j0 + q] : 1.0f;
-        load8(h + (int64_t)at * cols + c, live, v[q]);
+      for (int q = 0; q < Q; ++q) {
+        const int j = j0 + q < top ? j0 + q : top - 1;
+        const int at = place[p0 + j];
+        ok[q] = j0 + q < top && at >= 0 && at < rows;
+        g[q] = GATED ? gates[p0 + j] : 1.0f;
+        const T* row = h + (int64_t)(ok[q] ? at : 0) * cols + c;
+        if (WHOLE) load8_nt(row, v[q]);
+        else if (live >= 8) fp4_load(row, v[q]);
+        else fp4_load_tail(row, live, v[q]);
       }
-    }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < Q; ++q) {
+        T e8[8];
+        __builtin_memcpy(e8, v[q].w, sizeof(e8));
+        // an exact zero for a pick that is not there, whatever row 0 and its gate hold
+        const float w = ok[q] ? g[q] : 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(g[q], v[q][e], acc[e]);
+        for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(w, ok[q] ? ElemT<T>::cvt(e8[e]) : 0.0f, acc[e]);
+      }
     }
   }
   store8(y + (int64_t)t * cols + c, live, acc);
@@ -242,20 +288,22 @@ __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h,
 // dgate[t, j] = <dy[t], h[place[t, j]]>; zeros for rows past the last in
 // use and for picks without an expert.  Bound by HBM: dy is read once per
 // token and group of four picks, h read and dh written once.  W waves share a
-// token (4 where there are too few tokens to fill the card with one each); a
-// lane's share of the products is added in order of its columns, then over the
-// lanes of a wave and the waves of a token in a fixed order.
-template <typename T, int W>
-__global__ __launch_bounds__(256) void k_expert_combine_grad(const T* __restrict__ dy, const T* __restrict__ h,
-                                                             const int* __restrict__ place,
-                                                             const float* __restrict__ gates,
-                                                             const int* __restrict__ used, int tokens, int top,
-                                                             int rows, int cols, T* __restrict__ dh, float* __restrict__ dg) {
-  __shared__ float part[4][4];
+// token, one for each 512 columns (up to 8), so that a lane mostly has one
+// set of loads and stores and many tokens are under way.  The products of a
+// lane are added in order of its columns, then over the lanes of a wave and
+// the waves of a token in a fixed order.
+// WHOLE: columns in whole groups of 8 on 16 bytes; dh is then written past the
+// caches.
+template <typename T, int W, bool WHOLE>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_expert_combine_grad(
+    const T* __restrict__ dy, const T* __restrict__ h, const int* __restrict__ place, const float* __restrict__ gates,
+    const int* __restrict__ used, int tokens, int top, int rows, int cols, T* __restrict__ dh, float* __restrict__ dg) {
+  constexpr int PER = W > 4 ? 1 : 4 / W;  // tokens per workgroup
+  __shared__ float part[PER * W][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * (4 / W) + wave / W;
+  const int64_t t = (int64_t)blockIdx.x * PER + wave / W;
   const int w = wave % W;
-  const bool live_t = t < tokens;  // the waves of a group share t, and with W = 4 so does the workgroup
+  const bool live_t = t < tokens;
   const int64_t p0 = t * top;
   const int n_used = *used;
   const T* dyt = dy + t * cols;
@@ -267,27 +315,40 @@ __global__ __launch_bounds__(256) void k_expert_combine_grad(const T* __restrict
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const bool in = j0 + q < top;
-        at[q] = in ? place[p0 + j0 + q] : -1;
+        // the same for the whole wave: branches on it are scalar
+        at[q] = __builtin_amdgcn_readfirstlane(in ? place[p0 + j0 + q] : -1);
         if (at[q] >= rows) at[q] = -1;
         g[q] = in ? gates[p0 + j0 + q] : 0.0f;
       }
       for (int c = (w * 64 + lane) * 8; c < cols; c += W * 512) {
-        const int live = cols - c;
-        float d[8], v[4][8];
-        load8(dyt + c, live, d);
+        const int live = WHOLE ? 8 : cols - c;
+        FpWords<T, 8> d, v[4];
+        if (live >= 8) fp4_load(dyt + c, d);
+        else fp4_load_tail(dyt + c, live, d);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          if (at[q] >= 0) load8(h + (int64_t)at[q] * cols + c, live, v[q]);
+          if (at[q] >= 0) {
+            const T* row = h + (int64_t)at[q] * cols + c;
+            if (WHOLE) load8_nt(row, v[q]);
+            else if (live >= 8) fp4_load(row, v[q]);
+            else fp4_load_tail(row, live, v[q]);
+          }
+        T d8[8];
+        __builtin_memcpy(d8, d.w, sizeof(d8));
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (at[q] >= 0) {
+            T v8[8];
+            __builtin_memcpy(v8, v[q].w, sizeof(v8));
             float o[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              dot[q] = __builtin_fmaf(d[e], v[q][e], dot[q]);
-              o[e] = g[q] * d[e];
+              const float de = ElemT<T>::cvt(d8[e]);
+              dot[q] = __builtin_fmaf(de, ElemT<T>::cvt(v8[e]), dot[q]);
+              o[e] = g[q] * de;
             }
-            store8(dh + (int64_t)at[q] * cols + c, live, o);
+            if (WHOLE) store8_nt(dh + (int64_t)at[q] * cols + c, o);
+            else store8(dh + (int64_t)at[q] * cols + c, live, o);
           }
           if (j0 + q < top && p0 + j0 + q >= n_used) {  // row number p0 + j0 + q is in no one's use
             const float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -314,9 +375,11 @@ __global__ __launch_bounds__(256) void k_expert_combine_grad(const T* __restrict
         for (int q = 0; q < 4; ++q) part[wave][q] = dot[q];
       }
       __syncthreads();
-      if (live_t && threadIdx.x < 4 && j0 + (int)threadIdx.x < top) {
-        const int q = threadIdx.x;
-        dg[p0 + j0 + q] = (part[0][q] + part[1][q]) + (part[2][q] + part[3][q]);
+      if (live_t && w == 0 && lane < 4 && j0 + lane < top) {
+        float sum = part[wave][lane];
+#pragma unroll
+        for (int k = 1; k < W; ++k) sum += part[wave + k][lane];
+        dg[p0 + j0 + lane] = sum;
       }
       __syncthreads();
     }
@@ -381,21 +444,27 @@ int mxk_expert_gather(const void* x, int elem_bytes, int64_t tokens, int64_t col
     return fail(MXK_EINVAL, "expert_gather: bad sizes (rows at most tokens * top, below 2^31; cols below 2^28)");
   if (rows == 0 || cols == 0) return MXK_OK;
   if (!x || !order || !out) return fail(MXK_EINVAL, "expert_gather: null pointer");
-  const int64_t row_bytes = cols * elem_bytes, pieces = ceil_div(row_bytes, 16);
-  const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 31) / pieces - 1);
+  const int64_t row_bytes = cols * elem_bytes;
+  const bool whole = row_bytes % 16 == 0 && row_stride * elem_bytes % 16 == 0 && aligned16(x) && aligned16(out);
+  // eighths of at least two lines
+  const int64_t slices = whole && row_bytes % 2048 == 0 && rows * row_bytes >= ((int64_t)1 << 24) ? 8 : 1;
+  const int64_t pieces = ceil_div(row_bytes, 16) / slices;
+  const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 28) / pieces - 1);
   const DivU32 bt = make_divu32((uint32_t)top), bp = make_divu32((uint32_t)pieces);
   for (int64_t r0 = 0; r0 < rows; r0 += step) {
     const uint32_t total = (uint32_t)(std::min(step, rows - r0) * pieces);
     const uint8_t* xp = reinterpret_cast<const uint8_t*>(x);
     uint8_t* op = reinterpret_cast<uint8_t*>(out) + r0 * row_bytes;
-    const bool big = total >= 256u * 4u * 1024u;
-    const dim3 grid((unsigned)ceil_div(total, big ? 1024 : 256));
-    if (big)
-      hipLaunchKernelGGL((k_expert_gather<4>), grid, dim3(256), 0, st, xp, row_stride * elem_bytes, order + r0, bt,
-                         (uint32_t)tokens, total, bp, (uint32_t)pieces, (uint32_t)row_bytes, op);
-    else
-      hipLaunchKernelGGL((k_expert_gather<1>), grid, dim3(256), 0, st, xp, row_stride * elem_bytes, order + r0, bt,
-                         (uint32_t)tokens, total, bp, (uint32_t)pieces, (uint32_t)row_bytes, op);
+    const bool big = total * slices >= 256u * 4u * 1024u;
+    const dim3 grid((unsigned)(ceil_div(total, big ? 1024 : 256) * slices));
+#define MXK_GA(U, W)                                                                                              \
+  hipLaunchKernelGGL((k_expert_gather<U, W>), grid, dim3(256), 0, st, xp, row_stride * elem_bytes, order + r0, bt, \
+                     (uint32_t)tokens, total, bp, (uint32_t)pieces, (uint32_t)row_bytes, (uint32_t)slices, op)
+    if (big && whole) MXK_GA(4, true);
+    else if (big) MXK_GA(4, false);
+    else if (whole) MXK_GA(1, true);
+    else MXK_GA(1, false);
+#undef MXK_GA
   }
   return check_launch("expert_gather");
 }
@@ -409,6 +478,7 @@ int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* p
   if ((rows > 0 && !h) || !place || !y) return fail(MXK_EINVAL, "expert_combine: null pointer");
   if (h_type != MXK_IN_F32 && h_type != MXK_IN_F16 && h_type != MXK_IN_BF16)
     return fail(MXK_EINVAL, "expert_combine: unknown h_type");
+  const bool whole = cols % 8 == 0 && aligned16(h) && aligned16(y);
   const int64_t pieces = ceil_div(cols, 8), step = std::max<int64_t>(1, ((int64_t)1 << 31) / pieces - 1);
   const DivU32 bp = make_divu32((uint32_t)pieces);
   for (int64_t t0 = 0; t0 < tokens; t0 += step) {
@@ -416,21 +486,23 @@ int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* p
     const dim3 grid((unsigned)ceil_div(total, 256));
     const int* pl = place + t0 * top;
     const float* gt = gates ? gates + t0 * top : nullptr;
+#define MXK_CQ(T, G, Q)                                                                                           \
+  hipLaunchKernelGGL((whole ? k_expert_combine<T, G, Q, true> : k_expert_combine<T, G, Q, false>), grid,          \
+                     dim3(256), 0, st, hp, pl, gt, top, (int)rows, total, bp, (uint32_t)pieces, (int)cols, yp)
 #define MXK_C(T)                                                                                                  \
   do {                                                                                                            \
     const T* hp = reinterpret_cast<const T*>(h);                                                                  \
     T* yp = reinterpret_cast<T*>(y) + t0 * cols;                                                                  \
-    if (gt)                                                                                                       \
-      hipLaunchKernelGGL((k_expert_combine<T, true>), grid, dim3(256), 0, st, hp, pl, gt, top, (int)rows, total, bp, \
-                         (uint32_t)pieces, (int)cols, yp);                                                        \
-    else                                                                                                          \
-      hipLaunchKernelGGL((k_expert_combine<T, false>), grid, dim3(256), 0, st, hp, pl, gt, top, (int)rows, total, bp, \
-                         (uint32_t)pieces, (int)cols, yp);                                                        \
+    if (gt && top > 4) MXK_CQ(T, true, 8);                                                                        \
+    else if (gt) MXK_CQ(T, true, 4);                                                                              \
+    else if (top > 4) MXK_CQ(T, false, 8);                                                                        \
+    else MXK_CQ(T, false, 4);                                                                                     \
   } while (0)
     if (h_type == MXK_IN_F32) MXK_C(float);
     else if (h_type == MXK_IN_F16) MXK_C(__half);
     else MXK_C(hip_bfloat16);
 #undef MXK_C
+#undef MXK_CQ
   }
   return check_launch("expert_combine");
 }
@@ -447,24 +519,25 @@ int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t r
     return fail(MXK_EINVAL, "expert_combine_grad: null pointer");
   if (h_type != MXK_IN_F32 && h_type != MXK_IN_F16 && h_type != MXK_IN_BF16)
     return fail(MXK_EINVAL, "expert_combine_grad: unknown h_type");
-  // one wave a token where that fills the card (8 waves a CU), else four
-  const bool few = tokens < 8 * (int64_t)num_cus();
-#define MXK_G(T)                                                                                                    \
-  do {                                                                                                              \
-    const T* dp = reinterpret_cast<const T*>(dy);                                                                   \
-    const T* hp = reinterpret_cast<const T*>(h);                                                                    \
-    T* op = reinterpret_cast<T*>(dh);                                                                               \
-    if (few)                                                                                                        \
-      hipLaunchKernelGGL((k_expert_combine_grad<T, 4>), dim3((unsigned)tokens), dim3(256), 0, st, dp, hp, place,    \
-                         gates, used, (int)tokens, top, (int)rows, (int)cols, op, dgates);                                     \
-    else                                                                                                            \
-      hipLaunchKernelGGL((k_expert_combine_grad<T, 1>), dim3((unsigned)ceil_div(tokens, 4)), dim3(256), 0, st, dp,  \
-                         hp, place, gates, used, (int)tokens, top, (int)rows, (int)cols, op, dgates);                          \
+  const int64_t waves = ceil_div(cols, 512);
+  const bool whole = cols % 8 == 0 && aligned16(dy) && aligned16(h) && aligned16(dh);
+#define MXK_GW(T, W)                                                                                              \
+  hipLaunchKernelGGL((whole ? k_expert_combine_grad<T, W, true> : k_expert_combine_grad<T, W, false>),            \
+                     dim3((unsigned)ceil_div(tokens, W > 4 ? 1 : 4 / W)), dim3(W > 4 ? 64 * W : 256), 0, st, reinterpret_cast<const T*>(dy),                           \
+                     reinterpret_cast<const T*>(h), place, gates, used, (int)tokens, top, (int)rows, (int)cols,   \
+                     reinterpret_cast<T*>(dh), dgates)
+#define MXK_G(T)                        \
+  do {                                  \
+    if (waves <= 1) MXK_GW(T, 1);       \
+    else if (waves <= 2) MXK_GW(T, 2);  \
+    else if (waves <= 4) MXK_GW(T, 4);  \
+    else MXK_GW(T, 8);                  \
   } while (0)
   if (h_type == MXK_IN_F32) MXK_G(float);
   else if (h_type == MXK_IN_F16) MXK_G(__half);
   else MXK_G(hip_bfloat16);
 #undef MXK_G
+#undef MXK_GW
   return check_launch("expert_combine_grad");
 }
 

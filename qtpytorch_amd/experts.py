@@ -19,12 +19,10 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .microscale import (_bias_f32, _check_linear, _grad_a, _grad_b, _grad_bias, _linear, _pack_weight, _product,
+from .microscale import (_FLOATS, _bias_f32, _check_linear, _grad_a, _grad_b, _grad_bias, _linear, _pack_weight, _product,
                          _row_major, _wants_grad, mxfp4_quantize, mxfp4_tensor)
 
 Tensor = torch.Tensor
-
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 class expert_plan(NamedTuple):
@@ -62,18 +60,21 @@ def expert_sort(ids: Tensor, n_experts: int) -> expert_plan:
     with L.on_device(dev):
         rc = lib.mxk_expert_sort(ids.data_ptr(), ids.element_size(), P, n_experts, order.data_ptr(), place.data_ptr(),
                                  offsets.data_ptr(), L.ptr(ws), nbytes, L.stream_of(ids))
-    L.check(rc, f"expert_sort({P} picks, {n_experts} experts)")
+    if rc:
+        L.check(rc, f"expert_sort({P} picks, {n_experts} experts)")
     return expert_plan(order, place, offsets)
 
 
 def _check_plan(name: str, plan: expert_plan) -> None:
-    for field, t in zip(plan._fields, plan):
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise TypeError(f"{name}: plan.{field} is a contiguous int32 tensor, got {t.dtype}")
-    if plan.order.dim() != 1 or plan.place.dim() != 2 or plan.place.numel() != plan.order.numel() \
-            or plan.offsets.dim() != 1 or plan.offsets.numel() < 2:
+    order, place, offsets = plan
+    if not (order.dtype == place.dtype == offsets.dtype == torch.int32
+            and order.is_contiguous() and place.is_contiguous() and offsets.is_contiguous()):
+        raise TypeError(f"{name}: a plan's tensors are contiguous int32, got "
+                        f"{order.dtype}, {place.dtype} and {offsets.dtype}")
+    if order.dim() != 1 or place.dim() != 2 or place.numel() != order.numel() or offsets.dim() != 1 \
+            or offsets.numel() < 2:
         raise ValueError(f"{name}: a plan has order [tokens * top], place [tokens, top] and offsets [experts + 1], got "
-                         f"{tuple(plan.order.shape)}, {tuple(plan.place.shape)} and {tuple(plan.offsets.shape)}")
+                         f"{tuple(order.shape)}, {tuple(place.shape)} and {tuple(offsets.shape)}")
 
 
 def _float_rows(name: str, x: Tensor, rows: int, what: str) -> None:
@@ -87,11 +88,12 @@ def _gather(x: Tensor, plan: expert_plan) -> Tensor:
     dev = L.require_gpu(x, *plan)
     x = _row_major(x)
     tokens, top = plan.place.shape
-    out = torch.empty(tokens * top, x.shape[1], dtype=x.dtype, device=dev)
+    out = torch.empty((tokens * top, x.shape[1]), dtype=x.dtype, device=dev)
     with L.on_device(dev):
         rc = L.lib().mxk_expert_gather(x.data_ptr(), x.element_size(), tokens, x.shape[1], x.stride(0),
                                        plan.order.data_ptr(), tokens * top, top, out.data_ptr(), L.stream_of(x))
-    L.check(rc, f"expert_gather({tokens}x{x.shape[1]}, top {top})")
+    if rc:
+        L.check(rc, f"expert_gather({tokens}x{x.shape[1]}, top {top})")
     return out
 
 
@@ -99,11 +101,12 @@ def _combine(h: Tensor, plan: expert_plan, gates: Optional[Tensor]) -> Tensor:
     dev = L.require_gpu(h, gates, *plan)
     h = h.contiguous()
     tokens, top = plan.place.shape
-    y = torch.empty(tokens, h.shape[1], dtype=h.dtype, device=dev)
+    y = torch.empty((tokens, h.shape[1]), dtype=h.dtype, device=dev)
     with L.on_device(dev):
         rc = L.lib().mxk_expert_combine(h.data_ptr(), L.elem_type(h.dtype), h.shape[0], plan.place.data_ptr(),
                                         L.ptr(gates), tokens, top, h.shape[1], y.data_ptr(), L.stream_of(h))
-    L.check(rc, f"expert_combine({tokens}x{h.shape[1]}, top {top})")
+    if rc:
+        L.check(rc, f"expert_combine({tokens}x{h.shape[1]}, top {top})")
     return y
 
 
@@ -140,7 +143,8 @@ class _ExpertCombine(torch.autograd.Function):
                                                  plan.place.data_ptr(), gates.data_ptr(),
                                                  plan.offsets.data_ptr() + 4 * (plan.offsets.numel() - 1), tokens, top,
                                                  h.shape[1], dh.data_ptr(), dg.data_ptr(), L.stream_of(dy))
-        L.check(rc, f"expert_combine gradient({tokens}x{h.shape[1]}, top {top})")
+        if rc:
+            L.check(rc, f"expert_combine gradient({tokens}x{h.shape[1]}, top {top})")
         return dh, dg, None
 
 

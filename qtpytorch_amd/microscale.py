@@ -28,7 +28,7 @@ from . import _lib as L
 
 Tensor = torch.Tensor
 
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_FLOATS = {torch.float32: L.MXK_IN_F32, torch.float16: L.MXK_IN_F16, torch.bfloat16: L.MXK_IN_BF16}
 
 
 class mxfp4_tensor:
@@ -54,6 +54,13 @@ class mxfp4_tensor:
         self.scales = scales.contiguous()
         self.shape = shape
 
+    @classmethod
+    def _of(cls, codes: Tensor, scales: Tensor, shape: torch.Size) -> "mxfp4_tensor":
+        """Codes and scales that were allocated for this shape."""
+        q = cls.__new__(cls)
+        q.codes, q.scales, q.shape = codes, scales, shape
+        return q
+
     @property
     def device(self) -> torch.device:
         return self.codes.device
@@ -72,12 +79,15 @@ class mxfp4_tensor:
         """The values as float32, float16 or bfloat16 (exact in float32 and
         bfloat16 below their largest value; float16 rounds to nearest even)."""
         dev = L.require_gpu(self.codes)
-        y = torch.empty(self.shape, dtype=dtype, device=dev)
+        kind = L.elem_type(dtype)
+        shape = self.shape
+        y = torch.empty(shape, dtype=dtype, device=dev)
         if y.numel():
             with L.on_device(dev):
-                rc = L.lib().mxk_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _rows(self.shape),
-                                                  self.shape[-1], L.elem_type(dtype), y.data_ptr(), L.stream_of(y))
-            L.check(rc, "mxfp4 dequantize")
+                rc = L.lib().mxk_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _rows(shape),
+                                                  shape[-1], kind, y.data_ptr(), L.stream_of(y))
+            if rc:
+                L.check(rc, f"mxfp4 dequantize({tuple(shape)})")
         return y
 
     def __repr__(self):
@@ -90,7 +100,7 @@ def _aligned(codes: Tensor) -> Tensor:
 
 
 def _rows(shape) -> int:
-    return math.prod(shape[:-1])
+    return shape[0] if len(shape) == 2 else math.prod(shape[:-1])
 
 
 def mxfp4_quantize(x: Tensor) -> mxfp4_tensor:
@@ -99,25 +109,31 @@ def mxfp4_quantize(x: Tensor) -> mxfp4_tensor:
     Per block: scale byte = max(exponent of the largest magnitude - 2, -127) +
     127, code = the nearest grid value of x / 2**(scale - 127), ties to the
     even code, magnitudes above 6 to 6."""
-    if x.dim() < 1:
+    shape = x.shape
+    if len(shape) < 1:
         raise ValueError("mxfp4_quantize: a tensor of at least one dimension")
     dev = L.require_gpu(x)
-    x = x.detach()
-    if x.dtype not in _FLOATS:
-        x = x.float()
-    shape = x.shape
-    cols = shape[-1]
-    x = _row_major(x) if x.dim() == 2 else x.contiguous()
-    ld = max(x.stride(0), cols) if x.dim() == 2 else cols
+    kind = _FLOATS.get(x.dtype)
+    if kind is None:
+        x, kind = x.detach().float(), L.MXK_IN_F32
+    cols = ld = shape[-1]
     kb = -(-cols // 32)
-    codes = torch.empty(*shape[:-1], 16 * kb, dtype=torch.uint8, device=dev)
-    scales = torch.empty(*shape[:-1], kb, dtype=torch.uint8, device=dev)
-    if x.numel():
+    if len(shape) == 2:
+        x = _row_major(x)
+        ld = max(x.stride(0), cols)
+        codes = torch.empty((shape[0], 16 * kb), dtype=torch.uint8, device=dev)
+        scales = torch.empty((shape[0], kb), dtype=torch.uint8, device=dev)
+    else:
+        x = x.detach().contiguous()
+        codes = torch.empty((*shape[:-1], 16 * kb), dtype=torch.uint8, device=dev)
+        scales = torch.empty((*shape[:-1], kb), dtype=torch.uint8, device=dev)
+    if codes.numel():
         with L.on_device(dev):
-            rc = L.lib().mxk_mxfp4_quantize(x.data_ptr(), L.elem_type(x.dtype), _rows(shape), cols, ld,
-                                            codes.data_ptr(), scales.data_ptr(), L.stream_of(x))
-        L.check(rc, f"mxfp4_quantize({tuple(shape)})")
-    return mxfp4_tensor(codes, scales, shape)
+            rc = L.lib().mxk_mxfp4_quantize(x.data_ptr(), kind, _rows(shape), cols, ld, codes.data_ptr(),
+                                            scales.data_ptr(), L.stream_of(codes))
+        if rc:
+            L.check(rc, f"mxfp4_quantize({tuple(shape)})")
+    return mxfp4_tensor._of(codes, scales, shape)
 
 
 def _bias_f32(bias: Optional[Tensor], shape: Tuple[int, ...]) -> Optional[Tensor]:
@@ -142,13 +158,14 @@ def _product(a: mxfp4_tensor, b: mxfp4_tensor, rows: int, N: int, bias: Optional
                                   b.scales.data_ptr(), rows, N, K, L.ptr(bias), L.elem_type(out.dtype),
                                   out.data_ptr(), L.ptr(offsets), E, L.ptr(order), top, L.ptr(ws), nbytes,
                                   L.stream_of(out))
-    L.check(rc, f"mxfp4 product({rows}x{K} by {N})")
+    if rc:
+        L.check(rc, f"mxfp4 product({rows}x{K} by {N})")
     return out
 
 
 def _row_major(x: Tensor) -> Tensor:
     """x [rows, cols] itself if its rows are contiguous (they may lie apart), else a copy."""
-    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.detach().contiguous()
 
 
 def _linear(x: Tensor, b: mxfp4_tensor, rows: int, bias: Optional[Tensor], offsets: Optional[Tensor] = None,
@@ -156,18 +173,19 @@ def _linear(x: Tensor, b: mxfp4_tensor, rows: int, bias: Optional[Tensor], offse
     """Float rows x [*, K] packed and multiplied in one call, [rows, N] of x's dtype."""
     dev = L.require_gpu(x, b.codes, bias, offsets, order)
     lib = L.lib()
-    x = _row_major(x.detach())
+    x = _row_major(x)
     N, K = b.shape[-2:]
     E = 0 if offsets is None else offsets.numel() - 1
-    y = torch.empty(rows, N, dtype=x.dtype, device=dev)
-    kind, stride = L.elem_type(x.dtype), max(x.stride(0), K)
+    y = torch.empty((rows, N), dtype=x.dtype, device=dev)
+    kind, stride = _FLOATS[x.dtype], max(x.stride(0), K)
     nbytes = lib.mxk_mxfp4_linear_workspace(kind, x.shape[0], stride, rows, N, K, E, order is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with L.on_device(dev):
         rc = lib.mxk_mxfp4_linear(x.data_ptr(), kind, x.shape[0], stride, b.codes.data_ptr(),
-                                   b.scales.data_ptr(), rows, N, K, L.ptr(bias), y.data_ptr(),
+                                  b.scales.data_ptr(), rows, N, K, L.ptr(bias), y.data_ptr(),
                                   L.ptr(offsets), E, L.ptr(order), top, L.ptr(ws), nbytes, L.stream_of(y))
-    L.check(rc, f"mxfp4 linear({rows}x{K} by {N})")
+    if rc:
+        L.check(rc, f"mxfp4 linear({rows}x{K} by {N})")
     return y
 
 
@@ -195,7 +213,8 @@ def _grad(entry: str, dy: Tensor, q: mxfp4_tensor, out: Tensor, offsets: Optiona
         rc = getattr(lib, entry)(dy.data_ptr(), kind, M, N, q.codes.data_ptr(), q.scales.data_ptr(), K,
                                  L.elem_type(out.dtype), out.data_ptr(), L.ptr(offsets),
                                  0 if offsets is None else offsets.numel() - 1, L.ptr(ws), nbytes, L.stream_of(out))
-    L.check(rc, f"{entry[4:]}({M}x{N} by {K})")
+    if rc:
+        L.check(rc, f"{entry[4:]}({M}x{N} by {K})")
     return out
 
 
