@@ -204,9 +204,10 @@ __device__ __forceinline__ void wait_loads_if(uint32_t counted) {
 // 4h .. 4h+3, so one dword per row holds its four scale bytes and a step
 // selects its byte.  (Any order of K is right as long as both operands share it.)
 //
-// LDS rows are 128 bytes: 16-byte chunk c of row r sits at c ^ (r & 7), so
-// that 8 lanes of consecutive rows read all banks once.  The loads write LDS
-// in lane order, so the lane picks the chunk that belongs at its place.
+// LDS rows are 128 bytes, half of the banks: 16-byte chunk c of row r sits at
+// c ^ (r & 7) ^ (r >> 3 & 7), so that 16 lanes of consecutive rows read all
+// banks once (with c ^ (r & 7) rows r and r + 8 meet).  The loads write LDS in
+// lane order, so the lane picks the chunk that belongs at its place.
 //
 // The barrier of a stage sits before its last step: by then the next stage
 // has landed and this stage's last fragments are in registers, so the loads of the
@@ -239,8 +240,10 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
   int64_t lo = 0, hi = 0, n0 = 0;
   int e = 0;
   i32x4 ra, rb;
-  // loads of this wave: rows (wave * LI + i) * 8 + lane / 8 of either operand
+  // loads of this wave: rows (wave * LI + i) * 8 + lane / 8 of either operand,
+  // chunk (lane & 7) ^ (lane / 8) ^ (wave * LI + i & 7) of the stage
   const int lr = lane >> 3, chunk = (lane & 7) ^ lr;
+  const int flip = wave * LI & 7;
   const uint32_t off0 = (uint32_t)(wave * LI * 8 + lr) * row_bytes, step8 = 8u * row_bytes;
   uint32_t off_a[EXPERT ? LI : 1];  // by expert: of any rows
 
@@ -292,10 +295,10 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
   };
   // part q of F of the loads of stage t
   auto issue = [&](uint32_t t, uint32_t buf, int q) {
-    const uint32_t blk = 8u * t + chunk;
-    const uint32_t ok = blk < KB && t < to ? blk * 16u : MXK_FAR_BLOCK;
 #pragma unroll
     for (int i = q * LI / F; i < (q + 1) * LI / F; ++i) {
+      const uint32_t blk = 8u * t + (chunk ^ flip ^ i);
+      const uint32_t ok = blk < KB && t < to ? blk * 16u : MXK_FAR_BLOCK;
       const uint32_t off = off0 + i * step8 + ok;
       load_to_lds(ra, EXPERT ? off_a[EXPERT ? i : 0] + ok : off, buf * BUF + (wave * LI + i) * 1024u);
       load_to_lds(rb, off, buf * BUF + OP + (wave * LI + i) * 1024u);
@@ -319,7 +322,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
   const uint32_t rd_b = OP + (uint32_t)((wave & 1) * 32 * F + r32) * 128u;
   uint32_t at[4];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) at[s] = (uint32_t)((4 * h + s) ^ (lane & 7)) * 16u;
+  for (int s = 0; s < 4; ++s) at[s] = (uint32_t)((4 * h + s) ^ (lane & 7) ^ (r32 >> 3)) * 16u;
   const uint32_t rs_a = 2 * BUF + ((wave >> 1) * 32 * F + r32) * 8 + 4 * h;
   const uint32_t rs_b = 2 * BUF + SC + ((wave & 1) * 32 * F + r32) * 8 + 4 * h;
 
@@ -327,8 +330,9 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
   i32x4 fa[2][F], fb[2][F];
   int sa[2][F], sb[2][F];
   auto read_frag = [&](uint32_t buf, int s, int i, i32x4 (&xa)[F], i32x4 (&xb)[F]) {
-    xa[i] = *reinterpret_cast<const i32x4*>(lds + buf * BUF + rd_a + at[s] + i * 4096);
-    xb[i] = *reinterpret_cast<const i32x4*>(lds + buf * BUF + rd_b + at[s] + i * 4096);
+    const uint32_t c = at[s] ^ (i & 1 ? 64u : 0u);  // rows 32 i: bit 2 of r >> 3
+    xa[i] = *reinterpret_cast<const i32x4*>(lds + buf * BUF + rd_a + c + i * 4096);
+    xb[i] = *reinterpret_cast<const i32x4*>(lds + buf * BUF + rd_b + c + i * 4096);
   };
   auto read_scale = [&](uint32_t buf, int i, int (&xa)[F], int (&xb)[F]) {
     xa[i] = *reinterpret_cast<const int*>(lds + buf * SBUF + rs_a + i * 256);

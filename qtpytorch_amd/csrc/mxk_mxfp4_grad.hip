@@ -229,14 +229,24 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
     xa[i] = *reinterpret_cast<const bf16x8*>(lds + buf * BUF + (ra + 32 * i) * 128 + ((c ^ xra) << 4));
     xb[i] = *reinterpret_cast<const bf16x8*>(lds + buf * BUF + OP + (rb + 32 * i) * 128 + ((c ^ xrb) << 4));
   };
+  // A row of F MFMAs and what is issued between them: the conversions of a
+  // stage (some 240 VALU a wave) fit into the MFMAs' shadows only if they
+  // alternate with them
 #define MXK_STEP(XA, XB, BETWEEN)                                                              \
   _Pragma("unroll") for (int i = 0; i < F; ++i) {                                              \
     BETWEEN;                                                                                   \
-    __builtin_amdgcn_sched_barrier(0);                                                         \
     _Pragma("unroll") for (int j = 0; j < F; ++j)                                              \
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(XB[i], XA[j], acc[i][j], 0, 0, 0); \
+    _Pragma("unroll") for (int j = 0; j < F; ++j) {                                            \
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); /* MFMA */                            \
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); /* LDS read */                        \
+      __builtin_amdgcn_sched_group_barrier(0x002, SHADOW, 0); /* VALU */                       \
+      __builtin_amdgcn_sched_group_barrier(0x200, 1, 0); /* LDS write */                       \
+      __builtin_amdgcn_sched_group_barrier(0x020, 4, 0); /* loads */                           \
+    }                                                                                          \
     __builtin_amdgcn_sched_barrier(0);                                                         \
   }
+  constexpr int SHADOW = 48 / F;  // a row's share of the conversions, spread over its MFMAs
   // Quarters per row of MFMAs
   constexpr int Q = 4 / F;
   if (stages > 0) {
