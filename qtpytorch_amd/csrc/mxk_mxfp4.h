@@ -197,4 +197,19 @@ __device__ __forceinline__ void place_tile(uint32_t id, uint32_t tm, uint32_t tn
   m = group * 8u + (in - n * high);
 }
 
+// The same for products by expert, of whose tm rows of tiles only the first
+// ones are in use (how many is not known on the host): blocks of 8 x 4 tiles in
+// turn to the XCDs, so that each has its share of those.  false: no such tile.
+__device__ __forceinline__ bool place_block_tile(uint32_t id, uint32_t tm, uint32_t tn, uint32_t& m, uint32_t& n) {
+  const uint32_t local = id >> 3, block = (local >> 5) * 8u + (id & 7u), in = local & 31u;
+  const uint32_t across = (tn + 3u) >> 2, row = block / across;
+  m = row * 8u + (in & 7u);
+  n = (block - row * across) * 4u + (in >> 3);
+  return m < tm && n < tn;
+}
+// how many ids that takes
+inline int64_t block_tile_ids(int64_t tm, int64_t tn) {
+  return ceil_div(ceil_div(tm, 8) * ceil_div(tn, 4), 8) * 256;
+}
+
 }  // namespace mxk

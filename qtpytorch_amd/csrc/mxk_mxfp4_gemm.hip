@@ -216,7 +216,7 @@ __device__ __forceinline__ void wait_loads_if(uint32_t counted) {
 template <typename T, int F, bool EXPERT>
 __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8_t* __restrict__ ta,
                                                           const uint8_t* __restrict__ tb, int64_t b_rows, uint32_t tm,
-                                                          uint32_t tn, uint32_t splits) {
+                                                          uint32_t tn, uint32_t splits, uint32_t ids) {
   constexpr int B = 64 * F;                 // rows of a tile
   constexpr int OP = B * 128, SC = B * 8;   // bytes of an operand's stage and of its scales
   constexpr int BUF = 2 * OP, SBUF = 2 * SC;
@@ -250,9 +250,10 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
   // the next tile from `id` on that has products (rows without an expert are
   // written here): true, or false at the end
   auto next_tile = [&](uint32_t& id) -> bool {
-    for (; id < tm * tn * splits; id += gridDim.x) {
+    for (; id < ids; id += gridDim.x) {
       uint32_t mt, nt;
-      place_tile(id, tm, tn * splits, mt, nt);
+      if (!EXPERT) place_tile(id, tm, tn * splits, mt, nt);
+      else if (!place_block_tile(id, tm, tn, mt, nt)) continue;
       if (!EXPERT && splits > 1) {
         const uint32_t part = nt % splits;
         nt /= splits;
@@ -904,7 +905,7 @@ static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_byte
   const Shape t = tile_of(p);
   const int64_t B = t.F ? 64 * t.F : 64;
   const int64_t slots = ex ? segment_slots(p.M, p.E, (int)B) : ceil_div(p.M, B);
-  const int64_t tn = ceil_div(p.N, B), n = slots * tn * t.splits;
+  const int64_t tn = ceil_div(p.N, B), n = ex && t.F ? block_tile_ids(slots, tn) : slots * tn * t.splits;
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many tiles");
   const int64_t b_rows = ex ? p.E * p.N : p.N, na = stage_bytes(p.M, p.KB), nb = stage_bytes(b_rows, p.KB);
   if (t.F) {
@@ -917,7 +918,7 @@ static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_byte
   const int64_t cus = (num_cus() + 7) & ~7;  // a multiple of the XCDs: a workgroup's tiles stay on its own
 #define MXK_TILE(T, F, EX, P)                                                                                        \
   hipLaunchKernelGGL((k_fp4_gemm_tile<T, F, EX>), dim3((unsigned)std::min<int64_t>(n, (F == 4 ? 1 : 2) * cus)),      \
-                     dim3(256), 0, st, P, ws, ws + na, b_rows, (uint32_t)slots, (uint32_t)tn, (uint32_t)t.splits)
+                     dim3(256), 0, st, P, ws, ws + na, b_rows, (uint32_t)slots, (uint32_t)tn, (uint32_t)t.splits, (uint32_t)n)
 #define MXK_L(T, EX)                                                                                     \
   do {                                                                                                   \
     if (t.F == 4) MXK_TILE(T, 4, EX, p);                                                                 \

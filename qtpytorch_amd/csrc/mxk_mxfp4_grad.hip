@@ -100,7 +100,8 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
   uint32_t it, jt;
-  place_tile(blockIdx.x, tm, tn, it, jt);
+  if (OF_B || !p.offsets) place_tile(blockIdx.x, tm, tn, it, jt);
+  else if (!place_block_tile(blockIdx.x, tm, tn, it, jt)) return;
   const int64_t j0 = (int64_t)jt * B;
   int64_t i0 = (int64_t)it * B, i1 = p.I < i0 + B ? p.I : i0 + B, t0 = 0, t1 = p.T, v0 = 0, o0 = 0;
   if (p.offsets) {
@@ -369,8 +370,10 @@ static int launch_grad(const Fp4Grad& p, bool of_b, int out_type, hipStream_t st
   const int F = tiles(256) >= 160 ? 4 : 2;
   const int64_t B = 64 * F, n = tiles((int)B), tn = ceil_div(p.J, B);
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 gradient: too many tiles");
-  const dim3 grid((unsigned)n);
   const uint32_t tm = (uint32_t)(n / tn);
+  const int64_t ids = ex && !of_b ? block_tile_ids(tm, tn) : n;
+  if (ids >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 gradient: too many tiles");
+  const dim3 grid((unsigned)ids);
 #define MXK_G(O, F, OB) hipLaunchKernelGGL((k_fp4_grad<O, F, OB>), grid, dim3(256), 0, st, p, tm, (uint32_t)tn)
 #define MXK_O(O)                     \
   do {                               \
