@@ -120,19 +120,38 @@ __global__ __launch_bounds__(256) void k_fp4_gemm(Fp4Gemm p) {
 
 
 // ---------------------------------------------------------------- tiles through LDS
-// Scale bytes in the order in which the tile kernel's stages read them:
-// out[kt][row][8], kt = stages of 8 blocks (256 values of K), zeros past KB,
-// for the rows of the product (picked by `order` where there is one) and those of b.  One
-// launch for both operands: 17/16 of a byte moved per 32 values.
-__global__ __launch_bounds__(256) void k_fp4_stage_scales(Fp4Gemm p, int64_t b_rows, int64_t a_blocks,
-                                                          uint8_t* __restrict__ ta, uint8_t* __restrict__ tb) {
-  const bool of_a = (int64_t)blockIdx.x < a_blocks;
+// What the tile kernel reads in its own order, in one launch:
+//  - scale bytes by stages of 8 blocks (256 values of K): ta[kt][row of the
+//    product][8], tb[kt][row of b][8], zeros past KB; 17/16 of a byte moved
+//    per 32 values;
+//  - by expert, each slot's segment and rows, and the row of a behind each row
+//    of the product, which a tile would otherwise look up while nothing else is
+//    under way.
+struct Fp4Staged {
+  uint8_t *ta, *tb;
+  int4* slot;  // {expert, first row, end, 0}
+  int* row;    // -1: none
+};
+__global__ __launch_bounds__(256) void k_fp4_stage(Fp4Gemm p, Fp4Staged out, int64_t b_rows, int64_t a_blocks,
+                                                   int64_t b_blocks, int64_t slots, int tile) {
+  int64_t block = blockIdx.x;
+  if (block >= a_blocks + b_blocks) {  // a slot per wave
+    const int64_t slot = (block - a_blocks - b_blocks) * 4 + (threadIdx.x >> 6);
+    if (slot >= slots) return;
+    const Segment s = tile == 256 ? find_segment<256>(slot, p.offsets, p.E, p.M)
+                                  : find_segment<128>(slot, p.offsets, p.E, p.M);
+    if ((threadIdx.x & 63) == 0) out.slot[slot] = make_int4(s.e, (int)s.lo, (int)s.hi, 0);
+    return;
+  }
+  const bool of_a = block < a_blocks;
+  if (!of_a) block -= a_blocks;
   const int64_t rows = of_a ? p.M : b_rows;
-  const int64_t r = (of_a ? (int64_t)blockIdx.x : (int64_t)blockIdx.x - a_blocks) * 32 + (threadIdx.x >> 3);
+  const int64_t r = block * 32 + (threadIdx.x >> 3);
   if (r >= rows) return;
   const int64_t src = of_a ? source_row(p, r) : r;
+  if (of_a && p.offsets && (threadIdx.x & 7) == 0) out.row[r] = (int)src;
   const uint8_t* s = (of_a ? p.as : p.bs) + (src < 0 ? 0 : src) * p.KB;
-  uint8_t* out = of_a ? ta : tb;
+  uint8_t* to = of_a ? out.ta : out.tb;
   for (int64_t k = 8 * (threadIdx.x & 7); k < p.KB; k += 64) {
     uint64_t v = 0;
     if (src >= 0) {
@@ -143,7 +162,7 @@ __global__ __launch_bounds__(256) void k_fp4_stage_scales(Fp4Gemm p, int64_t b_r
           if (k + i < p.KB) v |= (uint64_t)s[k + i] << (8 * i);
       }
     }
-    *reinterpret_cast<uint64_t*>(out + ((k >> 3) * rows + r) * 8) = v;
+    *reinterpret_cast<uint64_t*>(to + ((k >> 3) * rows + r) * 8) = v;
   }
 }
 
@@ -213,93 +232,121 @@ __device__ __forceinline__ void wait_loads_if(uint32_t counted) {
 // has landed and this stage's last fragments are in registers, so the loads of the
 // stage after next go into the buffer just read, and the next stage's first
 // fragments are read while the last step multiplies.
+//
+// A workgroup takes tile after tile.  Its next tile's place (and, by expert,
+// its rows) is looked up before the products of this one, and that tile's first
+// two stages are requested between the stores of this one's result.
 template <typename T, int F, bool EXPERT>
-__global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8_t* __restrict__ ta,
-                                                          const uint8_t* __restrict__ tb, int64_t b_rows, uint32_t tm,
+__global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged in, int64_t b_rows, uint32_t tm,
                                                           uint32_t tn, uint32_t splits, uint32_t ids) {
   constexpr int B = 64 * F;                 // rows of a tile
   constexpr int OP = B * 128, SC = B * 8;   // bytes of an operand's stage and of its scales
   constexpr int BUF = 2 * OP, SBUF = 2 * SC;
   constexpr int LI = B / 32;                // load instructions per wave, operand and stage
+  constexpr int LOADS = 2 * LI + (F == 4 ? 1 : 2);  // all of a wave and stage
   constexpr int NW = 32 * F;                // columns of a wave
   constexpr int CB = F == 4 ? 128 : 64;     // bytes of a row that the result passes through LDS at once
   constexpr int CH = CB / 16, CC = CB / (int)sizeof(T), PASS = NW / CC;
-  constexpr int STORES = F * PASS * 32 * CH / 64;  // store instructions per wave and tile
+  // passes of the result, each with CH / 2 stores; every STEP of them one of
+  // the 2 F parts of the next tile's first two stages
+  constexpr int PASSES = F * PASS, STEP = PASSES / (2 * F);
+  // memory operations of a wave complete in order: what may be due behind the
+  // last load of stage 0 (the stores from its pass on and stage 1), of stage 1
+  constexpr int BEHIND0 = LOADS + (PASSES - (F - 1) * STEP) * (CH / 2);
+  constexpr int BEHIND1 = (PASSES - (2 * F - 1) * STEP) * (CH / 2);
+  static_assert(STEP >= 1 && BEHIND0 <= 63, "a part for every pass, counts that the wait can hold");
   __shared__ __align__(16) uint8_t lds[2 * BUF + 2 * SBUF + 4 * 32 * CB];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r32 = lane & 31, h = lane >> 5;
-  T* y = reinterpret_cast<T*>(p.y);
   const uint32_t row_bytes = (uint32_t)p.KB * 16u;
   const uint32_t KB = (uint32_t)p.KB, stages = (KB + 7u) >> 3;
-  uint32_t from = 0, to = stages;  // of the tile being loaded
-  const bool picked = EXPERT && p.order != nullptr;
   // whole 16-byte pieces of y: stores by buffer, as many for every tile
   const bool whole = p.N * (int)sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
 
-  // the tile that is being loaded, and the one whose result is due
-  int64_t lo = 0, hi = 0, n0 = 0;
-  int e = 0;
-  i32x4 ra, rb;
+  // a tile: rows lo .. hi of the product, columns from n0, stages from .. to
+  struct Tile {
+    int lo, hi, e;
+    int64_t n0;
+    uint32_t from, to;
+    T* y;
+  };
+  Tile cur = {}, next = {};
   // loads of this wave: rows (wave * LI + i) * 8 + lane / 8 of either operand,
   // chunk (lane & 7) ^ (lane / 8) ^ (wave * LI + i & 7) of the stage
   const int lr = lane >> 3, chunk = (lane & 7) ^ lr;
   const int flip = wave * LI & 7;
   const uint32_t off0 = (uint32_t)(wave * LI * 8 + lr) * row_bytes, step8 = 8u * row_bytes;
+  i32x4 ra, rb;
   uint32_t off_a[EXPERT ? LI : 1];  // by expert: of any rows
+  int src[EXPERT ? LI : 1];         // those of the next tile
 
   // the next tile from `id` on that has products (rows without an expert are
   // written here): true, or false at the end
-  auto next_tile = [&](uint32_t& id) -> bool {
+  auto look_ahead = [&](uint32_t& id) -> bool {
     for (; id < ids; id += gridDim.x) {
       uint32_t mt, nt;
-      if (!EXPERT) place_tile(id, tm, tn * splits, mt, nt);
-      else if (!place_block_tile(id, tm, tn, mt, nt)) continue;
-      if (!EXPERT && splits > 1) {
-        const uint32_t part = nt % splits;
-        nt /= splits;
-        from = part * stages / splits;
-        to = (part + 1u) * stages / splits;
-        y = reinterpret_cast<T*>(p.y) + (int64_t)part * p.M * p.N;
-      }
-      lo = (int64_t)mt * B;
-      hi = p.M < lo + B ? p.M : lo + B;
-      n0 = (int64_t)nt * B;
-      if (EXPERT) {
-        const Segment s = find_segment<B>(mt, p.offsets, p.E, p.M);
-        e = s.e;
-        lo = s.lo;
-        hi = s.hi;
-        if (e > p.E) continue;
-        if (e == p.E) {
-          const int64_t w = p.N - n0 < B ? p.N - n0 : B;
-          for (int64_t r = lo + wave; r < hi; r += 4)
-            for (int64_t c = lane; c < w; c += 64) y[r * p.N + n0 + c] = from_f32<T>(0.0f);
+      next.from = 0;
+      next.to = stages;
+      next.y = reinterpret_cast<T*>(p.y);
+      if constexpr (EXPERT) {
+        if (!place_block_tile(id, tm, tn, mt, nt)) continue;
+        next.n0 = (int64_t)nt * B;
+        const int4 s = in.slot[mt];
+        next.e = __builtin_amdgcn_readfirstlane(s.x);
+        next.lo = __builtin_amdgcn_readfirstlane(s.y);
+        next.hi = __builtin_amdgcn_readfirstlane(s.z);
+        if (next.e > p.E) continue;
+        if (next.e == p.E) {
+          const int64_t w = p.N - next.n0 < B ? p.N - next.n0 : B;
+          for (int64_t r = next.lo + wave; r < next.hi; r += 4)
+            for (int64_t c = lane; c < w; c += 64) next.y[r * p.N + next.n0 + c] = from_f32<T>(0.0f);
           continue;
         }
-      }
-      const int64_t rows_b = p.N - n0 < B ? p.N - n0 : B;
-      const uint8_t* a0 = picked ? p.a : p.a + lo * (int64_t)row_bytes;
-      const int64_t rows_a = picked ? p.a_rows : (p.M - lo < B ? p.M - lo : B);
-      ra = buffer_words(a0, (uint32_t)(rows_a * row_bytes));
-      rb = buffer_words(p.b + ((int64_t)e * p.N + n0) * row_bytes, (uint32_t)(rows_b * row_bytes));
-      if constexpr (EXPERT) {
 #pragma unroll
         for (int i = 0; i < LI; ++i) {
-          const int64_t r = lo + (wave * LI + i) * 8 + lr;
-          const int64_t src = r < hi ? (picked ? source_row(p, r) : r - lo) : -1;
-          off_a[i] = src >= 0 ? (uint32_t)src * row_bytes : MXK_FAR_ROW;
+          const int r = next.lo + (wave * LI + i) * 8 + lr;
+          src[i] = in.row[r < next.hi ? r : next.hi - 1];
         }
+      } else {
+        place_tile(id, tm, tn * splits, mt, nt);
+        if (splits > 1) {
+          const uint32_t part = nt % splits;
+          nt /= splits;
+          next.from = part * stages / splits;
+          next.to = (part + 1u) * stages / splits;
+          next.y += (int64_t)part * p.M * p.N;
+        }
+        next.n0 = (int64_t)nt * B;
+        next.lo = (int)mt * B;
+        next.hi = p.M < (int64_t)next.lo + B ? (int)p.M : next.lo + B;
       }
       return true;
     }
     return false;
+  };
+  // that tile is the one to load now
+  auto advance = [&]() {
+    cur = next;
+    const int64_t rows_b = p.N - cur.n0 < B ? p.N - cur.n0 : B;
+    rb = buffer_words(p.b + ((int64_t)cur.e * p.N + cur.n0) * row_bytes, (uint32_t)(rows_b * row_bytes));
+    if constexpr (EXPERT) {
+      // with an order, rows of all of a; without, of this tile's part of it
+      const bool picked = p.order != nullptr;
+      ra = buffer_words(picked ? p.a : p.a + cur.lo * (int64_t)row_bytes,
+                        (uint32_t)(picked ? p.a_rows : (int64_t)(cur.hi - cur.lo)) * row_bytes);
+#pragma unroll
+      for (int i = 0; i < LI; ++i)
+        off_a[i] = src[i] < 0 ? MXK_FAR_ROW : (uint32_t)(src[i] - (picked ? 0 : cur.lo)) * row_bytes;
+    } else {
+      ra = buffer_words(p.a + cur.lo * (int64_t)row_bytes, (uint32_t)(cur.hi - cur.lo) * row_bytes);
+    }
   };
   // part q of F of the loads of stage t
   auto issue = [&](uint32_t t, uint32_t buf, int q) {
 #pragma unroll
     for (int i = q * LI / F; i < (q + 1) * LI / F; ++i) {
       const uint32_t blk = 8u * t + (chunk ^ flip ^ i);
-      const uint32_t ok = blk < KB && t < to ? blk * 16u : MXK_FAR_BLOCK;
+      const uint32_t ok = blk < KB && t < cur.to ? blk * 16u : MXK_FAR_BLOCK;
       const uint32_t off = off0 + i * step8 + ok;
       load_to_lds(ra, EXPERT ? off_a[EXPERT ? i : 0] + ok : off, buf * BUF + (wave * LI + i) * 1024u);
       load_to_lds(rb, off, buf * BUF + OP + (wave * LI + i) * 1024u);
@@ -310,10 +357,11 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
       constexpr int R = B / 2;  // rows per wave
       const bool of_b = wave >= 2;
       const int64_t rows = of_b ? b_rows : p.M;
-      const int64_t first = (of_b ? (int64_t)e * p.N + n0 : lo) + R * (wave & 1);
+      const int64_t first = (of_b ? (int64_t)cur.e * p.N + cur.n0 : cur.lo) + R * (wave & 1);
       // past the last row: bytes of the next plane or of the kilobytes kept after the
       // last, for rows whose codes are zeros or whose results are not stored
-      const i32x4 rs = buffer_words((of_b ? tb : ta) + ((int64_t)t * rows + first) * 8, t < to ? R * 8u : 0u);
+      const i32x4 rs =
+          buffer_words((of_b ? in.tb : in.ta) + ((int64_t)t * rows + first) * 8, t < cur.to ? R * 8u : 0u);
       load_scales_to_lds<R>(rs, lane, 2u * BUF + buf * SBUF + (of_b ? SC : 0) + R * 8u * (wave & 1));
     }
   };
@@ -353,18 +401,12 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
     __builtin_amdgcn_sched_barrier(0);                                                                      \
   }
 
-  constexpr int LOADS = 2 * LI + (F == 4 ? 1 : 2);  // per wave and stage
   uint32_t id = blockIdx.x;
-  if (!next_tile(id)) return;
+  if (!look_ahead(id)) return;
+  advance();
 #pragma unroll
-  for (int q = 0; q < F; ++q) issue(from, 0, q);
-#pragma unroll
-  for (int q = 0; q < F; ++q) issue(from + 1, 1, q);
-  // stores of the tile before, issued after this tile's first loads: memory
-  // operations of a wave complete in order, so those loads are waited for
-  // without them
-  constexpr bool COUNTED = STORES + LOADS <= 63;  // as the wait's field has room for
-  uint32_t stores_due = 0;
+  for (int q = 0; q < 2 * F; ++q) issue(cur.from + q / F, q / F, q % F);
+  uint32_t behind = 0;  // whether stores are due behind and between this tile's first loads
   for (;;) {
     // sums start from the bias, which every row of a fragment shares
 #pragma unroll
@@ -373,11 +415,11 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
 #pragma unroll
       for (int q = 0; q < 16; ++q) b[q] = 0.0f;
       if (p.bias) {
-        const int64_t n = n0 + (wave & 1) * NW + 32 * i + 4 * h;
+        const int64_t n = cur.n0 + (wave & 1) * NW + 32 * i + 4 * h;
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
           const int64_t at = n + 8 * (q >> 2) + (q & 3);
-          b[q] = p.bias[(int64_t)e * p.N + (at < p.N ? at : p.N - 1)];
+          b[q] = p.bias[(int64_t)cur.e * p.N + (at < p.N ? at : p.N - 1)];
         }
       }
 #pragma unroll
@@ -385,7 +427,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
 #pragma unroll
         for (int q = 0; q < 16; ++q) acc[i][j][q] = b[q];
     }
-    if (COUNTED && stores_due) wait_loads<(COUNTED ? STORES : 0) + LOADS>();
+    if (behind) wait_loads<BEHIND0>();
     else wait_loads<LOADS>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -394,17 +436,15 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
       read_scale(0, i, sa[0], sb[0]);
       read_frag(0, 0, i, fa[0], fb[0]);
     }
+    id += gridDim.x;
+    const bool more = look_ahead(id);
     // past the last stage the loads bring zeros and the reads are not used
     uint32_t buf = 0;
-    for (uint32_t t = from; t < to; ++t) {
+    for (uint32_t t = cur.from; t < cur.to; ++t) {
       MXK_STEP(0, fa[0], fb[0], read_frag(buf, 1, i, fa[1], fb[1]))
       MXK_STEP(1, fa[1], fb[1], read_frag(buf, 2, i, fa[0], fb[0]))
       MXK_STEP(2, fa[0], fb[0], read_frag(buf, 3, i, fa[1], fb[1]))
-      if constexpr (COUNTED) {
-        wait_loads_if<STORES>(t == from ? stores_due : 0u);
-      } else {
-        wait_loads<0>();
-      }
+      wait_loads_if<BEHIND1>(t == cur.from ? behind : 0u);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       buf ^= 1u;
@@ -423,23 +463,13 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 
-    // the next tile's first two stages are under way while this one's result leaves
-    const int64_t m0 = lo, m1 = hi, c0 = n0;
-    T* const y0 = y;
-    id += gridDim.x;
-    const bool more = next_tile(id);
-    if (more) {
-#pragma unroll
-      for (int q = 0; q < F; ++q) issue(from, 0, q);
-#pragma unroll
-      for (int q = 0; q < F; ++q) issue(from + 1, 1, q);
-    }
-
     // The result through LDS, 32 rows of m and CB bytes of n at a time and
     // wave: a lane holds four consecutive n of one m; whole 64- or 128-byte
     // pieces of rows leave in 16-byte stores.
     uint8_t* mine = lds + 2 * BUF + 2 * SBUF + wave * 32 * CB;
-    const int64_t nw = c0 + (wave & 1) * NW, mw = m0 + (wave >> 1) * NW;
+    const int64_t nw = cur.n0 + (wave & 1) * NW, mw = cur.lo + (wave >> 1) * NW, m1 = cur.hi;
+    T* const y = cur.y;
+    if (more) advance();
     // the sums stay where they are until here: read earlier, they would push the loads' addresses into scratch
 #pragma unroll
     for (int i = 0; i < F; ++i)
@@ -449,7 +479,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
     const int64_t left = m1 - mw;
     const uint32_t pitch = (uint32_t)p.N * (uint32_t)sizeof(T);
     const __amdgpu_buffer_rsrc_t ry =
-        make_rsrc(y0 + mw * p.N, left <= 0 ? 0u : (uint32_t)(left < NW ? left : NW) * pitch);
+        make_rsrc(y + mw * p.N, left <= 0 ? 0u : (uint32_t)(left < NW ? left : NW) * pitch);
     uint32_t el = (uint32_t)lane;
     asm volatile("" : "+v"(el));  // the addresses below are not worth registers during the products
     const uint32_t col = (uint32_t)nw * (uint32_t)sizeof(T) + (el % CH) * 16u, out0 = (el / CH) * pitch + col;
@@ -458,6 +488,8 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
     for (int j = 0; j < F; ++j)
 #pragma unroll
       for (int s = 0; s < PASS; ++s) {
+        const int part = (j * PASS + s) / STEP;
+        if (more && (j * PASS + s) % STEP == 0 && part < 2 * F) issue(cur.from + part / F, part / F, part % F);
 #pragma unroll
         for (int u = 0; u < CC / 8; ++u) {
           const int iq = s * (CC / 8) + u, i = iq >> 2, q = iq & 3;
@@ -487,12 +519,12 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, const uint8
             __builtin_memcpy(t, &v[k], 16);
 #pragma unroll
             for (int q = 0; q < 16 / (int)sizeof(T); ++q)
-              if (n + q < p.N) y0[(mw + row) * p.N + n + q] = t[q];
+              if (n + q < p.N) y[(mw + row) * p.N + n + q] = t[q];
           }
         }
       }
     if (!more) return;
-    stores_due = whole ? 1u : 0u;
+    behind = whole ? 1u : 0u;
   }
 #undef MXK_STEP
 }
@@ -843,7 +875,8 @@ static Shape tile_of(const Fp4Gemm& p) {
 }
 static int64_t tile_bytes(const Fp4Gemm& p, const Shape& t) {
   const int64_t rows = p.offsets ? p.E * p.N : p.N;
-  return stage_bytes(p.M, p.KB) + stage_bytes(rows, p.KB) + (t.splits > 1 ? t.splits * p.M * p.N * 4 : 0);
+  const int64_t tables = p.offsets ? 16 * segment_slots(p.M, p.E, 64 * t.F) + 4 * p.M : 0;
+  return stage_bytes(p.M, p.KB) + stage_bytes(rows, p.KB) + tables + (t.splits > 1 ? t.splits * p.M * p.N * 4 : 0);
 }
 
 // Whether the kernel of few rows packs float x itself: a dense product of at
@@ -908,17 +941,23 @@ static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_byte
   const int64_t tn = ceil_div(p.N, B), n = ex && t.F ? block_tile_ids(slots, tn) : slots * tn * t.splits;
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many tiles");
   const int64_t b_rows = ex ? p.E * p.N : p.N, na = stage_bytes(p.M, p.KB), nb = stage_bytes(b_rows, p.KB);
+  Fp4Staged in = {};
   if (t.F) {
     if (!ws || !aligned16(ws) || ws_bytes < (size_t)tile_bytes(p, t))
       return fail(MXK_EINVAL, "mxfp4 product: workspace too small or not 16-byte aligned");
-    const int64_t ga = ceil_div(p.M, 32), gb = ceil_div(b_rows, 32);
-    if (ga + gb >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many rows");
-    hipLaunchKernelGGL(k_fp4_stage_scales, dim3((unsigned)(ga + gb)), dim3(256), 0, st, p, b_rows, ga, ws, ws + na);
+    const int64_t ga = ceil_div(p.M, 32), gb = ceil_div(b_rows, 32), gs = ex ? ceil_div(slots, 4) : 0;
+    if (ga + gb + gs >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many rows");
+    in.ta = ws;
+    in.tb = ws + na;
+    in.slot = reinterpret_cast<int4*>(ws + na + nb);
+    in.row = reinterpret_cast<int*>(in.slot + slots);
+    hipLaunchKernelGGL(k_fp4_stage, dim3((unsigned)(ga + gb + gs)), dim3(256), 0, st, p, in, b_rows, ga, gb, slots,
+                       (int)B);
   }
   const int64_t cus = (num_cus() + 7) & ~7;  // a multiple of the XCDs: a workgroup's tiles stay on its own
 #define MXK_TILE(T, F, EX, P)                                                                                        \
   hipLaunchKernelGGL((k_fp4_gemm_tile<T, F, EX>), dim3((unsigned)std::min<int64_t>(n, (F == 4 ? 1 : 2) * cus)),      \
-                     dim3(256), 0, st, P, ws, ws + na, b_rows, (uint32_t)slots, (uint32_t)tn, (uint32_t)t.splits, (uint32_t)n)
+                     dim3(256), 0, st, P, in, b_rows, (uint32_t)slots, (uint32_t)tn, (uint32_t)t.splits, (uint32_t)n)
 #define MXK_L(T, EX)                                                                                     \
   do {                                                                                                   \
     if (t.F == 4) MXK_TILE(T, 4, EX, p);                                                                 \
