@@ -24,11 +24,9 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 inline int64_t fp4_blocks(int64_t cols) { return (cols + 31) / 32; }
 
-// 2^(s - 127) as float32 (s = 0: the subnormal 2^-127; s = 255: NaN)
-__device__ __forceinline__ float e8m0_value(uint32_t s) {
-  const uint32_t b = max(s << 23, 0x00400000u);
-  return __uint_as_float(s == 255u ? 0x7FC00000u : b);
-}
+// Scale byte s as the conversions' scale operand, of which they read the
+// exponent field alone: 2^(s - 127), also for s = 0, and NaN for s = 255
+__device__ __forceinline__ float e8m0_operand(uint32_t s) { return __uint_as_float(s << 23); }
 
 // N elements of type T as the dwords that hold them
 template <typename T, int N>
@@ -88,7 +86,7 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t amax_bits) {
   return e == 255u ? 255u : max(e, 2u) - 2u;
 }
 
-// Codes of the N elements (N / 8 dwords) for scale s = e8m0_value(byte): the
+// Codes of the N elements (N / 8 dwords) for scale s = e8m0_operand(byte): the
 // conversion divides by the power of two, rounds to the nearest even code
 // and saturates at 6 (checked against the grid's midpoints)
 template <typename T, int N>

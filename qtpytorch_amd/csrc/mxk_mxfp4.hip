@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void k_fp4_quantize(const T* __restrict__ x, i
     // total is a multiple of 4: the lanes of a block are all in range or all out of it
     const uint32_t byte = fp4_scale_byte(group_max_u<4>(fp4_amax_bits(v[u])));
     uint32_t q[1];
-    fp4_codes(v[u], e8m0_value(byte), q);
+    fp4_codes(v[u], e8m0_operand(byte), q);
     if (i < total) {
       codes[i] = byte == 255u ? 0u : q[0];
       if ((threadIdx.x & 3u) == 0u) scales[i >> 2] = (uint8_t)byte;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void k_fp4_dequantize(const uint32_t* __restri
   for (int u = 0; u < U; ++u) {
     const uint64_t i = first + 256u * u;
     if (i >= total) continue;
-    const float f = e8m0_value(s[u]);
+    const float f = e8m0_operand(s[u]);
     FpWords<T, 8> o;
     if constexpr (__is_same(T, hip_bfloat16)) {
       o.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[u], f, 0));

@@ -752,7 +752,7 @@ __global__ __launch_bounds__(1024) void k_fp4_few(Fp4Gemm p) {
           for (int k = 0; k < 4; ++k) {
             byte[k] = fp4_scale_byte(group_max_u<4>(fp4_amax_bits(v[t][k])));
             uint32_t q[1];
-            fp4_codes(v[t][k], e8m0_value(byte[k]), q);
+            fp4_codes(v[t][k], e8m0_operand(byte[k]), q);
             a[k] = byte[k] == 255u ? 0u : q[0];
           }
           // out[d] of lane k = a[k] of lane d (lanes of four), one bit of the two at a time

@@ -13,6 +13,8 @@
 // continue one after the other.
 #include "mxk_mxfp4.h"
 
+#include <type_traits>
+
 namespace mxk {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -93,10 +95,12 @@ struct Fp4Grad {
 // take 8 consecutive rows, the transposing writes every eighth row.
 template <typename O, int F, bool OF_B>
 __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uint32_t tn) {
-  constexpr int B = 64 * F, OP = B * 128, BUF = 2 * OP;
+  // LDS: L of either buffer, then V of either, so that a buffer and a fragment
+  // are an immediate offset
+  constexpr int B = 64 * F, OP = B * 128;
   constexpr int NW = 32 * F, CB = F == 4 ? 128 : 64;
   constexpr int CH = CB / 16, CC = CB / (int)sizeof(O), PASS = NW / CC;
-  __shared__ __align__(16) uint8_t lds[2 * BUF];
+  __shared__ __align__(16) uint8_t lds[4 * OP];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
   uint32_t it, jt;
@@ -172,24 +176,31 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
       for (int k = q * B / 64; k < (q + 1) * B / 64; ++k) lw[k] = buf_load_b128(rl, (ld_off + k * 32u * pitch) | far, 0);
     }
   };
-  auto put = [&](uint32_t base, int row, int c, u32x4 w) {
-    *reinterpret_cast<u32x4*>(lds + base + row * 128 + ((c ^ (row & 7) ^ ((row >> 3) & 7)) << 4)) = w;
-  };
+  // where this thread's rows of LDS are: chunk tg of rows 8 g8 + k of a
+  // transposed operand, chunk tid % 8 of rows tid / 8 + 32 k of a copied one
+  // (those with k even and odd differ by 4 in bits 3 .. 5 of the row)
+  uint8_t* put_t[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) put_t[k] = lds + (8 * g8 + k) * 128 + ((tg ^ k ^ (g8 & 7)) << 4);
+  uint8_t* put_c[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    put_c[k] = lds + (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7) ^ (((tid >> 6) + 4 * k) & 7)) << 4);
   // two LDS rows of the transpose of an 8 x 8 block of 16-bit values: low and high halves of eight pairs
-  auto put_pairs = [&](uint32_t base, int q, const uint32_t (&a)[8]) {
+  auto put_pairs = [&](int base, int q, const uint32_t (&a)[8]) {
     u32x4 lo, hi;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       lo[k] = __builtin_amdgcn_perm(a[2 * k + 1], a[2 * k], 0x05040100u);
       hi[k] = __builtin_amdgcn_perm(a[2 * k + 1], a[2 * k], 0x07060302u);
     }
-    put(base, 8 * g8 + 2 * q, tg, lo);
-    put(base, 8 * g8 + 2 * q + 1, tg, hi);
+    *reinterpret_cast<u32x4*>(put_t[2 * q] + base) = lo;
+    *reinterpret_cast<u32x4*>(put_t[2 * q + 1] + base) = hi;
   };
 #define MXK_VPAIR(k, q) \
-  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[k], e8m0_value(vsc[k]), q))
+  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[k], e8m0_operand(vsc[k]), q))
   // quarter q of the staged V, of the staged L
-  auto stage_v = [&](uint32_t buf, int q) {
+  auto stage_v = [&](int buf, int q) {
     if (!does_v) return;
     uint32_t a[8];
 #pragma unroll
@@ -199,18 +210,19 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
       else if (q == 2) a[k] = MXK_VPAIR(k, 2);
       else a[k] = MXK_VPAIR(k, 3);
     }
-    put_pairs(buf * BUF + OP, q, a);
+    put_pairs((2 + buf) * OP, q, a);
   };
-  auto stage_l = [&](uint32_t buf, int q) {
+  auto stage_l = [&](int buf, int q) {
     if constexpr (OF_B) {
       if (!does_lt) return;
       uint32_t a[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) a[k] = lw[k][q];
-      put_pairs(buf * BUF, q, a);
+      put_pairs(buf * OP, q, a);
     } else {
 #pragma unroll
-      for (int k = q * B / 128; k < (q + 1) * B / 128; ++k) put(buf * BUF, (tid >> 3) + 32 * k, tid & 7, lw[k]);
+      for (int k = q * B / 128; k < (q + 1) * B / 128; ++k)
+        *reinterpret_cast<u32x4*>(put_c[k & 1] + buf * OP + 4096 * k) = lw[k];
     }
   };
 
@@ -223,12 +235,18 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
   bf16x8 fa[2][F], fb[2][F];
-  auto read_frag = [&](uint32_t buf, int s, int i, bf16x8 (&xa)[F], bf16x8 (&xb)[F]) {
-    // row 32 i + ra: its bits 3 .. 5 change with i by 4 (i & 1)
-    const int c = 2 * s + h;
-    const int xra = (ra & 7) ^ (((ra >> 3) + 4 * i) & 7), xrb = (rb & 7) ^ (((rb >> 3) + 4 * i) & 7);
-    xa[i] = *reinterpret_cast<const bf16x8*>(lds + buf * BUF + (ra + 32 * i) * 128 + ((c ^ xra) << 4));
-    xb[i] = *reinterpret_cast<const bf16x8*>(lds + buf * BUF + OP + (rb + 32 * i) * 128 + ((c ^ xrb) << 4));
+  // chunk 2 s + h of rows ra + 32 i; bits 3 .. 5 of the row change with i by 4 (i & 1)
+  const uint8_t *get_l[4], *get_v[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    get_l[s] = lds + ra * 128 + (((2 * s + h) ^ (ra & 7) ^ ((ra >> 3) & 7)) << 4);
+    get_v[s] = lds + 2 * OP + rb * 128 + (((2 * s + h) ^ (rb & 7) ^ ((rb >> 3) & 7)) << 4);
+  }
+  auto read_frag = [&](int buf, int s, int i, bf16x8 (&xa)[F], bf16x8 (&xb)[F]) {
+    // chunk c ^ 4 is that of step s ^ 2
+    const int at = i & 1 ? s ^ 2 : s;
+    xa[i] = *reinterpret_cast<const bf16x8*>(get_l[at] + buf * OP + i * 4096);
+    xb[i] = *reinterpret_cast<const bf16x8*>(get_v[at] + buf * OP + i * 4096);
   };
   // A row of F MFMAs and what is issued between them: the conversions of a
   // stage (some 240 VALU a wave) fit into the MFMAs' shadows only if they
@@ -265,15 +283,16 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < F; ++i) read_frag(0, 0, i, fa[0], fb[0]);
-    uint32_t buf = 0;
-    for (uint32_t s = 0; s < stages; ++s) {
+    // two stages a turn, one in each buffer; where their number is odd the last one's operands are zeros
+    auto stage = [&](auto which, uint32_t s) {
+      constexpr int buf = decltype(which)::value;
       MXK_STEP(fa[0], fb[0], {
         read_frag(buf, 1, i, fa[1], fb[1]);
-        _Pragma("unroll") for (int q = i * Q; q < (i + 1) * Q; ++q) stage_v(buf ^ 1u, q);
+        _Pragma("unroll") for (int q = i * Q; q < (i + 1) * Q; ++q) stage_v(buf ^ 1, q);
       })
       MXK_STEP(fa[1], fb[1], {
         read_frag(buf, 2, i, fa[0], fb[0]);
-        _Pragma("unroll") for (int q = i * Q; q < (i + 1) * Q; ++q) stage_l(buf ^ 1u, q);
+        _Pragma("unroll") for (int q = i * Q; q < (i + 1) * Q; ++q) stage_l(buf ^ 1, q);
       })
       MXK_STEP(fa[0], fb[0], {
         read_frag(buf, 3, i, fa[1], fb[1]);
@@ -282,8 +301,11 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      buf ^= 1u;
-      MXK_STEP(fa[1], fb[1], read_frag(buf, 0, i, fa[0], fb[0]))
+      MXK_STEP(fa[1], fb[1], read_frag(buf ^ 1, 0, i, fa[0], fb[0]))
+    };
+    for (uint32_t s = 0; s < stages; s += 2) {
+      stage(std::integral_constant<int, 0>(), s);
+      stage(std::integral_constant<int, 1>(), s + 1);
     }
   }
 #undef MXK_STEP
