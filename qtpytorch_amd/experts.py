@@ -17,6 +17,7 @@ from typing import NamedTuple, Optional, Union
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .microscale import (_FLOATS, _bias_f32, _check_linear, _grad_a, _grad_b, _grad_bias, _linear, _pack_weight, _product,
@@ -117,6 +118,7 @@ class _ExpertGather(torch.autograd.Function):
         return _gather(x, plan)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         return _combine(dy, expert_plan(*ctx.saved_tensors), None), None
 
@@ -129,6 +131,7 @@ class _ExpertCombine(torch.autograd.Function):
         return _combine(h, plan, gates)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         h, gates, *plan = ctx.saved_tensors
         plan = expert_plan(*plan)
@@ -189,6 +192,7 @@ class _ExpertLinear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         bc, bs, ac, as_, *plan = ctx.saved_tensors
         plan = expert_plan(*plan)
@@ -196,11 +200,11 @@ class _ExpertLinear(torch.autograd.Function):
         dy = dy.contiguous()
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
-            dx = _grad_a(dy, mxfp4_tensor(bc, bs, b_shape), x_dtype, plan.offsets)
+            dx = _grad_a(dy, mxfp4_tensor._of(bc, bs, b_shape), x_dtype, plan.offsets)
             if gather:
                 dx = _combine(dx, plan, None)
         if ctx.needs_input_grad[1]:
-            a = mxfp4_quantize(_gather(ac, plan)) if gather else mxfp4_tensor(ac, as_, a_shape)
+            a = mxfp4_quantize(_gather(ac, plan)) if gather else mxfp4_tensor._of(ac, as_, a_shape)
             dw = _grad_b(dy, a, w_dtype, plan.offsets)
         if ctx.needs_input_grad[2]:
             db = _grad_bias(dy, bias_dtype, plan.offsets)

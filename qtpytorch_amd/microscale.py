@@ -23,6 +23,7 @@ import math
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -263,12 +264,13 @@ class _MXFP4Linear(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         bc, bs, ac, as_ = ctx.saved_tensors
         a_shape, b_shape, x_dtype, w_dtype, bias_dtype = ctx.sizes
         dy = dy.contiguous()
-        dx = _grad_a(dy, mxfp4_tensor(bc, bs, b_shape), x_dtype) if ctx.needs_input_grad[0] else None
-        dw = _grad_b(dy, mxfp4_tensor(ac, as_, a_shape), w_dtype) if ctx.needs_input_grad[1] else None
+        dx = _grad_a(dy, mxfp4_tensor._of(bc, bs, b_shape), x_dtype) if ctx.needs_input_grad[0] else None
+        dw = _grad_b(dy, mxfp4_tensor._of(ac, as_, a_shape), w_dtype) if ctx.needs_input_grad[1] else None
         db = _grad_bias(dy, bias_dtype) if ctx.needs_input_grad[2] else None
         return dx, dw, db, None
 

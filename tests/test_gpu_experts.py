@@ -249,6 +249,98 @@ def test_expert_mlp(tokens):
     assert float((y[0].detach().cpu().double() - want).norm() / want.norm()) < 5e-3
 
 
+def test_rows_past_2_31_elements():
+    """Gather, combine and the gradients of rows whose offsets pass 32 bits."""
+    import qtpytorch_amd as qa
+    tokens, top, cols = 70000, 4, 8192
+    g = torch.Generator(device="cuda").manual_seed(0)
+    ids = torch.randint(0, 16, (tokens, top), device="cuda", generator=g)
+    plan = qa.expert_sort(ids, 16)
+    x = torch.empty(tokens, cols, dtype=torch.bfloat16, device="cuda").normal_(generator=g).requires_grad_()
+    y = qa.expert_gather(x, plan)
+    assert y.numel() > 1 << 31
+    pick = torch.tensor([0, 1, 262143, 262144, 279998, 279999], device="cuda")
+    assert torch.equal(y[pick], x[(plan.order[pick] // top).long()])
+    gates = torch.rand(tokens, top, device="cuda", generator=g).requires_grad_()
+    z = qa.expert_combine(y, plan, gates)
+    tok = torch.tensor([0, 3, 65535, 65536, 69999], device="cuda")
+    rows = y.detach()[plan.place[tok].long()].float()
+    assert torch.equal(z[tok], (gates[tok, :, None] * rows).sum(1).bfloat16()) or \
+        float((z[tok].float() - (gates[tok, :, None] * rows).sum(1)).norm() / z[tok].float().norm()) < 4e-3
+    dy = torch.empty_like(z).normal_(generator=g)
+    dx, dg = torch.autograd.grad(z, (x, gates), dy)
+    dots = (rows * dy[tok, None].float()).sum(-1)
+    assert float((dg[tok] - dots).norm() / dots.norm()) < 1e-4
+    # every row of a token is the token itself: its gradient is dy times the sum of its gates, each part rounded once
+    ref = dy[tok].float() * gates.detach()[tok].sum(1, keepdim=True)
+    assert float((dx[tok].float() - ref).norm() / ref.norm()) < 6e-3
+
+
+def test_no_tokens():
+    """A batch without tokens, and one whose picks are all other devices': empty or zero results and gradients."""
+    import qtpytorch_amd as qa
+    w = torch.randn(4, 48, 64, generator=_gen(1)).cuda().requires_grad_()
+    for ids in (torch.zeros(0, 2, dtype=torch.int64), torch.full((5, 2), -1)):
+        plan = _plan(ids, 4)
+        x = torch.randn(ids.shape[0], 64, generator=_gen(2)).cuda().requires_grad_()
+        gates = torch.ones(ids.shape, device="cuda", requires_grad=True)
+        y = qa.expert_combine(qa.expert_linear(x, w, plan, gather=True), plan, gates)
+        z = qa.expert_linear(qa.expert_gather(x, plan), w, plan)
+        assert y.shape == (ids.shape[0], 48) and z.shape == (ids.numel(), 48)
+        assert not y.any() and not z.any()
+        grads = torch.autograd.grad(y.sum() + z.sum(), (x, w, gates))
+        assert all(g.shape == t.shape and not g.any() for g, t in zip(grads, (x, w, gates)))
+
+
+def test_gradients_of_gradients_are_refused():
+    import qtpytorch_amd as qa
+    plan = _plan(_ids(6, 2, 4), 4)
+    x = torch.randn(6, 64, generator=_gen(1)).cuda().requires_grad_()
+    w = torch.randn(4, 32, 64, generator=_gen(2)).cuda().requires_grad_()
+    y = qa.expert_combine(qa.expert_linear(qa.expert_gather(x, plan), w, plan), plan)
+    (dx,) = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+# ---------------------------------------------------------------- graphs
+@pytest.mark.parametrize("tokens", [1, 12, 200])
+def test_expert_layer_in_a_graph(tokens):
+    """Replays of a captured layer and its gradient, with eager work in between, against eager calls bit for bit."""
+    import qtpytorch_amd as qa
+    E, D, F, top = 8, 256, 128, 2
+    g = _gen(0)
+    layer = qa.mxfp4_expert_mlp(torch.randn(E, D, generator=g).cuda(), (torch.randn(E, 2 * F, D, generator=g) * 0.1).cuda(),
+                                (torch.randn(E, D, F, generator=g) * 0.1).cuda(), top)
+    w = (torch.randn(D, D, generator=g) * 0.05).bfloat16().cuda().requires_grad_()
+    x = torch.zeros(tokens, D, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    dy = torch.zeros(tokens, D, device="cuda", dtype=torch.bfloat16)
+
+    def step():
+        with torch.no_grad():
+            routed = layer(x)
+        y = qa.mxfp4_linear(x, w)
+        return (routed, y.detach(), *torch.autograd.grad(y, (x, w), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(tokens, D, generator=_gen(10 + i)))
+            dy.copy_(torch.randn(tokens, D, generator=_gen(20 + i)))
+        graph.replay()
+        got = [t.clone() for t in out]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     import qtpytorch_amd as qa

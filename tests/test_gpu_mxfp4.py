@@ -268,7 +268,7 @@ def test_gradient_is_the_slope_between_representable_points():
     for m, k in ((0, 1), (1, 40), (2, 63)):
         moved = x.clone()
         moved[m, k] = 3.0
-        step = (qa.mxfp4_linear(moved.cuda(), w).double() - y.double()).mul(dy.double()).sum()
+        step = (qa.mxfp4_linear(moved.cuda(), w).double() - y.detach().double()).mul(dy.double()).sum()
         assert abs(float(step) - float(dx[m, k])) <= 2e-5 * (1 + abs(float(step)))
 
 
@@ -296,6 +296,80 @@ def test_gradient_of_a_strided_output_gradient():
     R.assert_close(dx, d @ rw, d.abs() @ rw.abs(), 8)
     (dx,) = torch.autograd.grad(qa.mxfp4_linear(x, held).sum(), x)  # a broadcast gradient of ones
     R.assert_close(dx, rw.sum(0).expand(10, 96), rw.abs().sum(0).expand(10, 96), 8)
+
+
+def test_product_of_views_that_start_anywhere():
+    """Codes and scales at odd addresses of larger buffers, as a loaded checkpoint has them."""
+    import qtpytorch_amd as qa
+    for M, N, K in ((9, 100, 544), (40, 70, 96), (300, 200, 1056)):
+        a, b, qa_, qb = _operands(M, N, K)
+        held = []
+        for q in (qa_, qb):
+            codes, scales = torch.zeros(q.codes.numel() + 3, dtype=torch.uint8).cuda(), \
+                torch.zeros(q.scales.numel() + 1, dtype=torch.uint8).cuda()
+            codes[3:].copy_(q.codes.view(-1))
+            scales[1:].copy_(q.scales.view(-1))
+            held.append(qa.mxfp4_tensor(codes[3:].view(q.codes.shape), scales[1:].view(q.scales.shape), q.shape))
+        want = qa.mxfp4_matmul(qa_, qb, out_dtype=torch.float32)
+        assert torch.equal(qa.mxfp4_matmul(*held, out_dtype=torch.float32), want)
+        y = torch.randn(M, N, generator=_gen(3)).cuda()
+        x = a.cuda().requires_grad_()
+        d0, = torch.autograd.grad(qa.mxfp4_linear(x, qb), x, y)
+        d1, = torch.autograd.grad(qa.mxfp4_linear(x, held[1]), x, y)
+        assert torch.equal(d0, d1)
+
+
+def test_tensor_moves_and_sizes():
+    import qtpytorch_amd as qa
+    q = qa.mxfp4_quantize(torch.randn(6, 70).cuda())
+    assert q.shape == (6, 70) and q.dim() == 2 and q.nbytes == 6 * 3 * 17 and "6, 70" in repr(q)
+    back = q.to("cpu").to("cuda")
+    assert torch.equal(back.dequantize(), q.dequantize())
+    with pytest.raises(qa._lib.MXKError):
+        q.to("cpu").dequantize()
+
+
+# ---------------------------------------------------------------- offsets past 32 bits
+def _random_packed(shape, seed):
+    """A packed tensor of random codes and scales from 2^-7 to 2^7, made on the GPU."""
+    import qtpytorch_amd as qa
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kb = -(-shape[-1] // 32)
+    codes = torch.randint(0, 256, (*shape[:-1], 16 * kb), dtype=torch.uint8, device="cuda", generator=g)
+    scales = torch.randint(120, 135, (*shape[:-1], kb), dtype=torch.uint8, device="cuda", generator=g)
+    return qa.mxfp4_tensor(codes, scales, shape)
+
+
+def test_quantize_of_more_than_2_31_elements():
+    import qtpytorch_amd as qa
+    rows, cols = 70001, 32768 + 64
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    q = qa.mxfp4_quantize(x)
+    y = q.dequantize(torch.bfloat16)
+    for lo in (0, 65530, rows - 3):
+        part = qa.mxfp4_quantize(x[lo:lo + 3])
+        assert torch.equal(q.codes[lo:lo + 3], part.codes) and torch.equal(q.scales[lo:lo + 3], part.scales)
+        assert torch.equal(y[lo:lo + 3], part.dequantize(torch.bfloat16))
+
+
+@pytest.mark.parametrize("rows", [3, 40, 400])
+def test_experts_of_more_than_2_31_bytes(rows):
+    """The last of many large experts: its product and its input's gradient are those of its weight alone."""
+    import qtpytorch_amd as qa
+    E, N, K = 40, 16384, 8192
+    w = _random_packed((E, N, K), 1)
+    assert w.codes.numel() > 1 << 31
+    ids = torch.full((rows, 1), E - 1, device="cuda")
+    plan = qa.expert_sort(ids, E)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(rows, K, device="cuda", generator=g).bfloat16().requires_grad_()
+    alone = qa.mxfp4_tensor(w.codes[-1], w.scales[-1], (N, K))
+    y, z = qa.expert_linear(x, w, plan, gather=True), qa.mxfp4_linear(x, alone)
+    dy = torch.randn(rows, N, device="cuda", generator=g).bfloat16()
+    # the kernels may differ in the order of their sums
+    assert float((y.detach().double() - z.detach().double()).norm() / z.detach().double().norm()) < 1e-3
+    dx, dz = torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(z, x, dy)[0]
+    assert float((dx.double() - dz.double()).norm() / dz.double().norm()) < 1e-3
 
 
 # ---------------------------------------------------------------- refusals
