@@ -50,11 +50,12 @@ def expert_sort(ids: Tensor, n_experts: int) -> expert_plan:
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"expert_sort: ids are int32 or int64, got {ids.dtype}")
     dev = L.require_gpu(ids)
-    ids = ids.contiguous()
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
     P = ids.numel()
-    order = torch.empty(P, dtype=torch.int32, device=dev)
-    place = torch.empty(ids.shape, dtype=torch.int32, device=dev)
-    offsets = torch.empty(n_experts + 1 if n_experts > 0 else 1, dtype=torch.int32, device=dev)
+    place = torch.empty_like(ids, dtype=torch.int32)
+    order = torch.empty((P,), dtype=torch.int32, device=dev)
+    offsets = torch.empty((max(n_experts, 0) + 1,), dtype=torch.int32, device=dev)
     lib = L.lib()
     nbytes = lib.mxk_expert_sort_workspace(P, n_experts)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
@@ -86,28 +87,32 @@ def _float_rows(name: str, x: Tensor, rows: int, what: str) -> None:
 
 
 def _gather(x: Tensor, plan: expert_plan) -> Tensor:
-    dev = L.require_gpu(x, *plan)
+    order = plan.order
+    dev = L.require_gpu(x, order)
     x = _row_major(x)
     tokens, top = plan.place.shape
-    out = torch.empty((tokens * top, x.shape[1]), dtype=x.dtype, device=dev)
+    cols = x.shape[1]
+    out = torch.empty((tokens * top, cols), dtype=x.dtype, device=dev)
     with L.on_device(dev):
-        rc = L.lib().mxk_expert_gather(x.data_ptr(), x.element_size(), tokens, x.shape[1], x.stride(0),
-                                       plan.order.data_ptr(), tokens * top, top, out.data_ptr(), L.stream_of(x))
+        rc = L.lib().mxk_expert_gather(x.data_ptr(), x.element_size(), tokens, cols, x.stride(0), order.data_ptr(),
+                                       tokens * top, top, out.data_ptr(), L.stream_of(out))
     if rc:
-        L.check(rc, f"expert_gather({tokens}x{x.shape[1]}, top {top})")
+        L.check(rc, f"expert_gather({tokens}x{cols}, top {top})")
     return out
 
 
 def _combine(h: Tensor, plan: expert_plan, gates: Optional[Tensor]) -> Tensor:
-    dev = L.require_gpu(h, gates, *plan)
+    place = plan.place
+    dev = L.require_gpu(h, gates, place)
     h = h.contiguous()
-    tokens, top = plan.place.shape
-    y = torch.empty((tokens, h.shape[1]), dtype=h.dtype, device=dev)
+    tokens, top = place.shape
+    rows, cols = h.shape
+    y = torch.empty((tokens, cols), dtype=h.dtype, device=dev)
     with L.on_device(dev):
-        rc = L.lib().mxk_expert_combine(h.data_ptr(), L.elem_type(h.dtype), h.shape[0], plan.place.data_ptr(),
-                                        L.ptr(gates), tokens, top, h.shape[1], y.data_ptr(), L.stream_of(h))
+        rc = L.lib().mxk_expert_combine(h.data_ptr(), _FLOATS[h.dtype], rows, place.data_ptr(), L.ptr(gates), tokens,
+                                        top, cols, y.data_ptr(), L.stream_of(y))
     if rc:
-        L.check(rc, f"expert_combine({tokens}x{h.shape[1]}, top {top})")
+        L.check(rc, f"expert_combine({tokens}x{cols}, top {top})")
     return y
 
 
@@ -138,7 +143,7 @@ class _ExpertCombine(torch.autograd.Function):
         dy = dy.contiguous()
         if gates is None:
             return _gather(dy, plan), None, None
-        dev = L.require_gpu(dy, h)
+        dev = L.require_gpu(dy, h, gates, *plan)
         tokens, top = plan.place.shape
         dh, dg = torch.empty_like(h), torch.empty_like(gates)
         with L.on_device(dev):
@@ -157,7 +162,9 @@ def expert_gather(x: Tensor, plan: expert_plan) -> Tensor:
     the sum of its rows' (in float32, by ascending pick)."""
     _check_plan("expert_gather", plan)
     _float_rows("expert_gather", x, plan.place.shape[0], "one row per token")
-    return _ExpertGather.apply(x, plan) if _wants_grad(x) else _gather(x, plan)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _ExpertGather.apply(x, plan)
+    return _gather(x, plan)
 
 
 def expert_combine(h: Tensor, plan: expert_plan, gates: Optional[Tensor] = None) -> Tensor:
@@ -171,7 +178,7 @@ def expert_combine(h: Tensor, plan: expert_plan, gates: Optional[Tensor] = None)
         if gates.shape != plan.place.shape:
             raise ValueError(f"expert_combine: gates {tuple(plan.place.shape)} expected, got {tuple(gates.shape)}")
         gates = gates.float().contiguous()
-    if _wants_grad(h, gates):
+    if (h.requires_grad or gates is not None and gates.requires_grad) and torch.is_grad_enabled():
         return _ExpertCombine.apply(h, gates, plan)
     return _combine(h, plan, gates)
 

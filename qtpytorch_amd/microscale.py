@@ -280,14 +280,16 @@ def _check_linear(name: str, x: Tensor, weight, dims: int) -> None:
         raise TypeError(f"{name}: x is float32, float16 or bfloat16, got {x.dtype}")
     if not isinstance(weight, mxfp4_tensor) and weight.dtype not in _FLOATS:
         raise TypeError(f"{name}: the weight is an mxfp4_tensor or a float tensor, got {weight.dtype}")
-    if weight.dim() != dims or x.dim() < 1 or x.shape[-1] != weight.shape[-1]:
+    shape = weight.shape
+    if len(shape) != dims or x.dim() < 1 or x.shape[-1] != shape[-1]:
         want = "[N, K]" if dims == 2 else "[E, N, K]"
         raise ValueError(f"{name}: x [..., K] and a weight {want} expected, got {tuple(x.shape)} and "
                          f"{tuple(weight.shape)}")
 
 
-def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in ts)
+def _wants_grad(x: Tensor, weight, bias: Optional[Tensor]) -> bool:
+    return (x.requires_grad or bias is not None and bias.requires_grad
+            or not isinstance(weight, mxfp4_tensor) and weight.requires_grad) and torch.is_grad_enabled()
 
 
 def mxfp4_linear(x: Tensor, weight: Union[Tensor, mxfp4_tensor], bias: Optional[Tensor] = None) -> Tensor:
