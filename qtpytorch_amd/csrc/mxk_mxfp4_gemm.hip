@@ -534,7 +534,9 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
 // over its waves in chunks of 512 and the waves' sums added through LDS in
 // their order.
 //
-// Bound by HBM (17/32 byte per weight, each read once).  A wave requests its
+// Bound by HBM (17/32 byte per weight, each read once): 16x8192x8192 with x in
+// bf16 12.3 us, packed 9.6 (3.8 TB/s of weights), 8 tokens to 4 of 32 experts
+// of 4096x4096 29 us (5.6 TB/s of the busy experts').  A wave requests its
 // chunk of a tile of b, 256 bytes a row, straight into LDS of its own, in
 // whole lines (lanes of an MFMA operand lie in different rows: read in that
 // order, each lane's 16 bytes would be a request by itself, 64 a wave
@@ -551,7 +553,7 @@ template <typename X> struct IsPacked { static constexpr bool V = false; };
 template <> struct IsPacked<uint8_t> { static constexpr bool V = true; };
 
 template <typename X, typename T, int MT, int NT, bool EXPERT>
-__global__ __launch_bounds__(1024) void k_fp4_few(Fp4Gemm p) {
+__global__ __launch_bounds__(MT > 2 ? 512 : 1024) void k_fp4_few(Fp4Gemm p) {
   constexpr bool PACKED = IsPacked<X>::V;
   constexpr int OWN = NT > 1 ? 8192 : 4096;           // bytes of LDS of a wave: two tiles, or the only one
   extern __shared__ __align__(16) uint8_t few_lds[];  // then the sums: [waves][MT * NT][64][4] floats
@@ -620,10 +622,13 @@ __global__ __launch_bounds__(1024) void k_fp4_few(Fp4Gemm p) {
     return p.bs + ((int64_t)e * p.N + (n < p.N ? n : p.N - 1)) * KB;
   };
   uint32_t bw[2][4];
-  // requests of a tile: 4 loads into LDS and, in whole chunks, one of scales
+  // requests of a tile: in whole chunks one load of scales, then 4 into LDS, in
+  // that order, which the waits below count on
   auto request = [&](int chunk, int i) {
-    fetch_b(chunk, i);
     load_scales(scales_of(i), chunk, bw[i & 1]);
+    asm volatile("" ::: "memory");
+    fetch_b(chunk, i);
+    asm volatile("" ::: "memory");
   };
   // the products of a chunk, once its first two tiles are requested
   auto multiply = [&](int chunk, const u32x4 (&xc)[MT][4], const uint32_t (&xs)[MT]) {
@@ -839,14 +844,23 @@ __global__ __launch_bounds__(256) void k_fp4_join(const float* __restrict__ part
 }
 
 // Bytes of the scales of `rows` rows in stage order, with room for the last tile's reads past the end
-static int64_t stage_bytes(int64_t rows, int64_t KB) { return ceil_div(KB, 8) * rows * 8 + 4096; }
+static int64_t stage_bytes(int64_t rows, int64_t KB) { return ceil_div(ceil_div(KB, 8) * rows, 2) * 16 + 4096; }
 
-// Tiles of 16 rows of k_fp4_few for a problem (0: another kernel): the rows
-// of a dense product, the rows an expert has on average
+// Tiles of 16 rows of k_fp4_few for a problem (0: another kernel).  Dense:
+// while one set of tiles holds every row, so that b is read once (64x8192x8192
+// 17.7 us against the tile kernel's 19.5, 64x4096x4096 9.2 against 13.4,
+// 32x8192x8192 12.7 against 18.3; two sets of 64 rows, 128x8192x8192: 33
+// against 22).  By expert the rows of one are known on average only, and those
+// above a set read the expert again: 32 experts of 4096x4096 with 16 rows each
+// 72 us against 86, with 25 rows 84 against 88, with 32 rows 108 against 91; one
+// tile of rows is best to 16 (12 rows 58 us, with two tiles 68).
 static int few_of(const Fp4Gemm& p) {
-  if (p.KB == 0 || p.KB > (1 << 18)) return 0;  // 32 rows of b in a buffer of at most 2^30 bytes
-  const int64_t rows = p.offsets ? ceil_div(p.M, p.E) : p.M;
-  return rows <= 16 ? 1 : (rows <= 32 ? 2 : 0);
+  if (p.KB == 0 || p.KB > (1 << 18)) return 0;  // 64 rows of b in a buffer of at most 2^28 bytes
+  if (p.offsets) {
+    const int64_t rows = ceil_div(p.M, p.E);
+    return rows <= 16 ? 1 : (rows <= 24 ? 2 : 0);
+  }
+  return p.M <= 16 ? 1 : (p.M <= 32 ? 2 : (p.M <= 64 ? 4 : 0));
 }
 
 // The tile kernel's shape for a problem: fragments a side of its waves (0:
@@ -856,7 +870,7 @@ struct Shape {
 };
 static Shape tile_of(const Fp4Gemm& p) {
   const int64_t row_bytes = p.KB * 16;
-  if (p.KB == 0 || few_of(p) || p.N < 64 || row_bytes > (1 << 22)) return {0, 1};
+  if (p.KB == 0 || few_of(p) || row_bytes > (1 << 22)) return {0, 1};
   if (p.order && p.a_rows * row_bytes > ((int64_t)1 << 30)) return {0, 1};
   if (p.N >= ((int64_t)1 << 21)) return {0, 1};  // 256 rows of 4-byte results within 2^31 bytes
   auto tiles = [&](int B) { return (p.offsets ? segment_slots(p.M, p.E, B) : ceil_div(p.M, B)) * ceil_div(p.N, B); };
@@ -897,10 +911,10 @@ static int launch_few_t(const Fp4Gemm& p, hipStream_t st) {
   const bool ex = p.offsets != nullptr;
   const int64_t n = (ex ? segment_slots(p.M, p.E, 16 * MT) : ceil_div(p.M, 16 * MT)) * ceil_div(p.N, 16 * NT);
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many tiles");
-  const int waves = (int)std::min<int64_t>(16, ceil_div(p.KB, 16));
+  const int waves = (int)std::min<int64_t>(MT > 2 ? 8 : 16, ceil_div(p.KB, 16));
   const size_t own = NT > 1 ? 8192 : 4096, sums = MT * NT * 1024;
   const size_t lds = waves * std::max(own, sums);
-  if constexpr (IsPacked<X>::V) {
+  if constexpr (IsPacked<X>::V && MT < 4) {
     if (ex) {
       hipLaunchKernelGGL((k_fp4_few<X, T, MT, NT, true>), dim3((unsigned)n), dim3(64 * waves), lds, st, p);
       return check_launch("mxfp4 product of few rows by expert");
@@ -925,6 +939,7 @@ static int launch_few_n(const Fp4Gemm& p, hipStream_t st) {
 template <typename T>
 static int launch_few_packed(const Fp4Gemm& p, int mt, hipStream_t st) {
   if (mt == 1) return launch_few_n<uint8_t, T, 1>(p, st);
+  if (mt == 4) return launch_few_n<uint8_t, T, 4>(p, st);
   return launch_few_n<uint8_t, T, 2>(p, st);
 }
 

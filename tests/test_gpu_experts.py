@@ -168,6 +168,13 @@ def test_expert_linear(tokens, top, experts, n, k, dropped, skew, gather, dtype)
     assert not y[int(offsets[-1]):].any()
 
 
+@pytest.mark.parametrize("tokens", [33, 34, 48, 50, 64])
+@pytest.mark.parametrize("n,k", [(17, 100), (130, 1056)])
+def test_expert_linear_of_16_to_32_rows_an_expert(tokens, n, k):
+    test_expert_linear(tokens, 2, 4, n, k, 0.1, 0.5, True, torch.float32)
+    test_expert_linear(tokens, 2, 4, n, k, 0.0, 0.0, False, torch.bfloat16)
+
+
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("gather", [True, False])
 @pytest.mark.parametrize("tokens,top,experts,n,k,dropped,skew", [c for c in EXPERT_CASES if c[2] < 100])

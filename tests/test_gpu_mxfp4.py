@@ -129,6 +129,24 @@ def test_product(shape, out):
     R.assert_close(y, ra @ rb.t(), ra.abs() @ rb.abs().t(), K / 32 + 2)
 
 
+@pytest.mark.parametrize("shape", [(33, 1, 1024), (34, 8208, 512), (49, 300, 4128), (64, 33, 8224), (64, 8193, 96), (65, 5, 3000),
+                                   (400, 1, 2080), (1000, 63, 96), (65, 8193, 64)])
+def test_product_of_33_to_64_rows_and_of_narrow_weights(shape):
+    test_product(shape, torch.float32)
+    test_product(shape, torch.bfloat16)
+
+
+def test_product_of_more_columns_than_a_tile_can_store_by_32_bits():
+    import qtpytorch_amd as qa
+    M, N, K = 65, (1 << 21) + 3, 64
+    a, b = _data((M, K), torch.float32, 3), _data((N, K), torch.float32, 4)
+    y = qa.mxfp4_matmul(qa.mxfp4_quantize(a.cuda()), qa.mxfp4_quantize(b.cuda()), out_dtype=torch.float32)
+    ra = R.rounded(a)
+    for lo in (0, N // 2, N - 301):
+        rb = R.rounded(b[lo:lo + 301])
+        R.assert_close(y[:, lo:lo + 301], ra @ rb.t(), ra.abs() @ rb.abs().t(), K / 32 + 2)
+
+
 @pytest.mark.parametrize("shape", [(16, 64, 128), (1, 48, 160), (70, 130, 320), (300, 300, 512)])
 def test_product_with_bias_and_leading_dimensions(shape):
     import qtpytorch_amd as qa
