@@ -134,74 +134,46 @@ __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __re
 
 // out[r] = x[order[r] / top], zeros where order[r] < 0: a copy, bound by
 // HBM's write rate (a token's row is read `top` times, from the caches after
-// the first).  Rows are copied in pieces of 16 bytes, U pieces a thread with
-// their loads issued first.  WHOLE: rows of whole aligned pieces, written past
-// the caches; else any alignment, and the last piece of a row may be shorter.
-template <int U, bool WHOLE>
+// the first).  A thread copies one piece of 16 bytes: four a thread with their loads
+// first took as long for large copies and longer for small ones (32000 rows of
+// 4096 bf16 63 us both, 4000 rows 7.7 against 6.5).  WHOLE: rows of whole aligned
+// pieces, written past the caches; else any alignment, and the last piece of a
+// row may be shorter.
+template <bool WHOLE>
 __global__ __launch_bounds__(256) void k_expert_gather(const uint8_t* __restrict__ x, int64_t x_stride,
                                                        const int* __restrict__ order, DivU32 by_top, uint32_t tokens,
-                                                       uint32_t total, DivU32 by_pieces, uint32_t pieces, uint32_t row_bytes,
-                                                       uint32_t slices, uint8_t* __restrict__ out) {
+                                                       uint32_t total, DivU32 by_pieces, uint32_t pieces,
+                                                       uint32_t row_bytes, uint32_t slices, uint8_t* __restrict__ out) {
   // slices = 8: workgroup b, on XCD b % 8, copies that eighth of the columns
   // (pieces and total are a slice's), so that an XCD's L2 sees an eighth of each
-  // token; slices = 1: whole rows
+  // token (32000 rows of 4096 bf16, 4 a token: 63 us against 74); slices = 1: whole rows
   const uint32_t slice = slices > 1 ? blockIdx.x & 7u : 0u, block = slices > 1 ? blockIdx.x >> 3 : blockIdx.x;
-  const uint32_t c0 = slice * pieces * 16u;
-  const uint64_t first = (uint64_t)block * (256u * U) + threadIdx.x;
-  u32x4 v[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint64_t i = first + 256u * u;
-    v[u] = u32x4{0u, 0u, 0u, 0u};
-    if (i < total) {
-      const uint32_t r = divu32((uint32_t)i, by_pieces), c = c0 + ((uint32_t)i - r * pieces) * 16u;
-      const int pick = order[r];
-      const uint32_t token = divu32((uint32_t)pick, by_top);
-      if (pick >= 0 && token < tokens) {
-        const uint8_t* p = x + (int64_t)token * x_stride + c;
-        if (WHOLE) {
-          v[u] = *reinterpret_cast<const u32x4*>(p);
-        } else if (c + 16u <= row_bytes) {
-          __builtin_memcpy(&v[u], p, 16);
-        } else {  // elements have an even number of bytes
-          uint16_t t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-          for (uint32_t k = 0; k < 8; ++k)
-            if (c + 2 * k < row_bytes) __builtin_memcpy(&t[k], p + 2 * k, 2);
-          __builtin_memcpy(&v[u], t, 16);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint64_t i = first + 256u * u;
-    if (i >= total) continue;
-    const uint32_t r = divu32((uint32_t)i, by_pieces), c = c0 + ((uint32_t)i - r * pieces) * 16u;
-    uint8_t* p = out + (int64_t)r * row_bytes + c;
-    if (WHOLE) {
-      __builtin_nontemporal_store(v[u], reinterpret_cast<u32x4*>(p));
-    } else if (c + 16u <= row_bytes) {
-      __builtin_memcpy(p, &v[u], 16);
-    } else {
-      uint16_t t[8];
-      __builtin_memcpy(t, &v[u], 16);
-      for (uint32_t k = 0; k < 8; ++k)
-        if (c + 2 * k < row_bytes) __builtin_memcpy(p + 2 * k, &t[k], 2);
+  const uint64_t i = (uint64_t)block * 256u + threadIdx.x;
+  if (i >= total) return;
+  const uint32_t r = divu32((uint32_t)i, by_pieces);
+  const uint32_t c = (slice * pieces + (uint32_t)i - r * pieces) * 16u;
+  const int pick = order[r];
+  const uint32_t token = divu32((uint32_t)pick, by_top);
+  const bool some = pick >= 0 && token < tokens;
+  const uint8_t* p = x + (int64_t)token * x_stride + c;
+  uint8_t* o = out + (int64_t)r * row_bytes + c;
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (WHOLE) {
+    if (some) v = *reinterpret_cast<const u32x4*>(p);
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(o));
+  } else if (c + 16u <= row_bytes) {
+    if (some) __builtin_memcpy(&v, p, 16);
+    __builtin_memcpy(o, &v, 16);
+  } else {  // elements have an even number of bytes
+    for (uint32_t k = c; k < row_bytes; k += 2, p += 2, o += 2) {
+      uint16_t t = 0;
+      if (some) __builtin_memcpy(&t, p, 2);
+      __builtin_memcpy(o, &t, 2);
     }
   }
 }
 
-// 8 elements at p (the first `live` where fewer are left) as float32
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int live, float (&v)[8]) {
-  FpWords<T, 8> w;
-  if (live >= 8) fp4_load(p, w);
-  else fp4_load_tail(p, live, w);
-  T t[8];
-  __builtin_memcpy(t, w.w, sizeof(t));
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = ElemT<T>::cvt(t[e]);
-}
+// 8 results at p (the first `live` where fewer are left)
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int live, const float (&v)[8]) {
   T t[8];
@@ -243,7 +215,7 @@ __device__ __forceinline__ void store8_nt(T* p, const float (&v)[8]) {
 // pick without an expert reads row 0 in place of a branch, and its values are
 // replaced by zeros.
 // WHOLE: columns in whole groups of 8 on 16 bytes.
-template <typename T, bool GATED, int Q, bool WHOLE>
+template <typename T, bool GATED, bool WHOLE>
 __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h, const int* __restrict__ place,
                                                         const float* __restrict__ gates, int top, int rows,
                                                         uint32_t total, DivU32 by_pieces, uint32_t pieces, int cols,
@@ -252,6 +224,7 @@ __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h,
   if (i >= total) return;
   const uint32_t t = divu32((uint32_t)i, by_pieces), c = 8u * ((uint32_t)i - t * pieces);
   const int live = WHOLE ? 8 : cols - (int)c;
+  constexpr int Q = 4;
   float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   const int64_t p0 = (int64_t)t * top;
   if (rows > 0) {
@@ -446,25 +419,18 @@ int mxk_expert_gather(const void* x, int elem_bytes, int64_t tokens, int64_t col
   if (!x || !order || !out) return fail(MXK_EINVAL, "expert_gather: null pointer");
   const int64_t row_bytes = cols * elem_bytes;
   const bool whole = row_bytes % 16 == 0 && row_stride * elem_bytes % 16 == 0 && aligned16(x) && aligned16(out);
-  // eighths of at least two lines
-  const int64_t slices = whole && row_bytes % 2048 == 0 && rows * row_bytes >= ((int64_t)1 << 24) ? 8 : 1;
+  // eighths of whole lines
+  const int64_t slices = whole && row_bytes % 1024 == 0 ? 8 : 1;
   const int64_t pieces = ceil_div(row_bytes, 16) / slices;
   const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 28) / pieces - 1);
   const DivU32 bt = make_divu32((uint32_t)top), bp = make_divu32((uint32_t)pieces);
+  const uint8_t* xp = reinterpret_cast<const uint8_t*>(x);
   for (int64_t r0 = 0; r0 < rows; r0 += step) {
     const uint32_t total = (uint32_t)(std::min(step, rows - r0) * pieces);
-    const uint8_t* xp = reinterpret_cast<const uint8_t*>(x);
-    uint8_t* op = reinterpret_cast<uint8_t*>(out) + r0 * row_bytes;
-    const bool big = total * slices >= 256u * 4u * 1024u;
-    const dim3 grid((unsigned)(ceil_div(total, big ? 1024 : 256) * slices));
-#define MXK_GA(U, W)                                                                                              \
-  hipLaunchKernelGGL((k_expert_gather<U, W>), grid, dim3(256), 0, st, xp, row_stride * elem_bytes, order + r0, bt, \
-                     (uint32_t)tokens, total, bp, (uint32_t)pieces, (uint32_t)row_bytes, (uint32_t)slices, op)
-    if (big && whole) MXK_GA(4, true);
-    else if (big) MXK_GA(4, false);
-    else if (whole) MXK_GA(1, true);
-    else MXK_GA(1, false);
-#undef MXK_GA
+    hipLaunchKernelGGL((whole ? k_expert_gather<true> : k_expert_gather<false>),
+                       dim3((unsigned)(ceil_div(total, 256) * slices)), dim3(256), 0, st, xp, row_stride * elem_bytes,
+                       order + r0, bt, (uint32_t)tokens, total, bp, (uint32_t)pieces, (uint32_t)row_bytes,
+                       (uint32_t)slices, reinterpret_cast<uint8_t*>(out) + r0 * row_bytes);
   }
   return check_launch("expert_gather");
 }
@@ -486,23 +452,21 @@ int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* p
     const dim3 grid((unsigned)ceil_div(total, 256));
     const int* pl = place + t0 * top;
     const float* gt = gates ? gates + t0 * top : nullptr;
-#define MXK_CQ(T, G, Q)                                                                                           \
-  hipLaunchKernelGGL((whole ? k_expert_combine<T, G, Q, true> : k_expert_combine<T, G, Q, false>), grid,          \
-                     dim3(256), 0, st, hp, pl, gt, top, (int)rows, total, bp, (uint32_t)pieces, (int)cols, yp)
+#define MXK_CG(T, G)                                                                                              \
+  hipLaunchKernelGGL((whole ? k_expert_combine<T, G, true> : k_expert_combine<T, G, false>), grid, dim3(256), 0, \
+                     st, hp, pl, gt, top, (int)rows, total, bp, (uint32_t)pieces, (int)cols, yp)
 #define MXK_C(T)                                                                                                  \
   do {                                                                                                            \
     const T* hp = reinterpret_cast<const T*>(h);                                                                  \
     T* yp = reinterpret_cast<T*>(y) + t0 * cols;                                                                  \
-    if (gt && top > 4) MXK_CQ(T, true, 8);                                                                        \
-    else if (gt) MXK_CQ(T, true, 4);                                                                              \
-    else if (top > 4) MXK_CQ(T, false, 8);                                                                        \
-    else MXK_CQ(T, false, 4);                                                                                     \
+    if (gt) MXK_CG(T, true);                                                                                      \
+    else MXK_CG(T, false);                                                                                        \
   } while (0)
     if (h_type == MXK_IN_F32) MXK_C(float);
     else if (h_type == MXK_IN_F16) MXK_C(__half);
     else MXK_C(hip_bfloat16);
 #undef MXK_C
-#undef MXK_CQ
+#undef MXK_CG
   }
   return check_launch("expert_combine");
 }

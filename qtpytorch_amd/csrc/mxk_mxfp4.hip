@@ -55,57 +55,47 @@ __global__ __launch_bounds__(256) void k_fp4_quantize(const T* __restrict__ x, i
 
 // Task i: one dword (8 codes).  f16 results go through float32, where the
 // value is exact, so that subnormal and overflowing ones round once.
-template <typename T, bool FLAT, int U>
+template <typename T, bool FLAT>
 __global__ __launch_bounds__(256) void k_fp4_dequantize(const uint32_t* __restrict__ codes,
                                                         const uint8_t* __restrict__ scales, uint32_t total, int cols,
                                                         DivU32 by_lanes, uint32_t lanes, T* __restrict__ y) {
-  const uint64_t first = (uint64_t)blockIdx.x * (256u * U) + threadIdx.x;
-  uint32_t q[U], s[U];
+  const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+  if (i >= total) return;
+  const uint32_t q = codes[i];
+  const float f = e8m0_operand(scales[i >> 2]);
+  FpWords<T, 8> o;
+  if constexpr (__is_same(T, hip_bfloat16)) {
+    o.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, f, 0));
+    o.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, f, 1));
+    o.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, f, 2));
+    o.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, f, 3));
+  } else {
+    f32x2f p[4];
+    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, f, 0);
+    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, f, 1);
+    p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, f, 2);
+    p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, f, 3);
+    T t[8];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint64_t i = first + 256u * u;
-    q[u] = i < total ? codes[i] : 0u;
-    s[u] = i < total ? scales[i >> 2] : 0u;
+    for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(p[e >> 1][e & 1]);
+    __builtin_memcpy(o.w, t, sizeof(o.w));
   }
+  if constexpr (FLAT) {
+    u32x4* d = reinterpret_cast<u32x4*>(y + 8 * i);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint64_t i = first + 256u * u;
-    if (i >= total) continue;
-    const float f = e8m0_operand(s[u]);
-    FpWords<T, 8> o;
-    if constexpr (__is_same(T, hip_bfloat16)) {
-      o.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[u], f, 0));
-      o.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[u], f, 1));
-      o.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[u], f, 2));
-      o.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[u], f, 3));
+    for (int k = 0; k < FpWords<T, 8>::NW / 4; ++k)
+      __builtin_nontemporal_store(u32x4{o.w[4 * k], o.w[4 * k + 1], o.w[4 * k + 2], o.w[4 * k + 3]}, d + k);
+  } else {
+    const uint32_t r = divu32((uint32_t)i, by_lanes), c = 8u * ((uint32_t)i - r * lanes);
+    T* p = y + (int64_t)r * cols + c;
+    const int live = cols - (int)c;
+    if (live >= 8) {
+      __builtin_memcpy(p, o.w, sizeof(o.w));
     } else {
-      f32x2f p[4];
-      p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[u], f, 0);
-      p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[u], f, 1);
-      p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[u], f, 2);
-      p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[u], f, 3);
-      T t[8];
+      const T* t = reinterpret_cast<const T*>(o.w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(p[e >> 1][e & 1]);
-      __builtin_memcpy(o.w, t, sizeof(o.w));
-    }
-    if constexpr (FLAT) {
-      u32x4* d = reinterpret_cast<u32x4*>(y + 8 * i);
-#pragma unroll
-      for (int k = 0; k < FpWords<T, 8>::NW / 4; ++k)
-        __builtin_nontemporal_store(u32x4{o.w[4 * k], o.w[4 * k + 1], o.w[4 * k + 2], o.w[4 * k + 3]}, d + k);
-    } else {
-      const uint32_t r = divu32((uint32_t)i, by_lanes), c = 8u * ((uint32_t)i - r * lanes);
-      T* p = y + (int64_t)r * cols + c;
-      const int live = cols - (int)c;
-      if (live >= 8) {
-        __builtin_memcpy(p, o.w, sizeof(o.w));
-      } else {
-        const T* t = reinterpret_cast<const T*>(o.w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < live) p[e] = t[e];
-      }
+      for (int e = 0; e < 8; ++e)
+        if (e < live) p[e] = t[e];
     }
   }
 }
@@ -153,16 +143,9 @@ static void launch_dequantize(const uint8_t* codes, const uint8_t* scales, int64
     const uint32_t* cp = reinterpret_cast<const uint32_t*>(codes + r0 * kb * 16);
     const uint8_t* sp = scales + r0 * kb;
     T* yp = y + r0 * cols;
-    const bool big = total >= 256u * 4u * 1024u;
-    const dim3 grid((unsigned)ceil_div(total, big ? 1024 : 256));
-#define MXK_D(F, U)                                                                                             \
-  hipLaunchKernelGGL((k_fp4_dequantize<T, F, U>), grid, dim3(256), 0, st, cp, sp, total, (int)cols, dv,        \
-                     (uint32_t)lanes, yp)
-    if (flat && big) MXK_D(true, 4);
-    else if (flat) MXK_D(true, 1);
-    else if (big) MXK_D(false, 4);
-    else MXK_D(false, 1);
-#undef MXK_D
+    const dim3 grid((unsigned)ceil_div(total, 256));
+    hipLaunchKernelGGL((flat ? k_fp4_dequantize<T, true> : k_fp4_dequantize<T, false>), grid, dim3(256), 0, st, cp, sp,
+                       total, (int)cols, dv, (uint32_t)lanes, yp);
   }
 }
 
