@@ -468,8 +468,8 @@ size_t mxk_mxfp4_linear_workspace(int x_type, int64_t x_rows, int64_t x_stride, 
                                   int experts, int picked);
 
 /* mxk_mxfp4_quantize of x [x_rows][K] (x_type, rows x_stride >= K elements
- * apart), then mxk_mxfp4_matmul, y of x_type.  Products of at most 16 rows (by
- * expert: on average) pack x inside the product's kernel. */
+ * apart), then mxk_mxfp4_matmul, y of x_type.  A dense product of at most 16
+ * rows of up to 8192 elements packs x inside its kernel. */
 int mxk_mxfp4_linear(const void* x, int x_type, int64_t x_rows, int64_t x_stride, const void* b_codes,
                      const void* b_scales, int64_t M, int64_t N, int64_t K, const float* bias, void* y,
                      const int32_t* offsets, int experts, const int32_t* order, int top, void* workspace,

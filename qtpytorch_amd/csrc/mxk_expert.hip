@@ -41,7 +41,8 @@ __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_count(const I* __re
 // shares' first places follow from the counts of the chunks before (`hist`,
 // which a single chunk does not need) and of the waves before, and a wave
 // then places 64 picks at a time, ranked among the lanes with the same expert by
-// ballots over the bits of the expert's number.
+// ballots over the bits of the expert's number.  64 picks 4 us; 65536 picks of 128
+// experts 8 us and 3 for the counts.
 template <typename I>
 __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __restrict__ ids, uint32_t P, uint32_t E,
                                                                    uint32_t chunk, const int* __restrict__ hist,
@@ -211,9 +212,11 @@ __device__ __forceinline__ void store8_nt(T* p, const float (&v)[8]) {
 // y[t] = sum over j of gate[t, j] * h[place[t, j]] (gate = 1 where gates is
 // null), in float32 by ascending j, picks without an expert left out.  Bound
 // by HBM: one read of the rows in use, one write of the tokens.  A thread
-// holds 8 columns of a token and requests the rows of Q picks at a time: a
-// pick without an expert reads row 0 in place of a branch, and its values are
-// replaced by zeros.
+// holds 8 columns of a token and requests the rows of Q picks at a time (eight in
+// place of four were no faster for 8 picks a token, 101 us for 8000 tokens of
+// 4096 bf16, and slower for 4: 68 against 54): a pick without an expert reads row 0 in
+// place of a branch, and its values are replaced by zeros.  8000 tokens of 4096
+// bf16, 4 picks (328 MB): 55 us, 6.0 TB/s.
 // WHOLE: columns in whole groups of 8 on 16 bytes.
 template <typename T, bool GATED, bool WHOLE>
 __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h, const int* __restrict__ place,
@@ -262,9 +265,11 @@ __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h,
 // use and for picks without an expert.  Bound by HBM: dy is read once per
 // token and group of four picks, h read and dh written once.  W waves share a
 // token, one for each 512 columns (up to 8), so that a lane mostly has one
-// set of loads and stores and many tokens are under way.  The products of a
-// lane are added in order of its columns, then over the lanes of a wave and
-// the waves of a token in a fixed order.
+// set of loads and stores and many tokens are under way (8 waves against 4 and
+// 1 for 4096 bf16: 8000 tokens of 4 picks 102, 106 and 125 us, 16 of 8 picks
+// 7.2, 8.3 and 20.7; 4000 of 2 picks 35, 30 and 30).  8000 tokens of 4 picks are
+// 590 MB, 5.6 TB/s.  The products of a lane are added in order of its columns,
+// then over the lanes of a wave and the waves of a token in a fixed order.
 // WHOLE: columns in whole groups of 8 on 16 bytes; dh is then written past the
 // caches.
 template <typename T, int W, bool WHOLE>
@@ -359,8 +364,10 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_expert_combine_grad(
   }
 }
 
-// Picks per chunk: one chunk (one launch) up to 2048; above it at most 128 chunks
-// of at least 2048 picks, whose counts every workgroup reads
+// Picks per chunk: one chunk (one launch) up to 2048 (2000 picks of 32 experts 6.3
+// us; chunks of 1024 and their counts 7.3); above it at most 128 chunks of at least
+// 2048 picks, whose counts every workgroup reads (128000 picks of 128 experts 11.7
+// us, in chunks of 1024 13.2, of 8192 16.4; 16000 of 256 9.6, 8.6 and 16.5)
 static int64_t sort_chunk(int64_t P) {
   if (P <= 2048) return 2048;
   const int64_t c = std::max<int64_t>(2048, ceil_div(P, 128));
@@ -395,7 +402,8 @@ size_t mxk_expert_sort_workspace(int64_t picks, int experts) {
 int mxk_expert_sort(const void* ids, int id_bytes, int64_t picks, int experts, int32_t* order, int32_t* place,
                     int32_t* offsets, void* workspace, size_t workspace_nbytes, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (picks < 0 || picks >= ((int64_t)1 << 31) - 65536) return fail(MXK_EINVAL, "expert_sort: 0 <= picks < 2^31 - 2^16");
+  if (picks < 0 || picks >= ((int64_t)1 << 31) - 65536)
+    return fail(MXK_EINVAL, "expert_sort: 0 <= picks < 2^31 - 2^16");
   // the waves' counters have to fit 64 KiB of LDS
   if (experts < 1 || experts > 1000) return fail(MXK_EINVAL, "expert_sort: 1 to 1000 experts");
   if (id_bytes != 4 && id_bytes != 8) return fail(MXK_EINVAL, "expert_sort: ids of 4 or 8 bytes");
@@ -438,7 +446,8 @@ int mxk_expert_gather(const void* x, int elem_bytes, int64_t tokens, int64_t col
 int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* place, const float* gates,
                        int64_t tokens, int top, int64_t cols, void* y, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (tokens < 0 || top < 1 || cols < 0 || rows < 0 || rows >= ((int64_t)1 << 31) || tokens * top >= ((int64_t)1 << 31) || cols >= ((int64_t)1 << 28))
+  if (tokens < 0 || top < 1 || cols < 0 || rows < 0 || rows >= ((int64_t)1 << 31) ||
+      tokens >= ((int64_t)1 << 31) || tokens * top >= ((int64_t)1 << 31) || cols >= ((int64_t)1 << 28))
     return fail(MXK_EINVAL, "expert_combine: bad sizes (tokens * top below 2^31, cols below 2^28)");
   if (tokens == 0 || cols == 0) return MXK_OK;
   if ((rows > 0 && !h) || !place || !y) return fail(MXK_EINVAL, "expert_combine: null pointer");
@@ -472,10 +481,11 @@ int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* p
 }
 
 int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t rows, const int32_t* place,
-                            const float* gates, const int32_t* used, int64_t tokens, int top, int64_t cols, void* dh, float* dgates,
-                            void* stream) {
+                            const float* gates, const int32_t* used, int64_t tokens, int top, int64_t cols,
+                            void* dh, float* dgates, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (tokens < 0 || top < 1 || cols < 0 || rows < 0 || rows >= ((int64_t)1 << 31) || tokens * top >= ((int64_t)1 << 31) || cols >= ((int64_t)1 << 28))
+  if (tokens < 0 || top < 1 || cols < 0 || rows < 0 || rows >= ((int64_t)1 << 31) ||
+      tokens >= ((int64_t)1 << 31) || tokens * top >= ((int64_t)1 << 31) || cols >= ((int64_t)1 << 28))
     return fail(MXK_EINVAL, "expert_combine_grad: bad sizes (tokens * top below 2^31, cols below 2^28)");
   if (tokens == 0) return MXK_OK;
   if (rows != tokens * top) return fail(MXK_EINVAL, "expert_combine_grad: rows must be tokens * top");
@@ -485,11 +495,11 @@ int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t r
     return fail(MXK_EINVAL, "expert_combine_grad: unknown h_type");
   const int64_t waves = ceil_div(cols, 512);
   const bool whole = cols % 8 == 0 && aligned16(dy) && aligned16(h) && aligned16(dh);
-#define MXK_GW(T, W)                                                                                              \
-  hipLaunchKernelGGL((whole ? k_expert_combine_grad<T, W, true> : k_expert_combine_grad<T, W, false>),            \
-                     dim3((unsigned)ceil_div(tokens, W > 4 ? 1 : 4 / W)), dim3(W > 4 ? 64 * W : 256), 0, st, reinterpret_cast<const T*>(dy),                           \
-                     reinterpret_cast<const T*>(h), place, gates, used, (int)tokens, top, (int)rows, (int)cols,   \
-                     reinterpret_cast<T*>(dh), dgates)
+#define MXK_GW(T, W)                                                                                           \
+  hipLaunchKernelGGL((whole ? k_expert_combine_grad<T, W, true> : k_expert_combine_grad<T, W, false>),         \
+                     dim3((unsigned)ceil_div(tokens, W > 4 ? 1 : 4 / W)), dim3(W > 4 ? 64 * W : 256), 0, st,  \
+                     reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(h), place, gates, used,        \
+                     (int)tokens, top, (int)rows, (int)cols, reinterpret_cast<T*>(dh), dgates)
 #define MXK_G(T)                        \
   do {                                  \
     if (waves <= 1) MXK_GW(T, 1);       \

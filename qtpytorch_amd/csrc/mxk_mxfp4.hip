@@ -7,6 +7,8 @@
 // wave stores 64 consecutive dwords of codes.  There is nothing to divide:
 // the scale is a power of two, so its exponent field comes from the bits of
 // the maximum and v_cvt_scalef32_pk_fp4_* rounds two elements at a time.
+// 16383x8192 bf16 (268 MB and 71 MB): quantize 56 us, dequantize 48, 6.1 and
+// 7.1 TB/s, above the 5.1 of a large copy.
 #include "mxk_mxfp4.h"
 
 namespace mxk {
@@ -53,8 +55,10 @@ __global__ __launch_bounds__(256) void k_fp4_quantize(const T* __restrict__ x, i
   }
 }
 
-// Task i: one dword (8 codes).  f16 results go through float32, where the
-// value is exact, so that subnormal and overflowing ones round once.
+// Task i, one a thread: one dword (8 codes).  Four a thread, as above, were no faster
+// anywhere (4000x4096 bf16 7.3 us against 6.5).  f16 results go through
+// float32, where the value is exact, so that subnormal and overflowing ones
+// round once.
 template <typename T, bool FLAT>
 __global__ __launch_bounds__(256) void k_fp4_dequantize(const uint32_t* __restrict__ codes,
                                                         const uint8_t* __restrict__ scales, uint32_t total, int cols,
@@ -116,8 +120,9 @@ static void launch_quantize(const T* x, int64_t rows, int64_t cols, int64_t ld, 
     const T* xp = x + r0 * ld;
     uint32_t* cp = reinterpret_cast<uint32_t*>(codes + r0 * kb * 16);
     uint8_t* sp = scales + r0 * kb;
-    // four tasks a thread hide the loads' latency; below 4 workgroups a CU
-    // of that size, more workgroups do
+    // four tasks a thread hide the loads' latency (4000x4096 bf16 6.2 us against
+    // 8.2 with one; 16383x8192 the same); below 4 workgroups a CU of that size, more
+    // workgroups do (2000x2000 3.4 us against 4.1 with four)
     const bool big = total >= 256u * 4u * 1024u;
     const dim3 grid((unsigned)ceil_div(total, big ? 1024 : 256));
 #define MXK_Q(F, U)                                                                                              \

@@ -39,7 +39,8 @@ __device__ __forceinline__ void split_bf16(float v, uint16_t (&t)[N]) {
 }
 
 // planes[k][M][pitch] = term k of dy [M][N], zeros in columns N .. pitch - 1
-// (pitch: N rounded up to 8).  One pass, 8 columns a thread.
+// (pitch: N rounded up to 8).  One pass, 8 columns a thread, bound by HBM: 4000x4096
+// f32 27 us, f16 17 (6.1 and 5.7 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void k_fp4_planes(const T* __restrict__ dy, int64_t M, int64_t N, int64_t pitch,
                                                     uint16_t* __restrict__ planes) {
@@ -93,6 +94,11 @@ struct Fp4Grad {
 // two before it multiplies, and written to LDS between the MFMAs of the stage before.
 // 16-byte chunk c of LDS row r sits at c ^ (r & 7) ^ (r >> 3 & 7): reads
 // take 8 consecutive rows, the transposing writes every eighth row.
+//
+// Bound by the matrix unit and by the conversions beside it (115 VALU a wave and
+// stage): 4000x4096x4096 of bf16 136 us for the gradient of a, 139 of b, 1.0
+// PFLOP/s (115 and 114 us in a row of calls without the profiler), where the
+// instruction alone runs at 1.75 on random values.  f16 takes two, f32 three times that.
 template <typename O, int F, bool OF_B>
 __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uint32_t tn) {
   // LDS: L of either buffer, then V of either, so that a buffer and a fragment
@@ -249,8 +255,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
     xb[i] = *reinterpret_cast<const bf16x8*>(get_v[at] + buf * OP + i * 4096);
   };
   // A row of F MFMAs and what is issued between them: the conversions of a
-  // stage (some 240 VALU a wave) fit into the MFMAs' shadows only if they
-  // alternate with them
+  // stage fit into the MFMAs' shadows only if they alternate with them
 #define MXK_STEP(XA, XB, BETWEEN)                                                              \
   _Pragma("unroll") for (int i = 0; i < F; ++i) {                                              \
     BETWEEN;                                                                                   \
@@ -389,6 +394,8 @@ static int launch_grad(const Fp4Grad& p, bool of_b, int out_type, hipStream_t st
     const int64_t ti = ceil_div(p.I, B);
     return (ex ? (of_b ? ti * p.E : segment_slots(p.I, p.E, B)) : ti) * ceil_div(p.J, B);
   };
+  // large tiles where they occupy most CUs (192 of them, 3000x4096x4096: 103 us
+  // against 130; 128, 2048x4096x4096: 101 against 80)
   const int F = tiles(256) >= 160 ? 4 : 2;
   const int64_t B = 64 * F, n = tiles((int)B), tn = ceil_div(p.J, B);
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 gradient: too many tiles");
