@@ -886,8 +886,9 @@ static Shape tile_of(const Fp4Gemm& p) {
   if (p.N >= ((int64_t)1 << 21)) return {0, 1};  // 256 rows of 4-byte results within 2^31 bytes
   auto tiles = [&](int B) { return (p.offsets ? segment_slots(p.M, p.E, B) : ceil_div(p.M, B)) * ceil_div(p.N, B); };
   // large tiles where they occupy most CUs (2048x8192x8192, 256 of them: 76 us
-  // against 92; 1024x8192x8192, 128: 61 against 48)
-  if (tiles(256) >= 192) return {4, 1};
+  // against 92; 1024x8192x8192, 128: 61 against 48) and where experts fill one (32 of
+  // 4096x4096: 250 rows each 129 us against 132, 62 rows 89 against 74)
+  if (tiles(256) >= 192 && (!p.offsets || p.M > 128 * (int64_t)p.E)) return {4, 1};
   if (p.offsets) return {2, 1};
   // K in parts where tiles leave CUs idle and the stages saved, some 0.45 us
   // each, outweigh a launch and the parts' way through memory (128x8192x8192
