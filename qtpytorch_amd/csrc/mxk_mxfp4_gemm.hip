@@ -122,14 +122,15 @@ __global__ __launch_bounds__(256) void k_fp4_gemm(Fp4Gemm p) {
 
 
 // ---------------------------------------------------------------- tiles through LDS
-// What the tile kernel reads in its own order, in one launch:
+// What the tile kernel reads in its own order, in one launch (products of few
+// stages read scales where they lie instead, tile_of):
 //  - scale bytes by stages of 8 blocks (256 values of K): ta[kt][row of the
 //    product][8], tb[kt][row of b][8], zeros past KB; 17/16 of a byte moved
 //    per 32 values;
 //  - by expert, each slot's segment and rows, and the row of a behind each row
 //    of the product, which a tile would otherwise look up while nothing else is
 //    under way.
-// Latency: 3.3 us for 2 x 1000 rows of 4096, 5.8 for 2 x 8192 of 8192.
+// Latency: 3.3 us for 3300 rows of 2080, 5.8 for 16384 of 8192.
 struct Fp4Staged {
   uint8_t *ta, *tb;
   int4* slot;  // {expert, first row, end, 0}
@@ -246,14 +247,16 @@ __device__ __forceinline__ void wait_loads_if(uint32_t counted) {
 // and the clock's fall leave more), 4000x4096x4096 43 us (3.1), 16000
 // rows over 32 experts of 4096x2048 118 us (2.3: 48 KB of stages per tile of
 // 256 rows filled 30 times a workgroup, stores of 131 MB).
-template <typename T, int F, bool EXPERT>
+template <typename T, int F, bool EXPERT, bool STAGED>
 __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged in, int64_t b_rows, uint32_t tm,
                                                           uint32_t tn, uint32_t splits, uint32_t ids) {
   constexpr int B = 64 * F;                 // rows of a tile
   constexpr int OP = B * 128, SC = B * 8;   // bytes of an operand's stage and of its scales
   constexpr int BUF = 2 * OP, SBUF = 2 * SC;
   constexpr int LI = B / 32;                // load instructions per wave, operand and stage
-  constexpr int LOADS = 2 * LI + (F == 4 ? 1 : 2);  // all of a wave and stage
+  // scales in stage order by k_fp4_stage, or each thread brings its row's of a stage
+  static_assert(STAGED || (F == 2 && !EXPERT), "rows of a and b as threads");
+  constexpr int LOADS = 2 * LI + (STAGED && F == 2 ? 2 : 1);  // all of a wave and stage
   constexpr int NW = 32 * F;                // columns of a wave
   constexpr int CB = F == 4 ? 128 : 64;     // bytes of a row that the result passes through LDS at once
   constexpr int CH = CB / 16, CC = CB / (int)sizeof(T), PASS = NW / CC;
@@ -289,6 +292,21 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
   i32x4 ra, rb;
   uint32_t off_a[EXPERT ? LI : 1];  // by expert: of any rows
   int src[EXPERT ? LI : 1];         // those of the next tile
+  // not STAGED: this thread's row of scales, the bytes from there to the last
+  // eight of all, and the stage's bytes that are on the way (of a tile's first
+  // stage in sc0).  Eight bytes are read wherever they are there; those of other
+  // rows and stages are taken out at their use.
+  const uint8_t* srow = nullptr;
+  int room = 0;
+  uint64_t sc = 0, sc0 = 0;
+  auto put_scales = [&](uint32_t t, uint32_t buf, uint64_t v) {
+    const int past = 8 * (int)t - room;  // 8 or more only where no block is left
+    const uint32_t live = KB > 8u * t ? KB - 8u * t : 0u;
+    const uint64_t mask = live >= 8u ? ~0ull : (1ull << (8u * live)) - 1u;
+    *reinterpret_cast<uint64_t*>(lds + 2 * BUF + buf * SBUF + threadIdx.x * 8u) =
+        (v >> (8 * (past > 0 ? past & 7 : 0))) & mask;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
 
   // the next tile from `id` on that has products (rows without an expert are
   // written here): true, or false at the end
@@ -349,10 +367,17 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
         off_a[i] = src[i] < 0 ? MXK_FAR_ROW : (uint32_t)(src[i] - (picked ? 0 : cur.lo)) * row_bytes;
     } else {
       ra = buffer_words(p.a + cur.lo * (int64_t)row_bytes, (uint32_t)(cur.hi - cur.lo) * row_bytes);
+      if constexpr (!STAGED) {
+        const bool of_b = threadIdx.x >= B;
+        const int64_t row = (of_b ? cur.n0 : cur.lo) + (threadIdx.x & (B - 1)), rows = of_b ? p.N : p.M;
+        const int64_t first = (row < rows ? row : rows - 1) * KB, last = rows * KB - 8 - first;
+        srow = (of_b ? p.bs : p.as) + first;
+        room = (int)(last < (1 << 24) ? last : (1 << 24));  // a row has at most 2^18 blocks
+      }
     }
   };
   // part q of F of the loads of stage t
-  auto issue = [&](uint32_t t, uint32_t buf, int q) {
+  auto issue = [&](uint32_t t, uint32_t buf, int q, uint64_t& by_thread) {
 #pragma unroll
     for (int i = q * LI / F; i < (q + 1) * LI / F; ++i) {
       const uint32_t blk = 8u * t + (chunk ^ flip ^ i);
@@ -363,7 +388,8 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
     }
     // scales: planes of [rows][8] bytes, B / 128 kilobytes an operand; waves 0, 1
     // take a's, 2, 3 b's (F = 2: each wave half a kilobyte, the upper lanes nothing)
-    if (q == 0) {
+    if (q == 0 && !STAGED) __builtin_memcpy(&by_thread, srow + min(8 * (int)t, room), 8);
+    if (q == 0 && STAGED) {
       constexpr int R = B / 2;  // rows per wave
       const bool of_b = wave >= 2;
       const int64_t rows = of_b ? b_rows : p.M;
@@ -415,7 +441,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
   if (!look_ahead(id)) return;
   advance();
 #pragma unroll
-  for (int q = 0; q < 2 * F; ++q) issue(cur.from + q / F, q / F, q % F);
+  for (int q = 0; q < 2 * F; ++q) issue(cur.from + q / F, q / F, q % F, q < F ? sc0 : sc);
   uint32_t behind = 0;  // whether stores are due behind and between this tile's first loads
   for (;;) {
     // sums start from the bias, which every row of a fragment shares
@@ -439,6 +465,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
     }
     if (behind) wait_loads<BEHIND0>();
     else wait_loads<LOADS>();
+    if constexpr (!STAGED) put_scales(cur.from, 0, sc0);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
@@ -455,13 +482,14 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
       MXK_STEP(1, fa[1], fb[1], read_frag(buf, 2, i, fa[0], fb[0]))
       MXK_STEP(2, fa[0], fb[0], read_frag(buf, 3, i, fa[1], fb[1]))
       wait_loads_if<BEHIND1>(t == cur.from ? behind : 0u);
+      if constexpr (!STAGED) put_scales(t + 1, buf ^ 1u, sc);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       buf ^= 1u;
       MXK_STEP(3, fa[1], fb[1], {
         read_scale(buf, i, sa[1], sb[1]);
         read_frag(buf, 0, i, fa[0], fb[0]);
-        issue(t + 2, buf ^ 1u, i);
+        issue(t + 2, buf ^ 1u, i, sc);
       })
 #pragma unroll
       for (int i = 0; i < F; ++i) {
@@ -499,7 +527,8 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
 #pragma unroll
       for (int s = 0; s < PASS; ++s) {
         const int part = (j * PASS + s) / STEP;
-        if (more && (j * PASS + s) % STEP == 0 && part < 2 * F) issue(cur.from + part / F, part / F, part % F);
+        if (more && (j * PASS + s) % STEP == 0 && part < 2 * F) 
+          issue(cur.from + part / F, part / F, part % F, part < F ? sc0 : sc);
 #pragma unroll
         for (int u = 0; u < CC / 8; ++u) {
           const int iq = s * (CC / 8) + u, i = iq >> 2, q = iq & 3;
@@ -878,31 +907,37 @@ static int few_of(const Fp4Gemm& p) {
 // the plain kernel) and parts of K
 struct Shape {
   int F, splits;
+  bool staged;
 };
 static Shape tile_of(const Fp4Gemm& p) {
   const int64_t row_bytes = p.KB * 16;
-  if (p.KB == 0 || few_of(p) || row_bytes > (1 << 22)) return {0, 1};
-  if (p.order && p.a_rows * row_bytes > ((int64_t)1 << 30)) return {0, 1};
-  if (p.N >= ((int64_t)1 << 21)) return {0, 1};  // 256 rows of 4-byte results within 2^31 bytes
+  if (p.KB == 0 || few_of(p) || row_bytes > (1 << 22)) return {0, 1, false};
+  if (p.order && p.a_rows * row_bytes > ((int64_t)1 << 30)) return {0, 1, false};
+  if (p.N >= ((int64_t)1 << 21)) return {0, 1, false};  // 256 rows of 4-byte results within 2^31 bytes
   auto tiles = [&](int B) { return (p.offsets ? segment_slots(p.M, p.E, B) : ceil_div(p.M, B)) * ceil_div(p.N, B); };
   // large tiles where they occupy most CUs (2048x8192x8192, 256 of them: 76 us
   // against 92; 1024x8192x8192, 128: 61 against 48) and where experts fill one (32 of
   // 4096x4096: 250 rows each 129 us against 132, 62 rows 89 against 74)
-  if (tiles(256) >= 192 && (!p.offsets || p.M > 128 * (int64_t)p.E)) return {4, 1};
-  if (p.offsets) return {2, 1};
+  if (tiles(256) >= 192 && (!p.offsets || p.M > 128 * (int64_t)p.E)) return {4, 1, true};
+  if (p.offsets) return {2, 1, true};
   // K in parts where tiles leave CUs idle and the stages saved, some 0.45 us
   // each, outweigh a launch and the parts' way through memory (128x8192x8192
   // in 4: 23 us against 30; 256x4096x4096 in 4: 22 against 16)
   const int64_t stages = ceil_div(p.KB, 8), n = tiles(128);
-  const int64_t parts = std::min<int64_t>({num_cus() / n, stages / 4, 16});
-  if (parts < 2) return {2, 1};
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({num_cus() / n, stages / 4, 16}));
   const double saved = 0.45 * (double)(stages - stages / parts), cost = 3.0 + (double)(parts * p.M * p.N) * 1.6e-6;
-  return {2, saved > cost ? (int)parts : 1};
+  const int64_t splits = parts > 1 && saved > cost ? parts : 1;
+  // scales straight from their rows, eight bytes of a line at a time, save a launch and
+  // cost some 0.1 us a stage (1500x1800x2080, 9 stages: 14.0 us against 15.3,
+  // 512x512x512 6.0 against 8.1; 1024x4096x4096, 16 stages: 21.3 against 20.6,
+  // 1024x8192x8192, 64: 57 against 50); they need eight bytes
+  const int64_t turns = ceil_div(n * splits, num_cus()) * ceil_div(stages, splits);
+  return {2, (int)splits, turns > 12 || p.N * p.KB < 8};
 }
 static int64_t tile_bytes(const Fp4Gemm& p, const Shape& t) {
-  const int64_t rows = p.offsets ? p.E * p.N : p.N;
-  const int64_t tables = p.offsets ? 16 * segment_slots(p.M, p.E, 64 * t.F) + 4 * p.M : 0;
-  return stage_bytes(p.M, p.KB) + stage_bytes(rows, p.KB) + tables + (t.splits > 1 ? t.splits * p.M * p.N * 4 : 0);
+  int64_t n = t.splits > 1 ? ceil_div(t.splits * p.M * p.N, 4) * 16 : 0;
+  if (t.staged) n += stage_bytes(p.M, p.KB) + stage_bytes(p.offsets ? p.E * p.N : p.N, p.KB);
+  return p.offsets ? n + 16 * segment_slots(p.M, p.E, 64 * t.F) + 4 * p.M : n;
 }
 
 // Whether the kernel of few rows packs float x itself: a dense product of at
@@ -967,11 +1002,13 @@ static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_byte
   const int64_t slots = ex ? segment_slots(p.M, p.E, (int)B) : ceil_div(p.M, B);
   const int64_t tn = ceil_div(p.N, B), n = ex && t.F ? block_tile_ids(slots, tn) : slots * tn * t.splits;
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many tiles");
-  const int64_t b_rows = ex ? p.E * p.N : p.N, na = stage_bytes(p.M, p.KB), nb = stage_bytes(b_rows, p.KB);
+  const size_t need = t.F ? (size_t)tile_bytes(p, t) : 0;
+  if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need))
+    return fail(MXK_EINVAL, "mxfp4 product: workspace too small or not 16-byte aligned");
+  const int64_t b_rows = ex ? p.E * p.N : p.N;
   Fp4Staged in = {};
-  if (t.F) {
-    if (!ws || !aligned16(ws) || ws_bytes < (size_t)tile_bytes(p, t))
-      return fail(MXK_EINVAL, "mxfp4 product: workspace too small or not 16-byte aligned");
+  if (t.staged) {
+    const int64_t na = stage_bytes(p.M, p.KB), nb = stage_bytes(b_rows, p.KB);
     const int64_t ga = ceil_div(p.M, 32), gb = ceil_div(b_rows, 32), gs = ex ? ceil_div(slots, 4) : 0;
     if (ga + gb + gs >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 product: too many rows");
     in.ta = ws;
@@ -982,13 +1019,14 @@ static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_byte
                        (int)B);
   }
   const int64_t cus = (num_cus() + 7) & ~7;  // a multiple of the XCDs: a workgroup's tiles stay on its own
-#define MXK_TILE(T, F, EX, P)                                                                                        \
-  hipLaunchKernelGGL((k_fp4_gemm_tile<T, F, EX>), dim3((unsigned)std::min<int64_t>(n, (F == 4 ? 1 : 2) * cus)),      \
+#define MXK_TILE(T, F, EX, ST, P)                                                                                    \
+  hipLaunchKernelGGL((k_fp4_gemm_tile<T, F, EX, ST>), dim3((unsigned)std::min<int64_t>(n, (F == 4 ? 1 : 2) * cus)), \
                      dim3(256), 0, st, P, in, b_rows, (uint32_t)slots, (uint32_t)tn, (uint32_t)t.splits, (uint32_t)n)
 #define MXK_L(T, EX)                                                                                     \
   do {                                                                                                   \
-    if (t.F == 4) MXK_TILE(T, 4, EX, p);                                                                 \
-    else if (t.F == 2) MXK_TILE(T, 2, EX, p);                                                            \
+    if (t.F == 4) MXK_TILE(T, 4, EX, true, p);                                                           \
+    else if (t.F == 2 && (EX || t.staged)) MXK_TILE(T, 2, EX, true, p);                                  \
+    else if (t.F == 2) MXK_TILE(T, 2, false, false, p);                                                  \
     else hipLaunchKernelGGL((k_fp4_gemm<T, EX>), dim3((unsigned)n), dim3(256), 0, st, p);                \
   } while (0)
 #define MXK_T(T)                \
@@ -997,11 +1035,13 @@ static int launch_gemm(const Fp4Gemm& p, int y_type, uint8_t* ws, size_t ws_byte
     else MXK_L(T, false);       \
   } while (0)
   if (t.splits > 1) {
-    float* parts = reinterpret_cast<float*>(ws + na + nb);
+    // behind the scales
+    float* parts = reinterpret_cast<float*>(t.staged ? ws + stage_bytes(p.M, p.KB) + stage_bytes(p.N, p.KB) : ws);
     Fp4Gemm q = p;
     q.y = parts;
     q.bias = nullptr;
-    MXK_TILE(float, 2, false, q);
+    if (t.staged) MXK_TILE(float, 2, false, true, q);
+    else MXK_TILE(float, 2, false, false, q);
     const int64_t total = p.M * p.N;
     const dim3 grid((unsigned)ceil_div(total, 1024));
 #define MXK_J(T)                                                                                                    \

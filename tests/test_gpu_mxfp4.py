@@ -136,6 +136,31 @@ def test_product_of_33_to_64_rows_and_of_narrow_weights(shape):
     test_product(shape, torch.bfloat16)
 
 
+@pytest.mark.parametrize("shape", [(65, 3, 64), (100, 4, 64), (65, 1, 256), (70, 1, 200), (3000, 3900, 96), (129, 130, 250), (300, 257, 288),
+                                   (129, 400, 3328), (300, 300, 12000), (66, 129, 2049)])
+def test_product_of_few_stages(shape):
+    test_product(shape, torch.float32)
+    test_product(shape, torch.float16)
+
+
+@pytest.mark.parametrize("shape", [(70, 40, 64), (130, 129, 288), (200, 70, 480), (1100, 1030, 5000)])
+def test_nan_of_a_row_reaches_no_other(shape):
+    """First and last blocks of rows next to each other, whose scale bytes are read together."""
+    import qtpytorch_amd as qa
+    M, N, K = shape
+    a, b, _, _ = _operands(M, N, K)
+    for m in (1, M // 2, M - 1):
+        a[m, 0] = float("nan")
+    for n in (2, N // 2, N - 1):
+        b[n, 0] = float("inf")
+        b[n, K - 1] = float("nan")
+    y = qa.mxfp4_matmul(qa.mxfp4_quantize(a.cuda()), qa.mxfp4_quantize(b.cuda()), out_dtype=torch.float32)
+    want = torch.zeros(M, N, dtype=torch.bool)
+    want[[1, M // 2, M - 1]] = True
+    want[:, [2, N // 2, N - 1]] = True
+    assert torch.equal(torch.isnan(y.cpu()), want)
+
+
 def test_product_of_more_columns_than_a_tile_can_store_by_32_bits():
     import qtpytorch_amd as qa
     M, N, K = 65, (1 << 21) + 3, 64
