@@ -376,20 +376,20 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
       }
     }
   };
-  // part q of F of the loads of stage t
-  auto issue = [&](uint32_t t, uint32_t buf, int q, uint64_t& by_thread) {
-#pragma unroll
-    for (int i = q * LI / F; i < (q + 1) * LI / F; ++i) {
-      const uint32_t blk = 8u * t + (chunk ^ flip ^ i);
-      const uint32_t ok = blk < KB && t < cur.to ? blk * 16u : MXK_FAR_BLOCK;
-      const uint32_t off = off0 + i * step8 + ok;
-      load_to_lds(ra, EXPERT ? off_a[EXPERT ? i : 0] + ok : off, buf * BUF + (wave * LI + i) * 1024u);
-      load_to_lds(rb, off, buf * BUF + OP + (wave * LI + i) * 1024u);
-    }
-    // scales: planes of [rows][8] bytes, B / 128 kilobytes an operand; waves 0, 1
-    // take a's, 2, 3 b's (F = 2: each wave half a kilobyte, the upper lanes nothing)
-    if (q == 0 && !STAGED) __builtin_memcpy(&by_thread, srow + min(8 * (int)t, room), 8);
-    if (q == 0 && STAGED) {
+  // load k of 2 LI of a stage's codes: of a and b in turn
+  auto issue_load = [&](uint32_t t, uint32_t buf, int k) {
+    const int i = k >> 1;
+    const uint32_t blk = 8u * t + (chunk ^ flip ^ i);
+    const uint32_t ok = blk < KB && t < cur.to ? blk * 16u : MXK_FAR_BLOCK;
+    if (k & 1) load_to_lds(rb, off0 + i * step8 + ok, buf * BUF + OP + (wave * LI + i) * 1024u);
+    else load_to_lds(ra, EXPERT ? off_a[EXPERT ? i : 0] + ok : off0 + i * step8 + ok, buf * BUF + (wave * LI + i) * 1024u);
+  };
+  // its scales: planes of [rows][8] bytes, B / 128 kilobytes an operand; waves 0, 1
+  // take a's, 2, 3 b's (F = 2: each wave half a kilobyte, the upper lanes nothing)
+  auto issue_scales = [&](uint32_t t, uint32_t buf, uint64_t& by_thread) {
+    if (!STAGED) {
+      __builtin_memcpy(&by_thread, srow + min(8 * (int)t, room), 8);
+    } else {
       constexpr int R = B / 2;  // rows per wave
       const bool of_b = wave >= 2;
       const int64_t rows = of_b ? b_rows : p.M;
@@ -400,6 +400,12 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
           buffer_words((of_b ? in.tb : in.ta) + ((int64_t)t * rows + first) * 8, t < cur.to ? R * 8u : 0u);
       load_scales_to_lds<R>(rs, lane, 2u * BUF + buf * SBUF + (of_b ? SC : 0) + R * 8u * (wave & 1));
     }
+  };
+  // part q of F of the loads of a stage
+  auto issue = [&](uint32_t t, uint32_t buf, int q, uint64_t& by_thread) {
+#pragma unroll
+    for (int k = q * 2 * LI / F; k < (q + 1) * 2 * LI / F; ++k) issue_load(t, buf, k);
+    if (q == F - 1) issue_scales(t, buf, by_thread);
   };
 
   // fragment reads: rows of this wave's half of a (wave / 2) and of b (wave % 2)
@@ -423,18 +429,19 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
     xa[i] = *reinterpret_cast<const int*>(lds + buf * SBUF + rs_a + i * 256);
     xb[i] = *reinterpret_cast<const int*>(lds + buf * SBUF + rs_b + i * 256);
   };
-  // One step: a row of F MFMAs at a time, after what `between` issues for it
+  // One step: F x F MFMAs, before each what `between` issues there, which fits
+  // into the shadow of the one before
 #define MXK_STEP(SEL, XA, XB, BETWEEN)                                                                       \
   _Pragma("unroll") for (int i = 0; i < F; ++i) {                                                           \
-    BETWEEN;                                                                                                \
-    __builtin_amdgcn_sched_barrier(0);                                                                      \
     _Pragma("unroll") for (int j = 0; j < F; ++j) {                                                         \
+      BETWEEN;                                                                                              \
+      __builtin_amdgcn_sched_barrier(0);                                                                    \
       const i32x8 va = {XA[j][0], XA[j][1], XA[j][2], XA[j][3], 0, 0, 0, 0};                                \
       const i32x8 vb = {XB[i][0], XB[i][1], XB[i][2], XB[i][3], 0, 0, 0, 0};                                \
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vb, va, acc[i][j], 4, 4, SEL, sb[0][i],   \
                                                                   SEL, sa[0][j]);                           \
+      __builtin_amdgcn_sched_barrier(0);                                                                    \
     }                                                                                                       \
-    __builtin_amdgcn_sched_barrier(0);                                                                      \
   }
 
   uint32_t id = blockIdx.x;
@@ -478,18 +485,21 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
     // past the last stage the loads bring zeros and the reads are not used
     uint32_t buf = 0;
     for (uint32_t t = cur.from; t < cur.to; ++t) {
-      MXK_STEP(0, fa[0], fb[0], read_frag(buf, 1, i, fa[1], fb[1]))
-      MXK_STEP(1, fa[1], fb[1], read_frag(buf, 2, i, fa[0], fb[0]))
-      MXK_STEP(2, fa[0], fb[0], read_frag(buf, 3, i, fa[1], fb[1]))
+      MXK_STEP(0, fa[0], fb[0], if (j == 0) read_frag(buf, 1, i, fa[1], fb[1]))
+      MXK_STEP(1, fa[1], fb[1], if (j == 0) read_frag(buf, 2, i, fa[0], fb[0]))
+      MXK_STEP(2, fa[0], fb[0], if (j == 0) read_frag(buf, 3, i, fa[1], fb[1]))
       wait_loads_if<BEHIND1>(t == cur.from ? behind : 0u);
       if constexpr (!STAGED) put_scales(t + 1, buf ^ 1u, sc);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       buf ^= 1u;
       MXK_STEP(3, fa[1], fb[1], {
-        read_scale(buf, i, sa[1], sb[1]);
-        read_frag(buf, 0, i, fa[0], fb[0]);
-        issue(t + 2, buf ^ 1u, i, sc);
+        if (j == 0) read_frag(buf, 0, i, fa[0], fb[0]);
+        if (j == 1) read_scale(buf, i, sa[1], sb[1]);
+        // 2 LI loads over F x F MFMAs
+        _Pragma("unroll") for (int k = (i * F + j) * 2 * LI / (F * F); k < (i * F + j + 1) * 2 * LI / (F * F); ++k)
+            issue_load(t + 2, buf ^ 1u, k);
+        if (i == F - 1 && j == F - 1) issue_scales(t + 2, buf ^ 1u, sc);
       })
 #pragma unroll
       for (int i = 0; i < F; ++i) {
