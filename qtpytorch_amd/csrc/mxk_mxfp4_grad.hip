@@ -151,14 +151,28 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
 
   uint32_t vw[8], vsc[8];
   u32x4 lw[OF_B ? 8 : B / 32];
-  // request half q (0, 1) of the operands of stage s
-  auto request = [&](uint32_t s, int q) {
+  // the buffers of stage s, and whether this thread's chunk of a copied L is past its end
+  __amdgpu_buffer_rsrc_t rv, rs, rl;
+  uint32_t far = 0;
+  auto prepare = [&](uint32_t s) {
     const uint32_t plane = s / per_plane, st = s - plane * per_plane;
     const int64_t t = t0 + 64 * (int64_t)st;
     const int64_t left = s < stages ? (t1 - t < 64 ? t1 - t : 64) : 0;
+    rv = make_rsrc(p.v + (v0 + t) * row_bytes, (uint32_t)left * row_bytes);
+    rs = make_rsrc(p.vs + (v0 + t) * KB, (uint32_t)left * KB);
+    if constexpr (OF_B) {
+      const int64_t cols = p.pitch - i0;  // of dy from this tile on
+      rl = make_rsrc(p.l + (plane * p.l_rows + t) * p.pitch + i0,
+                     left > 0 ? (uint32_t)((left - 1) * pitch + cols * 2) : 0u);
+    } else {
+      const int64_t rows = p.I - i0 < B ? p.I - i0 : B;
+      rl = make_rsrc(p.l + (plane * p.l_rows + i0) * p.pitch + t, left > 0 ? (uint32_t)(rows * pitch - (t * 2)) : 0u);
+      far = (tid & 7) * 8 < left ? 0u : MXK_FAR;
+    }
+  };
+  // request half q (0, 1) of its operands
+  auto request = [&](int q) {
     if (does_v) {
-      const __amdgpu_buffer_rsrc_t rv = make_rsrc(p.v + (v0 + t) * row_bytes, (uint32_t)left * row_bytes);
-      const __amdgpu_buffer_rsrc_t rs = make_rsrc(p.vs + (v0 + t) * KB, (uint32_t)left * KB);
 #pragma unroll
       for (int k = 4 * q; k < 4 * q + 4; ++k) {
         vw[k] = buf_load_b32(rv, v_off + k * row_bytes, 0);
@@ -167,19 +181,13 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
     }
     if constexpr (OF_B) {
       if (does_lt) {
-        const int64_t cols = p.pitch - i0;  // of dy from this tile on
-        const __amdgpu_buffer_rsrc_t rl =
-            make_rsrc(p.l + (plane * p.l_rows + t) * p.pitch + i0, left > 0 ? (uint32_t)((left - 1) * pitch + cols * 2) : 0u);
 #pragma unroll
         for (int k = 4 * q; k < 4 * q + 4; ++k) lw[k] = buf_load_b128(rl, lt_off + k * pitch, 0);
       }
     } else {
-      const int64_t rows = p.I - i0 < B ? p.I - i0 : B;
-      const __amdgpu_buffer_rsrc_t rl =
-          make_rsrc(p.l + (plane * p.l_rows + i0) * p.pitch + t, left > 0 ? (uint32_t)(rows * pitch - (t * 2)) : 0u);
-      const uint32_t far = (tid & 7) * 8 < left ? 0u : MXK_FAR;
 #pragma unroll
-      for (int k = q * B / 64; k < (q + 1) * B / 64; ++k) lw[k] = buf_load_b128(rl, (ld_off + k * 32u * pitch) | far, 0);
+      for (int k = q * B / 64; k < (q + 1) * B / 64; ++k)
+        lw[k] = buf_load_b128(rl, (ld_off + k * 32u * pitch) | far, 0);
     }
   };
   // where this thread's rows of LDS are: chunk tg of rows 8 g8 + k of a
@@ -270,19 +278,21 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
     }                                                                                          \
     __builtin_amdgcn_sched_barrier(0);                                                         \
   }
-  constexpr int SHADOW = 48 / F;  // a row's share of the conversions, spread over its MFMAs
+  constexpr int SHADOW = 24 / F;  // a row's share of the conversions, spread over its MFMAs
   // Quarters per row of MFMAs
   constexpr int Q = 4 / F;
   if (stages > 0) {
-    request(0, 0);
-    request(0, 1);
+    prepare(0);
+    request(0);
+    request(1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       stage_v(0, q);
       stage_l(0, q);
     }
-    request(1, 0);
-    request(1, 1);
+    prepare(1);
+    request(0);
+    request(1);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -298,10 +308,11 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
       MXK_STEP(fa[1], fb[1], {
         read_frag(buf, 2, i, fa[0], fb[0]);
         _Pragma("unroll") for (int q = i * Q; q < (i + 1) * Q; ++q) stage_l(buf ^ 1, q);
+        if (i == F - 1) prepare(s + 2);
       })
       MXK_STEP(fa[0], fb[0], {
         read_frag(buf, 3, i, fa[1], fb[1]);
-        if (i < 2) request(s + 2, i);
+        if (i < 2) request(i);
       })
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
