@@ -241,12 +241,15 @@ __device__ __forceinline__ void wait_loads_if(uint32_t counted) {
 // its rows) is looked up before the products of this one, and that tile's first
 // two stages are requested between the stores of this one's result.
 //
+// What an instruction loads and reads stands between single MFMAs, in their
+// shadow: in front of rows of four it took 5% longer.
+//
 // Bound by the matrix unit, whose rate falls with what the operands hold: this
 // instruction alone on random codes in registers 6.4 PFLOP/s, on zeros 9.1.
-// 8192x8192x8192 260 to 300 us (4.2 to 3.7 PFLOP/s; 206 on zeros, where LDS reads
-// and the clock's fall leave more), 4000x4096x4096 43 us (3.1), 16000
-// rows over 32 experts of 4096x2048 118 us (2.3: 48 KB of stages per tile of
-// 256 rows filled 30 times a workgroup, stores of 131 MB).
+// 8192x8192x8192 250 to 278 us (4.4 to 3.9 PFLOP/s; MFMAs 57% of the cycles,
+// waits 18%), 4000x4096x4096 43 us (3.1), 16000 rows over 32 experts of 4096x2048
+// 116 us (2.3: of a tile's 43000 cycles its eight stages take 29000, the stores
+// of all CUs at once 11000).
 template <typename T, int F, bool EXPERT, bool STAGED>
 __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged in, int64_t b_rows, uint32_t tm,
                                                           uint32_t tn, uint32_t splits, uint32_t ids) {
@@ -382,7 +385,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
     const uint32_t blk = 8u * t + (chunk ^ flip ^ i);
     const uint32_t ok = blk < KB && t < cur.to ? blk * 16u : MXK_FAR_BLOCK;
     if (k & 1) load_to_lds(rb, off0 + i * step8 + ok, buf * BUF + OP + (wave * LI + i) * 1024u);
-    else load_to_lds(ra, EXPERT ? off_a[EXPERT ? i : 0] + ok : off0 + i * step8 + ok, buf * BUF + (wave * LI + i) * 1024u);
+    else load_to_lds(ra, (EXPERT ? off_a[EXPERT ? i : 0] : off0 + i * step8) + ok, buf * BUF + (wave * LI + i) * 1024u);
   };
   // its scales: planes of [rows][8] bytes, B / 128 kilobytes an operand; waves 0, 1
   // take a's, 2, 3 b's (F = 2: each wave half a kilobyte, the upper lanes nothing)
@@ -584,7 +587,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
 // their order.
 //
 // Bound by HBM (17/32 byte per weight, each read once): 16x8192x8192 with x in
-// bf16 12.3 us, packed 9.6 (3.8 TB/s of weights), 8 tokens to 4 of 32 experts
+// bf16 11.2 us, packed 9.6 (3.8 TB/s of weights), 8 tokens to 4 of 32 experts
 // of 4096x4096 29 us (5.6 TB/s of the busy experts').  A wave requests its
 // chunk of a tile of b, 256 bytes a row, straight into LDS of its own, in
 // whole lines (lanes of an MFMA operand lie in different rows: read in that
@@ -952,8 +955,8 @@ static int64_t tile_bytes(const Fp4Gemm& p, const Shape& t) {
 
 // Whether the kernel of few rows packs float x itself: a dense product of at
 // most 16 rows and one chunk of K per wave, whole dwords a row, x a buffer of
-// less than 2^31 bytes.  The GPU takes as long either way (16x8192x8192 13.6
-// us, 1x4096x4096 6.3 against 5.9), the call 3 us less with one launch and no
+// less than 2^31 bytes.  The GPU takes as long either way (16x8192x8192 11.2
+// us against 9.6 and 2.4, 1x4096x4096 6.3 against 5.9), the call 3 us less with one launch and no
 // workspace.  By expert, where many workgroups would each pack mostly rows
 // that are not there, packing first is faster: 8 tokens to 4 of 32 experts of
 // 4096x4096 44 us against 29 and 2.5 for packing.

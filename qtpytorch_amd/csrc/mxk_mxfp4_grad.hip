@@ -96,9 +96,10 @@ struct Fp4Grad {
 // take 8 consecutive rows, the transposing writes every eighth row.
 //
 // Bound by the matrix unit and by the conversions beside it (115 VALU a wave and
-// stage): 4000x4096x4096 of bf16 136 us for the gradient of a, 139 of b, 1.0
-// PFLOP/s (115 and 114 us in a row of calls without the profiler), where the
-// instruction alone runs at 1.75 on random values.  f16 takes two, f32 three times that.
+// stage): 4000x4096x4096 of bf16 134 us for the gradient of a, 136 of b, 1.0
+// PFLOP/s (115 and 110 us in a row of calls without the profiler; 8192x8192x4096
+// 426 us, 1.3), where the instruction alone runs at 1.75 on random values.  MFMAs
+// take 55% of the cycles, waits 14%.  f16 takes two, f32 three times that.
 template <typename O, int F, bool OF_B>
 __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uint32_t tn) {
   // LDS: L of either buffer, then V of either, so that a buffer and a fragment
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
     }                                                                                          \
     __builtin_amdgcn_sched_barrier(0);                                                         \
   }
-  constexpr int SHADOW = 24 / F;  // a row's share of the conversions, spread over its MFMAs
+  constexpr int SHADOW = 24 / F;  // a row's share of the conversions, spread over its MFMAs (48 / F was 2% slower)
   // Quarters per row of MFMAs
   constexpr int Q = 4 / F;
   if (stages > 0) {
@@ -388,14 +389,13 @@ static int64_t planes_bytes(int dy_type, int64_t M, int64_t N) {
 static int launch_planes(const void* dy, int dy_type, int64_t M, int64_t N, uint16_t* planes, hipStream_t st) {
   const int64_t pitch = ceil_div(N, 8) * 8, n = ceil_div(M * (pitch / 8), 256);
   if (n >= ((int64_t)1 << 31)) return fail(MXK_EINVAL, "mxfp4 gradient: dy too large");
-  const dim3 grid((unsigned)n);
-  if (dy_type == MXK_IN_F32)
-    hipLaunchKernelGGL((k_fp4_planes<float>), grid, dim3(256), 0, st, reinterpret_cast<const float*>(dy), M, N, pitch, planes);
-  else if (dy_type == MXK_IN_F16)
-    hipLaunchKernelGGL((k_fp4_planes<__half>), grid, dim3(256), 0, st, reinterpret_cast<const __half*>(dy), M, N, pitch, planes);
-  else
-    hipLaunchKernelGGL((k_fp4_planes<hip_bfloat16>), grid, dim3(256), 0, st, reinterpret_cast<const hip_bfloat16*>(dy), M, N,
-                       pitch, planes);
+#define MXK_P(T)                                                                                                    \
+  hipLaunchKernelGGL((k_fp4_planes<T>), dim3((unsigned)n), dim3(256), 0, st, reinterpret_cast<const T*>(dy), M, N, \
+                     pitch, planes)
+  if (dy_type == MXK_IN_F32) MXK_P(float);
+  else if (dy_type == MXK_IN_F16) MXK_P(__half);
+  else MXK_P(hip_bfloat16);
+#undef MXK_P
   return check_launch("mxfp4 gradient: planes");
 }
 
