@@ -936,17 +936,18 @@ static Shape tile_of(const Fp4Gemm& p) {
   if (p.offsets) return {2, 1, true};
   // K in parts where tiles leave CUs idle and the stages saved, some 0.45 us
   // each, outweigh a launch and the parts' way through memory (128x8192x8192
-  // in 4: 23 us against 30; 256x4096x4096 in 4: 22 against 16)
+  // in 4: 20 us against 33, 256x8192x8192 in 2: 27 against 30, 1000x500x4096
+  // in 4: 14 against 16; 256x4096x4096 in 4: 22 against 16)
   const int64_t stages = ceil_div(p.KB, 8), n = tiles(128);
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({num_cus() / n, stages / 4, 16}));
-  const double saved = 0.45 * (double)(stages - stages / parts), cost = 3.0 + (double)(parts * p.M * p.N) * 1.6e-6;
+  const double saved = 0.45 * (double)(stages - stages / parts), cost = 3.0 + (double)(parts * p.M * p.N) * 0.8e-6;
   const int64_t splits = parts > 1 && saved > cost ? parts : 1;
   // scales straight from their rows, eight bytes of a line at a time, save a launch and
-  // cost some 0.1 us a stage (1500x1800x2080, 9 stages: 14.0 us against 15.3,
-  // 512x512x512 6.0 against 8.1; 1024x4096x4096, 16 stages: 21.3 against 20.6,
-  // 1024x8192x8192, 64: 57 against 50); they need eight bytes
-  const int64_t turns = ceil_div(n * splits, num_cus()) * ceil_div(stages, splits);
-  return {2, (int)splits, turns > 12 || p.N * p.KB < 8};
+  // cost some 0.1 us a stage where every CU takes part: up to 12 stages of a tile per
+  // CU on average (1500x1800x2080, 6 of them: 13.7 us against 15.3, 256x4096x4096, 4:
+  // 13.8 against 16.3; 1024x4096x4096, 16: 21.3 against 20.6, 1024x8192x8192, 64: 57
+  // against 50); they need eight bytes
+  return {2, (int)splits, n * stages > 12 * num_cus() || p.N * p.KB < 8};
 }
 static int64_t tile_bytes(const Fp4Gemm& p, const Shape& t) {
   int64_t n = t.splits > 1 ? ceil_div(t.splits * p.M * p.N, 4) * 16 : 0;
