@@ -49,15 +49,16 @@ def _compile(src: str, obj: str) -> None:
         raise RuntimeError(f"hipcc failed for {src}:\n{r.stderr[-6000:]}")
 
 
-def _check_waits(src: str) -> None:
+def _check(name: str, src: str) -> None:
+    """Run the assembly check `name`.py of this folder on a source."""
     import importlib.util
 
-    spec = importlib.util.spec_from_file_location("mxk_check_lgkm", os.path.join(HERE, "check_lgkm.py"))
-    check_lgkm = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(check_lgkm)
-    n, problems = check_lgkm.check_source(src, hipcc(), HIPCC_FLAGS)
+    spec = importlib.util.spec_from_file_location("mxk_" + name, os.path.join(HERE, name + ".py"))
+    check = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(check)
+    n, problems = check.check_source(os.path.join(HERE, src), hipcc(), HIPCC_FLAGS)
     if problems:
-        raise RuntimeError(f"LDS wait check failed for {os.path.basename(src)} ({n} kernels):\n" + "\n".join(problems))
+        raise RuntimeError(f"{name} failed for {src} ({n} checked):\n" + "\n".join(problems))
 
 
 def build(jobs: int = 4, verbose: bool = True) -> str:
@@ -67,11 +68,11 @@ def build(jobs: int = 4, verbose: bool = True) -> str:
     objs = [os.path.join(objdir, s.replace(".hip", ".o")) for s in srcs]
     with cf.ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
         futs = [ex.submit(_compile, s, o) for s, o in zip(srcs, objs)]
-        # the GEMM's hand-counted LDS waits, checked on its assembly (check_lgkm.py)
-        chk = ex.submit(_check_waits, os.path.join(HERE, "mxk_gemm.hip"))
+        # on the assembly: the GEMM's hand-counted LDS waits, the wait states of loads into LDS
+        futs.append(ex.submit(_check, "check_lgkm", "mxk_gemm.hip"))
+        futs.append(ex.submit(_check, "check_lds_loads", "mxk_mxfp4_gemm.hip"))
         for f in futs:
             f.result()
-        chk.result()
     tmp = OUT + ".tmp"
     cmd = [hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -181,8 +181,11 @@ __device__ __forceinline__ i32x4 buffer_words(const void* p, uint32_t bytes) {
 // 16 bytes per lane from a buffer into LDS at `lds` + 16 * lane.  In
 // assembly, so that the compiler does not order the tile's LDS reads behind
 // loads of the other buffer; the kernel waits for them itself (wait_loads).
+// A load into LDS needs one wait state behind the write of m0, which the
+// hardware does not insert, nor the compiler within assembly: the s_nop.  The
+// build checks it on the result (check_lds_loads.py).
 __device__ __forceinline__ void load_to_lds(i32x4 r, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds), "v"(off), "s"(r)
                : "memory");
@@ -194,8 +197,8 @@ __device__ __forceinline__ void load_scales_to_lds(i32x4 r, int lane, uint32_t l
     load_to_lds(r, 16u * lane, lds);
   } else {
     static_assert(R == 64, "16 or 8 bytes per lane");
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds\n\t"
-                 "s_mov_b32 m0, %3\n\tbuffer_load_dword %4, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds\n\t"
+                 "s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %4, %2, 0 offen lds"
                  :
                  : "s"(lds), "v"(4u * lane), "s"(r), "s"(lds + 256u), "v"(4u * lane + 256u)
                  : "memory");
