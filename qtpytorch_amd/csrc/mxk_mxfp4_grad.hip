@@ -435,7 +435,7 @@ static int launch_grad(const Fp4Grad& p, bool of_b, int out_type, hipStream_t st
 
 static bool known(int t) { return t == MXK_IN_F32 || t == MXK_IN_F16 || t == MXK_IN_BF16; }
 
-static int check_grad(const void* dy, int dy_type, int64_t M, int64_t N, int64_t K, const void* codes,
+static int check_grad(bool of_b, const void* dy, int dy_type, int64_t M, int64_t N, int64_t K, const void* codes,
                       const void* scales, int out_type, const void* out, const int32_t* offsets, int experts,
                       const void* ws, size_t ws_bytes) {
   if (M < 0 || N < 0 || K < 0) return fail(MXK_EINVAL, "mxfp4 gradient: negative size");
@@ -444,7 +444,8 @@ static int check_grad(const void* dy, int dy_type, int64_t M, int64_t N, int64_t
     return fail(MXK_EINVAL, "mxfp4 gradient: M below 2^31, N below 2^22, K below 2^26");
   if (!known(dy_type) || !known(out_type)) return fail(MXK_EINVAL, "mxfp4 gradient: unknown type");
   if (offsets && (experts < 1 || experts > 1000)) return fail(MXK_EINVAL, "mxfp4 gradient: 1 to 1000 experts");
-  if (!out && M * N * K > 0) return fail(MXK_EINVAL, "mxfp4 gradient: null pointer");
+  // an empty sum is written too: the result is there wherever it has elements
+  if (!out && (of_b ? N : M) > 0 && K > 0) return fail(MXK_EINVAL, "mxfp4 gradient: null pointer");
   if (M > 0 && N > 0 && K > 0 && (!dy || !codes || !scales)) return fail(MXK_EINVAL, "mxfp4 gradient: null pointer");
   if ((reinterpret_cast<uintptr_t>(codes) & 15u) != 0)
     return fail(MXK_EINVAL, "mxfp4 gradient: codes must be 16-byte aligned");
@@ -483,7 +484,7 @@ size_t mxk_mxfp4_grad_workspace(const void* dy, int dy_type, int64_t M, int64_t 
 int mxk_mxfp4_grad_a(const void* dy, int dy_type, int64_t M, int64_t N, const void* b_codes, const void* b_scales,
                      int64_t K, int out_type, void* da, const int32_t* offsets, int experts, void* workspace,
                      size_t workspace_nbytes, void* stream) {
-  int rc = check_grad(dy, dy_type, M, N, K, b_codes, b_scales, out_type, da, offsets, experts, workspace,
+  int rc = check_grad(false, dy, dy_type, M, N, K, b_codes, b_scales, out_type, da, offsets, experts, workspace,
                       workspace_nbytes);
   if (rc != MXK_OK || M == 0 || K == 0) return rc;
   Fp4Grad p;
@@ -502,7 +503,7 @@ int mxk_mxfp4_grad_a(const void* dy, int dy_type, int64_t M, int64_t N, const vo
 int mxk_mxfp4_grad_b(const void* dy, int dy_type, int64_t M, int64_t N, const void* a_codes, const void* a_scales,
                      int64_t K, int out_type, void* db, const int32_t* offsets, int experts, void* workspace,
                      size_t workspace_nbytes, void* stream) {
-  int rc = check_grad(dy, dy_type, M, N, K, a_codes, a_scales, out_type, db, offsets, experts, workspace,
+  int rc = check_grad(true, dy, dy_type, M, N, K, a_codes, a_scales, out_type, db, offsets, experts, workspace,
                       workspace_nbytes);
   if (rc != MXK_OK || N == 0 || K == 0) return rc;
   Fp4Grad p;
