@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define MXK_ABI_VERSION 12
+#define MXK_ABI_VERSION 13
 
 typedef enum {
   MXK_OK = 0,
@@ -521,10 +521,12 @@ int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* p
                        int64_t tokens, int top, int64_t cols, void* y, void* stream);
 
 /* Gradients of mxk_expert_combine: dh[place[t][j]] = gates[t][j] * dy[t],
- * zeros in rows from *used (device int32) on; dgates[t][j] = <dy[t],
- * h[place[t][j]]>, 0 without a place.  rows = tokens * top. */
-int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t rows, const int32_t* place,
-                            const float* gates, const int32_t* used, int64_t tokens, int top, int64_t cols, void* dh,
+ * zeros in rows that no place names; dgates[t][j] = <dy[t], h[place[t][j]]>, 0
+ * without a place.  gates NULL: ones, h and dgates are not used.  A row is
+ * named by one place at most; order as in mxk_expert_sort (the inverse of place
+ * where a pick has one).  rows = tokens * top. */
+int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t rows, const int32_t* order,
+                            const int32_t* place, const float* gates, int64_t tokens, int top, int64_t cols, void* dh,
                             float* dgates, void* stream);
 
 #ifdef __cplusplus

@@ -260,9 +260,38 @@ __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h,
   store8(y + (int64_t)t * cols + c, live, acc);
 }
 
+// Zeros in the rows of dh that no place names: the picks dropped from a plan, the
+// rows past the last in use.  A place names row r if it is that of the pick
+// order[r]; should a plan's order not be the inverse of its places, the row of a place is
+// written over by the launch behind this one.  A workgroup looks at 32 rows: 1.6 us
+// for 32000 rows that are all named, 15 where a quarter of them, 8 KB each, are not.
+// WHOLE: rows of whole aligned 16-byte pieces.
+template <bool WHOLE>
+__global__ __launch_bounds__(256) void k_expert_unnamed(const int* __restrict__ order, const int* __restrict__ place,
+                                                        int rows, int64_t row_bytes, uint8_t* __restrict__ dh) {
+  const int64_t r0 = (int64_t)blockIdx.x * 32, r = r0 + (threadIdx.x & 31);
+  bool none = false;
+  if (r < rows) {
+    const int pick = order[r];
+    none = pick < 0 || pick >= rows || place[pick] != r;
+  }
+  // the halves of a wave hold the same rows
+  for (uint32_t left = (uint32_t)__ballot(none); left; left &= left - 1u) {
+    uint8_t* row = dh + (r0 + __builtin_ctz(left)) * row_bytes;
+    if (WHOLE) {
+      for (int64_t c = threadIdx.x * 16; c < row_bytes; c += 4096)
+        __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u}, reinterpret_cast<u32x4*>(row + c));
+    } else {  // elements have an even number of bytes
+      const uint16_t z = 0;
+      for (int64_t c = threadIdx.x * 2; c < row_bytes; c += 512) __builtin_memcpy(row + c, &z, 2);
+    }
+  }
+}
+
 // Gradients of the weighted sum: dh[place[t, j]] = gate[t, j] * dy[t] and
-// dgate[t, j] = <dy[t], h[place[t, j]]>; zeros for rows past the last in
-// use and for picks without an expert.  Bound by HBM: dy is read once per
+// dgate[t, j] = <dy[t], h[place[t, j]]>; zero for picks without an expert.  Rows
+// that no place names are k_expert_unnamed's.  Not GATED: gates of 1, no dgate, h
+// is not read.  Bound by HBM: dy is read once per
 // token and group of four picks, h read and dh written once.  W waves share a
 // token, one for each 512 columns (up to 8), so that a lane mostly has one
 // set of loads and stores and many tokens are under way (8 waves against 4 and
@@ -272,10 +301,10 @@ __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h,
 // then over the lanes of a wave and the waves of a token in a fixed order.
 // WHOLE: columns in whole groups of 8 on 16 bytes; dh is then written past the
 // caches.
-template <typename T, int W, bool WHOLE>
+template <typename T, int W, bool WHOLE, bool GATED>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_expert_combine_grad(
     const T* __restrict__ dy, const T* __restrict__ h, const int* __restrict__ place, const float* __restrict__ gates,
-    const int* __restrict__ used, int tokens, int top, int rows, int cols, T* __restrict__ dh, float* __restrict__ dg) {
+    int tokens, int top, int rows, int cols, T* __restrict__ dh, float* __restrict__ dg) {
   constexpr int PER = W > 4 ? 1 : 4 / W;  // tokens per workgroup
   __shared__ float part[PER * W][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -283,7 +312,6 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_expert_combine_grad(
   const int w = wave % W;
   const bool live_t = t < tokens;
   const int64_t p0 = t * top;
-  const int n_used = *used;
   const T* dyt = dy + t * cols;
   for (int j0 = 0; j0 < top; j0 += 4) {
     float dot[4] = {0, 0, 0, 0};
@@ -296,58 +324,59 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_expert_combine_grad(
         // the same for the whole wave: branches on it are scalar
         at[q] = __builtin_amdgcn_readfirstlane(in ? place[p0 + j0 + q] : -1);
         if (at[q] >= rows) at[q] = -1;
-        g[q] = in ? gates[p0 + j0 + q] : 0.0f;
+        g[q] = GATED && in ? gates[p0 + j0 + q] : 1.0f;
       }
       for (int c = (w * 64 + lane) * 8; c < cols; c += W * 512) {
         const int live = WHOLE ? 8 : cols - c;
         FpWords<T, 8> d, v[4];
         if (live >= 8) fp4_load(dyt + c, d);
         else fp4_load_tail(dyt + c, live, d);
+        if (GATED) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (at[q] >= 0) {
-            const T* row = h + (int64_t)at[q] * cols + c;
-            if (WHOLE) load8_nt(row, v[q]);
-            else if (live >= 8) fp4_load(row, v[q]);
-            else fp4_load_tail(row, live, v[q]);
-          }
+          for (int q = 0; q < 4; ++q)
+            if (at[q] >= 0) {
+              const T* row = h + (int64_t)at[q] * cols + c;
+              if (WHOLE) load8_nt(row, v[q]);
+              else if (live >= 8) fp4_load(row, v[q]);
+              else fp4_load_tail(row, live, v[q]);
+            }
+        }
         T d8[8];
         __builtin_memcpy(d8, d.w, sizeof(d8));
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (at[q] >= 0) {
-            T v8[8];
-            __builtin_memcpy(v8, v[q].w, sizeof(v8));
             float o[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float de = ElemT<T>::cvt(d8[e]);
-              dot[q] = __builtin_fmaf(de, ElemT<T>::cvt(v8[e]), dot[q]);
-              o[e] = g[q] * de;
+            for (int e = 0; e < 8; ++e) o[e] = g[q] * ElemT<T>::cvt(d8[e]);
+            if (GATED) {
+              T v8[8];
+              __builtin_memcpy(v8, v[q].w, sizeof(v8));
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                dot[q] = __builtin_fmaf(ElemT<T>::cvt(d8[e]), ElemT<T>::cvt(v8[e]), dot[q]);
             }
             if (WHOLE) store8_nt(dh + (int64_t)at[q] * cols + c, o);
             else store8(dh + (int64_t)at[q] * cols + c, live, o);
           }
-          if (j0 + q < top && p0 + j0 + q >= n_used) {  // row number p0 + j0 + q is in no one's use
-            const float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            store8(dh + (p0 + j0 + q) * cols + c, live, z);
-          }
         }
       }
+      if (GATED) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 4; ++q) {
 #pragma unroll
-        for (int s = 32; s > 0; s >>= 1) dot[q] += __shfl_xor(dot[q], s);
-        if (at[q] < 0) dot[q] = 0.0f;
+          for (int s = 32; s > 0; s >>= 1) dot[q] += __shfl_xor(dot[q], s);
+          if (at[q] < 0) dot[q] = 0.0f;
+        }
       }
     }
-    if constexpr (W == 1) {
+    if constexpr (GATED && W == 1) {
       if (live_t && lane == 0) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (j0 + q < top) dg[p0 + j0 + q] = dot[q];
       }
-    } else {
+    } else if constexpr (GATED) {
       if (lane == 0) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) part[wave][q] = dot[q];
@@ -480,26 +509,36 @@ int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* p
   return check_launch("expert_combine");
 }
 
-int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t rows, const int32_t* place,
-                            const float* gates, const int32_t* used, int64_t tokens, int top, int64_t cols,
-                            void* dh, float* dgates, void* stream) {
+int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t rows, const int32_t* order,
+                            const int32_t* place, const float* gates, int64_t tokens, int top, int64_t cols, void* dh,
+                            float* dgates, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (tokens < 0 || top < 1 || cols < 0 || rows < 0 || rows >= ((int64_t)1 << 31) ||
       tokens >= ((int64_t)1 << 31) || tokens * top >= ((int64_t)1 << 31) || cols >= ((int64_t)1 << 28))
     return fail(MXK_EINVAL, "expert_combine_grad: bad sizes (tokens * top below 2^31, cols below 2^28)");
   if (tokens == 0) return MXK_OK;
   if (rows != tokens * top) return fail(MXK_EINVAL, "expert_combine_grad: rows must be tokens * top");
-  if (!place || !gates || !used || !dgates || (cols > 0 && (!dy || !h || !dh)))
+  if (!order || !place || (gates && !dgates) || (cols > 0 && (!dy || !dh || (gates && !h))))
     return fail(MXK_EINVAL, "expert_combine_grad: null pointer");
   if (h_type != MXK_IN_F32 && h_type != MXK_IN_F16 && h_type != MXK_IN_BF16)
     return fail(MXK_EINVAL, "expert_combine_grad: unknown h_type");
   const int64_t waves = ceil_div(cols, 512);
   const bool whole = cols % 8 == 0 && aligned16(dy) && aligned16(h) && aligned16(dh);
-#define MXK_GW(T, W)                                                                                           \
-  hipLaunchKernelGGL((whole ? k_expert_combine_grad<T, W, true> : k_expert_combine_grad<T, W, false>),         \
+  if (cols > 0) {
+    const int64_t row_bytes = cols * (h_type == MXK_IN_F32 ? 4 : 2);
+    hipLaunchKernelGGL((whole ? k_expert_unnamed<true> : k_expert_unnamed<false>), dim3((unsigned)ceil_div(rows, 32)),
+                       dim3(256), 0, st, order, place, (int)rows, row_bytes, reinterpret_cast<uint8_t*>(dh));
+  }
+#define MXK_GG(T, W, G)                                                                                        \
+  hipLaunchKernelGGL((whole ? k_expert_combine_grad<T, W, true, G> : k_expert_combine_grad<T, W, false, G>),   \
                      dim3((unsigned)ceil_div(tokens, W > 4 ? 1 : 4 / W)), dim3(W > 4 ? 64 * W : 256), 0, st,  \
-                     reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(h), place, gates, used,        \
-                     (int)tokens, top, (int)rows, (int)cols, reinterpret_cast<T*>(dh), dgates)
+                     reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(h), place, gates, (int)tokens, \
+                     top, (int)rows, (int)cols, reinterpret_cast<T*>(dh), dgates)
+#define MXK_GW(T, W)                    \
+  do {                                  \
+    if (gates) MXK_GG(T, W, true);      \
+    else MXK_GG(T, W, false);           \
+  } while (0)
 #define MXK_G(T)                        \
   do {                                  \
     if (waves <= 1) MXK_GW(T, 1);       \
@@ -512,6 +551,7 @@ int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t r
   else MXK_G(hip_bfloat16);
 #undef MXK_G
 #undef MXK_GW
+#undef MXK_GG
   return check_launch("expert_combine_grad");
 }
 

@@ -132,7 +132,7 @@ class _ExpertCombine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, gates, plan):
         h = h.contiguous()
-        ctx.save_for_backward(h, gates, *plan)
+        ctx.save_for_backward(None if gates is None else h, gates, *plan)
         return _combine(h, plan, gates)
 
     @staticmethod
@@ -141,18 +141,17 @@ class _ExpertCombine(torch.autograd.Function):
         h, gates, *plan = ctx.saved_tensors
         plan = expert_plan(*plan)
         dy = dy.contiguous()
-        if gates is None:
-            return _gather(dy, plan), None, None
         dev = L.require_gpu(dy, h, gates, *plan)
         tokens, top = plan.place.shape
-        dh, dg = torch.empty_like(h), torch.empty_like(gates)
+        rows, cols = tokens * top, dy.shape[1]
+        dh = torch.empty((rows, cols), dtype=dy.dtype, device=dev)
+        dg = None if gates is None else torch.empty_like(gates)
         with L.on_device(dev):
-            rc = L.lib().mxk_expert_combine_grad(dy.data_ptr(), h.data_ptr(), L.elem_type(h.dtype), h.shape[0],
-                                                 plan.place.data_ptr(), gates.data_ptr(),
-                                                 plan.offsets.data_ptr() + 4 * (plan.offsets.numel() - 1), tokens, top,
-                                                 h.shape[1], dh.data_ptr(), dg.data_ptr(), L.stream_of(dy))
+            rc = L.lib().mxk_expert_combine_grad(dy.data_ptr(), L.ptr(h), L.elem_type(dy.dtype), rows,
+                                                 plan.order.data_ptr(), plan.place.data_ptr(), L.ptr(gates), tokens,
+                                                 top, cols, dh.data_ptr(), L.ptr(dg), L.stream_of(dy))
         if rc:
-            L.check(rc, f"expert_combine gradient({tokens}x{h.shape[1]}, top {top})")
+            L.check(rc, f"expert_combine gradient({tokens}x{cols}, top {top})")
         return dh, dg, None
 
 
@@ -169,8 +168,9 @@ def expert_gather(x: Tensor, plan: expert_plan) -> Tensor:
 
 def expert_combine(h: Tensor, plan: expert_plan, gates: Optional[Tensor] = None) -> Tensor:
     """Sum over each token's picks of gates[t, j] * h[place[t, j]], [tokens, D],
-    added in float32 by ascending j and rounded once; a pick without an expert
-    adds nothing.  gates [tokens, top] (float; None: ones).  Differentiable
+    added in float32 by ascending j and rounded once; a pick without a place
+    adds nothing, and a row that no place names has a gradient of zero (one
+    place at most names a row).  gates [tokens, top] (float; None: ones).  Differentiable
     in h and gates."""
     _check_plan("expert_combine", plan)
     _float_rows("expert_combine", h, plan.order.numel(), "one row per pick")
