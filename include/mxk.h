@@ -454,7 +454,7 @@ size_t mxk_mxfp4_matmul_workspace(int64_t a_rows, int64_t M, int64_t N, int64_t 
  * Dense: offsets = order = NULL, a_rows = M.
  * By expert: offsets int32 [experts+1] on the device; rows offsets[e] to
  * offsets[e+1] of y are those of a times b[e] (b [experts][N][K], bias
- * [experts][N]); rows from offsets[experts] on are zeros.  With order (int32
+ * [experts][N]); rows before offsets[0] and from offsets[experts] on are zeros.  With order (int32
  * [M]) row r reads row order[r]/top of a (none, as zeros, if order[r] < 0 or
  * the row is past a_rows); without it a_rows = M.  Offsets are taken into
  * [0, M].  Codes 16-byte aligned; at most 1000 experts. */
@@ -482,7 +482,7 @@ size_t mxk_mxfp4_grad_workspace(const void* dy, int dy_type, int64_t M, int64_t 
 /* da [M][K] (out_type) = dy [M][N] (dy_type) @ dequantize(b) [N][K]: the
  * gradient of a, straight through its quantization.  dy is not rounded,
  * sums are float32.  N below 2^22, K below 2^26.  By expert as mxk_mxfp4_matmul: b [experts][N][K], rows
- * past the last expert's zeros. */
+ * of no expert zeros. */
 int mxk_mxfp4_grad_a(const void* dy, int dy_type, int64_t M, int64_t N, const void* b_codes, const void* b_scales,
                      int64_t K, int out_type, void* da, const int32_t* offsets, int experts, void* workspace,
                      size_t workspace_nbytes, void* stream);

@@ -132,7 +132,8 @@ __device__ __forceinline__ hip_bfloat16 from_f32<hip_bfloat16>(float v) {
 }
 
 // Slot s of the tiles of BM rows of all segments (the experts', then the rows
-// without one): its segment and rows.  Offsets are brought into [0, M], so
+// behind the last of them and those in front of the first, which a part of a
+// larger plan has): its segment and rows.  Offsets are brought into [0, M], so
 // that no row outside the product is named whatever they hold.
 struct Segment {
   int e;  // E: rows without an expert; E + 1: no tile
@@ -144,12 +145,12 @@ __device__ __forceinline__ Segment find_segment(int64_t slot, const int* offsets
   const int lane = threadIdx.x & 63;
   Segment g = {E + 1, 0, 0};
   int64_t before = 0;
-  for (int e0 = 0; e0 <= E; e0 += 64) {
+  for (int e0 = 0; e0 <= E + 1; e0 += 64) {
     const int e = e0 + lane;
     int64_t lo = 0, hi = 0;
-    if (e <= E) {
-      lo = e == 0 ? 0 : (int64_t)offsets[e];
-      hi = e == E ? M : (int64_t)offsets[e + 1];
+    if (e <= E + 1) {
+      lo = e > E ? 0 : (int64_t)offsets[e];
+      hi = e == E ? M : (int64_t)offsets[e > E ? 0 : e + 1];
       lo = lo < 0 ? 0 : (lo > M ? M : lo);
       hi = hi < lo ? lo : (hi > M ? M : hi);
     }
@@ -166,7 +167,7 @@ __device__ __forceinline__ Segment find_segment(int64_t slot, const int* offsets
       const int src = __builtin_ctzll(here);
       const int first = __shfl(upto - tiles, src);
       const int64_t slo = __shfl((int)lo, src), shi = __shfl((int)hi, src);
-      g.e = __builtin_amdgcn_readfirstlane(e0 + src);
+      g.e = __builtin_amdgcn_readfirstlane(min(e0 + src, E));
       g.lo = __builtin_amdgcn_readfirstlane((int)(slo + (at - first) * BM));
       g.hi = __builtin_amdgcn_readfirstlane((int)(shi < slo + (at - first + 1) * BM ? shi : slo + (at - first + 1) * BM));
       return g;
@@ -175,10 +176,10 @@ __device__ __forceinline__ Segment find_segment(int64_t slot, const int* offsets
   }
   return g;
 }
-// Slots that cover every case of M rows in E segments and the rows without an
-// expert: each segment wastes less than a tile, and no tile is empty
+// Slots that cover every case of M rows in E segments and the two of rows without
+// an expert: each segment wastes less than a tile, and no tile is empty
 inline int64_t segment_slots(int64_t M, int E, int BM) {
-  return std::min<int64_t>(M, (M + (int64_t)(E + 1) * (BM - 1)) / BM);
+  return std::min<int64_t>(M, (M + (int64_t)(E + 2) * (BM - 1)) / BM);
 }
 
 // Tile t of a grid of tm x tn, taken so that the workgroups of one XCD

@@ -8,7 +8,7 @@
 // the float32 accumulator.
 //
 // By expert: rows [offsets[e], offsets[e + 1]) of a go through b[e], and rows
-// past the last expert's are written as zeros; with `order` row r of the
+// in front of the first expert's and past the last's are written as zeros; with `order` row r of the
 // product is row order[r] / top of a.
 #include "mxk_mxfp4.h"
 

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uin
       const uint32_t e = it / per;
       i0 = (int64_t)(it - e * per) * B;
       i1 = p.I < i0 + B ? p.I : i0 + B;
-      const int64_t lo = e == 0 ? 0 : (int64_t)p.offsets[e], hi = p.offsets[e + 1];
+      const int64_t lo = p.offsets[e], hi = p.offsets[e + 1];
       t0 = lo < 0 ? 0 : (lo > p.T ? p.T : lo);
       t1 = hi < t0 ? t0 : (hi > p.T ? p.T : hi);
       v0 = 0;

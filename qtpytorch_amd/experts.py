@@ -230,7 +230,7 @@ def _expert_product(a: mxfp4_tensor, b: mxfp4_tensor, plan: expert_plan, bias: O
 def expert_linear(x: Tensor, weight: Union[Tensor, mxfp4_tensor], plan: expert_plan, bias: Optional[Tensor] = None,
                   *, gather: bool = False) -> Tensor:
     """Each expert's rows through its weight: y[r] = x[r] @ weight[e].T (+
-    bias[e]) for the rows r of expert e, zeros past the places in use.
+    bias[e]) for the rows r of expert e, zeros in rows that no expert has.
 
     x [tokens * top, K] in the plan's order, packed to 4 bits in the call; with
     gather x is [tokens, K] and row r reads token order[r] // top, so that a

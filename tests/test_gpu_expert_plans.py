@@ -1,4 +1,5 @@
-"""Plans with places dropped after the sort (an expert over its capacity)."""
+"""Plans that a routing makes by hand: places dropped after the sort (an expert's
+capacity), and some experts' part of a larger plan."""
 import pytest
 import torch
 
@@ -107,3 +108,65 @@ def test_a_layer_without_the_dropped(tokens, gather):
     want = step(qa.expert_sort(ids.masked_fill(out, -1).cuda(), E))
     for a, b in zip(got, want):  # the same sums, of rows in other places
         assert torch.isfinite(a).all() and float((a - b).norm()) <= 1e-6 * float(b.norm())
+
+
+# ---------------------------------------------------------------- some experts of a larger plan
+SLICES = [  # tokens, top, experts, the first of them and their number, n, k
+    (6, 2, 5, 1, 3, 40, 96), (64, 4, 9, 2, 4, 130, 320), (300, 2, 8, 3, 4, 257, 544), (500, 2, 4, 2, 2, 64, 160),
+    (40, 1, 70, 3, 64, 20, 64), (300, 1, 66, 1, 63, 20, 64), (30, 2, 4, 3, 1, 8, 32)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gather", [True, False])
+@pytest.mark.parametrize("tokens,top,experts,first,held,n,k", SLICES)
+def test_experts_of_a_part_of_a_plan(tokens, top, experts, first, held, n, k, gather, dtype):
+    """offsets[first : first + held + 1]: those experts' rows are computed, all others are zeros."""
+    import qtpytorch_amd as qa
+    ids = _ids(tokens, top, experts, dropped=0.1)
+    order, place, offsets = R.plan(ids, experts)
+    part = offsets[first:first + held + 1]
+    plan = _cuda((order, place, part))
+    x = torch.randn(tokens if gather else tokens * top, k, generator=_gen(1)).to(dtype)
+    w = (torch.randn(held, n, k, generator=_gen(2)) * 0.1).to(dtype)
+    bias = torch.randn(held, n, generator=_gen(3))
+    dy = torch.randn(tokens * top, n, generator=_gen(4)).to(dtype)
+    xg, wg, bg = x.cuda().requires_grad_(), w.cuda().requires_grad_(), bias.cuda().requires_grad_()
+    rx, rw, d = R.rounded(x), R.rounded(w), dy.double()
+    ref, mass = (torch.zeros(tokens * top, n, dtype=torch.float64) for _ in range(2))
+    rows_dx, mass_dx = (torch.zeros(tokens * top, k, dtype=torch.float64) for _ in range(2))
+    y = qa.expert_linear(xg, wg, plan, bg, gather=gather)
+    dx, dw, db = torch.autograd.grad(y, (xg, wg, bg), dy.cuda())
+    for e in range(held):
+        lo, hi = int(part[e]), int(part[e + 1])
+        rows = rx[order[lo:hi] // top] if gather else rx[lo:hi]
+        ref[lo:hi] = rows @ rw[e].t() + bias[e].double()
+        mass[lo:hi] = rows.abs() @ rw[e].abs().t() + bias[e].double().abs()
+        rows_dx[lo:hi], mass_dx[lo:hi] = d[lo:hi] @ rw[e], d[lo:hi].abs() @ rw[e].abs()
+        terms = 3 * ((hi - lo) / 8 + 2)
+        R.assert_close(dw[e], d[lo:hi].t() @ rows, d[lo:hi].abs().t() @ rows.abs(), terms)
+        R.assert_close(db[e], d[lo:hi].sum(0), d[lo:hi].abs().sum(0), terms)
+    R.assert_close(y, ref, mass, k / 32 + 3)
+    assert not y[:int(part[0])].any() and not y[int(part[-1]):].any()
+    if not gather:
+        R.assert_close(dx, rows_dx, mass_dx, 3 * (n / 8 + 2))
+        assert not dx[:int(part[0])].any() and not dx[int(part[-1]):].any()
+    held_w = qa.mxfp4_quantize(w.cuda())
+    assert torch.equal(qa.expert_linear(x.cuda(), held_w, plan, bias.cuda(), gather=gather), y)
+
+
+@pytest.mark.parametrize("gated", [True, False])
+def test_gradients_of_a_sum_over_a_part_of_a_plan(gated):
+    """The sum takes every row that a place names, in or out of the part."""
+    import qtpytorch_amd as qa
+    ids = _ids(50, 4, 8, dropped=0.2)
+    plan = qa.expert_sort(ids.cuda(), 8)
+    h = torch.randn(200, 64, generator=_gen(1)).cuda().requires_grad_()
+    gates = torch.rand(50, 4, generator=_gen(2)).cuda().requires_grad_() if gated else None
+    dy = torch.randn(50, 64, generator=_gen(3)).cuda()
+    want = torch.autograd.grad(qa.expert_combine(h, plan, gates), (h, gates) if gated else (h,), dy)
+    part = plan._replace(offsets=plan.offsets[2:5])
+    for _ in range(4):
+        y = qa.expert_combine(h, part, gates)
+        _poison(200, 64, dtype=torch.float32)
+        got = torch.autograd.grad(y, (h, gates) if gated else (h,), dy)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
