@@ -35,6 +35,16 @@ class expert_plan(NamedTuple):
                              expert here (its id is outside [0, n_experts))
     offsets  [n_experts + 1] first place of each expert's rows; the last entry
                              is the number of places in use
+
+    A pick may be dropped after the sort (an expert over its capacity) by a
+    place of -1: expert_combine follows the places alone and passes the pick's
+    row a gradient of zero.  expert_gather and expert_linear follow order, so that
+    the row is still computed unless its order is -1 too; a row without a place passes
+    a gathered x no gradient.
+
+    Some experts' part of a plan (those of this device) is the plan with
+    offsets[first : first + number + 1]: expert_linear computes their rows and
+    leaves zeros in all others, in front of them and behind.
     """
     order: Tensor
     place: Tensor
