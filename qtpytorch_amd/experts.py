@@ -20,8 +20,8 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from .microscale import (_FLOATS, _bias_f32, _check_linear, _grad_a, _grad_b, _grad_bias, _linear, _pack_weight, _product,
-                         _row_major, _wants_grad, mxfp4_quantize, mxfp4_tensor)
+from .microscale import (_FLOATS, _bias_f32, _check_linear, _grad_a, _grad_b, _grad_bias, _linear, _no_tangents,
+                         _pack_weight, _product, _row_major, _wants_grad, mxfp4_quantize, mxfp4_tensor)
 
 Tensor = torch.Tensor
 
@@ -171,6 +171,7 @@ def expert_gather(x: Tensor, plan: expert_plan) -> Tensor:
     the sum of its rows' (in float32, by ascending pick)."""
     _check_plan("expert_gather", plan)
     _float_rows("expert_gather", x, plan.place.shape[0], "one row per token")
+    _no_tangents("expert_gather", x)
     if x.requires_grad and torch.is_grad_enabled():
         return _ExpertGather.apply(x, plan)
     return _gather(x, plan)
@@ -184,6 +185,7 @@ def expert_combine(h: Tensor, plan: expert_plan, gates: Optional[Tensor] = None)
     in h and gates."""
     _check_plan("expert_combine", plan)
     _float_rows("expert_combine", h, plan.order.numel(), "one row per pick")
+    _no_tangents("expert_combine", h, gates)
     if gates is not None:
         if gates.shape != plan.place.shape:
             raise ValueError(f"expert_combine: gates {tuple(plan.place.shape)} expected, got {tuple(gates.shape)}")
@@ -248,6 +250,7 @@ def expert_linear(x: Tensor, weight: Union[Tensor, mxfp4_tensor], plan: expert_p
     a float tensor, packed in the call and differentiable.  Returns
     [tokens * top, N] of x's dtype; gradients as for mxfp4_linear."""
     _check_linear("expert_linear", x, weight, 3)
+    _no_tangents("expert_linear", x, weight, bias)
     _check_plan("expert_linear", plan)
     tokens, top = plan.place.shape
     _float_rows("expert_linear", x, tokens if gather else tokens * top,

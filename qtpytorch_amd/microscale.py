@@ -15,7 +15,8 @@ block of any length) are decoded first.
 
 ``mxfp4_linear`` passes gradients straight through the quantizer:
 ``dx = dy @ dequantize(weight)`` and, for a float weight, ``dw = dy.T @
-dequantize(quantize(x))``, both with dy unrounded and sums in float32.
+dequantize(quantize(x))``, both with dy unrounded and sums in float32.  There is
+no forward-mode derivative: a dual tensor is refused.
 """
 from __future__ import annotations
 
@@ -23,6 +24,7 @@ import math
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -196,6 +198,7 @@ def mxfp4_matmul(a: mxfp4_tensor, b: mxfp4_tensor, bias: Optional[Tensor] = None
     Products are exact, sums in float32, rounded once to out_dtype."""
     if not isinstance(a, mxfp4_tensor) or not isinstance(b, mxfp4_tensor):
         raise TypeError("mxfp4_matmul: two mxfp4_tensors (mxfp4_quantize packs a float tensor)")
+    _no_tangents("mxfp4_matmul", bias)
     if b.dim() != 2 or a.shape[-1] != b.shape[1]:
         raise ValueError(f"mxfp4_matmul: [..., K] and [N, K] expected, got {tuple(a.shape)} and {tuple(b.shape)}")
     out = torch.empty(*a.shape[:-1], b.shape[0], dtype=out_dtype, device=a.device)
@@ -275,6 +278,13 @@ class _MXFP4Linear(torch.autograd.Function):
         return dx, dw, db, None
 
 
+def _no_tangents(name: str, *tensors) -> None:
+    """Refuse dual tensors: the kernels read the values alone, and a result would lose its tangent."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise L.MXKError(f"{name} has no forward-mode derivative")
+
+
 def _check_linear(name: str, x: Tensor, weight, dims: int) -> None:
     if x.dtype not in _FLOATS:
         raise TypeError(f"{name}: x is float32, float16 or bfloat16, got {x.dtype}")
@@ -297,6 +307,7 @@ def mxfp4_linear(x: Tensor, weight: Union[Tensor, mxfp4_tensor], bias: Optional[
     dtype.  weight: an mxfp4_tensor (held packed, no gradient) or a float
     tensor, packed in the call and differentiable."""
     _check_linear("mxfp4_linear", x, weight, 2)
+    _no_tangents("mxfp4_linear", x, weight, bias)
     N, K = weight.shape
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     if _wants_grad(x, weight, bias):

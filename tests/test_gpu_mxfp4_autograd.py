@@ -1,0 +1,48 @@
+"""What the differentiable calls on microscaled 4-bit operands take, refuse and round."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from tests import _mxfp4 as R
+from tests.test_gpu_experts import _gen, _ids
+
+pytestmark = pytest.mark.gpu
+
+
+def _rand(*shape, seed=0, scale=1.0):
+    return (torch.randn(*shape, generator=_gen(seed)) * scale).cuda()
+
+
+# ---------------------------------------------------------------- tangents
+def _calls():
+    """name, arguments that may have a tangent, the call."""
+    import qtpytorch_amd as qa
+    plan = qa.expert_sort(_ids(6, 2, 4).cuda(), 4)
+    held, experts = qa.mxfp4_quantize(_rand(20, 64, seed=1)), qa.mxfp4_quantize(_rand(4, 20, 64, seed=2))
+    return [
+        ("linear", (_rand(6, 64), _rand(20, 64), _rand(20)), lambda x, w, b: qa.mxfp4_linear(x, w, b)),
+        ("linear, held weight", (_rand(2, 3, 64), _rand(20)), lambda x, b: qa.mxfp4_linear(x, held, b)),
+        ("matmul", (_rand(20),), lambda b: qa.mxfp4_matmul(held, held, b)),
+        ("gather", (_rand(6, 64),), lambda x: qa.expert_gather(x, plan)),
+        ("expert linear", (_rand(12, 64), _rand(4, 20, 64), _rand(4, 20)),
+         lambda x, w, b: qa.expert_linear(x, w, plan, b)),
+        ("expert linear, gathered", (_rand(6, 64),), lambda x: qa.expert_linear(x, experts, plan, gather=True)),
+        ("combine", (_rand(12, 64), _rand(6, 2)), lambda h, g: qa.expert_combine(h, plan, g)),
+        ("combine without gates", (_rand(12, 64),), lambda h: qa.expert_combine(h, plan)),
+    ]
+
+
+@pytest.mark.parametrize("call", range(8))
+def test_a_tangent_is_refused(call):
+    """No forward-mode derivative: an error in place of a result without its tangent."""
+    import qtpytorch_amd as qa
+    name, args, run = _calls()[call]
+    want = run(*args)
+    with forward_ad.dual_level():
+        assert torch.equal(run(*args), want)  # no tangents: as ever
+        for i in range(len(args)):
+            duals = list(args)
+            duals[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(qa._lib.MXKError, match="forward-mode"):
+                run(*duals)
+    assert torch.equal(run(*args), want)
