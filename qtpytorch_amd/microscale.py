@@ -237,12 +237,13 @@ def _grad_b(dy: Tensor, a: mxfp4_tensor, dtype: torch.dtype, offsets: Optional[T
 
 def _grad_bias(dy: Tensor, dtype: torch.dtype, offsets: Optional[Tensor] = None) -> Tensor:
     """Column sums of dy, per expert where offsets are given: the gradient of b
-    against one column of ones."""
+    against one column of ones.  Of a float64 bias too, which the product rounds
+    to float32."""
     codes = torch.zeros(dy.shape[0], 16, dtype=torch.uint8, device=dy.device)
     codes[:, 0] = 2  # the code of 1.0
     ones = mxfp4_tensor(codes, torch.full((dy.shape[0], 1), 127, dtype=torch.uint8, device=dy.device),
                         (dy.shape[0], 1))
-    return _grad_b(dy, ones, dtype, offsets).squeeze(-1)
+    return _grad_b(dy, ones, dtype if dtype in _FLOATS else torch.float32, offsets).squeeze(-1).to(dtype)
 
 
 def _pack_weight(weight: Union[Tensor, mxfp4_tensor]) -> mxfp4_tensor:

@@ -46,3 +46,32 @@ def test_a_tangent_is_refused(call):
             with pytest.raises(qa._lib.MXKError, match="forward-mode"):
                 run(*duals)
     assert torch.equal(run(*args), want)
+
+
+# ---------------------------------------------------------------- biases
+@pytest.mark.parametrize("m", [3, 70])
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16, torch.float16])
+def test_gradient_of_a_bias_of_any_float_type(dtype, m):
+    """Sums in float32, then the bias's own type."""
+    import qtpytorch_amd as qa
+    x, w, bias = _rand(m, 64), _rand(20, 64, seed=1), _rand(20, seed=2).to(dtype).requires_grad_()
+    dy = _rand(m, 20, seed=3)
+    d = dy.double().cpu()
+    as32 = torch.float32 if dtype == torch.float64 else dtype
+    held = qa.mxfp4_quantize(w)
+    for y in (qa.mxfp4_linear(x, held, bias), qa.mxfp4_linear(x, w, bias)):
+        (db,) = torch.autograd.grad(y, bias, dy)
+        assert db.dtype == dtype
+        R.assert_close(db.to(as32), d.sum(0), d.abs().sum(0), 3 * (m / 8 + 2))
+    E, top = 4, 2
+    ids = _ids(m, top, E)
+    order, _, offsets = R.plan(ids, E)
+    bias = _rand(E, 20, seed=4).to(dtype).requires_grad_()
+    dy = _rand(m * top, 20, seed=5)
+    d = dy.double().cpu()
+    y = qa.expert_linear(x, qa.mxfp4_quantize(_rand(E, 20, 64, seed=6)), qa.expert_sort(ids.cuda(), E), bias, gather=True)
+    (db,) = torch.autograd.grad(y, bias, dy)
+    assert db.dtype == dtype
+    for e in range(E):
+        part = d[int(offsets[e]):int(offsets[e + 1])]
+        R.assert_close(db[e].to(as32), part.sum(0), part.abs().sum(0), 3 * (len(part) / 8 + 2))
