@@ -192,17 +192,39 @@ def _linear(x: Tensor, b: mxfp4_tensor, rows: int, bias: Optional[Tensor], offse
     return y
 
 
+def _matmul(a: mxfp4_tensor, b: mxfp4_tensor, bias: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
+    out = torch.empty(*a.shape[:-1], b.shape[0], dtype=out_dtype, device=a.device)
+    return _product(a, b, _rows(a.shape), b.shape[0], _bias_f32(bias, (b.shape[0],)), out)
+
+
+class _MXFP4MatmulBias(torch.autograd.Function):
+    """mxfp4_matmul, differentiable in its bias; the packed operands are constants."""
+
+    @staticmethod
+    def forward(ctx, bias, a, b, out_dtype):
+        ctx.dtype = bias.dtype
+        return _matmul(a, b, bias, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        N = dy.shape[-1]
+        return _grad_bias(dy.reshape(math.prod(dy.shape[:-1]), N).contiguous(), ctx.dtype), None, None, None
+
+
 def mxfp4_matmul(a: mxfp4_tensor, b: mxfp4_tensor, bias: Optional[Tensor] = None,
                  out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """a [..., K] @ b [N, K].T (+ bias [N]) of packed operands, [..., N].
-    Products are exact, sums in float32, rounded once to out_dtype."""
+    Products are exact, sums in float32, rounded once to out_dtype.  The bias has
+    a gradient, packed operands have none."""
     if not isinstance(a, mxfp4_tensor) or not isinstance(b, mxfp4_tensor):
         raise TypeError("mxfp4_matmul: two mxfp4_tensors (mxfp4_quantize packs a float tensor)")
     _no_tangents("mxfp4_matmul", bias)
     if b.dim() != 2 or a.shape[-1] != b.shape[1]:
         raise ValueError(f"mxfp4_matmul: [..., K] and [N, K] expected, got {tuple(a.shape)} and {tuple(b.shape)}")
-    out = torch.empty(*a.shape[:-1], b.shape[0], dtype=out_dtype, device=a.device)
-    return _product(a, b, _rows(a.shape), b.shape[0], _bias_f32(bias, (b.shape[0],)), out)
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        return _MXFP4MatmulBias.apply(bias, a, b, out_dtype)
+    return _matmul(a, b, bias, out_dtype)
 
 
 def _grad(entry: str, dy: Tensor, q: mxfp4_tensor, out: Tensor, offsets: Optional[Tensor]) -> Tensor:

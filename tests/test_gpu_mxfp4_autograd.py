@@ -59,7 +59,9 @@ def test_gradient_of_a_bias_of_any_float_type(dtype, m):
     d = dy.double().cpu()
     as32 = torch.float32 if dtype == torch.float64 else dtype
     held = qa.mxfp4_quantize(w)
-    for y in (qa.mxfp4_linear(x, held, bias), qa.mxfp4_linear(x, w, bias)):
+    for y in (qa.mxfp4_linear(x, held, bias), qa.mxfp4_linear(x, w, bias),
+              qa.mxfp4_matmul(qa.mxfp4_quantize(x), held, bias, torch.float32),
+              qa.mxfp4_matmul(qa.mxfp4_quantize(x.view(1, m, 64)), held, bias, torch.float32)[0]):
         (db,) = torch.autograd.grad(y, bias, dy)
         assert db.dtype == dtype
         R.assert_close(db.to(as32), d.sum(0), d.abs().sum(0), 3 * (m / 8 + 2))
@@ -75,3 +77,13 @@ def test_gradient_of_a_bias_of_any_float_type(dtype, m):
     for e in range(E):
         part = d[int(offsets[e]):int(offsets[e + 1])]
         R.assert_close(db[e].to(as32), part.sum(0), part.abs().sum(0), 3 * (len(part) / 8 + 2))
+
+
+def test_packed_operands_alone_have_no_gradient():
+    import qtpytorch_amd as qa
+    q = qa.mxfp4_quantize(_rand(8, 64))
+    bias = _rand(8).requires_grad_()
+    assert not qa.mxfp4_matmul(q, q).requires_grad
+    with torch.no_grad():
+        assert not qa.mxfp4_matmul(q, q, bias).requires_grad
+    assert torch.equal(qa.mxfp4_matmul(q, q, bias), qa.mxfp4_matmul(q, q, bias.detach()))
