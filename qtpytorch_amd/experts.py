@@ -189,6 +189,8 @@ def expert_combine(h: Tensor, plan: expert_plan, gates: Optional[Tensor] = None)
     if gates is not None:
         if gates.shape != plan.place.shape:
             raise ValueError(f"expert_combine: gates {tuple(plan.place.shape)} expected, got {tuple(gates.shape)}")
+        if gates.is_complex():
+            raise TypeError(f"expert_combine: real gates expected, got {gates.dtype}")
         gates = gates.float().contiguous()
     if (h.requires_grad or gates is not None and gates.requires_grad) and torch.is_grad_enabled():
         return _ExpertCombine.apply(h, gates, plan)

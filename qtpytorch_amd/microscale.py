@@ -107,7 +107,8 @@ def _rows(shape) -> int:
 
 
 def mxfp4_quantize(x: Tensor) -> mxfp4_tensor:
-    """Pack a [..., K] tensor in blocks of 32 along its last dimension.
+    """Pack a [..., K] tensor of float32, float16 or bfloat16 in blocks of 32
+    along its last dimension.
 
     Per block: scale byte = max(exponent of the largest magnitude - 2, -127) +
     127, code = the nearest grid value of x / 2**(scale - 127), ties to the
@@ -117,8 +118,8 @@ def mxfp4_quantize(x: Tensor) -> mxfp4_tensor:
         raise ValueError("mxfp4_quantize: a tensor of at least one dimension")
     dev = L.require_gpu(x)
     kind = _FLOATS.get(x.dtype)
-    if kind is None:
-        x, kind = x.detach().float(), L.MXK_IN_F32
+    if kind is None:  # by way of float32 they would be rounded twice, or leave its range
+        raise TypeError(f"mxfp4_quantize: float32, float16 or bfloat16 expected, got {x.dtype}")
     cols = ld = shape[-1]
     kb = -(-cols // 32)
     if len(shape) == 2:
@@ -144,6 +145,8 @@ def _bias_f32(bias: Optional[Tensor], shape: Tuple[int, ...]) -> Optional[Tensor
         return None
     if tuple(bias.shape) != shape:
         raise ValueError(f"bias of shape {shape} expected, got {tuple(bias.shape)}")
+    if bias.is_complex():
+        raise TypeError(f"a real bias expected, got {bias.dtype}")
     return bias.detach().float().contiguous()
 
 

@@ -87,3 +87,28 @@ def test_packed_operands_alone_have_no_gradient():
     with torch.no_grad():
         assert not qa.mxfp4_matmul(q, q, bias).requires_grad
     assert torch.equal(qa.mxfp4_matmul(q, q, bias), qa.mxfp4_matmul(q, q, bias.detach()))
+
+
+# ---------------------------------------------------------------- types
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int8, torch.uint8, torch.int32, torch.int64, torch.bool,
+                                   torch.complex64])
+def test_quantize_of_other_types_is_refused(dtype):
+    """They would pass float32 on the way: rounded twice, out of its range, or without their imaginary part."""
+    import qtpytorch_amd as qa
+    for shape in ((4, 64), (2, 3, 32), (0, 32)):
+        with pytest.raises(TypeError, match="float32, float16 or bfloat16"):
+            qa.mxfp4_quantize(torch.zeros(shape, dtype=dtype, device="cuda"))
+
+
+def test_complex_biases_and_gates_are_refused():
+    import qtpytorch_amd as qa
+    x, plan = _rand(6, 64), qa.expert_sort(_ids(6, 2, 4).cuda(), 4)
+    q, experts = qa.mxfp4_quantize(x), qa.mxfp4_quantize(_rand(4, 20, 64, seed=2))
+    with pytest.raises(TypeError, match="real"):
+        qa.mxfp4_matmul(q, q, torch.ones(6, dtype=torch.complex64, device="cuda"))
+    with pytest.raises(TypeError, match="real"):
+        qa.mxfp4_linear(x, q, torch.ones(6, dtype=torch.complex64, device="cuda"))
+    with pytest.raises(TypeError, match="real"):
+        qa.expert_linear(x, experts, plan, torch.ones(4, 20, dtype=torch.complex64, device="cuda"), gather=True)
+    with pytest.raises(TypeError, match="real"):
+        qa.expert_combine(_rand(12, 64), plan, torch.ones(6, 2, dtype=torch.complex64, device="cuda"))
