@@ -335,7 +335,7 @@ def mxfp4_linear(x: Tensor, weight: Union[Tensor, mxfp4_tensor], bias: Optional[
     _check_linear("mxfp4_linear", x, weight, 2)
     _no_tangents("mxfp4_linear", x, weight, bias)
     N, K = weight.shape
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    x2 = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), K)
     if _wants_grad(x, weight, bias):
         held = isinstance(weight, mxfp4_tensor)
         y = _MXFP4Linear.apply(x2, None if held else weight, bias, weight if held else None)

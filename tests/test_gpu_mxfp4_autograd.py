@@ -112,3 +112,20 @@ def test_complex_biases_and_gates_are_refused():
         qa.expert_linear(x, experts, plan, torch.ones(4, 20, dtype=torch.complex64, device="cuda"), gather=True)
     with pytest.raises(TypeError, match="real"):
         qa.expert_combine(_rand(12, 64), plan, torch.ones(6, 2, dtype=torch.complex64, device="cuda"))
+
+
+# ---------------------------------------------------------------- rows without columns
+def test_linear_over_rows_without_columns():
+    """K = 0: the bias, for leading dimensions of any number."""
+    import qtpytorch_amd as qa
+    bias, w = _rand(7), torch.empty(7, 0).cuda()
+    for lead in ((4,), (2, 3), (2, 1, 3), (0, 3), ()):
+        x = torch.empty(*lead, 0).cuda()
+        want = bias.expand(*lead, 7)
+        assert torch.equal(qa.mxfp4_linear(x, qa.mxfp4_quantize(w), bias), want)
+        xg, wg, bg = x.requires_grad_(), w.clone().requires_grad_(), bias.clone().requires_grad_()
+        y = qa.mxfp4_linear(xg, wg, bg)
+        assert torch.equal(y, want)
+        dx, dw, db = torch.autograd.grad(y, (xg, wg, bg), torch.ones_like(y))
+        assert dx.shape == x.shape and dw.shape == w.shape
+        assert torch.equal(db, torch.full_like(db, want.numel() // 7))
