@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define MXK_ABI_VERSION 13
+#define MXK_ABI_VERSION 14
 
 typedef enum {
   MXK_OK = 0,
@@ -516,9 +516,10 @@ int mxk_expert_gather(const void* x, int elem_bytes, int64_t tokens, int64_t col
                       const int32_t* order, int64_t rows, int top, void* out, void* stream);
 
 /* y [tokens][cols] = sum over j of gates[t][j] * h[place[t][j]] in float32
- * by ascending j (gates NULL: ones); places outside [0, rows) add nothing. */
+ * by ascending j (gates NULL: ones); places outside [0, rows) add nothing.
+ * y_type: h_type, or any for float32 rows. */
 int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* place, const float* gates,
-                       int64_t tokens, int top, int64_t cols, void* y, void* stream);
+                       int64_t tokens, int top, int64_t cols, int y_type, void* y, void* stream);
 
 /* Gradients of mxk_expert_combine: dh[place[t][j]] = gates[t][j] * dy[t],
  * zeros in rows that no place names; dgates[t][j] = <dy[t], h[place[t][j]]>, 0

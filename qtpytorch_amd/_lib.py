@@ -21,7 +21,7 @@ MXK_IN_F32, MXK_IN_F16, MXK_IN_BF16 = 0, 1, 2
 MXK_KIND_INT, MXK_KIND_FLOAT = 0, 1
 MXK_VAR_BASE, MXK_VAR_HADAMARD, MXK_VAR_VECTOR = 0, 1, 2
 MXK_DYN_PER_TOKEN, MXK_DYN_PER_CHANNEL, MXK_DYN_PER_TENSOR = 0, 1, 2
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 _lock = threading.Lock()
 _lib = None
@@ -94,7 +94,7 @@ SIGNATURES = {
     "mxk_expert_sort_workspace": (c_sz, [c_i64, c_int]),
     "mxk_expert_sort": (c_int, [c_vp, c_int, c_i64, c_int, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "mxk_expert_gather": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_int, c_vp, c_vp]),
-    "mxk_expert_combine": (c_int, [c_vp, c_int, c_i64, c_vp, c_vp, c_i64, c_int, c_i64, c_vp, c_vp]),
+    "mxk_expert_combine": (c_int, [c_vp, c_int, c_i64, c_vp, c_vp, c_i64, c_int, c_i64, c_int, c_vp, c_vp]),
     "mxk_expert_combine_grad": (c_int, [c_vp, c_vp, c_int, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_i64, c_vp, c_vp,
                                         c_vp]),
 }

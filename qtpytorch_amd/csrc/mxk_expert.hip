@@ -217,12 +217,13 @@ __device__ __forceinline__ void store8_nt(T* p, const float (&v)[8]) {
 // 4096 bf16, and slower for 4: 68 against 54): a pick without an expert reads row 0 in
 // place of a branch, and its values are replaced by zeros.  8000 tokens of 4096
 // bf16, 4 picks (328 MB): 55 us, 6.0 TB/s.
+// The result's type O is the rows' or, for float32 rows, any: rounded once.
 // WHOLE: columns in whole groups of 8 on 16 bytes.
-template <typename T, bool GATED, bool WHOLE>
+template <typename T, typename O, bool GATED, bool WHOLE>
 __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h, const int* __restrict__ place,
                                                         const float* __restrict__ gates, int top, int rows,
                                                         uint32_t total, DivU32 by_pieces, uint32_t pieces, int cols,
-                                                        T* __restrict__ y) {
+                                                        O* __restrict__ y) {
   const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
   if (i >= total) return;
   const uint32_t t = divu32((uint32_t)i, by_pieces), c = 8u * ((uint32_t)i - t * pieces);
@@ -473,7 +474,7 @@ int mxk_expert_gather(const void* x, int elem_bytes, int64_t tokens, int64_t col
 }
 
 int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* place, const float* gates,
-                       int64_t tokens, int top, int64_t cols, void* y, void* stream) {
+                       int64_t tokens, int top, int64_t cols, int y_type, void* y, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (tokens < 0 || top < 1 || cols < 0 || rows < 0 || rows >= ((int64_t)1 << 31) ||
       tokens >= ((int64_t)1 << 31) || tokens * top >= ((int64_t)1 << 31) || cols >= ((int64_t)1 << 28))
@@ -482,6 +483,8 @@ int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* p
   if ((rows > 0 && !h) || !place || !y) return fail(MXK_EINVAL, "expert_combine: null pointer");
   if (h_type != MXK_IN_F32 && h_type != MXK_IN_F16 && h_type != MXK_IN_BF16)
     return fail(MXK_EINVAL, "expert_combine: unknown h_type");
+  if (y_type != h_type && (h_type != MXK_IN_F32 || (y_type != MXK_IN_F16 && y_type != MXK_IN_BF16)))
+    return fail(MXK_EINVAL, "expert_combine: y of the rows' type, or any for float32 rows");
   const bool whole = cols % 8 == 0 && aligned16(h) && aligned16(y);
   const int64_t pieces = ceil_div(cols, 8), step = std::max<int64_t>(1, ((int64_t)1 << 31) / pieces - 1);
   const DivU32 bp = make_divu32((uint32_t)pieces);
@@ -490,19 +493,21 @@ int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* p
     const dim3 grid((unsigned)ceil_div(total, 256));
     const int* pl = place + t0 * top;
     const float* gt = gates ? gates + t0 * top : nullptr;
-#define MXK_CG(T, G)                                                                                              \
-  hipLaunchKernelGGL((whole ? k_expert_combine<T, G, true> : k_expert_combine<T, G, false>), grid, dim3(256), 0, \
-                     st, hp, pl, gt, top, (int)rows, total, bp, (uint32_t)pieces, (int)cols, yp)
-#define MXK_C(T)                                                                                                  \
+#define MXK_CG(T, O, G)                                                                                             \
+  hipLaunchKernelGGL((whole ? k_expert_combine<T, O, G, true> : k_expert_combine<T, O, G, false>), grid, dim3(256), \
+                     0, st, hp, pl, gt, top, (int)rows, total, bp, (uint32_t)pieces, (int)cols, yp)
+#define MXK_C(T, O)                                                                                               \
   do {                                                                                                            \
     const T* hp = reinterpret_cast<const T*>(h);                                                                  \
-    T* yp = reinterpret_cast<T*>(y) + t0 * cols;                                                                  \
-    if (gt) MXK_CG(T, true);                                                                                      \
-    else MXK_CG(T, false);                                                                                        \
+    O* yp = reinterpret_cast<O*>(y) + t0 * cols;                                                                  \
+    if (gt) MXK_CG(T, O, true);                                                                                   \
+    else MXK_CG(T, O, false);                                                                                     \
   } while (0)
-    if (h_type == MXK_IN_F32) MXK_C(float);
-    else if (h_type == MXK_IN_F16) MXK_C(__half);
-    else MXK_C(hip_bfloat16);
+    if (h_type == MXK_IN_F16) MXK_C(__half, __half);
+    else if (h_type == MXK_IN_BF16) MXK_C(hip_bfloat16, hip_bfloat16);
+    else if (y_type == MXK_IN_F16) MXK_C(float, __half);
+    else if (y_type == MXK_IN_BF16) MXK_C(float, hip_bfloat16);
+    else MXK_C(float, float);
 #undef MXK_C
 #undef MXK_CG
   }

@@ -111,16 +111,16 @@ def _gather(x: Tensor, plan: expert_plan) -> Tensor:
     return out
 
 
-def _combine(h: Tensor, plan: expert_plan, gates: Optional[Tensor]) -> Tensor:
-    place = plan.place
+def _combine(h: Tensor, plan: expert_plan, gates: Optional[Tensor], dtype: Optional[torch.dtype] = None) -> Tensor:
+    place, dtype = plan.place, dtype or h.dtype
     dev = L.require_gpu(h, gates, place)
     h = h.contiguous()
     tokens, top = place.shape
     rows, cols = h.shape
-    y = torch.empty((tokens, cols), dtype=h.dtype, device=dev)
+    y = torch.empty((tokens, cols), dtype=dtype, device=dev)
     with L.on_device(dev):
         rc = L.lib().mxk_expert_combine(h.data_ptr(), _FLOATS[h.dtype], rows, place.data_ptr(), L.ptr(gates), tokens,
-                                        top, cols, y.data_ptr(), L.stream_of(y))
+                                        top, cols, _FLOATS[dtype], y.data_ptr(), L.stream_of(y))
     if rc:
         L.check(rc, f"expert_combine({tokens}x{cols}, top {top})")
     return y
@@ -221,9 +221,10 @@ class _ExpertLinear(torch.autograd.Function):
         dy = dy.contiguous()
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
-            dx = _grad_a(dy, mxfp4_tensor._of(bc, bs, b_shape), x_dtype, plan.offsets)
+            # a token's rows are added in float32, where parts beyond float16's range may cancel
+            dx = _grad_a(dy, mxfp4_tensor._of(bc, bs, b_shape), torch.float32 if gather else x_dtype, plan.offsets)
             if gather:
-                dx = _combine(dx, plan, None)
+                dx = _combine(dx, plan, None, x_dtype)
         if ctx.needs_input_grad[1]:
             a = mxfp4_quantize(_gather(ac, plan)) if gather else mxfp4_tensor._of(ac, as_, a_shape)
             dw = _grad_b(dy, a, w_dtype, plan.offsets)

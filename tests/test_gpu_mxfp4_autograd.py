@@ -8,6 +8,8 @@ from tests.test_gpu_experts import _gen, _ids
 
 pytestmark = pytest.mark.gpu
 
+FLOATS = [torch.float32, torch.float16, torch.bfloat16]
+
 
 def _rand(*shape, seed=0, scale=1.0):
     return (torch.randn(*shape, generator=_gen(seed)) * scale).cuda()
@@ -129,3 +131,42 @@ def test_linear_over_rows_without_columns():
         dx, dw, db = torch.autograd.grad(y, (xg, wg, bg), torch.ones_like(y))
         assert dx.shape == x.shape and dw.shape == w.shape
         assert torch.equal(db, torch.full_like(db, want.numel() // 7))
+
+
+# ---------------------------------------------------------------- gathered rows
+def test_gathered_gradient_beyond_float16_in_its_parts():
+    """A token's rows are added in float32: parts above float16's range that cancel leave what is left."""
+    import qtpytorch_amd as qa
+    plan = qa.expert_sort(torch.tensor([[0, 1]] * 5).cuda(), 2)
+    x = torch.ones(5, 64, dtype=torch.float16, device="cuda", requires_grad=True)
+    w = torch.full((2, 8, 64), 4.0, device="cuda")
+    w[1] = -3.0
+    held = qa.mxfp4_quantize(w)
+    dy = torch.full((10, 8), 5000.0, dtype=torch.float16, device="cuda")
+    (dx,) = torch.autograd.grad(qa.expert_linear(x, held, plan, gather=True), x, dy)
+    # 8 columns of 5000 * 4 and of 5000 * -3, 160000 and -120000
+    assert torch.equal(dx, torch.full_like(dx, 40000.0))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("tokens,top,experts,n,k,dropped", [(1, 4, 8, 16, 32, 0.0), (64, 8, 16, 130, 320, 0.2),
+                                                            (200, 4, 3, 257, 543, 0.3), (300, 2, 8, 64, 96, 0.0)])
+def test_gathered_gradient_is_rounded_once(tokens, top, experts, n, k, dropped, dtype):
+    import qtpytorch_amd as qa
+    ids = _ids(tokens, top, experts, dropped=dropped)
+    order, place, offsets = R.plan(ids, experts)
+    x = _rand(tokens, k).to(dtype).requires_grad_()
+    w = _rand(experts, n, k, seed=1, scale=0.1)
+    dy = _rand(tokens * top, n, seed=2).to(dtype)
+    y = qa.expert_linear(x, qa.mxfp4_quantize(w), qa.expert_sort(ids.cuda(), experts), gather=True)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    assert dx.dtype == dtype
+    rw, d = R.rounded(w), dy.double().cpu()
+    rows, mass = (torch.zeros(tokens * top, k, dtype=torch.float64) for _ in range(2))
+    for e in range(experts):
+        lo, hi = int(offsets[e]), int(offsets[e + 1])
+        rows[lo:hi], mass[lo:hi] = d[lo:hi] @ rw[e], d[lo:hi].abs() @ rw[e].abs()
+    live = (place >= 0)[..., None]
+    parts = torch.where(live, rows[place.clamp(min=0)], 0.0)
+    masses = torch.where(live, mass[place.clamp(min=0)], 0.0)
+    R.assert_close(dx, parts.sum(1), masses.sum(1), 3 * (n / 8 + 2) + top)
