@@ -60,56 +60,52 @@ __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __re
   int* mine = start + wave * (E + 1);
   for (uint32_t i = lo + lane; i < hi; i += 64) atomicAdd(&mine[expert_of(ids[i], E)], 1);
   __syncthreads();
-  // experts in groups of 1024, one per thread: totals, exclusive scan, first places
-  int base = 0;
-  for (uint32_t e0 = 0; e0 < E; e0 += MXK_SORT_THREADS) {
-    const uint32_t e = e0 + tid;
-    int before = 0, total = 0;
-    if (e < E) {
-      if (gridDim.x > 1) {
-        for (uint32_t c0 = 0; c0 < gridDim.x; c0 += 16) {  // sixteen chunks' counts at a time
-          int n[16];
+  // an expert per thread (there are at most 1000): totals, exclusive scan, first places
+  int before = 0, total = 0;
+  if (tid < E) {
+    if (gridDim.x > 1) {
+      for (uint32_t c0 = 0; c0 < gridDim.x; c0 += 16) {  // sixteen chunks' counts at a time
+        int n[16];
 #pragma unroll
-          for (uint32_t k = 0; k < 16; ++k) n[k] = c0 + k < gridDim.x ? hist[(int64_t)(c0 + k) * E + e] : 0;
+        for (uint32_t k = 0; k < 16; ++k) n[k] = c0 + k < gridDim.x ? hist[(int64_t)(c0 + k) * E + tid] : 0;
 #pragma unroll
-          for (uint32_t k = 0; k < 16; ++k) {
-            total += n[k];
-            before += c0 + k < blockIdx.x ? n[k] : 0;
-          }
+        for (uint32_t k = 0; k < 16; ++k) {
+          total += n[k];
+          before += c0 + k < blockIdx.x ? n[k] : 0;
         }
-      } else {
-        for (int w = 0; w < MXK_SORT_WAVES; ++w) total += start[w * (E + 1) + e];
       }
+    } else {
+      for (int w = 0; w < MXK_SORT_WAVES; ++w) total += start[w * (E + 1) + tid];
     }
-    int scan = total;  // inclusive over the wave
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(scan, d);
-      if ((int)lane >= d) scan += up;
-    }
-    if (lane == 63) sums[wave] = scan;
-    __syncthreads();
-    int left = base;
-    for (uint32_t w = 0; w < MXK_SORT_WAVES; ++w) {
-      if (w < wave) left += sums[w];
-      base += sums[w];
-    }
-    if (e < E) {
-      const int at = left + scan - total;
-      if (blockIdx.x == 0) offsets[e] = at;
-      int next = at + before;
-      for (int w = 0; w < MXK_SORT_WAVES; ++w) {
-        const int n = start[w * (E + 1) + e];
-        start[w * (E + 1) + e] = next;
-        next += n;
-      }
-    }
-    __syncthreads();
   }
-  if (blockIdx.x == 0 && tid == 0) offsets[E] = base;
+  int scan = total;  // inclusive over the wave
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(scan, d);
+    if ((int)lane >= d) scan += up;
+  }
+  if (lane == 63) sums[wave] = scan;
+  __syncthreads();
+  int left = 0, used = 0;
+  for (uint32_t w = 0; w < MXK_SORT_WAVES; ++w) {
+    if (w < wave) left += sums[w];
+    used += sums[w];
+  }
+  if (tid < E) {
+    const int at = left + scan - total;
+    if (blockIdx.x == 0) offsets[tid] = at;
+    int next = at + before;
+    for (int w = 0; w < MXK_SORT_WAVES; ++w) {
+      const int n = start[w * (E + 1) + tid];
+      start[w * (E + 1) + tid] = next;
+      next += n;
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && tid == 0) offsets[E] = used;
   // places past the last one in use
   for (uint32_t i = first + tid; i < last; i += MXK_SORT_THREADS)
-    if (i >= (uint32_t)base) order[i] = -1;
+    if (i >= (uint32_t)used) order[i] = -1;
   const int bits = 32 - __builtin_clz(E | 1u);  // of 0 .. E
   for (uint32_t i0 = lo; i0 < hi; i0 += 64) {
     const uint32_t i = i0 + lane;
