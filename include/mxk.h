@@ -480,9 +480,10 @@ int mxk_mxfp4_linear(const void* x, int x_type, int64_t x_rows, int64_t x_stride
 size_t mxk_mxfp4_grad_workspace(const void* dy, int dy_type, int64_t M, int64_t N);
 
 /* da [M][K] (out_type) = dy [M][N] (dy_type) @ dequantize(b) [N][K]: the
- * gradient of a, straight through its quantization.  dy is not rounded,
- * sums are float32.  N below 2^22, K below 2^26.  By expert as mxk_mxfp4_matmul: b [experts][N][K], rows
- * of no expert zeros. */
+ * gradient of a, straight through its quantization.  dy is not rounded
+ * (float32 below 2^-110 counts down to 2^-133), sums are float32.
+ * N below 2^22, K below 2^26.  By expert as mxk_mxfp4_matmul: b
+ * [experts][N][K], rows of no expert zeros. */
 int mxk_mxfp4_grad_a(const void* dy, int dy_type, int64_t M, int64_t N, const void* b_codes, const void* b_scales,
                      int64_t K, int out_type, void* da, const int32_t* offsets, int experts, void* workspace,
                      size_t workspace_nbytes, void* stream);

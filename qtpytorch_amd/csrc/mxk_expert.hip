@@ -41,8 +41,8 @@ __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_count(const I* __re
 // shares' first places follow from the counts of the chunks before (`hist`,
 // which a single chunk does not need) and of the waves before, and a wave
 // then places 64 picks at a time, ranked among the lanes with the same expert by
-// ballots over the bits of the expert's number.  64 picks 4 us; 65536 picks of 128
-// experts 8 us and 3 for the counts.
+// ballots over the bits of the expert's number.  64 picks 3.5 us; 65536 picks of 128
+// experts 7.2 us and 3.1 for the counts.
 template <typename I>
 __global__ __launch_bounds__(MXK_SORT_THREADS) void k_expert_place(const I* __restrict__ ids, uint32_t P, uint32_t E,
                                                                    uint32_t chunk, const int* __restrict__ hist,
@@ -212,7 +212,7 @@ __device__ __forceinline__ void store8_nt(T* p, const float (&v)[8]) {
 // place of four were no faster for 8 picks a token, 101 us for 8000 tokens of
 // 4096 bf16, and slower for 4: 68 against 54): a pick without an expert reads row 0 in
 // place of a branch, and its values are replaced by zeros.  8000 tokens of 4096
-// bf16, 4 picks (328 MB): 55 us, 6.0 TB/s.
+// bf16, 4 picks (328 MB): 53 us, 6.1 TB/s.
 // The result's type O is the rows' or, for float32 rows, any: rounded once.
 // WHOLE: columns in whole groups of 8 on 16 bytes.
 template <typename T, typename O, bool GATED, bool WHOLE>
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256) void k_expert_combine(const T* __restrict__ h,
 // Zeros in the rows of dh that no place names: the picks dropped from a plan, the
 // rows past the last in use.  A place names row r if it is that of the pick
 // order[r]; should a plan's order not be the inverse of its places, the row of a place is
-// written over by the launch behind this one.  A workgroup looks at 32 rows: 1.6 us
+// written over by the launch behind this one.  A workgroup looks at 32 rows: 1.5 to 2.7 us
 // for 32000 rows that are all named, 15 where a quarter of them, 8 KB each, are not.
 // WHOLE: rows of whole aligned 16-byte pieces.
 template <bool WHOLE>
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(256) void k_expert_unnamed(const int* __restrict__ 
 // set of loads and stores and many tokens are under way (8 waves against 4 and
 // 1 for 4096 bf16: 8000 tokens of 4 picks 102, 106 and 125 us, 16 of 8 picks
 // 7.2, 8.3 and 20.7; 4000 of 2 picks 35, 30 and 30).  8000 tokens of 4 picks are
-// 590 MB, 5.6 TB/s.  The products of a lane are added in order of its columns,
+// 590 MB, 99 us, 6.0 TB/s.  The products of a lane are added in order of its columns,
 // then over the lanes of a wave and the waves of a token in a fixed order.
 // WHOLE: columns in whole groups of 8 on 16 bytes; dh is then written past the
 // caches.

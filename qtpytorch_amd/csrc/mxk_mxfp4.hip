@@ -7,8 +7,8 @@
 // wave stores 64 consecutive dwords of codes.  There is nothing to divide:
 // the scale is a power of two, so its exponent field comes from the bits of
 // the maximum and v_cvt_scalef32_pk_fp4_* rounds two elements at a time.
-// 16383x8192 bf16 (268 MB and 71 MB): quantize 56 us, dequantize 48, 6.1 and
-// 7.1 TB/s, above the 5.1 of a large copy.
+// 16383x8192 bf16 (268 MB and 71 MB): quantize 56 us, dequantize 48, 6.0 and
+// 7.0 TB/s, above the 5.1 of a large copy.
 #include "mxk_mxfp4.h"
 
 namespace mxk {

@@ -243,17 +243,21 @@ __device__ __forceinline__ void wait_loads_if(uint32_t counted) {
 //
 // A workgroup takes tile after tile.  Its next tile's place (and, by expert,
 // its rows) is looked up before the products of this one, and that tile's first
-// two stages are requested between the stores of this one's result.
+// two stages are requested between the stores of this one's result.  The
+// stores are not hidden behind its products, though: the compiler waits for all of
+// vector memory in front of a tile's first MFMA, where the sums start from a
+// bias that may be there or not, and by expert for the look-up's loads too.
 //
 // What an instruction loads and reads stands between single MFMAs, in their
 // shadow: in front of rows of four it took 5% longer.
 //
 // Bound by the matrix unit, whose rate falls with what the operands hold: this
 // instruction alone on random codes in registers 6.4 PFLOP/s, on zeros 9.1.
-// 8192x8192x8192 250 to 278 us (4.4 to 3.9 PFLOP/s; MFMAs 57% of the cycles,
-// waits 18%), 4000x4096x4096 43 us (3.1), 16000 rows over 32 experts of 4096x2048
-// 116 us (2.3: of a tile's 43000 cycles its eight stages take 29000, the stores
-// of all CUs at once 11000).
+// 8192x8192x8192 255 to 299 us (4.3 to 3.7 PFLOP/s; MFMAs 59% of the cycles,
+// waits 20%), 4000x4096x4096 43 us (3.1; MFMAs 45%, waits 30%), 16000 rows over
+// 32 experts of 4096x2048 116 us (2.3; MFMAs 35%, waits 26%: of a tile's
+// cycles its eight stages take some 29000, the stores of all CUs at once 11000).
+// 1500x1800x2080, one tile of 9 stages on 180 CUs, 13.9 us: MFMAs 11%, waits 48%.
 template <typename T, int F, bool EXPERT, bool STAGED>
 __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged in, int64_t b_rows, uint32_t tm,
                                                           uint32_t tn, uint32_t splits, uint32_t ids) {
@@ -271,7 +275,9 @@ __global__ __launch_bounds__(256, 1) void k_fp4_gemm_tile(Fp4Gemm p, Fp4Staged i
   // the 2 F parts of the next tile's first two stages
   constexpr int PASSES = F * PASS, STEP = PASSES / (2 * F);
   // memory operations of a wave complete in order: what may be due behind the
-  // last load of stage 0 (the stores from its pass on and stage 1), of stage 1
+  // last load of stage 0 (the stores from its pass on and stage 1), of stage 1.
+  // They are right by themselves; the compiler's own wait of today, which comes
+  // behind the first, leaves nothing due at the second.
   constexpr int BEHIND0 = LOADS + (PASSES - (F - 1) * STEP) * (CH / 2);
   constexpr int BEHIND1 = (PASSES - (2 * F - 1) * STEP) * (CH / 2);
   static_assert(STEP >= 1 && BEHIND0 <= 63, "a part for every pass, counts that the wait can hold");

@@ -6,7 +6,8 @@
 // dy is not quantized.  A code times its power-of-two scale has two
 // significant bits and is exact in bfloat16, so the product runs on bf16
 // MFMAs with dy as one bf16 term (bf16), two (f16) or three (f32) that add
-// up to it exactly: every product is exact, sums are in float32.
+// up to it exactly: every product is exact, sums are in float32.  (Of an f32 dy
+// below 2^-110 what lies under 2^-133, the smallest bf16, is left out.)
 //
 // The terms of f16 and f32 (and rows of bf16 that do not start on 16 bytes)
 // are laid out first as planes of aligned bf16 rows, whose sums simply
@@ -96,10 +97,11 @@ struct Fp4Grad {
 // take 8 consecutive rows, the transposing writes every eighth row.
 //
 // Bound by the matrix unit and by the conversions beside it (115 VALU a wave and
-// stage): 4000x4096x4096 of bf16 134 us for the gradient of a, 136 of b, 1.0
-// PFLOP/s (115 and 110 us in a row of calls without the profiler; 8192x8192x4096
+// stage): 4000x4096x4096 of bf16 131 us for the gradient of a, 134 of b, 1.0
+// PFLOP/s (115 and 116 us in a row of calls without the profiler; 8192x8192x4096
 // 426 us, 1.3), where the instruction alone runs at 1.75 on random values.  MFMAs
-// take 55% of the cycles, waits 14%.  f16 takes two, f32 three times that.
+// take 56% of the cycles, waits 15%.  f16 takes two, f32 three times that.  The
+// sum over t is one workgroup's whatever I is: 1 to 256 rows of 8192x8192 115 us.
 template <typename O, int F, bool OF_B>
 __global__ __launch_bounds__(256, 1) void k_fp4_grad(Fp4Grad p, uint32_t tm, uint32_t tn) {
   // LDS: L of either buffer, then V of either, so that a buffer and a fragment

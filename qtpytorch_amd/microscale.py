@@ -15,8 +15,9 @@ block of any length) are decoded first.
 
 ``mxfp4_linear`` passes gradients straight through the quantizer:
 ``dx = dy @ dequantize(weight)`` and, for a float weight, ``dw = dy.T @
-dequantize(quantize(x))``, both with dy unrounded and sums in float32.  There is
-no forward-mode derivative: a dual tensor is refused.
+dequantize(quantize(x))``, both with dy unrounded (a float32 dy below 2**-110
+counts down to 2**-133) and sums in float32.  There is no forward-mode
+derivative: a dual tensor is refused.
 """
 from __future__ import annotations
 
