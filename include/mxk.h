@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define MXK_ABI_VERSION 14
+#define MXK_ABI_VERSION 15
 
 typedef enum {
   MXK_OK = 0,
@@ -530,6 +530,77 @@ int mxk_expert_combine(const void* h, int h_type, int64_t rows, const int32_t* p
 int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t rows, const int32_t* order,
                             const int32_t* place, const float* gates, int64_t tokens, int top, int64_t cols, void* dh,
                             float* dgates, void* stream);
+
+/* ------------------------------------------------ rotary positions
+ * Pair i of the first 2*pairs elements of a head, (u, w) = (x[i], x[i+pairs])
+ * or, interleaved, (x[2i], x[2i+1]), becomes (u cos a - w sin a, w cos a +
+ * u sin a), a = pos[axis[i]] * freqs[i] reduced in float64; later elements stay.
+ * No counterpart in the reference.
+ */
+
+/* y [tokens][heads][D] (contiguous) = x rotated (backward: by the opposite
+ * angles, the gradient).  x: x_type, tokens token_stride and heads head_stride
+ * elements apart.  freqs float64 [pairs], axis int32 [pairs] (NULL: axis 0; an
+ * axis outside [0, axes) has position 0), pos [tokens][axes] of pos_bytes 4 or
+ * 8 (signed). */
+int mxk_rotary(const void* x, int x_type, int64_t tokens, int heads, int64_t D, int64_t token_stride,
+               int64_t head_stride, const double* freqs, const int32_t* axis, int pairs, int interleaved,
+               const void* pos, int pos_bytes, int axes, int backward, void* y, void* stream);
+
+/* ------------------------------------------------ paged 8-bit key-value cache
+ * codes int8 [pages][2][heads][page][D] (keys, values) and scales float32
+ * [pages][2][heads][page], value = code * scale, both on 16 bytes; page a
+ * power of two from 16 on, D 64, 128 or 256.  A batch, int32 on the device:
+ * table [B][width] the page of each run of `page` positions of a sequence,
+ * lengths [B] the positions it holds, offsets [B+1] (ascending) the first of
+ * each one's new tokens among the call's `tokens`; new token i of sequence b
+ * has position lengths[b] + i.  Pages outside [0, pages) and positions past
+ * the table hold nothing: they are not written, read as zeros and are not
+ * attended.  No counterpart in the reference.
+ */
+
+/* Keys and values of the batch's new tokens to their positions as
+ * round(x / scale), scale = max(max|x|, 1e-12) / 127 of a head's row; a row
+ * with a NaN or an infinity gets a scale of NaN and codes of 0.  k, v
+ * [tokens][heads][D] and q [tokens][q_heads][D] (q_heads 0: none) of x_type,
+ * their tokens and heads *_token and *_head elements apart.  Keys and queries are
+ * rotated first (mxk_rotary; pairs 0: not; pos NULL: the token's position); q_out
+ * [tokens][q_heads][D] takes the queries, zeros for tokens of no sequence. */
+int mxk_kv_pages_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                        int64_t v_head, const void* q, int64_t q_token, int64_t q_head, int q_heads, int x_type,
+                        void* codes, float* scales, int64_t pages, int page, int heads, int D, const int32_t* table,
+                        const int32_t* lengths, const int32_t* offsets, int64_t B, int64_t width, int64_t tokens,
+                        const double* freqs, const int32_t* axis, int pairs, int interleaved, const void* pos,
+                        int pos_bytes, int axes, void* q_out, void* stream);
+
+/* k, v [tokens][heads][D] (y_type) = the values at the batch's new positions. */
+int mxk_kv_pages_read(const void* codes, const float* scales, int64_t pages, int page, int heads, int D,
+                      const int32_t* table, const int32_t* lengths, const int32_t* offsets, int64_t B, int64_t width,
+                      int64_t tokens, int y_type, void* k, void* v, void* stream);
+
+/* Workspace bytes (16-byte aligned) mxk_kv_pages_attend needs (0 if none). */
+size_t mxk_kv_pages_attend_workspace(int64_t tokens, int64_t B, int64_t width, int page, int heads, int q_heads,
+                                     int D);
+
+/* out [tokens][q_heads][D] (q_type) = softmax(scale * q k^T) v over the keys
+ * that a new token sees: the lengths[b] held ones, and of the new ones (which
+ * are in the pages already) those up to itself, or with mask (uint64
+ * [tokens][words]) those whose bit j its words have.  Query head i reads head
+ * i / (q_heads / heads).  Rows that see nothing, and tokens of no sequence, are
+ * zeros; a row of q with a NaN or an infinity that sees a key is NaN.  Scores
+ * and sums float32, probabilities 11 significant bits (22 for float32 q). */
+int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_head, int q_heads, const void* codes,
+                        const float* scales, int64_t pages, int page, int heads, int D, const int32_t* table,
+                        const int32_t* lengths, const int32_t* offsets, int64_t B, int64_t width, int64_t tokens,
+                        const void* mask, int words, float scale, void* out, void* workspace,
+                        size_t workspace_nbytes, void* stream);
+
+/* Position lengths[b] + j takes the row of new token path[b][j] (int32
+ * [B][steps], steps at most 64), for entries inside [0, new tokens of b); all
+ * rows are read before any is written. */
+int mxk_kv_pages_keep(void* codes, float* scales, int64_t pages, int page, int heads, int D, const int32_t* table,
+                      const int32_t* lengths, const int32_t* offsets, int64_t B, int64_t width, int64_t tokens,
+                      const int32_t* path, int steps, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,7 @@ from .microscale import mxfp4_linear, mxfp4_matmul, mxfp4_quantize, mxfp4_tensor
 from .nn import (install_module_to, mx_dynamic_linear, mx_layer_norm, mx_linear, mx_multihead_attention,
                  mx_transformer_encoder_layer, to_mx, uninstall_module_to)
 from .ops import HADAMARD_DEQUANT_MODE, _dequant, quantize, vector_dequantize, vector_quantize
+from .pages import kv_batch, kv_pages, kv_tree_mask, rotary, rotary_table
 from .tensor import (_dispatch_qgemm, _mx_linear_forward, _mx_mm, _MXLinearAutograd, _QGemmSTE,
                      dynamic_quantize, fused_int8_linear, mx_fused_ops, mx_matmul, mx_quantize, mx_tensor)
 
@@ -34,4 +35,5 @@ __all__ = ["mx_dtype", "get_mx_dtype", "matmul_output_dtype", "mx_tensor", "quan
            "dynamic_quantize", "fused_int8_linear", "mx_fused_ops", "mx_dynamic_linear", "_MXLinearAutograd",
            "_mx_linear_forward", "mx_layer_norm", "mx_multihead_attention", "mx_transformer_encoder_layer",
            "vector_quantize", "vector_dequantize", "mxfp4_tensor", "mxfp4_quantize", "mxfp4_matmul", "mxfp4_linear",
-           "expert_plan", "expert_sort", "expert_gather", "expert_linear", "expert_combine", "mxfp4_expert_mlp"]
+           "expert_plan", "expert_sort", "expert_gather", "expert_linear", "expert_combine", "mxfp4_expert_mlp",
+           "rotary_table", "rotary", "kv_batch", "kv_pages", "kv_tree_mask"]

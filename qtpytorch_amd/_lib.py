@@ -21,7 +21,7 @@ MXK_IN_F32, MXK_IN_F16, MXK_IN_BF16 = 0, 1, 2
 MXK_KIND_INT, MXK_KIND_FLOAT = 0, 1
 MXK_VAR_BASE, MXK_VAR_HADAMARD, MXK_VAR_VECTOR = 0, 1, 2
 MXK_DYN_PER_TOKEN, MXK_DYN_PER_CHANNEL, MXK_DYN_PER_TENSOR = 0, 1, 2
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 _lock = threading.Lock()
 _lib = None
@@ -30,6 +30,7 @@ c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 c_vp = ctypes.c_void_p
 c_sz = ctypes.c_size_t
+c_float = ctypes.c_float
 
 # symbol -> (restype, argtypes)
 SIGNATURES = {
@@ -97,6 +98,18 @@ SIGNATURES = {
     "mxk_expert_combine": (c_int, [c_vp, c_int, c_i64, c_vp, c_vp, c_i64, c_int, c_i64, c_int, c_vp, c_vp]),
     "mxk_expert_combine_grad": (c_int, [c_vp, c_vp, c_int, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_i64, c_vp, c_vp,
                                         c_vp]),
+    "mxk_rotary": (c_int, [c_vp, c_int, c_i64, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_int, c_vp, c_int, c_int,
+                           c_int, c_vp, c_vp]),
+    "mxk_kv_pages_append": (c_int, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_int, c_vp, c_vp,
+                                    c_i64, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_int,
+                                    c_int, c_vp, c_int, c_int, c_vp, c_vp]),
+    "mxk_kv_pages_read": (c_int, [c_vp, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int,
+                                  c_vp, c_vp, c_vp]),
+    "mxk_kv_pages_attend_workspace": (c_sz, [c_i64, c_i64, c_i64, c_int, c_int, c_int, c_int]),
+    "mxk_kv_pages_attend": (c_int, [c_vp, c_int, c_i64, c_i64, c_int, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_vp,
+                                    c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_float, c_vp, c_vp, c_sz, c_vp]),
+    "mxk_kv_pages_keep": (c_int, [c_vp, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp,
+                                  c_int, c_vp]),
 }
 
 

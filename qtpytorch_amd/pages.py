@@ -1,0 +1,406 @@
+"""Serving from a paged 8-bit key-value cache: rotary positions, new tokens into
+the pages, attention over them, and the accepted path of a drafted tree.
+
+  rotary_table(freqs, axis)          how positions turn a head's pairs
+  rotary(x, positions, table)        heads rotated; differentiable
+  kv_batch(table, lengths, offsets)  the sequences of a step
+  kv_pages(codes, scales)            the pool of pages (kv_pages.empty makes one)
+    .append(k, v, batch, ...)        keys (and queries) rotated, keys and values packed
+    .attend(q, batch, mask)          attention of the new tokens, causal or by a mask
+    .keep(batch, path)               accepted drafted tokens moved behind the context
+    .read(batch, tokens)             values of positions
+
+``kv_cache_quantizer`` holds one batch's steps in a ring and gives them back
+as float32; here sequences share a pool, and the attention reads the codes
+as they lie.  No call waits for the GPU: lengths and pages stay on the
+device, so that a step can be recorded in a graph and replayed with others.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional, Sequence, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from .microscale import _FLOATS, _no_tangents
+
+Tensor = torch.Tensor
+
+_HEADS = (64, 128, 256)
+_MANY = (1 << 31) - 65  # more tokens than a batch has
+
+
+# ---------------------------------------------------------------- rotary positions
+class rotary_table:
+    """Angles of rotary positions: pair i of a head turns by ``freqs[i]`` radians
+    for each position on axis ``axis[i]``.
+
+    freqs float64 [pairs] and axis int32 [pairs] (None: one axis) on the GPU.
+    Pair i is elements (i, i + pairs), or (2i, 2i + 1) where ``interleaved``;
+    a head's elements from 2 * pairs on are not rotated."""
+
+    __slots__ = ("freqs", "axis", "interleaved")
+
+    def __init__(self, freqs: Tensor, axis: Optional[Tensor] = None, *, interleaved: bool = False):
+        if freqs.dtype != torch.float64 or freqs.dim() != 1:
+            raise TypeError(f"rotary_table: freqs [pairs] in float64 expected, got {tuple(freqs.shape)} in {freqs.dtype}")
+        if axis is not None and (axis.dtype != torch.int32 or axis.shape != freqs.shape):
+            raise TypeError(f"rotary_table: axis [pairs] in int32 expected, got {tuple(axis.shape)} in {axis.dtype}")
+        L.require_gpu(freqs, axis)
+        self.freqs = freqs.contiguous()
+        self.axis = None if axis is None else axis.contiguous()
+        self.interleaved = bool(interleaved)
+
+    @classmethod
+    def make(cls, rotated: int, base: float = 10000.0, *, sections: Optional[Sequence[int]] = None,
+             restart: bool = False, interleaved: bool = False, device="cuda") -> "rotary_table":
+        """The table of frequencies base ** (-i / pairs) for the pairs i of `rotated` elements.
+
+        sections: how many pairs each axis has, one after the other (time,
+        height, width); restart begins each axis' frequencies anew, as for
+        images whose axes are alike."""
+        if rotated < 0 or rotated % 2:
+            raise ValueError(f"rotary_table: an even number of rotated elements expected, got {rotated}")
+        pairs = rotated // 2
+        if sections is not None and (sum(sections) != pairs or any(s < 0 for s in sections)):
+            raise ValueError(f"rotary_table: sections that add up to {pairs} pairs expected, got {tuple(sections)}")
+        parts = [pairs] if sections is None else list(sections)
+        spans = parts if restart else [pairs] * len(parts)
+        freqs, axis, first = [], [], 0
+        for a, (n, span) in enumerate(zip(parts, spans)):
+            freqs += [float(base) ** (-(i if restart else first + i) / span) for i in range(n)]
+            axis += [a] * n
+            first += n
+        return cls(torch.tensor(freqs, dtype=torch.float64, device=device),
+                   None if sections is None else torch.tensor(axis, dtype=torch.int32, device=device),
+                   interleaved=interleaved)
+
+    def __repr__(self):
+        return f"rotary_table(pairs={self.freqs.numel()}, interleaved={self.interleaved})"
+
+
+def _positions(name: str, positions: Tensor, lead) -> Tuple[Tensor, int]:
+    """Contiguous positions and their number of axes; lead: the shape of the tokens."""
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name}: positions are int32 or int64, got {positions.dtype}")
+    if positions.shape == lead:
+        axes = 1
+    elif positions.dim() == len(lead) + 1 and positions.shape[:-1] == lead and positions.shape[-1] > 0:
+        axes = positions.shape[-1]
+    else:
+        raise ValueError(f"{name}: positions {tuple(lead)}, or with their axes last, expected, got "
+                         f"{tuple(positions.shape)}")
+    return positions.contiguous(), axes
+
+
+def _token_rows(x: Tensor) -> Tensor:
+    """x [..., H, D] as [tokens, H, D] with D contiguous, without a copy where its strides allow."""
+    if x.dim() != 3:
+        x = x.reshape(math.prod(x.shape[:-2]), *x.shape[-2:])
+    return x if x.stride(2) == 1 or x.shape[2] <= 1 else x.contiguous()
+
+
+def _rotary(x: Tensor, positions: Tensor, axes: int, table: rotary_table, backward: bool) -> Tensor:
+    freqs, axis = table.freqs, table.axis
+    dev = L.require_gpu(x, positions, freqs, axis)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    rows = _token_rows(x)
+    tokens, H, D = rows.shape
+    with L.on_device(dev):
+        rc = L.lib().mxk_rotary(rows.data_ptr(), _FLOATS[x.dtype], tokens, H, D, rows.stride(0), rows.stride(1),
+                                freqs.data_ptr(), L.ptr(axis), freqs.numel(), table.interleaved, positions.data_ptr(),
+                                positions.element_size(), axes, backward, y.data_ptr(), L.stream_of(y))
+    if rc:
+        L.check(rc, f"rotary({tokens}x{H}x{D})")
+    return y
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, axes, table):
+        ctx.save_for_backward(positions)
+        ctx.axes, ctx.table = axes, table
+        return _rotary(x.detach(), positions, axes, table, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (positions,) = ctx.saved_tensors
+        return _rotary(dy, positions, ctx.axes, ctx.table, True), None, None, None
+
+
+def rotary(x: Tensor, positions: Tensor, table: rotary_table) -> Tensor:
+    """Heads x [..., heads, D] (float32, float16 or bfloat16, any strides)
+    rotated by their tokens' positions [...] or [..., axes] (int32 or int64).
+
+    Angles are reduced in float64, so that far positions keep them; products
+    and sums are float32, rounded once.  The gradient is the opposite rotation
+    of the output's."""
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"rotary: float32, float16 or bfloat16 expected, got {x.dtype}")
+    if x.dim() < 2:
+        raise ValueError(f"rotary: [..., heads, D] expected, got {tuple(x.shape)}")
+    _no_tangents("rotary", x)
+    positions, axes = _positions("rotary", positions, x.shape[:-2])
+    if 2 * table.freqs.numel() > x.shape[-1]:
+        raise ValueError(f"rotary: the table rotates {2 * table.freqs.numel()} elements, a head has {x.shape[-1]}")
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Rotary.apply(x, positions, axes, table)
+    return _rotary(x, positions, axes, table, False)
+
+
+# ---------------------------------------------------------------- the paged cache
+class kv_batch(NamedTuple):
+    """The sequences of one step, int32 tensors on the GPU.
+
+    table    [B, width]  page of each run of page_size positions; entries that
+                         a sequence does not use may be anything outside the pool (-1)
+    lengths  [B]         positions each sequence holds before the step
+    offsets  [B + 1]     ascending: sequence b's new tokens are rows offsets[b] to
+                         offsets[b + 1] of the step's tensors (none for an idle one)
+
+    New token i of sequence b has position lengths[b] + i.  Rows in front of
+    offsets[0] and from offsets[B] on are padding: nothing is stored for them,
+    and results have zeros there."""
+    table: Tensor
+    lengths: Tensor
+    offsets: Tensor
+
+
+def kv_tree_mask(parents: Sequence[int], device="cuda") -> Tuple[Tensor, Tensor]:
+    """Mask words int64 [n, words] and depths int32 [n] of a tree of drafted
+    tokens: parents[i] < i, or negative for a root.  A token sees itself and the
+    tokens on its way from the root.  Host data to device tensors: made once for a
+    tree, repeated for the sequences that draft with it."""
+    seen, depth = [], []
+    for i, p in enumerate(parents):
+        p = int(p)
+        if p >= i:
+            raise ValueError(f"kv_tree_mask: token {i} comes before its parent {p}")
+        seen.append((seen[p] if p >= 0 else 0) | 1 << i)
+        depth.append(depth[p] + 1 if p >= 0 else 0)
+    words = max(1, -(-len(seen) // 64))
+    full = (1 << 64) - 1
+    rows = [[(m >> 64 * w & full) - (1 << 64 if m >> 64 * w + 63 & 1 else 0) for w in range(words)] for m in seen]
+    return (torch.tensor(rows, dtype=torch.int64, device=device).view(-1, words),
+            torch.tensor(depth, dtype=torch.int32, device=device))
+
+
+def _check_batch(name: str, batch: kv_batch) -> None:
+    table, lengths, offsets = batch
+    if not (table.dtype == lengths.dtype == offsets.dtype == torch.int32
+            and table.is_contiguous() and lengths.is_contiguous() and offsets.is_contiguous()):
+        raise TypeError(f"{name}: a batch's tensors are contiguous int32, got {table.dtype}, {lengths.dtype} and "
+                        f"{offsets.dtype}")
+    if table.dim() != 2 or lengths.shape != table.shape[:1] or offsets.shape != (table.shape[0] + 1,):
+        raise ValueError(f"{name}: a batch has table [B, width], lengths [B] and offsets [B + 1], got "
+                         f"{tuple(table.shape)}, {tuple(lengths.shape)} and {tuple(offsets.shape)}")
+
+
+class kv_pages:
+    """A pool of pages of 8-bit keys and values: ``codes`` int8 [pages, 2, heads,
+    page_size, head_dim] (keys, then values) and ``scales`` float32 [pages, 2,
+    heads, page_size], value = code * scale, as kv_cache_quantizer's "int8dv".
+
+    page_size is a power of two from 16 on, head_dim 64, 128 or 256.  Which
+    sequence has which page is the caller's: pages are named by a kv_batch alone.
+    A page may stand in several tables (a shared prefix) while nobody writes to it."""
+
+    __slots__ = ("codes", "scales")
+
+    def __init__(self, codes: Tensor, scales: Tensor):
+        if codes.dtype != torch.int8 or scales.dtype != torch.float32:
+            raise TypeError(f"kv_pages: int8 codes and float32 scales expected, got {codes.dtype} and {scales.dtype}")
+        shape = codes.shape
+        if len(shape) != 5 or shape[1] != 2 or scales.shape != shape[:-1]:
+            raise ValueError(f"kv_pages: codes [pages, 2, heads, page_size, head_dim] and scales [pages, 2, heads, "
+                             f"page_size] expected, got {tuple(shape)} and {tuple(scales.shape)}")
+        if shape[2] < 1 or shape[3] < 16 or shape[3] & (shape[3] - 1) or shape[4] not in _HEADS:
+            raise ValueError(f"kv_pages: one head at least, a page of a power of two of positions from 16 on and heads "
+                             f"of 64, 128 or 256 expected, got {tuple(shape)}")
+        if not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("kv_pages: codes and scales are written in place: contiguous tensors expected")
+        L.require_gpu(codes, scales)
+        if codes.data_ptr() % 16 or scales.data_ptr() % 16:
+            raise ValueError("kv_pages: codes and scales start on 16 bytes")
+        self.codes, self.scales = codes, scales
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, n_heads: int, head_dim: int, device="cuda") -> "kv_pages":
+        """A pool of its own; what its pages hold before they are written is never attended."""
+        return cls(torch.empty(n_pages, 2, n_heads, page_size, head_dim, dtype=torch.int8, device=device),
+                   torch.empty(n_pages, 2, n_heads, page_size, dtype=torch.float32, device=device))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + 4 * self.scales.numel()
+
+    def _pool(self):
+        n, _, H, page, D = self.codes.shape
+        return self.codes.data_ptr(), self.scales.data_ptr(), n, page, H, D
+
+    def _rows(self, name: str, what: str, x: Tensor, heads: Optional[int] = None) -> Tensor:
+        D = self.codes.shape[4]
+        if x.dim() != 3 or x.shape[2] != D or heads is not None and x.shape[1] != heads:
+            raise ValueError(f"{name}: {what} [tokens, {'heads' if heads is None else heads}, {D}] expected, got "
+                             f"{tuple(x.shape)}")
+        x = x.detach()
+        return x if x.stride(2) == 1 else x.contiguous()
+
+    def _queries(self, name: str, q: Tensor) -> Tensor:
+        H = self.codes.shape[2]
+        q = self._rows(name, "q", q)
+        if q.shape[1] < H or q.shape[1] % H:
+            raise ValueError(f"{name}: query heads in groups of one size for each of {H} heads expected, got {q.shape[1]}")
+        return q
+
+    def append(self, k: Tensor, v: Tensor, batch: kv_batch, *, rotary: Optional[rotary_table] = None,
+               positions: Optional[Tensor] = None, q: Optional[Tensor] = None) -> Optional[Tensor]:
+        """Store the new tokens' keys and values k, v [tokens, heads, head_dim]
+        (float32, float16 or bfloat16, heads contiguous) at their positions.
+
+        With a rotary table keys are rotated on the way, by positions [tokens] or
+        [tokens, axes] (None: each token's position in its sequence, on every
+        axis); they are packed from the unrounded rotation.  q [tokens, q_heads,
+        head_dim] is rotated along and returned.  A head's row with a NaN or an
+        infinity reads as NaN.  Nothing is differentiable."""
+        H = self.codes.shape[2]
+        if k.dtype not in _FLOATS or v.dtype != k.dtype or q is not None and q.dtype != k.dtype:
+            raise TypeError(f"kv_pages.append: keys, values and queries of one type (float32, float16 or bfloat16) "
+                            f"expected, got {k.dtype}, {v.dtype}{'' if q is None else f' and {q.dtype}'}")
+        k, v = self._rows("kv_pages.append", "k", k, H), self._rows("kv_pages.append", "v", v, H)
+        T = k.shape[0]
+        if q is not None:
+            q = self._queries("kv_pages.append", q)
+        if v.shape[0] != T or q is not None and q.shape[0] != T:
+            raise ValueError(f"kv_pages.append: one row for each of {T} tokens expected, got {v.shape[0]} of v"
+                             f"{'' if q is None else f' and {q.shape[0]} of q'}")
+        _check_batch("kv_pages.append", batch)
+        freqs = axis = None
+        pairs = axes = 0
+        if rotary is not None:
+            freqs, axis, pairs = rotary.freqs, rotary.axis, rotary.freqs.numel()
+            if 2 * pairs > self.codes.shape[4]:
+                raise ValueError(f"kv_pages.append: the table rotates {2 * pairs} elements, a head has "
+                                 f"{self.codes.shape[4]}")
+            if positions is not None:
+                positions, axes = _positions("kv_pages.append", positions, (T,))
+        elif positions is not None or q is not None:
+            raise ValueError("kv_pages.append: positions and queries go with a rotary table")
+        dev = L.require_gpu(self.codes, k, v, q, positions, freqs, axis, *batch)
+        out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=dev)
+        codes, scales, n, page, _, D = self._pool()
+        table, lengths, offsets = batch
+        qt, qh, Hq = (0, 0, 0) if q is None else (q.stride(0), q.stride(1), q.shape[1])
+        with L.on_device(dev):
+            rc = L.lib().mxk_kv_pages_append(
+                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), L.ptr(q), qt, qh, Hq,
+                _FLOATS[k.dtype], codes, scales, n, page, H, D, table.data_ptr(), lengths.data_ptr(),
+                offsets.data_ptr(), table.shape[0], table.shape[1], T, L.ptr(freqs), L.ptr(axis), pairs,
+                rotary is not None and rotary.interleaved, L.ptr(positions),
+                0 if positions is None else positions.element_size(), axes, L.ptr(out), L.stream_of(k))
+        if rc:
+            L.check(rc, f"kv_pages.append({T} tokens, {H} heads of {D})")
+        return out
+
+    def attend(self, q: Tensor, batch: kv_batch, *, mask: Optional[Tensor] = None,
+               scale: Optional[float] = None) -> Tensor:
+        """Attention of the new tokens' queries q [tokens, q_heads, head_dim]
+        over the pages of their sequences, whose new keys and values are stored
+        already (append).  q_heads is a multiple of the pool's heads: query
+        head i reads head i // (q_heads // heads).
+
+        A token sees all positions its sequence held before the step, and of
+        the step's own tokens those up to itself; with mask (int64 [tokens,
+        words]) those, in any order, whose bit is set: bit j % 64 of word j // 64
+        is new token j of the same sequence.  scale: of the scores, 1 /
+        sqrt(head_dim) unless given.  A row that sees nothing is zeros.
+
+        Codes are used as they are, q to 16 bits of its row's largest element
+        (24 where it is float32), probabilities to 11 bits (22), sums in float32.
+        Nothing is differentiable."""
+        if q.dtype not in _FLOATS:
+            raise TypeError(f"kv_pages.attend: float32, float16 or bfloat16 expected, got {q.dtype}")
+        q = self._queries("kv_pages.attend", q)
+        _check_batch("kv_pages.attend", batch)
+        T, Hq, D = q.shape
+        words = 0
+        if mask is not None:
+            if mask.dtype != torch.int64:
+                raise TypeError(f"kv_pages.attend: a mask of int64 words expected, got {mask.dtype}")
+            if mask.dim() != 2 or mask.shape[0] != T or mask.shape[1] < 1:
+                raise ValueError(f"kv_pages.attend: a mask [{T}, words] expected, got {tuple(mask.shape)}")
+            mask = mask.contiguous()
+            words = mask.shape[1]
+        scale = D ** -0.5 if scale is None else float(scale)
+        if not (scale > 0.0 and math.isfinite(scale)):
+            raise ValueError(f"kv_pages.attend: a positive scale expected, got {scale}")
+        table, lengths, offsets = batch
+        dev = L.require_gpu(self.codes, q, mask, *batch)
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+        codes, scales, n, page, H, _ = self._pool()
+        lib = L.lib()
+        B, width = table.shape
+        nbytes = lib.mxk_kv_pages_attend_workspace(T, B, width, page, H, Hq, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with L.on_device(dev):
+            rc = lib.mxk_kv_pages_attend(q.data_ptr(), _FLOATS[q.dtype], q.stride(0), q.stride(1), Hq, codes, scales, n,
+                                         page, H, D, table.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), B, width,
+                                         T, L.ptr(mask), words, scale, out.data_ptr(), L.ptr(ws), nbytes,
+                                         L.stream_of(out))
+        if rc:
+            L.check(rc, f"kv_pages.attend({T} tokens, {Hq} heads of {D})")
+        return out
+
+    def keep(self, batch: kv_batch, path: Tensor) -> None:
+        """Move the accepted tokens of a step behind the context: position
+        lengths[b] + j takes the keys and values of the step's token path[b, j]
+        (int32 [B, steps], at most 64 steps; an entry outside the sequence's new
+        tokens, as -1, moves nothing).  All are read before any is written.  The
+        caller then adds the number accepted to lengths."""
+        _check_batch("kv_pages.keep", batch)
+        table, lengths, offsets = batch
+        if path.dtype != torch.int32:
+            raise TypeError(f"kv_pages.keep: a path of int32 expected, got {path.dtype}")
+        if path.dim() != 2 or path.shape[0] != table.shape[0]:
+            raise ValueError(f"kv_pages.keep: a path [{table.shape[0]}, steps] expected, got {tuple(path.shape)}")
+        path = path.contiguous()
+        dev = L.require_gpu(self.codes, path, *batch)
+        codes, scales, n, page, H, D = self._pool()
+        with L.on_device(dev):
+            rc = L.lib().mxk_kv_pages_keep(codes, scales, n, page, H, D, table.data_ptr(), lengths.data_ptr(),
+                                           offsets.data_ptr(), table.shape[0], table.shape[1], _MANY, path.data_ptr(),
+                                           path.shape[1], L.stream_of(path))
+        if rc:
+            L.check(rc, f"kv_pages.keep({tuple(path.shape)})")
+
+    def read(self, batch: kv_batch, tokens: int, dtype: torch.dtype = torch.bfloat16) -> Tuple[Tensor, Tensor]:
+        """Keys and values [tokens, heads, head_dim] at positions lengths[b] + i,
+        row offsets[b] + i; zeros where there is none.  (A sequence's whole history:
+        lengths of 0 and offsets that count it.)  tokens: rows of the result."""
+        _check_batch("kv_pages.read", batch)
+        if tokens < 0:
+            raise ValueError(f"kv_pages.read: a number of tokens expected, got {tokens}")
+        kind = L.elem_type(dtype)
+        dev = L.require_gpu(self.codes, *batch)
+        codes, scales, n, page, H, D = self._pool()
+        table, lengths, offsets = batch
+        k = torch.empty((tokens, H, D), dtype=dtype, device=dev)
+        v = torch.empty((tokens, H, D), dtype=dtype, device=dev)
+        with L.on_device(dev):
+            rc = L.lib().mxk_kv_pages_read(codes, scales, n, page, H, D, table.data_ptr(), lengths.data_ptr(),
+                                           offsets.data_ptr(), table.shape[0], table.shape[1], tokens, kind,
+                                           k.data_ptr(), v.data_ptr(), L.stream_of(k))
+        if rc:
+            L.check(rc, f"kv_pages.read({tokens} tokens)")
+        return k, v
+
+    def __repr__(self):
+        n, _, H, page, D = self.codes.shape
+        return f"kv_pages(pages={n}, page_size={page}, heads={H}, head_dim={D}, device={self.device})"
