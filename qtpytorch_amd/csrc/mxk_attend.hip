@@ -36,10 +36,10 @@ namespace mxk {
 
 typedef int i32x4a __attribute__((ext_vector_type(4)));
 typedef float f32x4a __attribute__((ext_vector_type(4)));
+typedef float f32x16a __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x2a __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8a __attribute__((ext_vector_type(8)));
 
-#define MXK_KEYS 128  // keys of a block
 
 struct AttendArgs {
   const void* q;
@@ -50,7 +50,8 @@ struct AttendArgs {
   int words;
   float scale;  // of the scores, times log2(e)
   int Hq, G;    // query heads; of one key head
-  int TT, GC, chunks;  // a tile: TT tokens (a power of two) of GC heads, chunks of them over G
+  int keys;            // of a block: 128 or 256
+  int TT, GC, chunks;  // a tile: TT tokens (a power of two, at most keys) of GC heads, chunks of them over G
   void* out;
   float* part_o;  // [shares][2][rows][D], of their own maximum
   float2* part_s;  // [shares][2][rows]: maximum, sum
@@ -64,7 +65,7 @@ __device__ __forceinline__ int64_t sum_floor(int64_t x, int s) {
 }
 
 struct Line {
-  int rs;  // log2(MXK_KEYS / TT)
+  int rs;  // log2(keys / TT)
   int ts;  // log2(TT)
   int64_t cap;   // positions of the table
   int64_t most;  // blocks that a tile has at most: the table's, at least one.  The workspace is sized by it.
@@ -98,9 +99,9 @@ __device__ __forceinline__ SeqWork seq_work(const AttendArgs& A, const Line& L, 
   w.n = kv_count(A.batch, b);
   w.ctx = min(max((int64_t)A.batch.lengths[b], (int64_t)0), L.cap);
   w.tiles = (w.n + A.TT - 1) >> L.ts;
-  w.a = (w.ctx + A.TT + MXK_KEYS - 1) >> L.ts;
+  w.a = (w.ctx + A.TT + A.keys - 1) >> L.ts;
   w.full = max((int64_t)0, (L.most << L.rs) - w.a);
-  w.blocks = min((w.ctx + w.n + MXK_KEYS - 1) / MXK_KEYS, L.most);
+  w.blocks = min((w.ctx + w.n + A.keys - 1) >> (L.ts + L.rs), L.most);
   w.head = blocks_below(A, L, w, w.tiles);
   return w;
 }
@@ -108,9 +109,9 @@ __device__ __forceinline__ SeqWork seq_work(const AttendArgs& A, const Line& L, 
 __device__ __forceinline__ Line make_line(const AttendArgs& A) {
   Line L;
   L.ts = 31 - __builtin_clz(A.TT);
-  L.rs = 31 - __builtin_clz(MXK_KEYS / A.TT);
+  L.rs = 31 - __builtin_clz(A.keys) - L.ts;
   L.cap = (int64_t)A.batch.width << A.pool.shift;
-  L.most = max((int64_t)1, (L.cap + MXK_KEYS - 1) / MXK_KEYS);
+  L.most = max((int64_t)1, (L.cap + A.keys - 1) >> (L.ts + L.rs));
   return L;
 }
 
@@ -392,6 +393,32 @@ __device__ __forceinline__ bool tile_row(const AttendArgs& A, const SeqWork& w, 
   return i < A.TT && tok < w.n && hh < A.G;
 }
 
+// Rows of tokens that no sequence has
+template <typename T, int D, int THREADS>
+__device__ __forceinline__ void zero_padding(const AttendArgs& A, int shares) {
+  const int B = A.batch.B;
+  const int lo = B ? min(max(A.batch.offsets[0], 0), A.batch.T) : 0;
+  const int hi = B ? min(max(A.batch.offsets[B], 0), A.batch.T) : 0;
+  const int64_t row = (int64_t)A.Hq * D, n = (lo + (A.batch.T - hi)) * row;
+  T* out = reinterpret_cast<T*>(A.out);
+  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)shares * THREADS)
+    out[i < lo * row ? i : i - lo * row + hi * row] = out_cvt<T>(0.0f);
+}
+
+// The next tile on the line (there is one)
+__device__ __forceinline__ void next_tile(const AttendArgs& A, const Line& L, SeqWork& w, Place& p) {
+  p.k = 0;
+  if (++p.x == w.tiles * A.chunks) {
+    p.x = 0;
+    if (++p.h == A.pool.H) {
+      p.h = 0;
+      do ++p.b, w = seq_work(A, L, p.b);
+      while (w.head == 0);
+    }
+  }
+  p.blocks = tile_blocks(A, L, w, p.x / A.chunks);
+}
+
 // Tiles of 16 rows
 template <typename T, int D, int QT, int PT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A, int shares) {
@@ -405,16 +432,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A, 
   const int64_t per = line_share(total, shares);
   const int64_t from = (int64_t)blockIdx.x * per, to = min(total, from + per);
 
-  // tokens of no sequence: zeros
-  {
-    const int B = A.batch.B;
-    const int lo = B ? min(max(A.batch.offsets[0], 0), A.batch.T) : 0;
-    const int hi = B ? min(max(A.batch.offsets[B], 0), A.batch.T) : 0;
-    const int64_t row = (int64_t)A.Hq * D, n = (lo + (A.batch.T - hi)) * row;
-    T* out = reinterpret_cast<T*>(A.out);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)shares * 256)
-      out[i < lo * row ? i : i - lo * row + hi * row] = out_cvt<T>(0.0f);
-  }
+  zero_padding<T, D, 256>(A, shares);
   if (from >= to) return;
 
   SeqWork w;
@@ -440,8 +458,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A, 
     st.m = -__builtin_inff();
     st.l = 0.0f;
     st.e = -100;  // smaller scales lose bits
-    int64_t key = p.k * MXK_KEYS + wave * 32;
-    const int64_t stop = min(end, k1 * MXK_KEYS);
+    int64_t key = p.k * 128 + wave * 32;
+    const int64_t stop = min(end, k1 * 128);
     if (key < stop) {
       Keys32<D> cur, nxt;
       int page[2];
@@ -449,7 +467,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A, 
       for (int a = 0; a < 2; ++a) page[a] = kv_page(A.batch, A.pool, p.b, (key + 16 * a) >> A.pool.shift);
       load_keys<D>(A.pool, p.h, key, page, lane, cur);
       while (true) {
-        const int64_t next = key + MXK_KEYS;
+        const int64_t next = key + 128;
         const bool more = next < stop;
         if (more) {
 #pragma unroll
@@ -508,17 +526,368 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A, 
     at += k1 - p.k;
     if (at >= to) break;
     __syncthreads();
-    // the next tile on the line
-    p.k = 0;
-    if (++p.x == w.tiles * A.chunks) {
-      p.x = 0;
-      if (++p.h == A.pool.H) {
-        p.h = 0;
-        do ++p.b, w = seq_work(A, L, p.b);
-        while (w.head == 0);
-      }
+    next_tile(A, L, w, p);
+  }
+}
+
+// ---------------------------------------------------------------- tiles of many rows
+// NW waves of 32 rows each share the keys, 64 at a time: their codes are
+// made float16 (code * 2^-9, exact) once for the workgroup on the way into LDS,
+// values transposed, and both products run on the 32x32x16 MFMA.  As above S^T
+// leaves a lane with one row's keys, which are the second product's operand as
+// they are; only the keys' order in LDS follows it: values lie by element, and
+// there 16 keys s of a block as two runs of 8, keys 16s + 4h + {0..3, 8..11} for
+// the lanes' half h.
+//
+// Element d of the values is row (d % 4) * (D/4) + d / 4 of LDS: a thread reads
+// four elements of four keys, and its writes, like the MFMA's reads, take
+// rows that follow each other.  16-byte pieces are swizzled so that neither
+// meets itself in a bank.
+#define MXK_TILE 64
+
+template <typename T, int D, int QT>
+__device__ __forceinline__ void query_halves(const T* __restrict__ row, int h, f16x8a (&q)[QT][D / 16], float& unit) {
+  float x[D / 16][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    T e[8];
+    if (row) __builtin_memcpy(e, row + i * 16 + h * 8, sizeof(e));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[i][j] = row ? ElemT<T>::cvt(e[j]) : 0.0f;
+      m = max(m, mag_bits(x[i][j]));
     }
-    p.blocks = tile_blocks(A, L, w, p.x / A.chunks);
+  }
+  m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+  // a power of two takes the largest to 2^14 .. 2^15; zeros and NaN as in query_terms
+  const bool some = m >= 0x0D800000u && m < 0x7F800000u;
+  const int e = some ? (int)(m >> 23) - 127 : 0;
+  const float up = some ? scale_of_exp(14 - e) : 0.0f;
+  unit = m >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : scale_of_exp(e - 14 + 9);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v = some ? x[i][j] * up : 0.0f;
+      if constexpr (QT == 2) asm("" : "+v"(v));  // one rounding for both terms, as for the probabilities
+      q[0][i][j] = (_Float16)v;
+      if constexpr (QT == 2) q[1][i][j] = (_Float16)(v - (float)q[0][i][j]);
+    }
+}
+
+// two codes, in the low bytes of the halves (plus 128), as float16 code * 2^-9
+__device__ __forceinline__ uint32_t codes_f16(uint32_t pair) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2a, pair),
+                                                                f16x2a{32768.0f, 32768.0f}, f16x2a{-0.25f, -0.25f}));
+}
+
+// Swizzle of the 16-byte pieces of a key's row (D * 2 bytes): 16 rows in a row
+// take 16 places of the 256 bytes of all banks
+template <int D>
+__device__ __forceinline__ int key_swizzle(int row) {
+  return D == 64 ? (row >> 1) & 7 : row & 15;
+}
+
+template <int D, int NW>
+struct TileLds {
+  uint32_t k[2][MXK_TILE * D / 2];  // [key][D] float16, pieces of 8 swizzled
+  uint32_t v[2][MXK_TILE * D / 2];  // [row][64 keys] float16, pieces of 8 swizzled
+  float ks[2][MXK_TILE], vs[2][MXK_TILE];  // vs times 2^(10 - e)
+  int e[2];
+  uint32_t ok[2];  // bits of the block's runs of 16 keys that have a page
+};
+
+template <typename T, int D, int QT, int PT, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void k_attend_tile(AttendArgs A, int shares) {
+  constexpr int P = 8 / NW;          // pieces of 16 bytes of keys (and of values) a thread and D = 128
+  constexpr int KP = P * D / 128 > 0 ? P * D / 128 : 1;
+  constexpr int CPR = D / 16;        // 16-byte pieces of a row of codes
+  constexpr int PIECES = MXK_TILE * CPR;
+  __shared__ TileLds<D, NW> S;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, h = lane >> 5;
+  const Line L = make_line(A);
+  const int64_t total = line_length(A, L);
+  const int64_t per = line_share(total, shares);
+  // neighbours on the line read the same keys: they go to one XCD
+  const int share = shares % 8 == 0 ? (blockIdx.x & 7) * (shares >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+  const int64_t from = (int64_t)share * per, to = min(total, from + per);
+  zero_padding<T, D, 64 * NW>(A, shares);
+  if (from >= to) return;
+
+  SeqWork w;
+  Place p = line_place(A, L, from, w);
+  int64_t at = from;
+  while (true) {
+    const int64_t k1 = min(p.blocks, p.k + (to - at));
+    const bool whole = p.k == 0 && k1 == p.blocks;
+    int tok, head;
+    const bool row_ok = tile_row(A, w, p, wave * 32 + l32, tok, head);
+    const bool busy = __ballot(row_ok) != 0;
+    f16x8a q[QT][D / 16];
+    float unit;
+    query_halves<T, D, QT>(row_ok ? reinterpret_cast<const T*>(A.q) + (int64_t)(w.first + tok) * A.q_token +
+                                        (int64_t)head * A.q_head
+                                  : nullptr,
+                           h, q, unit);
+    unit *= A.scale;
+    const uint64_t* bits = A.mask && row_ok ? A.mask + (int64_t)(w.first + tok) * A.words : A.mask;
+    const int64_t end = min(L.cap, w.ctx + (A.mask ? w.n : min(w.n, (p.x / A.chunks + 1) * A.TT)));
+    const int64_t key0 = p.k * A.keys, stop = min(end, k1 * A.keys);
+    // the wave's first and last token: between them a causal block needs its mask
+    int lo_tok = row_ok ? tok : 0x7FFFFFFF, hi_tok = row_ok ? tok : -1;
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) lo_tok = min(lo_tok, __shfl_xor(lo_tok, i)), hi_tok = max(hi_tok, __shfl_xor(hi_tok, i));
+    lo_tok = __builtin_amdgcn_readfirstlane(lo_tok);
+    hi_tok = __builtin_amdgcn_readfirstlane(hi_tok);
+
+    f32x16a o[D / 32];
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[j][i] = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;
+    int e = -100;
+
+    // codes of a block on their way: the thread's pieces of keys, and four keys by four elements of values
+    u32x4 kr[KP];
+    uint32_t vr[KP][4];
+    float sr = 0.0f;
+    int run_ok = 0;
+    auto fetch = [&](int64_t key) {
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        const int piece = tid + i * 64 * NW, row = piece / CPR, c = piece % CPR;
+        if (piece >= PIECES) break;
+        const int64_t kk = key + row;
+        const int page = kv_page(A.batch, A.pool, p.b, kk >> A.pool.shift);
+        const int64_t src = kv_row(A.pool, max(page, 0), 0, p.h, (int)(kk & ((1 << A.pool.shift) - 1)));
+        kr[i] = *reinterpret_cast<const u32x4*>(A.pool.codes + src * D + c * 16);
+      }
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        const int piece = tid + i * 64 * NW, four = piece / (D / 4), c = piece % (D / 4);
+        if (piece >= PIECES) break;
+        const int64_t kk = key + four * 4;
+        const int page = kv_page(A.batch, A.pool, p.b, kk >> A.pool.shift);
+        const int64_t src = kv_row(A.pool, max(page, 0), 1, p.h, (int)(kk & ((1 << A.pool.shift) - 1)));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          vr[i][r] = *reinterpret_cast<const uint32_t*>(A.pool.codes + (src + r) * D + c * 4);
+      }
+      if (wave < 2) {
+        const int64_t kk = key + lane;
+        const int page = kk < end ? kv_page(A.batch, A.pool, p.b, kk >> A.pool.shift) : -1;
+        sr = 0.0f;
+        if (page >= 0) sr = A.pool.scales[kv_row(A.pool, page, wave, p.h, (int)(kk & ((1 << A.pool.shift) - 1)))];
+        run_ok = page >= 0;
+      }
+    };
+    int e_run = -100;  // of wave 1, which finds the exponent for all
+    auto put = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        const int piece = tid + i * 64 * NW, row = piece / CPR, c = piece % CPR;
+        if (piece >= PIECES) break;
+        u32x4 half[2];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t u = kr[i][x] ^ 0x80808080u;
+          half[x >> 1][2 * (x & 1)] = codes_f16(__builtin_amdgcn_perm(0u, u, 0x0C010C00u));
+          half[x >> 1][2 * (x & 1) + 1] = codes_f16(__builtin_amdgcn_perm(0u, u, 0x0C030C02u));
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          *reinterpret_cast<u32x4*>(&S.k[buf][row * (D / 2) + (((2 * c + x) ^ key_swizzle<D>(row)) * 4)]) = half[x];
+      }
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        const int piece = tid + i * 64 * NW, four = piece / (D / 4), c = piece % (D / 4);
+        if (piece >= PIECES) break;
+        // keys 16s + 8b + 4h': run s*2 + h', its half b
+        const int run = (four >> 2) * 2 + (four & 1), b = (four >> 1) & 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t sel = 0x0C000C00u | (uint32_t)j | (uint32_t)(4 + j) << 16;
+          u32x2 two;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            two[x] = codes_f16(__builtin_amdgcn_perm(vr[i][2 * x + 1] ^ 0x80808080u, vr[i][2 * x] ^ 0x80808080u, sel));
+          const int row = j * (D / 4) + c;
+          *reinterpret_cast<u32x2*>(&S.v[buf][row * (MXK_TILE / 2) + ((run ^ ((row >> 1) & 7)) * 4) + b * 2]) = two;
+        }
+      }
+      if (wave == 0) S.ks[buf][lane] = sr;
+      if (wave == 1) {
+        const uint32_t bb = mag_bits(sr);
+        int top = (int)((bb < 0x7F800000u ? bb : 0u) >> 23) - 127;
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) top = max(top, __shfl_xor(top, i));
+        e_run = max(e_run, top);
+        S.vs[buf][lane] = sr * scale_of_exp(10 - e_run);
+        const uint64_t b = __ballot(run_ok);
+        if (lane == 0) {
+          S.e[buf] = e_run;
+          S.ok[buf] = (uint32_t)(b & 1) | (uint32_t)(b >> 16 & 1) << 1 | (uint32_t)(b >> 32 & 1) << 2 |
+                      (uint32_t)(b >> 48 & 1) << 3;
+        }
+      }
+    };
+
+    __syncthreads();  // the tile before is read
+    if (key0 < stop) {
+      fetch(key0);
+      put(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int64_t key = key0; key < stop; key += MXK_TILE, buf ^= 1) {
+      const bool more = key + MXK_TILE < stop;
+      if (more) fetch(key + MXK_TILE);
+      const int e_new = __builtin_amdgcn_readfirstlane(S.e[buf]);
+      const uint32_t ok = __builtin_amdgcn_readfirstlane(S.ok[buf]);
+      const int64_t j0 = key - w.ctx;  // the first key among the new tokens
+      // rows of tokens before the whole block see none of it
+      if (busy && (A.mask || j0 <= hi_tok)) {
+        const bool open = key + MXK_TILE <= end && ok == 15 && (j0 + MXK_TILE <= 0 || (!A.mask && j0 + MXK_TILE - 1 <= lo_tok));
+        uint64_t see = ~0ull;
+        if (!open) {
+          if (A.mask) {
+            const int64_t word = j0 >= 0 ? j0 >> 6 : -1;
+            const uint64_t none = 0;
+            if (j0 >= 0) {
+              const int sh = (int)(j0 & 63);
+              const uint64_t one = word < A.words ? bits[word] : none;
+              const uint64_t two = word + 1 < A.words ? bits[word + 1] : none;
+              see = sh ? one >> sh | two << (64 - sh) : one;
+            } else if (j0 > -MXK_TILE) {
+              see = bits[0] << (int)-j0 | ((1ull << (int)-j0) - 1);
+            }
+          } else {
+            const int64_t last = tok - j0;  // the last key of the block that the row sees
+            see = last < 0 ? 0 : last >= 63 ? ~0ull : (2ull << (int)last) - 1;
+          }
+          if (key + MXK_TILE > end) see &= (1ull << (int)(end - key)) - 1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(ok >> i & 1)) see &= ~(0xFFFFull << (16 * i));
+          see >>= 4 * h;
+        }
+        float t[2][16];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          f32x16a acc;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+          const int row = kt * 32 + l32;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            const f16x8a kf = *reinterpret_cast<const f16x8a*>(&S.k[buf][row * (D / 2) + (((2 * i + h) ^ key_swizzle<D>(row)) * 4)]);
+#pragma unroll
+            for (int n = 0; n < QT; ++n) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[n][i], acc, 0, 0, 0);
+          }
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const f32x4a s4 = *reinterpret_cast<const f32x4a*>(&S.ks[buf][kt * 32 + a * 8 + h * 4]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[kt][4 * a + r] = acc[4 * a + r] * s4[r];
+          }
+        }
+        if (!open) {
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (!((uint32_t)(see >> (32 * kt)) >> (8 * (i >> 2) + (i & 3)) & 1)) t[kt][i] = -__builtin_inff();
+        }
+        float top = t[0][0];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, t[kt][i]);
+        top *= unit;
+        if (__ballot(top > m + 4.0f) || e_new != e) {
+          top = fmaxf(top, __shfl_xor(top, 32));
+          const float mm = fmaxf(m, top);
+          const float shrink = mm == m ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
+          const float both = shrink * scale_of_exp(e - e_new);
+          l *= shrink;
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[j][i] *= both;
+          m = mm;
+          e = e_new;
+        }
+        const float ms = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          f16x8a pr[PT][2];
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const f32x4a s4 = *reinterpret_cast<const f32x4a*>(&S.vs[buf][kt * 32 + a * 8 + h * 4]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t[kt][4 * a + r], unit, -ms));
+              float c = x * s4[r];
+              if (!open && !((uint32_t)(see >> (32 * kt)) >> (8 * a + r) & 1)) x = c = 0.0f;
+              l += x;
+              if constexpr (PT == 2) asm("" : "+v"(c));
+              const int s = a >> 1, i = 4 * (a & 1) + r;
+              pr[0][s][i] = (_Float16)c;
+              if constexpr (PT == 2) pr[1][s][i] = (_Float16)(c - (float)pr[0][s][i]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const int row = j * 32 + l32;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const int run = (kt * 2 + s) * 2 + h;
+              const f16x8a vf =
+                  *reinterpret_cast<const f16x8a*>(&S.v[buf][row * (MXK_TILE / 2) + ((run ^ ((row >> 1) & 7)) * 4)]);
+#pragma unroll
+              for (int n = 0; n < PT; ++n) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pr[n][s], o[j], 0, 0, 0);
+            }
+          }
+        }
+      }
+      if (more) put(buf ^ 1);
+      __syncthreads();
+    }
+
+    // a lane has its row's elements 4c .. 4c+3 for every c with bit 2 of c equal to h
+    l += __shfl_xor(l, 32);
+    if (row_ok) {
+      const float down = scale_of_exp(e - 1), inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int64_t slot = ((int64_t)share * 2 + (p.k == 0 ? 1 : 0)) * (32 * NW) + wave * 32 + l32;
+      T* dst = reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D;
+#pragma unroll
+      for (int a = 0; a < D / 32; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int row = j * (D / 4) + 8 * a + r;
+            x[j] = o[row / 32][(row % 32 / 8) * 4 + row % 4] * down;
+          }
+          const int d = 4 * (8 * a + 4 * h + r);
+          if (whole) {
+            T y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = out_cvt<T>(x[j] * inv);
+            __builtin_memcpy(dst + d, y, sizeof(y));
+          } else {
+            __builtin_memcpy(A.part_o + slot * D + d, x, sizeof(x));
+          }
+        }
+      if (!whole && h == 0) A.part_s[slot] = make_float2(m, l);
+    }
+    at += k1 - p.k;
+    if (at >= to) break;
+    next_tile(A, L, w, p);
   }
 }
 
@@ -568,28 +937,40 @@ __global__ __launch_bounds__(64) void k_attend_join(AttendArgs A, int shares, in
 
 // ---------------------------------------------------------------- host
 struct AttendPlan {
-  int rows, TT, GC, chunks, shares;
+  int rows, keys, TT, GC, chunks, shares;
   bool cut;  // a tile may be cut
 };
 
-static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int H, int G) {
+static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int H, int G, int D) {
   AttendPlan a;
-  a.rows = 16;
+  // rows of a sequence and key head, on average
+  const double each = B > 0 ? (double)T * G / (double)std::min(B, T) : 0.0;
+  a.rows = each <= 32 ? 16 : each <= 128 || D == 256 ? 128 : 256;
+  a.keys = a.rows == 16 ? 128 : 256;
   a.GC = std::min(G, a.rows);
   a.chunks = (int)ceil_div(G, a.GC);
   a.TT = 1;
   while (a.TT * 2 * a.GC <= a.rows) a.TT *= 2;
   // no more shares than blocks there can be
   const double tiles = ((double)T / a.TT + (double)std::min(B, T)) * a.chunks * H;
-  const double blocks = std::ceil((double)width * page / MXK_KEYS);
+  const double blocks = std::ceil((double)width * page / a.keys);
   a.cut = blocks > 1 && B > 0;
-  a.shares = (int)std::max(1.0, std::min(2.0 * num_cus(), tiles * std::max(1.0, blocks)));
+  const double most = (a.rows == 256 || D == 256 ? 1.0 : 2.0) * num_cus();  // workgroups that run at once
+  a.shares = (int)std::max(1.0, std::min(most, tiles * std::max(1.0, blocks)));
   return a;
 }
 
 template <typename T, int D, int QT, int PT>
 static int launch_attend(const AttendArgs& A, const AttendPlan& a, hipStream_t st) {
-  hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A, a.shares);
+  constexpr int QH = sizeof(T) == 4 ? 2 : 1;  // float16 terms of a query
+  if (a.rows == 16) {
+    hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A, a.shares);
+  } else if (a.rows == 128) {
+    hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 4>), dim3(a.shares), dim3(256), 0, st, A, a.shares);
+  } else {
+    if constexpr (D < 256)
+      hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 8>), dim3(a.shares), dim3(512), 0, st, A, a.shares);
+  }
   if (a.cut && a.shares > 1)
     hipLaunchKernelGGL((k_attend_join<T, D>), dim3(a.shares - 1, a.rows), dim3(64), 0, st, A, a.shares, a.rows);
   return check_launch("kv_attend");
@@ -612,7 +993,7 @@ size_t mxk_kv_pages_attend_workspace(int64_t tokens, int64_t B, int64_t width, i
                                      int D) {
   if (tokens <= 0 || B <= 0 || width < 0 || heads < 1 || q_heads < heads || q_heads % heads || !kv_page_ok(page))
     return 0;
-  const AttendPlan a = plan_attend(tokens, B, width, page, heads, q_heads / heads);
+  const AttendPlan a = plan_attend(tokens, B, width, page, heads, q_heads / heads, D);
   return a.cut ? (size_t)a.shares * 2 * a.rows * ((size_t)D * 4 + 8) : 0;
 }
 
@@ -642,7 +1023,7 @@ int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_he
   if (!aligned16(codes) || !aligned16(scales))
     return fail(MXK_EINVAL, "kv_attend: codes and scales start on 16 bytes");
   const int G = q_heads / heads;
-  const AttendPlan a = plan_attend(tokens, B, width, page, heads, G);
+  const AttendPlan a = plan_attend(tokens, B, width, page, heads, G, D);
   const size_t part = (size_t)a.shares * 2 * a.rows;
   if (a.cut && a.shares > 1 && (!workspace || workspace_nbytes < part * ((size_t)D * 4 + 8) || !aligned16(workspace)))
     return fail(MXK_EINVAL, "kv_attend: workspace too small (mxk_kv_pages_attend_workspace) or not on 16 bytes");
@@ -658,6 +1039,7 @@ int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_he
   A.scale = scale * 1.4426950408889634f;
   A.Hq = q_heads;
   A.G = G;
+  A.keys = a.keys;
   A.TT = a.TT;
   A.GC = a.GC;
   A.chunks = a.chunks;

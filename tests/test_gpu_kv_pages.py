@@ -260,9 +260,18 @@ def test_attend_groups(heads, group, dtype):
 
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("held,new,page,group", [([0], [200], 16, 2), ([100, 0], [70, 33], 32, 1), ([10, 300, 0, 7], [0, 129, 1, 64], 16, 3),
-                                                 ([129], [127], 128, 4), ([64], [300], 64, 8)])
+                                                 ([129], [127], 128, 4), ([64], [300], 64, 8), ([2100], [40], 16, 4)])
 def test_attend_chunks(held, new, page, group, dtype):
     _check_attend(R.Batch(held, new, page), 1, group, 128, dtype)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("held,new,page,group", [([0], [1], 16, 40), ([3, 600], [20, 20], 16, 4), ([70, 0], [63, 64], 32, 2),
+                                                 ([0, 255, 9], [65, 33, 0], 64, 5), ([190], [300], 16, 1)])
+def test_attend_tiles(held, new, page, group, dim, dtype):
+    """Tiles of 128 and of 256 rows, for every size of head."""
+    _check_attend(R.Batch(held, new, page, front=1), 2 if group < 3 else 1, group, dim, dtype)
 
 
 def _tree(batch, seed=0, words=None):
@@ -278,11 +287,12 @@ def _tree(batch, seed=0, words=None):
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
-@pytest.mark.parametrize("held,new,group", [([0], [5], 1), ([40, 7], [16, 17], 4), ([100, 0, 33], [64, 0, 65], 2), ([300], [130], 3),
-                                            ([126, 127, 128], [3, 3, 3], 8)])
-def test_attend_trees(held, new, group, dtype):
+@pytest.mark.parametrize("held,new,group,dim", [([0], [5], 1, 64), ([40, 7], [16, 17], 4, 64), ([100, 0, 33], [64, 0, 65], 2, 128),
+                                                ([300], [130], 3, 64), ([126, 127, 128], [3, 3, 3], 8, 64), ([63, 64, 65], [30, 66, 2], 3, 256),
+                                                ([1000, 70], [60, 90], 6, 128), ([1, 513], [200, 10], 2, 64)])
+def test_attend_trees(held, new, group, dim, dtype):
     batch = R.Batch(held, new, 16, front=1, back=2)
-    got = _check_attend(batch, 2, group, 64, dtype, mask=_tree(batch))
+    got = _check_attend(batch, 2, group, dim, dtype, mask=_tree(batch))
     inside = torch.zeros(batch.tokens, dtype=torch.bool)
     for b, n in enumerate(new):
         inside[batch.first[b]:batch.first[b] + n] = True
@@ -300,10 +310,13 @@ def test_attend_any_mask():
     assert (got[[3 + 0, 5, 7]].cpu()[1:] == 0).all()
     # fewer words than tokens: later tokens are not seen
     _check_attend(batch, 1, 2, 64, torch.float32, mask=mask[:, :1].contiguous())
+    for group in (1, 8):
+        _check_attend(batch, 1, group, 128, torch.bfloat16, mask=mask)
 
 
+@pytest.mark.parametrize("group", [2, 16, 50])
 @pytest.mark.parametrize("masked", [False, True])
-def test_attend_non_finite_where_it_is_not_seen(masked):
+def test_attend_non_finite_where_it_is_not_seen(masked, group):
     """Scales of NaN and infinity in places that a row does not see leave it alone; where it sees them it is NaN."""
     batch = R.Batch([40, 7], [6, 5], 16)
     codes, scales = R.pool(batch, 1, 64)
@@ -311,7 +324,7 @@ def test_attend_non_finite_where_it_is_not_seen(masked):
     for b, i, bad in ((0, 3, math.nan), (1, 2, math.inf)):
         p = batch.place(b, batch.held[b] + i)
         scales[p[0], b, :, p[1]] = bad  # a key of the first, a value of the second
-    q = _rand((batch.tokens, 2, 64), 1)
+    q = _rand((batch.tokens, group, 64), 1)
     got = _pages(codes, scales).attend(q.cuda(), batch.gpu(), mask=None if mask is None else mask.cuda()).cpu()
     for b, i in ((0, 3), (1, 2)):
         see = R.seen(batch, b, mask)[:, batch.held[b] + i]
@@ -323,10 +336,11 @@ def test_attend_non_finite_where_it_is_not_seen(masked):
     R.near(got[fine], want[fine], error[fine])
 
 
-def test_attend_rows_of_q_that_are_not_finite():
+@pytest.mark.parametrize("group", [2, 32, 100])
+def test_attend_rows_of_q_that_are_not_finite(group):
     batch = R.Batch([40, 0], [1, 2], 16)
     codes, scales = R.pool(batch, 1, 64)
-    q = _rand((3, 2, 64), 1)
+    q = _rand((3, group, 64), 1)
     q[0, 1, 5], q[2, 0, 0] = math.nan, -math.inf
     mask = torch.tensor([[1], [1], [0]])  # the last row sees nothing
     got = _pages(codes, scales).attend(q.cuda(), batch.gpu(), mask=mask.cuda()).cpu()
@@ -336,51 +350,56 @@ def test_attend_rows_of_q_that_are_not_finite():
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_attend_sharp_and_flat(dtype):
     batch = R.Batch([900, 500], [1, 20], 16)
-    _check_attend(batch, 1, 4, 64, dtype, scale=3.0)
-    _check_attend(batch, 1, 4, 64, dtype, scale=1e-6)
-    _check_attend(batch, 1, 4, 64, dtype, qscale=0.0)
+    for group in (2, 4, 20):
+        _check_attend(batch, 1, group, 64, dtype, scale=3.0)
+        _check_attend(batch, 1, group, 64, dtype, scale=1e-6)
+        _check_attend(batch, 1, group, 64, dtype, qscale=0.0)
 
 
+@pytest.mark.parametrize("group", [3, 20, 80])
 @pytest.mark.parametrize("dtype", FLOATS)
-def test_attend_values_of_far_apart_scales(dtype):
+def test_attend_values_of_far_apart_scales(dtype, group):
     """A key that takes nearly all of the weight has small values; the others' still count."""
     batch = R.Batch([600], [2], 16)
     codes, scales = R.pool(batch, 1, 128)
     p = batch.place(0, 0)
     scales[p[0], 0, 0, p[1]] *= 6.0
     scales[p[0], 1, 0, p[1]] *= 1e-5
-    q = _rand((2, 3, 128), 1, dtype, 0.2)
+    q = _rand((2, group, 128), 1, dtype, 0.2)
     q[:, 0] = (codes[p[0], 0, 0, p[1]].float() / 40).to(dtype)
     want, error = R.attend(batch, codes, scales, q)
     R.near(_pages(codes, scales).attend(q.cuda(), batch.gpu()), want, error)
 
 
+@pytest.mark.parametrize("group", [2, 64])
 @pytest.mark.parametrize("factor", [1e-30, 1e20])
-def test_attend_scales_at_both_ends(factor):
+def test_attend_scales_at_both_ends(factor, group):
     batch = R.Batch([300], [2], 16)
     codes, scales = R.pool(batch, 1, 64)
     scales[:, 1] *= factor
-    q = _rand((2, 2, 64), 1)
+    q = _rand((2, group, 64), 1)
     want, error = R.attend(batch, codes, scales, q)
     R.near(_pages(codes, scales).attend(q.cuda(), batch.gpu()), want, error)
 
 
-def test_attend_absent_pages():
+@pytest.mark.parametrize("group", [2, 32])
+def test_attend_absent_pages(group):
     batch = R.Batch([100, 70], [4, 1], 16)
     codes, scales = R.pool(batch, 2, 64)
     batch.table[0, 1], batch.table[0, 6], batch.table[1, 4] = batch.pages + 5, -1, -(1 << 31)
-    q = _rand((5, 4, 64), 1)
+    q = _rand((5, 2 * group, 64), 1)
     want, error = R.attend(batch, codes, scales, q)
     R.near(_pages(codes, scales).attend(q.cuda(), batch.gpu()), want, error)
     batch.table[:] = -1
     assert (_pages(codes, scales).attend(q.cuda(), batch.gpu()).cpu() == 0).all()
 
 
-def test_attend_more_positions_than_the_table():
+@pytest.mark.parametrize("group", [2, 10])
+def test_attend_more_positions_than_the_table(group):
     batch = R.Batch([100, 70], [40, 1], 16)
     codes, scales = R.pool(batch, 1, 64)
     batch.table, batch.width = batch.table[:, :7].contiguous(), 7  # 112 positions
-    q = _rand((41, 2, 64), 1)
+    q = _rand((41, group, 64), 1)
     want, error = R.attend(batch, codes, scales, q)
     R.near(_pages(codes, scales).attend(q.cuda(), batch.gpu()), want, error)
     batch.table, batch.width = batch.table[:, :0].contiguous(), 0
@@ -415,9 +434,10 @@ def test_attend_layouts(layout, dtype):
 def test_repeats_bit_for_bit():
     batch = R.Batch([5000, 300, 2], [1, 1, 1], 16)
     pages = _pages(*R.pool(batch, 2, 128))
-    q = _rand((3, 8, 128), 1, torch.bfloat16).cuda()
-    first = pages.attend(q, batch.gpu())
-    assert all(torch.equal(first, pages.attend(q, batch.gpu())) for _ in range(5))
+    for group in (4, 50, 200):
+        q = _rand((3, 2 * group, 128), 1, torch.bfloat16).cuda()
+        first = pages.attend(q, batch.gpu())
+        assert all(torch.equal(first, pages.attend(q, batch.gpu())) for _ in range(5))
 
 
 def test_empty_calls():
