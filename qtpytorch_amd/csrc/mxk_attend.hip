@@ -50,58 +50,70 @@ struct AttendArgs {
   int words;
   float scale;  // of the scores, times log2(e)
   int Hq, G;    // query heads; of one key head
-  int keys;            // of a block: 128 or 256
+  int keys;     // of a block: 128 or 256
   int TT, GC, chunks;  // a tile: TT tokens (a power of two, at most keys) of GC heads, chunks of them over G
+  int cap, most;       // positions of the table (below 2^31 - 2^16); blocks of a tile at most, at least one
+  int rows, shares;    // of a tile; the line's
   void* out;
-  float* part_o;  // [shares][2][rows][D], of their own maximum
-  float2* part_s;  // [shares][2][rows]: maximum, sum
+  // of tiles that are cut, null where none can be: sums [shares][2][rows][D] of their own maximum, the maximum and
+  // weight of each row, and the tile that a share leaves to the shares after it
+  float* part_o;
+  float2* part_s;
+  struct PartTile* part_t;
+};
+
+struct PartTile {
+  int first, n, h, x;  // of the sequence's new tokens; key head, tile
+  int last;            // share with the tile's last block, -1: no tile
+  int pad[3];
 };
 
 // ---------------------------------------------------------------- the line of blocks
-// sum of floor(i / 2^s) over i < x
-__device__ __forceinline__ int64_t sum_floor(int64_t x, int s) {
-  const int64_t q = x >> s;
-  return ((q * (q - 1) / 2) << s) + q * (x - (q << s));
+// All places on the line are below 2^31 (the host has seen to it).
+
+// sum of floor(i / 2^s) over i < x, modulo 2^32: differences of two are exact
+__device__ __forceinline__ uint32_t sum_floor(uint32_t x, int s) {
+  const uint32_t q = x >> s;
+  const uint32_t half = q & 1 ? q * ((q - 1) >> 1) : (q >> 1) * (q - 1);
+  return (half << s) + q * (x - (q << s));
 }
 
 struct Line {
-  int rs;  // log2(keys / TT)
-  int ts;  // log2(TT)
-  int64_t cap;   // positions of the table
-  int64_t most;  // blocks that a tile has at most: the table's, at least one.  The workspace is sized by it.
+  int ts, rs;  // log2 of TT and of keys / TT
 };
 
 // A sequence on the line: per key head, its tiles' blocks one after the other
 struct SeqWork {
-  int first, n;    // new tokens
-  int64_t ctx;     // keys held
-  int64_t a;       // causal: token tile t has floor((a + t) / 2^rs) blocks, at most Line::most
-  int64_t full;    // causal: the first token tile that has that many
-  int64_t blocks;  // masked: of every tile
-  int tiles;       // token tiles
-  int64_t head;    // blocks of one key head
+  int first, n, ctx;  // new tokens, keys held
+  int a;              // causal: token tile t has floor((a + t) / 2^rs) blocks, at most AttendArgs::most
+  int full;           // causal: the first token tile that has that many
+  int blocks;         // masked: of every tile
+  int tiles;          // token tiles
+  uint32_t head;      // blocks of one key head
 };
 
-__device__ __forceinline__ int64_t tile_blocks(const AttendArgs& A, const Line& L, const SeqWork& w, int t) {
-  return A.mask ? w.blocks : min((w.a + t) >> L.rs, L.most);
+__device__ __forceinline__ int tile_blocks(const AttendArgs& A, const Line& L, const SeqWork& w, int t) {
+  return A.mask ? w.blocks : t >= w.full ? A.most : (w.a + t) >> L.rs;
 }
 
 // Blocks of a key head's token tiles below t
-__device__ __forceinline__ int64_t blocks_below(const AttendArgs& A, const Line& L, const SeqWork& w, int t) {
-  if (A.mask) return A.chunks * (t * w.blocks);
-  const int64_t some = min((int64_t)t, w.full);
-  return A.chunks * (sum_floor(w.a + some, L.rs) - sum_floor(w.a, L.rs) + (t - some) * L.most);
+__device__ __forceinline__ uint32_t blocks_below(const AttendArgs& A, const Line& L, const SeqWork& w, int t) {
+  if (A.mask) return (uint32_t)A.chunks * ((uint32_t)t * (uint32_t)w.blocks);
+  const int some = min(t, w.full);
+  return (uint32_t)A.chunks * (sum_floor((uint32_t)(w.a + some), L.rs) - sum_floor((uint32_t)w.a, L.rs) +
+                               (uint32_t)(t - some) * (uint32_t)A.most);
 }
 
 __device__ __forceinline__ SeqWork seq_work(const AttendArgs& A, const Line& L, int b) {
   SeqWork w;
-  w.first = kv_first(A.batch, b);
-  w.n = kv_count(A.batch, b);
-  w.ctx = min(max((int64_t)A.batch.lengths[b], (int64_t)0), L.cap);
+  const int held = A.batch.lengths[b], o0 = A.batch.offsets[b], o1 = A.batch.offsets[b + 1];
+  w.first = min(max(o0, 0), A.batch.T);
+  w.n = max(0, min(o1, A.batch.T) - max(o0, 0));
+  w.ctx = min(max(held, 0), A.cap);
   w.tiles = (w.n + A.TT - 1) >> L.ts;
   w.a = (w.ctx + A.TT + A.keys - 1) >> L.ts;
-  w.full = max((int64_t)0, (L.most << L.rs) - w.a);
-  w.blocks = min((w.ctx + w.n + A.keys - 1) >> (L.ts + L.rs), L.most);
+  w.full = max(0, (int)(((int64_t)A.most << L.rs) - w.a));
+  w.blocks = min((int)(((int64_t)w.ctx + w.n + A.keys - 1) >> (L.ts + L.rs)), A.most);
   w.head = blocks_below(A, L, w, w.tiles);
   return w;
 }
@@ -110,86 +122,130 @@ __device__ __forceinline__ Line make_line(const AttendArgs& A) {
   Line L;
   L.ts = 31 - __builtin_clz(A.TT);
   L.rs = 31 - __builtin_clz(A.keys) - L.ts;
-  L.cap = (int64_t)A.batch.width << A.pool.shift;
-  L.most = max((int64_t)1, (L.cap + A.keys - 1) >> (L.ts + L.rs));
   return L;
 }
 
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
-// Blocks of all sequences; every lane of every wave ends with the sum
-__device__ __forceinline__ int64_t line_length(const AttendArgs& A, const Line& L) {
-  const int lane = threadIdx.x & 63;
-  int64_t sum = 0;
-  for (int b = lane; b < A.batch.B; b += 64) sum += seq_work(A, L, b).head * A.pool.H;
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
-  return uniform64(sum);
-}
-
-// Share of the line that each of `shares` workgroups takes
-__device__ __forceinline__ int64_t line_share(int64_t total, int shares) {
-  int64_t per = (int64_t)((double)total / (double)shares);
-  while (per * shares < total) ++per;
-  return per;
-}
-
-// A place on the line: the tile it lies in and the tile's own blocks
+// A place on the line: the tile it lies in and the block of the tile
 struct Place {
-  int b, h, x;       // sequence, key head, tile (token tile * chunks + chunk)
-  int64_t k;         // block within the tile
-  int64_t blocks;    // of the tile
+  int b, h, x;  // sequence, key head, tile (token tile * chunks + chunk)
+  int k;        // block within the tile
+  int blocks;   // of the tile
 };
 
-// at: below line_length; found by a whole wave, uniform in it
-__device__ __forceinline__ Place line_place(const AttendArgs& A, const Line& L, int64_t at, SeqWork& w) {
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {  // inclusive
   const int lane = threadIdx.x & 63;
-  int b = 0;
-  for (int b0 = 0; b0 < A.batch.B; b0 += 64) {
-    const int64_t own = b0 + lane < A.batch.B ? seq_work(A, L, b0 + lane).head * A.pool.H : 0;
-    int64_t upto = own;
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) {
-      const int64_t o = __shfl_up(upto, i);
-      if (lane >= i) upto += o;
-    }
-    const uint64_t beyond = __ballot(upto > at);
-    if (beyond) {
-      const int l = __builtin_ctzll(beyond);
-      at -= __shfl(upto - own, l);
-      b = b0 + l;
-      break;
-    }
-    at -= __shfl(upto, 63);
+  for (int i = 1; i < 64; i <<= 1) {
+    const uint32_t o = __shfl_up(v, i);
+    if (lane >= i) v += o;
   }
-  Place p;
-  p.b = __builtin_amdgcn_readfirstlane(b);
-  at = uniform64(at);
-  w = seq_work(A, L, p.b);
-  p.h = 0;
-  while (at >= w.head && p.h < A.pool.H - 1) {  // at most 1024 heads, 64 at once below
-    if (at >= 64 * w.head && p.h + 64 < A.pool.H) p.h += 64, at -= 64 * w.head;
-    else ++p.h, at -= w.head;
+  return v;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ int lane_of(int v, int lane) { return (int)__builtin_amdgcn_readlane((uint32_t)v, lane); }
+
+// Share `share` of the line, [from, to), and the place it begins at.  Found by
+// a whole wave, which holds a sequence a lane: for up to 64 of them one round of loads.
+// false: an empty share.
+__device__ __forceinline__ bool line_share(const AttendArgs& A, const Line& L, int share, uint32_t& from, uint32_t& to,
+                                           uint32_t& per, SeqWork& w, Place& p) {
+  const int lane = threadIdx.x & 63, B = A.batch.B;
+  if (B == 0) return false;
+  SeqWork mine = seq_work(A, L, min(lane, B - 1));
+  uint32_t own = lane < B ? mine.head * (uint32_t)A.pool.H : 0;
+  uint32_t upto = wave_scan(own);
+  uint32_t total = lane_of(upto, 63);
+  if (B > 64) {
+    uint32_t sum = 0;
+    for (int b = 64 + lane; b < B; b += 64) sum += seq_work(A, L, b).head * (uint32_t)A.pool.H;
+    total += lane_of(wave_scan(sum), 63);
   }
+  per = (total + (uint32_t)A.shares - 1) / (uint32_t)A.shares;
+  from = (uint32_t)share * per;
+  to = min(total, from + per);
+  if (from >= to) return false;
+  uint32_t at = from;
+  int b0 = 0;
+  while (at >= lane_of(upto, 63)) {  // below the total: it ends
+    at -= lane_of(upto, 63);
+    b0 += 64;
+    mine = seq_work(A, L, min(b0 + lane, B - 1));
+    own = b0 + lane < B ? mine.head * (uint32_t)A.pool.H : 0;
+    upto = wave_scan(own);
+  }
+  const int l = __builtin_ctzll(__ballot(upto > at));
+  at -= lane_of(upto - own, l);
+  w.first = lane_of(mine.first, l);
+  w.n = lane_of(mine.n, l);
+  w.ctx = lane_of(mine.ctx, l);
+  w.a = lane_of(mine.a, l);
+  w.full = lane_of(mine.full, l);
+  w.blocks = lane_of(mine.blocks, l);
+  w.tiles = lane_of(mine.tiles, l);
+  w.head = lane_of(mine.head, l);
+  p.b = b0 + l;
+  p.h = (int)__builtin_amdgcn_readfirstlane(at / w.head);
+  at -= (uint32_t)p.h * w.head;
   int lo = 0, hi = w.tiles - 1;  // the last token tile that begins at or before `at`
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (blocks_below(A, L, w, mid) <= at) lo = mid;
     else hi = mid - 1;
   }
-  const int t = lo;
-  at -= blocks_below(A, L, w, t);
-  p.blocks = tile_blocks(A, L, w, t);
+  at -= blocks_below(A, L, w, lo);
+  p.blocks = tile_blocks(A, L, w, lo);
   int c = 0;
-  while (at >= p.blocks && c < A.chunks - 1) ++c, at -= p.blocks;
-  p.x = t * A.chunks + c;
-  p.k = at;
-  return p;
+  while (at >= (uint32_t)p.blocks) ++c, at -= (uint32_t)p.blocks;  // below chunks
+  p.x = lo * A.chunks + c;
+  p.k = (int)at;
+  return true;
 }
+
+// The next tile on the line (there is one)
+__device__ __forceinline__ void next_tile(const AttendArgs& A, const Line& L, SeqWork& w, Place& p) {
+  p.k = 0;
+  if (++p.x == w.tiles * A.chunks) {
+    p.x = 0;
+    if (++p.h == A.pool.H) {
+      p.h = 0;
+      do ++p.b, w = seq_work(A, L, p.b);
+      while (w.head == 0);
+    }
+  }
+  p.blocks = tile_blocks(A, L, w, p.x / A.chunks);
+}
+
+// The tile that a share ends in and does not end, if it begins there too
+__device__ __forceinline__ void leave_part(const AttendArgs& A, int share, bool some, uint32_t end, uint32_t per,
+                                           const SeqWork& w, const Place& p) {
+  if (!A.part_t || threadIdx.x != 0) return;
+  PartTile t = {};
+  t.last = -1;
+  if (some) t = PartTile{w.first, w.n, p.h, p.x, (int)((end - 1) / per), {0, 0, 0}};
+  A.part_t[share] = t;
+}
+
+// First position past the keys that a tile's last token may see
+__device__ __forceinline__ int tile_end(const AttendArgs& A, const SeqWork& w, const Place& p) {
+  const int new_ones = A.mask ? w.n : min(w.n, (p.x / A.chunks + 1) * A.TT);
+  return w.ctx + min(A.cap - w.ctx, new_ones);
+}
+
+// Pages of a tile's runs of 16 keys, 64 runs a lane each, a batch ahead of its use
+struct RunPages {
+  int cur, next;
+  __device__ __forceinline__ int load(const AttendArgs& A, int b, int run) const {
+    return kv_page(A.batch, A.pool, b, ((int64_t)run << 4) >> A.pool.shift);
+  }
+  __device__ __forceinline__ void start(const AttendArgs& A, int b, int run) {
+    cur = load(A, b, run + (int)(threadIdx.x & 63));
+    next = load(A, b, run + 64 + (int)(threadIdx.x & 63));
+  }
+  __device__ __forceinline__ void advance(const AttendArgs& A, int b, int run) {  // run: of the batch after the next
+    cur = next;
+    next = load(A, b, run + (int)(threadIdx.x & 63));
+  }
+};
 
 // ---------------------------------------------------------------- query rows
 // QT int8 terms of a lane's D/4 elements of query row `row` (null: zeros): elements
@@ -246,23 +302,24 @@ struct Keys32 {
 };
 
 template <int D>
-__device__ __forceinline__ void load_keys(const KvPool& p, int h, int64_t key, const int (&page)[2], int lane,
-                                          Keys32<D>& s) {
+__device__ __forceinline__ void load_keys(const KvPool& p, int h, int key, int page0, int page1, int lane, Keys32<D>& s) {
   const int l = lane & 15, g = lane >> 4;
   const int64_t values = (int64_t)p.H << p.shift;
 #pragma unroll
   for (int a = 0; a < 2; ++a) {
-    s.ok[a] = page[a] >= 0;
+    const int page = a ? page1 : page0;
+    s.ok[a] = page >= 0;
     // without a page: some row of the pool, whose keys nobody sees
-    const int64_t row = kv_row(p, max(page[a], 0), 0, h, (int)((key + 16 * a) & ((1 << p.shift) - 1)));
+    const int64_t row = kv_row(p, max(page, 0), 0, h, (key + 16 * a) & ((1 << p.shift) - 1));
     const int8_t* kc = p.codes + row * D;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i)
-      s.k[a][i] = *reinterpret_cast<const i32x4a*>(kc + l * D + i * 64 + g * 16);
+      s.k[a][i] = *reinterpret_cast<const i32x4a*>(kc + (uint32_t)(l * D + i * 64 + g * 16));
     const int8_t* vc = p.codes + (row + values) * D;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      __builtin_memcpy(s.v[4 * a + j], vc + (g * 4 + j) * D + l * (D / 16), D / 16);
+      __builtin_memcpy(s.v[4 * a + j], __builtin_assume_aligned(vc + (uint32_t)((g * 4 + j) * D + l * (D / 16)), D / 16),
+                       D / 16);
     s.ks[a] = *reinterpret_cast<const f32x4a*>(p.scales + row + g * 4);
     s.vs[a] = *reinterpret_cast<const f32x4a*>(p.scales + row + values + g * 4);
   }
@@ -282,7 +339,7 @@ struct TileState {
 
 template <typename T, int D, int QT, int PT>
 __device__ __forceinline__ void step32(const AttendArgs& A, const i32x4a (&q)[QT][D / 64], float unit, Keys32<D>& s,
-                                       int64_t key, int64_t ctx, int64_t end, int tok, const uint64_t* __restrict__ bits,
+                                       int key, int ctx, int end, int tok, const uint64_t* __restrict__ bits,
                                        int lane, TileState<T, D, QT, PT>& st) {
   const int g = lane >> 4;
   float t[8];
@@ -308,9 +365,9 @@ __device__ __forceinline__ void step32(const AttendArgs& A, const i32x4a (&q)[QT
   if (key + 32 > min(ctx, end) || !s.ok[0] || !s.ok[1]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int64_t at = key + 16 * (i >> 2) + 4 * g + (i & 3), j = at - ctx;
+      const int at = key + 16 * (i >> 2) + 4 * g + (i & 3), j = at - ctx;
       bool see = at < end && s.ok[i >> 2];
-      if (see && j >= 0) see = bits ? j < 64 * (int64_t)A.words && (bits[j >> 6] >> (j & 63) & 1) : j <= tok;
+      if (see && j >= 0) see = bits ? (j >> 6) < A.words && (bits[j >> 6] >> (j & 63) & 1) : j <= tok;
       if (!see) t[i] = -__builtin_inff(), vs[i] = 0.0f;
     }
   }
@@ -395,54 +452,47 @@ __device__ __forceinline__ bool tile_row(const AttendArgs& A, const SeqWork& w, 
 
 // Rows of tokens that no sequence has
 template <typename T, int D, int THREADS>
-__device__ __forceinline__ void zero_padding(const AttendArgs& A, int shares) {
+__device__ __forceinline__ void zero_padding(const AttendArgs& A) {
   const int B = A.batch.B;
   const int lo = B ? min(max(A.batch.offsets[0], 0), A.batch.T) : 0;
   const int hi = B ? min(max(A.batch.offsets[B], 0), A.batch.T) : 0;
   const int64_t row = (int64_t)A.Hq * D, n = (lo + (A.batch.T - hi)) * row;
   T* out = reinterpret_cast<T*>(A.out);
-  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)shares * THREADS)
+  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)A.shares * THREADS)
     out[i < lo * row ? i : i - lo * row + hi * row] = out_cvt<T>(0.0f);
-}
-
-// The next tile on the line (there is one)
-__device__ __forceinline__ void next_tile(const AttendArgs& A, const Line& L, SeqWork& w, Place& p) {
-  p.k = 0;
-  if (++p.x == w.tiles * A.chunks) {
-    p.x = 0;
-    if (++p.h == A.pool.H) {
-      p.h = 0;
-      do ++p.b, w = seq_work(A, L, p.b);
-      while (w.head == 0);
-    }
-  }
-  p.blocks = tile_blocks(A, L, w, p.x / A.chunks);
 }
 
 // Tiles of 16 rows
 template <typename T, int D, int QT, int PT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A, int shares) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) {
   constexpr int LD = D + 4;
   __shared__ float so[4][16][LD];
   __shared__ float sm[4][16], sl[4][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int l16 = lane & 15, g = lane >> 4;
+  const int l16 = lane & 15, g = lane >> 4, share = blockIdx.x;
   const Line L = make_line(A);
-  const int64_t total = line_length(A, L);
-  const int64_t per = line_share(total, shares);
-  const int64_t from = (int64_t)blockIdx.x * per, to = min(total, from + per);
-
-  zero_padding<T, D, 256>(A, shares);
-  if (from >= to) return;
-
+  zero_padding<T, D, 256>(A);
+  uint32_t from, to, per;
   SeqWork w;
-  Place p = line_place(A, L, from, w);
-  int64_t at = from;
+  Place p;
+  if (!line_share(A, L, share, from, to, per, w, p)) {
+    leave_part(A, share, false, 0, 1, w, p);
+    return;
+  }
+  uint32_t at = from;
   while (true) {
-    const int64_t k1 = min(p.blocks, p.k + (to - at));
+    const int k1 = (int)min((uint32_t)p.blocks, (uint32_t)p.k + (to - at));
     const bool whole = p.k == 0 && k1 == p.blocks;
     int tok, head;
     const bool row_ok = tile_row(A, w, p, l16, tok, head);
+    const int end = tile_end(A, w, p);
+    const int stop = (int)min((int64_t)end, (int64_t)k1 * 128);
+    // a wave's keys: 32 of each block, so its runs of 16 are blocks * 8 + wave * 2 + 0, 1; lane i holds run i & 1 of
+    // the block i / 2 after the first
+    auto pages_of = [&](int block) {
+      return kv_page(A.batch, A.pool, p.b, ((int64_t)(block + (lane >> 1)) * 128 + wave * 32 + (lane & 1) * 16) >> A.pool.shift);
+    };
+    int pages = pages_of(p.k), ahead = pages_of(p.k + 32);
     i32x4a q[QT][D / 64];
     float unit;
     query_terms<T, D, QT>(row_ok ? reinterpret_cast<const T*>(A.q) + (int64_t)(w.first + tok) * A.q_token +
@@ -451,28 +501,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A, 
                           g, q, unit);
     unit *= A.scale;
     const uint64_t* bits = A.mask && row_ok ? A.mask + (int64_t)(w.first + tok) * A.words : A.mask;
-    const int64_t end = min(L.cap, w.ctx + (A.mask ? w.n : min(w.n, (p.x / A.chunks + 1) * A.TT)));
     TileState<T, D, QT, PT> st;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) st.o[j] = f32x4a{0, 0, 0, 0};
     st.m = -__builtin_inff();
     st.l = 0.0f;
     st.e = -100;  // smaller scales lose bits
-    int64_t key = p.k * 128 + wave * 32;
-    const int64_t stop = min(end, k1 * 128);
+    int key = p.k * 128 + wave * 32;
     if (key < stop) {
       Keys32<D> cur, nxt;
-      int page[2];
-#pragma unroll
-      for (int a = 0; a < 2; ++a) page[a] = kv_page(A.batch, A.pool, p.b, (key + 16 * a) >> A.pool.shift);
-      load_keys<D>(A.pool, p.h, key, page, lane, cur);
-      while (true) {
-        const int64_t next = key + 128;
+      load_keys<D>(A.pool, p.h, key, lane_of(pages, 0), lane_of(pages, 1), lane, cur);
+      for (int i = 1;; ++i) {
+        const int next = key + 128;
         const bool more = next < stop;
         if (more) {
-#pragma unroll
-          for (int a = 0; a < 2; ++a) page[a] = kv_page(A.batch, A.pool, p.b, (next + 16 * a) >> A.pool.shift);
-          load_keys<D>(A.pool, p.h, next, page, lane, nxt);
+          if ((i & 31) == 0) {
+            pages = ahead;
+            ahead = pages_of(p.k + i + 32);
+          }
+          load_keys<D>(A.pool, p.h, next, lane_of(pages, 2 * (i & 31)), lane_of(pages, 2 * (i & 31) + 1), lane, nxt);
         }
         step32<T, D, QT, PT>(A, q, unit, cur, key, w.ctx, end, tok, bits, lane, st);
         if (!more) break;
@@ -517,14 +564,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A, 
           for (int j = 0; j < D / 16; ++j) e[j] = out_cvt<T>(acc[j] * inv);
           __builtin_memcpy(dst, e, sizeof(e));
         } else {
-          const int64_t slot = ((int64_t)blockIdx.x * 2 + (p.k == 0 ? 1 : 0)) * 16 + r;
+          const int64_t slot = ((int64_t)share * 2 + (p.k == 0 ? 1 : 0)) * 16 + r;
           __builtin_memcpy(A.part_o + slot * D + d0, acc, sizeof(acc));
           if ((threadIdx.x & 15) == 0) A.part_s[slot] = make_float2(m, sum);
         }
       }
     }
-    at += k1 - p.k;
-    if (at >= to) break;
+    at += (uint32_t)(k1 - p.k);
+    if (at >= to) {
+      leave_part(A, share, p.k == 0 && k1 < p.blocks, at + (uint32_t)(p.blocks - k1), per, w, p);
+      break;
+    }
     __syncthreads();
     next_tile(A, L, w, p);
   }
@@ -589,39 +639,260 @@ __device__ __forceinline__ int key_swizzle(int row) {
   return D == 64 ? (row >> 1) & 7 : row & 15;
 }
 
+// Keys of a step: at heads of 256 half as many, so that two steps fit LDS and the registers
+template <int D>
+constexpr int tile_keys() { return D == 256 ? 32 : 64; }
+
 template <int D, int NW>
 struct TileLds {
-  uint32_t k[2][MXK_TILE * D / 2];  // [key][D] float16, pieces of 8 swizzled
-  uint32_t v[2][MXK_TILE * D / 2];  // [row][64 keys] float16, pieces of 8 swizzled
-  float ks[2][MXK_TILE], vs[2][MXK_TILE];  // vs times 2^(10 - e)
+  static constexpr int K = tile_keys<D>();
+  u32x4 k[2][K * D / 8];  // [key][D] float16, pieces of 8 swizzled
+  u32x4 v[2][K * D / 8];  // [row][K keys] float16, pieces of 8 swizzled
+  float ks[2][K], vs[2][K];  // vs times 2^(10 - e)
   int e[2];
-  uint32_t ok[2];  // bits of the block's runs of 16 keys that have a page
+  uint32_t ok[2];  // bits of the step's runs of 16 keys that have a page
 };
 
-template <typename T, int D, int QT, int PT, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void k_attend_tile(AttendArgs A, int shares) {
-  constexpr int P = 8 / NW;          // pieces of 16 bytes of keys (and of values) a thread and D = 128
-  constexpr int KP = P * D / 128 > 0 ? P * D / 128 : 1;
-  constexpr int CPR = D / 16;        // 16-byte pieces of a row of codes
-  constexpr int PIECES = MXK_TILE * CPR;
-  __shared__ TileLds<D, NW> S;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l32 = lane & 31, h = lane >> 5;
-  const Line L = make_line(A);
-  const int64_t total = line_length(A, L);
-  const int64_t per = line_share(total, shares);
-  // neighbours on the line read the same keys: they go to one XCD
-  const int share = shares % 8 == 0 ? (blockIdx.x & 7) * (shares >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-  const int64_t from = (int64_t)share * per, to = min(total, from + per);
-  zero_padding<T, D, 64 * NW>(A, shares);
-  if (from >= to) return;
+// Swizzle of the 16-byte pieces of a value row (K * 2 bytes)
+template <int D>
+__device__ __forceinline__ int value_swizzle(int row) {
+  return D == 256 ? (row >> 2) & 3 : (row >> 1) & 7;
+}
 
+// What a thread fetches of a step, on its way from memory to LDS
+template <int D, int NW>
+struct Fetched {
+  static constexpr int PIECES = tile_keys<D>() * D / 16, N = PIECES / (64 * NW) > 0 ? PIECES / (64 * NW) : 1;
+  u32x4 k[N];        // 16 elements of a key
+  uint32_t v[N][4];  // four elements of four keys
+  float scale;       // wave 0: of a key, wave 1: of a value
+  int page;          // of that key, waves 0 and 1
+};
+
+template <int D, int NW>
+__device__ __forceinline__ void tile_fetch(const AttendArgs& A, int h, int key, int end, int pages, int first_run,
+                                           Fetched<D, NW>& f) {
+  using F = Fetched<D, NW>;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int in = (1 << A.pool.shift) - 1;
+  const int64_t values = (int64_t)A.pool.H << A.pool.shift;
+#pragma unroll
+  for (int i = 0; i < F::N; ++i) {
+    // D pieces are 16 keys: a wave's lie in one run, with one page
+    const int first = (wave + i * NW) * 64, run = first / D, piece = (first + lane) % D;
+    if (first >= F::PIECES) break;
+    const int page = lane_of(pages, first_run + run);
+    const int64_t row = kv_row(A.pool, max(page, 0), 0, h, (key + run * 16) & in);
+    const int8_t* k = A.pool.codes + row * D;
+    const int8_t* v = k + values * D;
+    f.k[i] = *reinterpret_cast<const u32x4*>(k + (uint32_t)(piece * 16));
+    const int four = piece / (D / 4), c = piece % (D / 4);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      f.v[i][r] = *reinterpret_cast<const uint32_t*>(v + (uint32_t)((four * 4 + r) * D + c * 4));
+  }
+  if (wave < 2) {
+    const int l = lane & (tile_keys<D>() - 1), at = key + l;
+    const int there = __shfl(pages, first_run + (l >> 4));  // with all lanes: they hold each other's pages
+    const int page = at < end ? there : -1;
+    f.page = page;
+    f.scale = 0.0f;
+    if (page >= 0) f.scale = A.pool.scales[kv_row(A.pool, page, wave, h, at & in)];
+  }
+}
+
+template <int D, int NW>
+__device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>& S, int buf, int& e_run) {
+  using F = Fetched<D, NW>;
+  constexpr int K = tile_keys<D>(), RUNS = K / 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+  for (int i = 0; i < F::N; ++i) {
+    const int first = (wave + i * NW) * 64, piece = first + lane;
+    if (first >= F::PIECES) break;
+    {
+      const int row = piece / (D / 16), c = piece % (D / 16);
+      u32x4 half[2];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t u = f.k[i][x] ^ 0x80808080u;
+        half[x >> 1][2 * (x & 1)] = codes_f16(__builtin_amdgcn_perm(0u, u, 0x0C010C00u));
+        half[x >> 1][2 * (x & 1) + 1] = codes_f16(__builtin_amdgcn_perm(0u, u, 0x0C030C02u));
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) S.k[buf][row * (D / 8) + ((2 * c + x) ^ key_swizzle<D>(row))] = half[x];
+    }
+    // keys 16s + 8b + 4h': run s*2 + h', its half b
+    const int four = piece / (D / 4), c = piece % (D / 4);
+    const int run = (four >> 2) * 2 + (four & 1), b = (four >> 1) & 1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t sel = 0x0C000C00u | (uint32_t)j | (uint32_t)(4 + j) << 16;
+      u32x2 two;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        two[x] = codes_f16(__builtin_amdgcn_perm(f.v[i][2 * x + 1] ^ 0x80808080u, f.v[i][2 * x] ^ 0x80808080u, sel));
+      const int row = j * (D / 4) + c;
+      reinterpret_cast<u32x2*>(&S.v[buf][row * (K / 8) + (run ^ value_swizzle<D>(row))])[b] = two;
+    }
+  }
+  if (wave == 0 && lane < K) S.ks[buf][lane] = f.scale;
+  if (wave == 1) {
+    const uint32_t bb = mag_bits(f.scale);
+    int top = (int)((bb < 0x7F800000u ? bb : 0u) >> 23) - 127;
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) top = max(top, __shfl_xor(top, i));
+    e_run = max(e_run, top);
+    if (lane < K) S.vs[buf][lane] = f.scale * scale_of_exp(10 - e_run);
+    const uint64_t there = __ballot(f.page >= 0);
+    uint32_t ok = 0;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) ok |= (uint32_t)(there >> (16 * i) & 1) << i;
+    if (lane == 0) {
+      S.e[buf] = e_run;
+      S.ok[buf] = ok;
+    }
+  }
+}
+
+// Sums of a lane's row; of its elements those that query_halves' half h names
+template <int D>
+struct RowState {
+  f32x16a o[D / 32];
+  float m, l;
+  int e;
+};
+
+// A step's keys for a wave's 32 rows.  OPEN: every row sees all of them; else `see` has a bit for
+// each (shifted down by the lane's 4h).
+template <int D, int QT, int PT, int NW, bool OPEN>
+__device__ __forceinline__ void tile_step(const TileLds<D, NW>& S, int buf, const f16x8a (&q)[QT][D / 16], float unit,
+                                          uint64_t see, RowState<D>& st) {
+  constexpr int K = tile_keys<D>(), KT = K / 32;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int e_new = __builtin_amdgcn_readfirstlane(S.e[buf]);
+  f32x16a t[KT];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[kt][i] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int row = kt * 32 + l32;
+      const f16x8a kf = __builtin_bit_cast(f16x8a, S.k[buf][row * (D / 8) + ((2 * i + h) ^ key_swizzle<D>(row))]);
+#pragma unroll
+      for (int n = 0; n < QT; ++n) t[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[n][i], t[kt], 0, 0, 0);
+    }
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const f32x4a s4 = *reinterpret_cast<const f32x4a*>(&S.ks[buf][kt * 32 + a * 8 + h * 4]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = t[kt][4 * a + r] * s4[r];
+        if (!OPEN && !((uint32_t)(see >> (32 * kt)) >> (8 * a + r) & 1)) x = -__builtin_inff();
+        t[kt][4 * a + r] = x;
+        top = fmaxf(top, x);
+      }
+    }
+  top *= unit;
+  // the running maximum follows the largest score by steps of at least 2^4, as in step32
+  if (__ballot(top > st.m + 4.0f) || e_new != st.e) {
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float m = fmaxf(st.m, top);
+    const float shrink = m == st.m ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
+    const float both = shrink * scale_of_exp(st.e - e_new);
+    st.l *= shrink;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[j][i] *= both;
+    st.m = m;
+    st.e = e_new;
+  }
+  const float m = st.m == -__builtin_inff() ? 0.0f : st.m;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    f16x8a p[PT][2];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const f32x4a s4 = *reinterpret_cast<const f32x4a*>(&S.vs[buf][kt * 32 + a * 8 + h * 4]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t[kt][4 * a + r], unit, -m));
+        float c = x * s4[r];
+        if (!OPEN && !((uint32_t)(see >> (32 * kt)) >> (8 * a + r) & 1)) x = c = 0.0f;
+        st.l += x;
+        if constexpr (PT == 2) asm("" : "+v"(c));
+        const int s = a >> 1, i = 4 * (a & 1) + r;
+        p[0][s][i] = (_Float16)c;
+        if constexpr (PT == 2) p[1][s][i] = (_Float16)(c - (float)p[0][s][i]);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const int row = j * 32 + l32, run = (kt * 2 + s) * 2 + h;
+        const f16x8a vf = __builtin_bit_cast(f16x8a, S.v[buf][row * (K / 8) + (run ^ value_swizzle<D>(row))]);
+#pragma unroll
+        for (int n = 0; n < PT; ++n) st.o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[n][s], st.o[j], 0, 0, 0);
+      }
+  }
+}
+
+// Which of a step's K keys from `key` on a row sees, a bit each
+template <int K>
+__device__ __forceinline__ uint64_t row_sees(const AttendArgs& A, const uint64_t* __restrict__ bits, int key, int ctx, int end,
+                                             int tok, uint32_t ok) {
+  const int j0 = key - ctx;  // the first key among the new tokens
+  uint64_t see = ~0ull;
+  if (!A.mask) {
+    const int last = tok - j0;  // the last key of the step that the row sees
+    see = last < 0 ? 0 : last >= 63 ? ~0ull : (2ull << last) - 1;
+  } else if (j0 >= 0) {
+    const int word = j0 >> 6, sh = j0 & 63;
+    const uint64_t one = word < A.words ? bits[word] : 0, two = word + 1 < A.words ? bits[word + 1] : 0;
+    see = sh ? one >> sh | two << (64 - sh) : one;
+  } else if (j0 > -64) {
+    see = bits[0] << -j0 | ((1ull << -j0) - 1);
+  }
+  if (end - key < 64) see &= (1ull << (end - key)) - 1;  // keys past the end; there is one before it
+#pragma unroll
+  for (int i = 0; i < K / 16; ++i)
+    if (!(ok >> i & 1)) see &= ~(0xFFFFull << (16 * i));
+  return see;
+}
+
+template <typename T, int D, int QT, int PT, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_attend_tile(AttendArgs A) {
+  constexpr int K = tile_keys<D>(), RUNS = K / 16, BATCH = 64 / RUNS;  // runs of a step, steps of a batch of pages
+  __shared__ TileLds<D, NW> S;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l32 = lane & 31, h = lane >> 5;
+  // neighbours on the line read the same keys: they go to one XCD
+  const int share = A.shares % 8 == 0 ? (blockIdx.x & 7) * (A.shares >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+  const Line L = make_line(A);
+  zero_padding<T, D, 64 * NW>(A);
+  uint32_t from, to, per;
   SeqWork w;
-  Place p = line_place(A, L, from, w);
-  int64_t at = from;
+  Place p;
+  if (!line_share(A, L, share, from, to, per, w, p)) {
+    leave_part(A, share, false, 0, 1, w, p);
+    return;
+  }
+  uint32_t at = from;
   while (true) {
-    const int64_t k1 = min(p.blocks, p.k + (to - at));
+    const int k1 = (int)min((uint32_t)p.blocks, (uint32_t)p.k + (to - at));
     const bool whole = p.k == 0 && k1 == p.blocks;
+    const int end = tile_end(A, w, p);
+    const int key0 = p.k * A.keys, stop = (int)min((int64_t)end, (int64_t)k1 * A.keys);
+    RunPages pages;
+    pages.start(A, p.b, key0 >> 4);
     int tok, head;
     const bool row_ok = tile_row(A, w, p, wave * 32 + l32, tok, head);
     const bool busy = __ballot(row_ok) != 0;
@@ -633,245 +904,64 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void k_attend
                            h, q, unit);
     unit *= A.scale;
     const uint64_t* bits = A.mask && row_ok ? A.mask + (int64_t)(w.first + tok) * A.words : A.mask;
-    const int64_t end = min(L.cap, w.ctx + (A.mask ? w.n : min(w.n, (p.x / A.chunks + 1) * A.TT)));
-    const int64_t key0 = p.k * A.keys, stop = min(end, k1 * A.keys);
-    // the wave's first and last token: between them a causal block needs its mask
+    // the wave's first and last token: between them a causal step needs its mask
     int lo_tok = row_ok ? tok : 0x7FFFFFFF, hi_tok = row_ok ? tok : -1;
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) lo_tok = min(lo_tok, __shfl_xor(lo_tok, i)), hi_tok = max(hi_tok, __shfl_xor(hi_tok, i));
     lo_tok = __builtin_amdgcn_readfirstlane(lo_tok);
     hi_tok = __builtin_amdgcn_readfirstlane(hi_tok);
 
-    f32x16a o[D / 32];
+    RowState<D> st;
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[j][i] = 0.0f;
-    float m = -__builtin_inff(), l = 0.0f;
-    int e = -100;
-
-    // codes of a block on their way: the thread's pieces of keys, and four keys by four elements of values
-    u32x4 kr[KP];
-    uint32_t vr[KP][4];
-    float sr = 0.0f;
-    int run_ok = 0;
-    auto fetch = [&](int64_t key) {
-#pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        const int piece = tid + i * 64 * NW, row = piece / CPR, c = piece % CPR;
-        if (piece >= PIECES) break;
-        const int64_t kk = key + row;
-        const int page = kv_page(A.batch, A.pool, p.b, kk >> A.pool.shift);
-        const int64_t src = kv_row(A.pool, max(page, 0), 0, p.h, (int)(kk & ((1 << A.pool.shift) - 1)));
-        kr[i] = *reinterpret_cast<const u32x4*>(A.pool.codes + src * D + c * 16);
-      }
-#pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        const int piece = tid + i * 64 * NW, four = piece / (D / 4), c = piece % (D / 4);
-        if (piece >= PIECES) break;
-        const int64_t kk = key + four * 4;
-        const int page = kv_page(A.batch, A.pool, p.b, kk >> A.pool.shift);
-        const int64_t src = kv_row(A.pool, max(page, 0), 1, p.h, (int)(kk & ((1 << A.pool.shift) - 1)));
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          vr[i][r] = *reinterpret_cast<const uint32_t*>(A.pool.codes + (src + r) * D + c * 4);
-      }
-      if (wave < 2) {
-        const int64_t kk = key + lane;
-        const int page = kk < end ? kv_page(A.batch, A.pool, p.b, kk >> A.pool.shift) : -1;
-        sr = 0.0f;
-        if (page >= 0) sr = A.pool.scales[kv_row(A.pool, page, wave, p.h, (int)(kk & ((1 << A.pool.shift) - 1)))];
-        run_ok = page >= 0;
-      }
-    };
+      for (int i = 0; i < 16; ++i) st.o[j][i] = 0.0f;
+    st.m = -__builtin_inff();
+    st.l = 0.0f;
+    st.e = -100;
     int e_run = -100;  // of wave 1, which finds the exponent for all
-    auto put = [&](int buf) {
-#pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        const int piece = tid + i * 64 * NW, row = piece / CPR, c = piece % CPR;
-        if (piece >= PIECES) break;
-        u32x4 half[2];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t u = kr[i][x] ^ 0x80808080u;
-          half[x >> 1][2 * (x & 1)] = codes_f16(__builtin_amdgcn_perm(0u, u, 0x0C010C00u));
-          half[x >> 1][2 * (x & 1) + 1] = codes_f16(__builtin_amdgcn_perm(0u, u, 0x0C030C02u));
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          *reinterpret_cast<u32x4*>(&S.k[buf][row * (D / 2) + (((2 * c + x) ^ key_swizzle<D>(row)) * 4)]) = half[x];
-      }
-#pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        const int piece = tid + i * 64 * NW, four = piece / (D / 4), c = piece % (D / 4);
-        if (piece >= PIECES) break;
-        // keys 16s + 8b + 4h': run s*2 + h', its half b
-        const int run = (four >> 2) * 2 + (four & 1), b = (four >> 1) & 1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t sel = 0x0C000C00u | (uint32_t)j | (uint32_t)(4 + j) << 16;
-          u32x2 two;
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            two[x] = codes_f16(__builtin_amdgcn_perm(vr[i][2 * x + 1] ^ 0x80808080u, vr[i][2 * x] ^ 0x80808080u, sel));
-          const int row = j * (D / 4) + c;
-          *reinterpret_cast<u32x2*>(&S.v[buf][row * (MXK_TILE / 2) + ((run ^ ((row >> 1) & 7)) * 4) + b * 2]) = two;
-        }
-      }
-      if (wave == 0) S.ks[buf][lane] = sr;
-      if (wave == 1) {
-        const uint32_t bb = mag_bits(sr);
-        int top = (int)((bb < 0x7F800000u ? bb : 0u) >> 23) - 127;
-#pragma unroll
-        for (int i = 1; i < 64; i <<= 1) top = max(top, __shfl_xor(top, i));
-        e_run = max(e_run, top);
-        S.vs[buf][lane] = sr * scale_of_exp(10 - e_run);
-        const uint64_t b = __ballot(run_ok);
-        if (lane == 0) {
-          S.e[buf] = e_run;
-          S.ok[buf] = (uint32_t)(b & 1) | (uint32_t)(b >> 16 & 1) << 1 | (uint32_t)(b >> 32 & 1) << 2 |
-                      (uint32_t)(b >> 48 & 1) << 3;
-        }
-      }
-    };
-
+    Fetched<D, NW> f;
     __syncthreads();  // the tile before is read
     if (key0 < stop) {
-      fetch(key0);
-      put(0);
+      tile_fetch<D, NW>(A, p.h, key0, end, pages.cur, 0, f);
+      tile_put<D, NW>(f, S, 0, e_run);
     }
     __syncthreads();
-    int buf = 0;
-    for (int64_t key = key0; key < stop; key += MXK_TILE, buf ^= 1) {
-      const bool more = key + MXK_TILE < stop;
-      if (more) fetch(key + MXK_TILE);
-      const int e_new = __builtin_amdgcn_readfirstlane(S.e[buf]);
-      const uint32_t ok = __builtin_amdgcn_readfirstlane(S.ok[buf]);
-      const int64_t j0 = key - w.ctx;  // the first key among the new tokens
-      // rows of tokens before the whole block see none of it
-      if (busy && (A.mask || j0 <= hi_tok)) {
-        const bool open = key + MXK_TILE <= end && ok == 15 && (j0 + MXK_TILE <= 0 || (!A.mask && j0 + MXK_TILE - 1 <= lo_tok));
-        uint64_t see = ~0ull;
-        if (!open) {
-          if (A.mask) {
-            const int64_t word = j0 >= 0 ? j0 >> 6 : -1;
-            const uint64_t none = 0;
-            if (j0 >= 0) {
-              const int sh = (int)(j0 & 63);
-              const uint64_t one = word < A.words ? bits[word] : none;
-              const uint64_t two = word + 1 < A.words ? bits[word + 1] : none;
-              see = sh ? one >> sh | two << (64 - sh) : one;
-            } else if (j0 > -MXK_TILE) {
-              see = bits[0] << (int)-j0 | ((1ull << (int)-j0) - 1);
-            }
-          } else {
-            const int64_t last = tok - j0;  // the last key of the block that the row sees
-            see = last < 0 ? 0 : last >= 63 ? ~0ull : (2ull << (int)last) - 1;
-          }
-          if (key + MXK_TILE > end) see &= (1ull << (int)(end - key)) - 1;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!(ok >> i & 1)) see &= ~(0xFFFFull << (16 * i));
-          see >>= 4 * h;
-        }
-        float t[2][16];
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          f32x16a acc;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-          const int row = kt * 32 + l32;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            const f16x8a kf = *reinterpret_cast<const f16x8a*>(&S.k[buf][row * (D / 2) + (((2 * i + h) ^ key_swizzle<D>(row)) * 4)]);
-#pragma unroll
-            for (int n = 0; n < QT; ++n) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[n][i], acc, 0, 0, 0);
-          }
-#pragma unroll
-          for (int a = 0; a < 4; ++a) {
-            const f32x4a s4 = *reinterpret_cast<const f32x4a*>(&S.ks[buf][kt * 32 + a * 8 + h * 4]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) t[kt][4 * a + r] = acc[4 * a + r] * s4[r];
-          }
-        }
-        if (!open) {
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (!((uint32_t)(see >> (32 * kt)) >> (8 * (i >> 2) + (i & 3)) & 1)) t[kt][i] = -__builtin_inff();
-        }
-        float top = t[0][0];
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, t[kt][i]);
-        top *= unit;
-        if (__ballot(top > m + 4.0f) || e_new != e) {
-          top = fmaxf(top, __shfl_xor(top, 32));
-          const float mm = fmaxf(m, top);
-          const float shrink = mm == m ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
-          const float both = shrink * scale_of_exp(e - e_new);
-          l *= shrink;
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[j][i] *= both;
-          m = mm;
-          e = e_new;
-        }
-        const float ms = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          f16x8a pr[PT][2];
-#pragma unroll
-          for (int a = 0; a < 4; ++a) {
-            const f32x4a s4 = *reinterpret_cast<const f32x4a*>(&S.vs[buf][kt * 32 + a * 8 + h * 4]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t[kt][4 * a + r], unit, -ms));
-              float c = x * s4[r];
-              if (!open && !((uint32_t)(see >> (32 * kt)) >> (8 * a + r) & 1)) x = c = 0.0f;
-              l += x;
-              if constexpr (PT == 2) asm("" : "+v"(c));
-              const int s = a >> 1, i = 4 * (a & 1) + r;
-              pr[0][s][i] = (_Float16)c;
-              if constexpr (PT == 2) pr[1][s][i] = (_Float16)(c - (float)pr[0][s][i]);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j) {
-            const int row = j * 32 + l32;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              const int run = (kt * 2 + s) * 2 + h;
-              const f16x8a vf =
-                  *reinterpret_cast<const f16x8a*>(&S.v[buf][row * (MXK_TILE / 2) + ((run ^ ((row >> 1) & 7)) * 4)]);
-#pragma unroll
-              for (int n = 0; n < PT; ++n) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pr[n][s], o[j], 0, 0, 0);
-            }
-          }
-        }
+    int buf = 0, step = 1;
+    for (int key = key0; key < stop; key += K, buf ^= 1, ++step) {
+      const bool more = key + K < stop;
+      if (more) {
+        if (step % BATCH == 0) pages.advance(A, p.b, (key0 >> 4) + (step + BATCH) * RUNS);
+        tile_fetch<D, NW>(A, p.h, key + K, end, pages.cur, (step % BATCH) * RUNS, f);
       }
-      if (more) put(buf ^ 1);
+      const uint32_t ok = __builtin_amdgcn_readfirstlane(S.ok[buf]);
+      const int j0 = key - w.ctx;
+      if (busy && (A.mask || j0 <= hi_tok)) {  // else every row's token comes before these keys
+        if (key + K <= end && ok == (1u << RUNS) - 1 && (j0 + K <= 0 || (!A.mask && j0 + K - 1 <= lo_tok)))
+          tile_step<D, QT, PT, NW, true>(S, buf, q, unit, 0, st);
+        else
+          tile_step<D, QT, PT, NW, false>(S, buf, q, unit, row_sees<K>(A, bits, key, w.ctx, end, tok, ok) >> (4 * h), st);
+      }
+      if (more) tile_put<D, NW>(f, S, buf ^ 1, e_run);
       __syncthreads();
     }
 
     // a lane has its row's elements 4c .. 4c+3 for every c with bit 2 of c equal to h
+    float l = st.l;
     l += __shfl_xor(l, 32);
     if (row_ok) {
-      const float down = scale_of_exp(e - 1), inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float down = scale_of_exp(st.e - 1), inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t slot = ((int64_t)share * 2 + (p.k == 0 ? 1 : 0)) * (32 * NW) + wave * 32 + l32;
       T* dst = reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D;
 #pragma unroll
       for (int a = 0; a < D / 32; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float x[4];
+          f32x4a x;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int row = j * (D / 4) + 8 * a + r;
-            x[j] = o[row / 32][(row % 32 / 8) * 4 + row % 4] * down;
+            x[j] = st.o[row / 32][(row % 32 / 8) * 4 + row % 4] * down;
           }
           const int d = 4 * (8 * a + 4 * h + r);
           if (whole) {
@@ -880,65 +970,81 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D == 256 ? 1 : 2) void k_attend
             for (int j = 0; j < 4; ++j) y[j] = out_cvt<T>(x[j] * inv);
             __builtin_memcpy(dst + d, y, sizeof(y));
           } else {
-            __builtin_memcpy(A.part_o + slot * D + d, x, sizeof(x));
+            *reinterpret_cast<f32x4a*>(A.part_o + slot * D + d) = x;
           }
         }
-      if (!whole && h == 0) A.part_s[slot] = make_float2(m, l);
+      if (!whole && h == 0) A.part_s[slot] = make_float2(st.m, l);
     }
-    at += k1 - p.k;
-    if (at >= to) break;
+    at += (uint32_t)(k1 - p.k);
+    if (at >= to) {
+      leave_part(A, share, p.k == 0 && k1 < p.blocks, at + (uint32_t)(p.blocks - k1), per, w, p);
+      break;
+    }
     next_tile(A, L, w, p);
   }
 }
 
-// A tile whose first block lies in share s and whose last one does not: its
-// parts are share s's second one and the first ones of the shares after it, up to the one
-// with its last block.  A wave a row.
+// A tile that share s begins and does not end: its parts are share s's second
+// one and the first ones of the shares after it, up to the one with its last
+// block.  A wave a row, 64 parts at a time: a lane finds a part's weight, then
+// all lanes add the parts' sums in their order.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void k_attend_join(AttendArgs A, int shares, int rows) {
+__global__ __launch_bounds__(256) void k_attend_join(AttendArgs A) {
   constexpr int E = D / 64;
-  const Line L = make_line(A);
-  const int64_t total = line_length(A, L);
-  const int64_t per = line_share(total, shares);
-  const int s = blockIdx.x, r = blockIdx.y;
-  const int64_t from = s * per, to = min(total, from + per);
-  if (from >= to || to == total) return;
+  const int s = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const PartTile t = A.part_t[s];
+  if (t.last < 0) return;
   SeqWork w;
-  const Place p = line_place(A, L, to - 1, w);
-  const int64_t begin = to - 1 - p.k, end = begin + p.blocks;
-  if (end <= to || begin < from) return;
-  int tok, head;
-  if (!tile_row(A, w, p, r, tok, head)) return;
-  const int last = (int)((end - 1) / per);
-  const int lane = threadIdx.x;
-  float m = -__builtin_inff();
-  for (int i = s + lane; i <= last; i += 64) m = fmaxf(m, A.part_s[((int64_t)i * 2 + (i == s)) * rows + r].x);
+  w.first = t.first;
+  w.n = t.n;
+  Place p;
+  p.h = t.h;
+  p.x = t.x;
+  const int parts = t.last - s + 1;
+  for (int r = blockIdx.y * 4 + wave; r < A.rows; r += gridDim.y * 4) {
+    int tok, head;
+    if (!tile_row(A, w, p, r, tok, head)) continue;
+    auto slot = [&](int i) { return ((int64_t)(s + i) * 2 + (i == 0)) * A.rows + r; };
+    float m = -__builtin_inff();
+    for (int i = lane; i < parts; i += 64) m = fmaxf(m, A.part_s[slot(i)].x);
 #pragma unroll
-  for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
-  float sum = 0.0f, acc[E];
+    for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
+    float sum = 0.0f, acc[E];
 #pragma unroll
-  for (int j = 0; j < E; ++j) acc[j] = 0.0f;
-  for (int i = s; i <= last; ++i) {
-    const int64_t slot = ((int64_t)i * 2 + (i == s)) * rows + r;
-    const float2 ms = A.part_s[slot];
-    const float f = ms.x == m ? 1.0f : __builtin_amdgcn_exp2f(ms.x - m);
-    sum += f * ms.y;
-    float v[E];
-    __builtin_memcpy(v, A.part_o + slot * D + lane * E, sizeof(v));
+    for (int j = 0; j < E; ++j) acc[j] = 0.0f;
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+      const int n = min(64, parts - i0);
+      const float2 ms = A.part_s[slot(i0 + min(lane, n - 1))];
+      const float f = lane >= n ? 0.0f : ms.x == m ? 1.0f : __builtin_amdgcn_exp2f(ms.x - m);
+      if (lane < n) sum += f * ms.y;
+      for (int i = 0; i < n; i += 8) {
+        float v[8][E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) acc[j] = __builtin_fmaf(f, v[j], acc[j]);
+        for (int u = 0; u < 8; ++u)  // past the last part: it again, with a weight of zero
+          __builtin_memcpy(v[u], A.part_o + slot(i0 + min(i + u, n - 1)) * D + lane * E, sizeof(v[u]));
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float g = __uint_as_float(lane_of(__float_as_uint(f), min(i + u, 63)));
+#pragma unroll
+          for (int j = 0; j < E; ++j) acc[j] = __builtin_fmaf(i + u < n ? g : 0.0f, v[u][j], acc[j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T e[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) e[j] = out_cvt<T>(acc[j] * inv);
+    __builtin_memcpy(reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D + lane * E, e, sizeof(e));
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  T e[E];
-#pragma unroll
-  for (int j = 0; j < E; ++j) e[j] = out_cvt<T>(acc[j] * inv);
-  __builtin_memcpy(reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D + lane * E, e, sizeof(e));
 }
 
 // ---------------------------------------------------------------- host
 struct AttendPlan {
-  int rows, keys, TT, GC, chunks, shares;
+  int rows, keys, TT, GC, chunks, shares, cap, most;
   bool cut;  // a tile may be cut
+  bool fits;  // the line is below 2^31 blocks
 };
 
 static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int H, int G, int D) {
@@ -953,26 +1059,33 @@ static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int
   while (a.TT * 2 * a.GC <= a.rows) a.TT *= 2;
   // no more shares than blocks there can be
   const double tiles = ((double)T / a.TT + (double)std::min(B, T)) * a.chunks * H;
-  const double blocks = std::ceil((double)width * page / a.keys);
-  a.cut = blocks > 1 && B > 0;
+  a.cap = (int)std::min<int64_t>(width * page, ((int64_t)1 << 31) - ((int64_t)1 << 16));
+  a.most = std::max(1, (a.cap + a.keys - 1) / a.keys);
+  a.cut = a.most > 1 && B > 0;
+  a.fits = tiles * a.most < 2147483648.0;
   const double most = (a.rows == 256 || D == 256 ? 1.0 : 2.0) * num_cus();  // workgroups that run at once
-  a.shares = (int)std::max(1.0, std::min(most, tiles * std::max(1.0, blocks)));
+  a.shares = (int)std::max(1.0, std::min(most, tiles * a.most));
   return a;
+}
+
+static size_t attend_bytes(const AttendPlan& a, int D) {
+  if (!a.cut || a.shares == 1) return 0;
+  return (size_t)a.shares * (2 * (size_t)a.rows * ((size_t)D * 4 + sizeof(float2)) + sizeof(PartTile));
 }
 
 template <typename T, int D, int QT, int PT>
 static int launch_attend(const AttendArgs& A, const AttendPlan& a, hipStream_t st) {
   constexpr int QH = sizeof(T) == 4 ? 2 : 1;  // float16 terms of a query
   if (a.rows == 16) {
-    hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A, a.shares);
+    hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A);
   } else if (a.rows == 128) {
-    hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 4>), dim3(a.shares), dim3(256), 0, st, A, a.shares);
+    hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 4>), dim3(a.shares), dim3(256), 0, st, A);
   } else {
     if constexpr (D < 256)
-      hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 8>), dim3(a.shares), dim3(512), 0, st, A, a.shares);
+      hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 8>), dim3(a.shares), dim3(512), 0, st, A);
   }
   if (a.cut && a.shares > 1)
-    hipLaunchKernelGGL((k_attend_join<T, D>), dim3(a.shares - 1, a.rows), dim3(64), 0, st, A, a.shares, a.rows);
+    hipLaunchKernelGGL((k_attend_join<T, D>), dim3(a.shares - 1, a.rows == 16 ? 4 : 16), dim3(256), 0, st, A);
   return check_launch("kv_attend");
 }
 
@@ -994,7 +1107,7 @@ size_t mxk_kv_pages_attend_workspace(int64_t tokens, int64_t B, int64_t width, i
   if (tokens <= 0 || B <= 0 || width < 0 || heads < 1 || q_heads < heads || q_heads % heads || !kv_page_ok(page))
     return 0;
   const AttendPlan a = plan_attend(tokens, B, width, page, heads, q_heads / heads, D);
-  return a.cut ? (size_t)a.shares * 2 * a.rows * ((size_t)D * 4 + 8) : 0;
+  return attend_bytes(a, D);
 }
 
 int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_head, int q_heads, const void* codes,
@@ -1024,8 +1137,9 @@ int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_he
     return fail(MXK_EINVAL, "kv_attend: codes and scales start on 16 bytes");
   const int G = q_heads / heads;
   const AttendPlan a = plan_attend(tokens, B, width, page, heads, G, D);
-  const size_t part = (size_t)a.shares * 2 * a.rows;
-  if (a.cut && a.shares > 1 && (!workspace || workspace_nbytes < part * ((size_t)D * 4 + 8) || !aligned16(workspace)))
+  if (!a.fits) return fail(MXK_EINVAL, "kv_attend: more than 2^31 blocks of keys that the table has room for");
+  const size_t need = attend_bytes(a, D), part = (size_t)a.shares * 2 * a.rows;
+  if (need && (!workspace || workspace_nbytes < need || !aligned16(workspace)))
     return fail(MXK_EINVAL, "kv_attend: workspace too small (mxk_kv_pages_attend_workspace) or not on 16 bytes");
   AttendArgs A;
   A.q = q;
@@ -1044,8 +1158,13 @@ int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_he
   A.GC = a.GC;
   A.chunks = a.chunks;
   A.out = out;
-  A.part_o = reinterpret_cast<float*>(workspace);
-  A.part_s = workspace ? reinterpret_cast<float2*>(A.part_o + part * D) : nullptr;
+  A.cap = a.cap;
+  A.most = a.most;
+  A.rows = a.rows;
+  A.shares = a.shares;
+  A.part_o = need ? reinterpret_cast<float*>(workspace) : nullptr;
+  A.part_s = need ? reinterpret_cast<float2*>(A.part_o + part * D) : nullptr;
+  A.part_t = need ? reinterpret_cast<PartTile*>(A.part_s + part) : nullptr;
   if (q_type == MXK_IN_F32) return launch_attend_d<float, 3, 2>(D, A, a, st);
   if (q_type == MXK_IN_F16) return launch_attend_d<__half, 2, 1>(D, A, a, st);
   return launch_attend_d<hip_bfloat16, 2, 1>(D, A, a, st);
