@@ -579,8 +579,8 @@ int mxk_kv_pages_read(const void* codes, const float* scales, int64_t pages, int
                       int64_t tokens, int y_type, void* k, void* v, void* stream);
 
 /* Workspace bytes (16-byte aligned) mxk_kv_pages_attend needs (0 if none). */
-size_t mxk_kv_pages_attend_workspace(int64_t tokens, int64_t B, int64_t width, int page, int heads, int q_heads,
-                                     int D);
+size_t mxk_kv_pages_attend_workspace(int q_type, int64_t tokens, int64_t B, int64_t width, int page, int heads,
+                                     int q_heads, int D);
 
 /* out [tokens][q_heads][D] (q_type) = softmax(scale * q k^T) v over the keys
  * that a new token sees: the lengths[b] held ones, and of the new ones (which

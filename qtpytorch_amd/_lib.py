@@ -105,7 +105,7 @@ SIGNATURES = {
                                     c_int, c_vp, c_int, c_int, c_vp, c_vp]),
     "mxk_kv_pages_read": (c_int, [c_vp, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int,
                                   c_vp, c_vp, c_vp]),
-    "mxk_kv_pages_attend_workspace": (c_sz, [c_i64, c_i64, c_i64, c_int, c_int, c_int, c_int]),
+    "mxk_kv_pages_attend_workspace": (c_sz, [c_int, c_i64, c_i64, c_i64, c_int, c_int, c_int, c_int]),
     "mxk_kv_pages_attend": (c_int, [c_vp, c_int, c_i64, c_i64, c_int, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_vp,
                                     c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_float, c_vp, c_vp, c_sz, c_vp]),
     "mxk_kv_pages_keep": (c_int, [c_vp, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp,

@@ -31,6 +31,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace mxk {
 
@@ -596,7 +597,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
 #define MXK_TILE 64
 
 template <typename T, int D, int QT>
-__device__ __forceinline__ void query_halves(const T* __restrict__ row, int h, f16x8a (&q)[QT][D / 16], float& unit) {
+__device__ __forceinline__ void query_halves(const T* __restrict__ row, int h, f16x8a (&q)[QT][D / 16], float& unit,
+                                             bool& nan) {
   float x[D / 16][8];
   uint32_t m = 0;
 #pragma unroll
@@ -610,11 +612,13 @@ __device__ __forceinline__ void query_halves(const T* __restrict__ row, int h, f
     }
   }
   m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-  // a power of two takes the largest to 2^14 .. 2^15; zeros and NaN as in query_terms
+  // a power of two takes the largest to 2^14 .. 2^15; rows below 2^-100 count as zeros, and so do, at first, those
+  // with a NaN or an infinity
   const bool some = m >= 0x0D800000u && m < 0x7F800000u;
   const int e = some ? (int)(m >> 23) - 127 : 0;
   const float up = some ? scale_of_exp(14 - e) : 0.0f;
-  unit = m >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : scale_of_exp(e - 14 + 9);
+  unit = scale_of_exp(e - 14 + 9);
+  nan = m >= 0x7F800000u;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -647,10 +651,10 @@ template <int D, int NW>
 struct TileLds {
   static constexpr int K = tile_keys<D>();
   u32x4 k[2][K * D / 8];  // [key][D] float16, pieces of 8 swizzled
-  u32x4 v[2][K * D / 8];  // [row][K keys] float16, pieces of 8 swizzled
-  float ks[2][K], vs[2][K];  // vs times 2^(10 - e)
-  int e[2];
-  uint32_t ok[2];  // bits of the step's runs of 16 keys that have a page
+  u32x4 v[3][K * D / 8];  // [row][K keys] float16, pieces of 8 swizzled
+  float ks[3][K], vs[3][K];  // vs times 2^(10 - e)
+  int e[3];
+  uint32_t ok[3];  // bits of the step's runs of 16 keys that have a page; bit 31: a value's scale is not finite
 };
 
 // Swizzle of the 16-byte pieces of a value row (K * 2 bytes)
@@ -702,10 +706,11 @@ __device__ __forceinline__ void tile_fetch(const AttendArgs& A, int h, int key, 
 }
 
 template <int D, int NW>
-__device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>& S, int buf, int& e_run) {
+__device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>& S, int step, int& e_run) {
   using F = Fetched<D, NW>;
   constexpr int K = tile_keys<D>(), RUNS = K / 16;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int buf = step % 3;
 #pragma unroll
   for (int i = 0; i < F::N; ++i) {
     const int first = (wave + i * NW) * 64, piece = first + lane;
@@ -720,7 +725,7 @@ __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>
         half[x >> 1][2 * (x & 1) + 1] = codes_f16(__builtin_amdgcn_perm(0u, u, 0x0C030C02u));
       }
 #pragma unroll
-      for (int x = 0; x < 2; ++x) S.k[buf][row * (D / 8) + ((2 * c + x) ^ key_swizzle<D>(row))] = half[x];
+      for (int x = 0; x < 2; ++x) S.k[step & 1][row * (D / 8) + ((2 * c + x) ^ key_swizzle<D>(row))] = half[x];
     }
     // keys 16s + 8b + 4h': run s*2 + h', its half b
     const int four = piece / (D / 4), c = piece % (D / 4);
@@ -748,6 +753,7 @@ __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>
     uint32_t ok = 0;
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) ok |= (uint32_t)(there >> (16 * i) & 1) << i;
+    if (__ballot(bb >= 0x7F800000u)) ok |= 1u << 31;
     if (lane == 0) {
       S.e[buf] = e_run;
       S.ok[buf] = ok;
@@ -763,42 +769,70 @@ struct RowState {
   int e;
 };
 
-// A step's keys for a wave's 32 rows.  OPEN: every row sees all of them; else `see` has a bit for
-// each (shifted down by the lane's 4h).
-template <int D, int QT, int PT, int NW, bool OPEN>
-__device__ __forceinline__ void tile_step(const TileLds<D, NW>& S, int buf, const f16x8a (&q)[QT][D / 16], float unit,
-                                          uint64_t see, RowState<D>& st) {
-  constexpr int K = tile_keys<D>(), KT = K / 32;
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
-  const int e_new = __builtin_amdgcn_readfirstlane(S.e[buf]);
-  f32x16a t[KT];
+// Scores of a wave's 32 rows against a step's keys, but for the row's unit.  The stages' LDS reads are issued
+// a stage ahead and held there: left to itself the compiler waits for each of them in front of its MFMA.
+template <int D, int QT, int NW>
+__device__ __forceinline__ void tile_scores(const TileLds<D, NW>& S, int step, const f16x8a (&q)[QT][D / 16],
+                                            f32x16a (&t)[tile_keys<D>() / 32]) {
+  constexpr int KT = tile_keys<D>() / 32, N = D / 16;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, buf = step % 3;
+  auto key = [&](int kt, int i) {
+    const int row = kt * 32 + l32;
+    return __builtin_bit_cast(f16x8a, S.k[step & 1][row * (D / 8) + ((2 * i + h) ^ key_swizzle<D>(row))]);
+  };
+  f16x8a a[N], b[N];
+  f32x4a ks[KT][4];
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = key(0, i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) t[0][i] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (KT == 2) b[i] = key(1, i);
+#pragma unroll
+    for (int n = 0; n < QT; ++n) t[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i], q[n][i], t[0], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t[kt][i] = 0.0f;
+    for (int x = 0; x < 4; ++x) ks[kt][x] = *reinterpret_cast<const f32x4a*>(&S.ks[buf][kt * 32 + x * 8 + h * 4]);
+  if constexpr (KT == 2) {
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i)
+    for (int i = 0; i < 16; ++i) t[1][i] = 0.0f;
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const int row = kt * 32 + l32;
-      const f16x8a kf = __builtin_bit_cast(f16x8a, S.k[buf][row * (D / 8) + ((2 * i + h) ^ key_swizzle<D>(row))]);
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int n = 0; n < QT; ++n) t[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[n][i], t[kt], 0, 0, 0);
-    }
+      for (int n = 0; n < QT; ++n) t[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[i], q[n][i], t[1], 0, 0, 0);
+  }
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[kt][i] *= ks[kt][i >> 2][i & 3];
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Scores to probabilities and their product with the step's values.  see: a bit for each key that the
+// row sees (shifted down by the lane's 4h), used where not `all` of the rows see all keys.
+template <int D, int PT, int NW>
+__device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f32x16a (&t)[tile_keys<D>() / 32], float unit,
+                                            bool all, bool finite, uint64_t see, RowState<D>& st) {
+  constexpr int K = tile_keys<D>(), KT = K / 32, N = D / 16;  // N fragments of values for 32 keys
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, buf = step % 3;
+  const int e_new = __builtin_amdgcn_readfirstlane(S.e[buf]);
+  if (!all) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (!((uint32_t)(see >> (32 * kt)) >> (8 * (i >> 2) + (i & 3)) & 1)) t[kt][i] = -__builtin_inff();
+  }
   float top = -__builtin_inff();
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const f32x4a s4 = *reinterpret_cast<const f32x4a*>(&S.ks[buf][kt * 32 + a * 8 + h * 4]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = t[kt][4 * a + r] * s4[r];
-        if (!OPEN && !((uint32_t)(see >> (32 * kt)) >> (8 * a + r) & 1)) x = -__builtin_inff();
-        t[kt][4 * a + r] = x;
-        top = fmaxf(top, x);
-      }
-    }
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, t[kt][i]);
   top *= unit;
   // the running maximum follows the largest score by steps of at least 2^4, as in step32
   if (__ballot(top > st.m + 4.0f) || e_new != st.e) {
@@ -817,32 +851,41 @@ __device__ __forceinline__ void tile_step(const TileLds<D, NW>& S, int buf, cons
   const float m = st.m == -__builtin_inff() ? 0.0f : st.m;
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
+    __builtin_amdgcn_sched_barrier(0);
+    f16x8a vf[N];
+    f32x4a vs[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) vs[x] = *reinterpret_cast<const f32x4a*>(&S.vs[buf][kt * 32 + x * 8 + h * 4]);
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const int s = x / (N / 2), row = x % (N / 2) * 32 + l32, run = (kt * 2 + s) * 2 + h;
+      vf[x] = __builtin_bit_cast(f16x8a, S.v[buf][row * (K / 8) + (run ^ value_swizzle<D>(row))]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     f16x8a p[PT][2];
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const f32x4a s4 = *reinterpret_cast<const f32x4a*>(&S.vs[buf][kt * 32 + a * 8 + h * 4]);
+    for (int i = 0; i < 16; ++i) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t[kt][i], unit, -m));
+      float c = x * vs[i >> 2][i & 3];
+      st.l += x;
+      if constexpr (PT == 2) asm("" : "+v"(c));
+      p[0][i >> 3][i & 7] = (_Float16)c;
+      if constexpr (PT == 2) p[1][i >> 3][i & 7] = (_Float16)(c - (float)p[0][i >> 3][i & 7]);
+    }
+    if (!finite) {  // zero times such a scale: what a row does not see adds nothing to it all the same
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t[kt][4 * a + r], unit, -m));
-        float c = x * s4[r];
-        if (!OPEN && !((uint32_t)(see >> (32 * kt)) >> (8 * a + r) & 1)) x = c = 0.0f;
-        st.l += x;
-        if constexpr (PT == 2) asm("" : "+v"(c));
-        const int s = a >> 1, i = 4 * (a & 1) + r;
-        p[0][s][i] = (_Float16)c;
-        if constexpr (PT == 2) p[1][s][i] = (_Float16)(c - (float)p[0][s][i]);
-      }
+      for (int n = 0; n < PT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!((uint32_t)(see >> (32 * kt)) >> (8 * (i >> 2) + (i & 3)) & 1)) p[n][i >> 3][i & 7] = (_Float16)0.0f;
     }
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int x = 0; x < N; ++x)
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const int row = j * 32 + l32, run = (kt * 2 + s) * 2 + h;
-        const f16x8a vf = __builtin_bit_cast(f16x8a, S.v[buf][row * (K / 8) + (run ^ value_swizzle<D>(row))]);
-#pragma unroll
-        for (int n = 0; n < PT; ++n) st.o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[n][s], st.o[j], 0, 0, 0);
-      }
+      for (int n = 0; n < PT; ++n)
+        st.o[x % (N / 2)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x], p[n][x / (N / 2)], st.o[x % (N / 2)], 0, 0, 0);
   }
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // Which of a step's K keys from `key` on a row sees, a bit each
@@ -869,7 +912,7 @@ __device__ __forceinline__ uint64_t row_sees(const AttendArgs& A, const uint64_t
 }
 
 template <typename T, int D, int QT, int PT, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_attend_tile(AttendArgs A) {
+__global__ __launch_bounds__(64 * NW, D == 256 || (NW == 4 && sizeof(T) == 4) ? 1 : 2) void k_attend_tile(AttendArgs A) {
   constexpr int K = tile_keys<D>(), RUNS = K / 16, BATCH = 64 / RUNS;  // runs of a step, steps of a batch of pages
   __shared__ TileLds<D, NW> S;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -898,18 +941,18 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_attend_tile(Attend
     const bool busy = __ballot(row_ok) != 0;
     f16x8a q[QT][D / 16];
     float unit;
+    bool nan;
     query_halves<T, D, QT>(row_ok ? reinterpret_cast<const T*>(A.q) + (int64_t)(w.first + tok) * A.q_token +
                                         (int64_t)head * A.q_head
                                   : nullptr,
-                           h, q, unit);
+                           h, q, unit, nan);
     unit *= A.scale;
     const uint64_t* bits = A.mask && row_ok ? A.mask + (int64_t)(w.first + tok) * A.words : A.mask;
-    // the wave's first and last token: between them a causal step needs its mask
-    int lo_tok = row_ok ? tok : 0x7FFFFFFF, hi_tok = row_ok ? tok : -1;
+    // the wave's first token: it sees all keys up to it, and a causal step past it needs its mask
+    int lo_tok = row_ok ? tok : 0x7FFFFFFF;
 #pragma unroll
-    for (int i = 1; i < 32; i <<= 1) lo_tok = min(lo_tok, __shfl_xor(lo_tok, i)), hi_tok = max(hi_tok, __shfl_xor(hi_tok, i));
+    for (int i = 1; i < 32; i <<= 1) lo_tok = min(lo_tok, __shfl_xor(lo_tok, i));
     lo_tok = __builtin_amdgcn_readfirstlane(lo_tok);
-    hi_tok = __builtin_amdgcn_readfirstlane(hi_tok);
 
     RowState<D> st;
 #pragma unroll
@@ -921,34 +964,52 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_attend_tile(Attend
     st.e = -100;
     int e_run = -100;  // of wave 1, which finds the exponent for all
     Fetched<D, NW> f;
+    const int steps = stop > key0 ? (stop - key0 + K - 1) / K : 0;
+    auto fetch = [&](int n) {
+      if (n >= steps) return;
+      if (n % BATCH == 0 && n) pages.advance(A, p.b, (key0 >> 4) + (n + BATCH) * RUNS);
+      tile_fetch<D, NW>(A, p.h, key0 + n * K, end, pages.cur, (n % BATCH) * RUNS, f);
+    };
+    fetch(0);
     __syncthreads();  // the tile before is read
-    if (key0 < stop) {
-      tile_fetch<D, NW>(A, p.h, key0, end, pages.cur, 0, f);
-      tile_put<D, NW>(f, S, 0, e_run);
-    }
+    if (steps) tile_put<D, NW>(f, S, 0, e_run);
     __syncthreads();
-    int buf = 0, step = 1;
-    for (int key = key0; key < stop; key += K, buf ^= 1, ++step) {
-      const bool more = key + K < stop;
-      if (more) {
-        if (step % BATCH == 0) pages.advance(A, p.b, (key0 >> 4) + (step + BATCH) * RUNS);
-        tile_fetch<D, NW>(A, p.h, key + K, end, pages.cur, (step % BATCH) * RUNS, f);
-      }
-      const uint32_t ok = __builtin_amdgcn_readfirstlane(S.ok[buf]);
-      const int j0 = key - w.ctx;
-      if (busy && (A.mask || j0 <= hi_tok)) {  // else every row's token comes before these keys
-        if (key + K <= end && ok == (1u << RUNS) - 1 && (j0 + K <= 0 || (!A.mask && j0 + K - 1 <= lo_tok)))
-          tile_step<D, QT, PT, NW, true>(S, buf, q, unit, 0, st);
-        else
-          tile_step<D, QT, PT, NW, false>(S, buf, q, unit, row_sees<K>(A, bits, key, w.ctx, end, tok, ok) >> (4 * h), st);
-      }
-      if (more) tile_put<D, NW>(f, S, buf ^ 1, e_run);
+    fetch(1);
+    // Between two barriers the first half of the waves takes a step's scores and then its values, the second half the
+    // values of the step before and then the scores: on a SIMD one wave's MFMAs meet the other's exponentials.
+    // Values stay in LDS for one step more than keys.
+    auto pass_on = [&](int n) {
+      if (n + 1 < steps) tile_put<D, NW>(f, S, n + 1, e_run);
       __syncthreads();
+      fetch(n + 2);
+    };
+    auto loop = [&](auto late) {
+      for (int n = 0; n < steps; ++n) {
+        const int key = key0 + n * K, j0 = key - w.ctx;
+        f32x16a t[K / 32];
+        tile_scores<D, QT, NW>(S, n, q, t);
+        const uint32_t ok = __builtin_amdgcn_readfirstlane(S.ok[n % 3]);
+        if constexpr (decltype(late)::value) pass_on(n);
+        const bool all = key + K <= end && (ok & 0xFFFFu) == (1u << RUNS) - 1 &&
+                         (j0 + K <= 0 || (!A.mask && j0 + K - 1 <= lo_tok));
+        uint64_t see = ~0ull;
+        if (!all) see = row_sees<K>(A, bits, key, w.ctx, end, tok, ok) >> (4 * h);
+        tile_values<D, PT, NW>(S, n, t, unit, all, ok >> 31 == 0, see, st);
+        if constexpr (!decltype(late)::value) pass_on(n);
+      }
+    };
+    if (!busy) {
+      for (int n = 0; n < steps; ++n) pass_on(n);
+    } else if (wave >= NW / 2) {
+      loop(std::true_type{});
+    } else {
+      loop(std::false_type{});
     }
 
     // a lane has its row's elements 4c .. 4c+3 for every c with bit 2 of c equal to h
     float l = st.l;
     l += __shfl_xor(l, 32);
+    if (nan && l != 0.0f) l = __uint_as_float(0x7FC00000u);  // of a row that sees a key
     if (row_ok) {
       const float down = scale_of_exp(st.e - 1), inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t slot = ((int64_t)share * 2 + (p.k == 0 ? 1 : 0)) * (32 * NW) + wave * 32 + l32;
@@ -1047,11 +1108,11 @@ struct AttendPlan {
   bool fits;  // the line is below 2^31 blocks
 };
 
-static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int H, int G, int D) {
+static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int H, int G, int D, bool wide) {
   AttendPlan a;
   // rows of a sequence and key head, on average
   const double each = B > 0 ? (double)T * G / (double)std::min(B, T) : 0.0;
-  a.rows = each <= 32 ? 16 : each <= 128 || D == 256 ? 128 : 256;
+  a.rows = each <= 32 ? 16 : each <= 128 || D == 256 || wide ? 128 : 256;
   a.keys = a.rows == 16 ? 128 : 256;
   a.GC = std::min(G, a.rows);
   a.chunks = (int)ceil_div(G, a.GC);
@@ -1063,7 +1124,7 @@ static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int
   a.most = std::max(1, (a.cap + a.keys - 1) / a.keys);
   a.cut = a.most > 1 && B > 0;
   a.fits = tiles * a.most < 2147483648.0;
-  const double most = (a.rows == 256 || D == 256 ? 1.0 : 2.0) * num_cus();  // workgroups that run at once
+  const double most = (a.rows == 256 || D == 256 || (a.rows == 128 && wide) ? 1.0 : 2.0) * num_cus();  // workgroups that run at once
   a.shares = (int)std::max(1.0, std::min(most, tiles * a.most));
   return a;
 }
@@ -1081,7 +1142,7 @@ static int launch_attend(const AttendArgs& A, const AttendPlan& a, hipStream_t s
   } else if (a.rows == 128) {
     hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 4>), dim3(a.shares), dim3(256), 0, st, A);
   } else {
-    if constexpr (D < 256)
+    if constexpr (D < 256 && sizeof(T) == 2)
       hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 8>), dim3(a.shares), dim3(512), 0, st, A);
   }
   if (a.cut && a.shares > 1)
@@ -1102,11 +1163,11 @@ using namespace mxk;
 
 extern "C" {
 
-size_t mxk_kv_pages_attend_workspace(int64_t tokens, int64_t B, int64_t width, int page, int heads, int q_heads,
-                                     int D) {
+size_t mxk_kv_pages_attend_workspace(int q_type, int64_t tokens, int64_t B, int64_t width, int page, int heads,
+                                     int q_heads, int D) {
   if (tokens <= 0 || B <= 0 || width < 0 || heads < 1 || q_heads < heads || q_heads % heads || !kv_page_ok(page))
     return 0;
-  const AttendPlan a = plan_attend(tokens, B, width, page, heads, q_heads / heads, D);
+  const AttendPlan a = plan_attend(tokens, B, width, page, heads, q_heads / heads, D, q_type == MXK_IN_F32);
   return attend_bytes(a, D);
 }
 
@@ -1136,7 +1197,7 @@ int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_he
   if (!aligned16(codes) || !aligned16(scales))
     return fail(MXK_EINVAL, "kv_attend: codes and scales start on 16 bytes");
   const int G = q_heads / heads;
-  const AttendPlan a = plan_attend(tokens, B, width, page, heads, G, D);
+  const AttendPlan a = plan_attend(tokens, B, width, page, heads, G, D, q_type == MXK_IN_F32);
   if (!a.fits) return fail(MXK_EINVAL, "kv_attend: more than 2^31 blocks of keys that the table has room for");
   const size_t need = attend_bytes(a, D), part = (size_t)a.shares * 2 * a.rows;
   if (need && (!workspace || workspace_nbytes < need || !aligned16(workspace)))

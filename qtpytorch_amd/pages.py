@@ -347,7 +347,7 @@ class kv_pages:
         codes, scales, n, page, H, _ = self._pool()
         lib = L.lib()
         B, width = table.shape
-        nbytes = lib.mxk_kv_pages_attend_workspace(T, B, width, page, H, Hq, D)
+        nbytes = lib.mxk_kv_pages_attend_workspace(_FLOATS[q.dtype], T, B, width, page, H, Hq, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with L.on_device(dev):
             rc = lib.mxk_kv_pages_attend(q.data_ptr(), _FLOATS[q.dtype], q.stride(0), q.stride(1), Hq, codes, scales, n,
