@@ -677,31 +677,31 @@ template <int D, int NW>
 __device__ __forceinline__ void tile_fetch(const AttendArgs& A, int h, int key, int end, int pages, int first_run,
                                            Fetched<D, NW>& f) {
   using F = Fetched<D, NW>;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int in = (1 << A.pool.shift) - 1;
   const int64_t values = (int64_t)A.pool.H << A.pool.shift;
 #pragma unroll
   for (int i = 0; i < F::N; ++i) {
     // D pieces are 16 keys: a wave's lie in one run, with one page
-    const int first = (wave + i * NW) * 64, run = first / D, piece = (first + lane) % D;
+    const uint32_t first = (wave + i * NW) * 64, run = first / D, piece = (first + lane) % D;
     if (first >= F::PIECES) break;
-    const int page = lane_of(pages, first_run + run);
-    const int64_t row = kv_row(A.pool, max(page, 0), 0, h, (key + run * 16) & in);
+    const int page = lane_of(pages, first_run + (int)run);
+    const int64_t row = kv_row(A.pool, max(page, 0), 0, h, (key + (int)run * 16) & in);
     const int8_t* k = A.pool.codes + row * D;
     const int8_t* v = k + values * D;
     f.k[i] = *reinterpret_cast<const u32x4*>(k + (uint32_t)(piece * 16));
-    const int four = piece / (D / 4), c = piece % (D / 4);
+    const uint32_t four = piece / (D / 4), c = piece % (D / 4);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       f.v[i][r] = *reinterpret_cast<const uint32_t*>(v + (uint32_t)((four * 4 + r) * D + c * 4));
   }
   if (wave < 2) {
-    const int l = lane & (tile_keys<D>() - 1), at = key + l;
+    const int l = (int)lane & (tile_keys<D>() - 1), at = key + l;
     const int there = __shfl(pages, first_run + (l >> 4));  // with all lanes: they hold each other's pages
     const int page = at < end ? there : -1;
     f.page = page;
     f.scale = 0.0f;
-    if (page >= 0) f.scale = A.pool.scales[kv_row(A.pool, page, wave, h, at & in)];
+    if (page >= 0) f.scale = A.pool.scales[kv_row(A.pool, page, (int)wave, h, at & in)];
   }
 }
 
@@ -709,14 +709,14 @@ template <int D, int NW>
 __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>& S, int step, int& e_run) {
   using F = Fetched<D, NW>;
   constexpr int K = tile_keys<D>(), RUNS = K / 16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int buf = step % 3;
 #pragma unroll
   for (int i = 0; i < F::N; ++i) {
-    const int first = (wave + i * NW) * 64, piece = first + lane;
+    const uint32_t first = (wave + i * NW) * 64, piece = first + lane;
     if (first >= F::PIECES) break;
     {
-      const int row = piece / (D / 16), c = piece % (D / 16);
+      const uint32_t row = piece / (D / 16), c = piece % (D / 16);
       u32x4 half[2];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -728,8 +728,8 @@ __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>
       for (int x = 0; x < 2; ++x) S.k[step & 1][row * (D / 8) + ((2 * c + x) ^ key_swizzle<D>(row))] = half[x];
     }
     // keys 16s + 8b + 4h': run s*2 + h', its half b
-    const int four = piece / (D / 4), c = piece % (D / 4);
-    const int run = (four >> 2) * 2 + (four & 1), b = (four >> 1) & 1;
+    const uint32_t four = piece / (D / 4), c = piece % (D / 4);
+    const uint32_t run = (four >> 2) * 2 + (four & 1), b = (four >> 1) & 1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t sel = 0x0C000C00u | (uint32_t)j | (uint32_t)(4 + j) << 16;
@@ -737,7 +737,7 @@ __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>
 #pragma unroll
       for (int x = 0; x < 2; ++x)
         two[x] = codes_f16(__builtin_amdgcn_perm(f.v[i][2 * x + 1] ^ 0x80808080u, f.v[i][2 * x] ^ 0x80808080u, sel));
-      const int row = j * (D / 4) + c;
+      const uint32_t row = j * (D / 4) + c;
       reinterpret_cast<u32x2*>(&S.v[buf][row * (K / 8) + (run ^ value_swizzle<D>(row))])[b] = two;
     }
   }
