@@ -169,6 +169,20 @@ def on_device(dev: torch.device):
     return torch.cuda.device(dev)
 
 
+def stream_on(index: int) -> int:
+    """stream_of for the GPU of this index."""
+    if _RAW_STREAM is not None:
+        return _RAW_STREAM(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def on_gpu(index: int):
+    """on_device for the GPU of this index."""
+    if _GET_DEVICE is not None and index == _GET_DEVICE():
+        return _SAME_DEVICE
+    return torch.cuda.device(index)
+
+
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 

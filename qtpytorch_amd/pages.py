@@ -32,6 +32,17 @@ _HEADS = (64, 128, 256)
 _MANY = (1 << 31) - 65  # more tokens than a batch has
 
 
+def _together(first: Tensor, *rest: Optional[Tensor]) -> int:
+    """The GPU that all tensors are on."""
+    index = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            L.require_gpu(first, *rest)  # names the two
+    if index < 0:
+        L.require_gpu(first)
+    return index
+
+
 # ---------------------------------------------------------------- rotary positions
 class rotary_table:
     """Angles of rotary positions: pair i of a head turns by ``freqs[i]`` radians
@@ -85,10 +96,11 @@ def _positions(name: str, positions: Tensor, lead) -> Tuple[Tensor, int]:
     """Contiguous positions and their number of axes; lead: the shape of the tokens."""
     if positions.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name}: positions are int32 or int64, got {positions.dtype}")
-    if positions.shape == lead:
+    shape = positions.shape
+    if shape == lead:
         axes = 1
-    elif positions.dim() == len(lead) + 1 and positions.shape[:-1] == lead and positions.shape[-1] > 0:
-        axes = positions.shape[-1]
+    elif len(shape) == len(lead) + 1 and shape[:-1] == lead and shape[-1] > 0:
+        axes = shape[-1]
     else:
         raise ValueError(f"{name}: positions {tuple(lead)}, or with their axes last, expected, got "
                          f"{tuple(positions.shape)}")
@@ -104,14 +116,15 @@ def _token_rows(x: Tensor) -> Tensor:
 
 def _rotary(x: Tensor, positions: Tensor, axes: int, table: rotary_table, backward: bool) -> Tensor:
     freqs, axis = table.freqs, table.axis
-    dev = L.require_gpu(x, positions, freqs, axis)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    gpu = _together(x, positions, freqs, axis)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     rows = _token_rows(x)
     tokens, H, D = rows.shape
-    with L.on_device(dev):
-        rc = L.lib().mxk_rotary(rows.data_ptr(), _FLOATS[x.dtype], tokens, H, D, rows.stride(0), rows.stride(1),
-                                freqs.data_ptr(), L.ptr(axis), freqs.numel(), table.interleaved, positions.data_ptr(),
-                                positions.element_size(), axes, backward, y.data_ptr(), L.stream_of(y))
+    token, head, _ = rows.stride()
+    with L.on_gpu(gpu):
+        rc = L.lib().mxk_rotary(rows.data_ptr(), _FLOATS[x.dtype], tokens, H, D, token, head, freqs.data_ptr(),
+                                L.ptr(axis), freqs.numel(), table.interleaved, positions.data_ptr(),
+                                positions.element_size(), axes, backward, y.data_ptr(), L.stream_on(gpu))
     if rc:
         L.check(rc, f"rotary({tokens}x{H}x{D})")
     return y
@@ -122,7 +135,7 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, x, positions, axes, table):
         ctx.save_for_backward(positions)
         ctx.axes, ctx.table = axes, table
-        return _rotary(x.detach(), positions, axes, table, False)
+        return _rotary(x, positions, axes, table, False)
 
     @staticmethod
     @once_differentiable
@@ -194,7 +207,8 @@ def _check_batch(name: str, batch: kv_batch) -> None:
             and table.is_contiguous() and lengths.is_contiguous() and offsets.is_contiguous()):
         raise TypeError(f"{name}: a batch's tensors are contiguous int32, got {table.dtype}, {lengths.dtype} and "
                         f"{offsets.dtype}")
-    if table.dim() != 2 or lengths.shape != table.shape[:1] or offsets.shape != (table.shape[0] + 1,):
+    shape = table.shape
+    if len(shape) != 2 or lengths.shape != shape[:1] or offsets.shape != (shape[0] + 1,):
         raise ValueError(f"{name}: a batch has table [B, width], lengths [B] and offsets [B + 1], got "
                          f"{tuple(table.shape)}, {tuple(lengths.shape)} and {tuple(offsets.shape)}")
 
@@ -245,20 +259,14 @@ class kv_pages:
         n, _, H, page, D = self.codes.shape
         return self.codes.data_ptr(), self.scales.data_ptr(), n, page, H, D
 
-    def _rows(self, name: str, what: str, x: Tensor, heads: Optional[int] = None) -> Tensor:
-        D = self.codes.shape[4]
-        if x.dim() != 3 or x.shape[2] != D or heads is not None and x.shape[1] != heads:
-            raise ValueError(f"{name}: {what} [tokens, {'heads' if heads is None else heads}, {D}] expected, got "
-                             f"{tuple(x.shape)}")
-        x = x.detach()
+    def _rows(self, name: str, what: str, x: Tensor, H: int, D: int) -> Tensor:
+        """x [tokens, heads, D] with D contiguous; H: heads of keys and values, whose multiple queries have."""
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != D or (what != "q" and shape[1] != H):
+            raise ValueError(f"{name}: {what} [tokens, {'heads' if what == 'q' else H}, {D}] expected, got {tuple(shape)}")
+        if what == "q" and (shape[1] < H or shape[1] % H):
+            raise ValueError(f"{name}: query heads in groups of one size for each of {H} heads expected, got {shape[1]}")
         return x if x.stride(2) == 1 else x.contiguous()
-
-    def _queries(self, name: str, q: Tensor) -> Tensor:
-        H = self.codes.shape[2]
-        q = self._rows(name, "q", q)
-        if q.shape[1] < H or q.shape[1] % H:
-            raise ValueError(f"{name}: query heads in groups of one size for each of {H} heads expected, got {q.shape[1]}")
-        return q
 
     def append(self, k: Tensor, v: Tensor, batch: kv_batch, *, rotary: Optional[rotary_table] = None,
                positions: Optional[Tensor] = None, q: Optional[Tensor] = None) -> Optional[Tensor]:
@@ -270,41 +278,43 @@ class kv_pages:
         axis); they are packed from the unrounded rotation.  q [tokens, q_heads,
         head_dim] is rotated along and returned.  A head's row with a NaN or an
         infinity reads as NaN.  Nothing is differentiable."""
-        H = self.codes.shape[2]
-        if k.dtype not in _FLOATS or v.dtype != k.dtype or q is not None and q.dtype != k.dtype:
+        kind = _FLOATS.get(k.dtype)
+        if kind is None or v.dtype != k.dtype or q is not None and q.dtype != k.dtype:
             raise TypeError(f"kv_pages.append: keys, values and queries of one type (float32, float16 or bfloat16) "
                             f"expected, got {k.dtype}, {v.dtype}{'' if q is None else f' and {q.dtype}'}")
-        k, v = self._rows("kv_pages.append", "k", k, H), self._rows("kv_pages.append", "v", v, H)
+        codes, scales, n, page, H, D = self._pool()
+        k, v = self._rows("kv_pages.append", "k", k, H, D), self._rows("kv_pages.append", "v", v, H, D)
         T = k.shape[0]
         if q is not None:
-            q = self._queries("kv_pages.append", q)
+            q = self._rows("kv_pages.append", "q", q, H, D)
         if v.shape[0] != T or q is not None and q.shape[0] != T:
             raise ValueError(f"kv_pages.append: one row for each of {T} tokens expected, got {v.shape[0]} of v"
                              f"{'' if q is None else f' and {q.shape[0]} of q'}")
         _check_batch("kv_pages.append", batch)
+        table, lengths, offsets = batch
         freqs = axis = None
-        pairs = axes = 0
+        pairs = axes = bytes_ = interleaved = 0
         if rotary is not None:
-            freqs, axis, pairs = rotary.freqs, rotary.axis, rotary.freqs.numel()
-            if 2 * pairs > self.codes.shape[4]:
-                raise ValueError(f"kv_pages.append: the table rotates {2 * pairs} elements, a head has "
-                                 f"{self.codes.shape[4]}")
+            freqs, axis, interleaved = rotary.freqs, rotary.axis, rotary.interleaved
+            pairs = freqs.numel()
+            if 2 * pairs > D:
+                raise ValueError(f"kv_pages.append: the table rotates {2 * pairs} elements, a head has {D}")
             if positions is not None:
                 positions, axes = _positions("kv_pages.append", positions, (T,))
+                bytes_ = positions.element_size()
         elif positions is not None or q is not None:
             raise ValueError("kv_pages.append: positions and queries go with a rotary table")
-        dev = L.require_gpu(self.codes, k, v, q, positions, freqs, axis, *batch)
-        out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=dev)
-        codes, scales, n, page, _, D = self._pool()
-        table, lengths, offsets = batch
-        qt, qh, Hq = (0, 0, 0) if q is None else (q.stride(0), q.stride(1), q.shape[1])
-        with L.on_device(dev):
+        gpu = _together(self.codes, k, v, q, positions, freqs, axis, table, lengths, offsets)
+        out, qt, qh, Hq = None, 0, 0, 0
+        if q is not None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            (qt, qh, _), Hq = q.stride(), q.shape[1]
+        (kt, kh, _), (vt, vh, _), (B, width) = k.stride(), v.stride(), table.shape
+        with L.on_gpu(gpu):
             rc = L.lib().mxk_kv_pages_append(
-                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), L.ptr(q), qt, qh, Hq,
-                _FLOATS[k.dtype], codes, scales, n, page, H, D, table.data_ptr(), lengths.data_ptr(),
-                offsets.data_ptr(), table.shape[0], table.shape[1], T, L.ptr(freqs), L.ptr(axis), pairs,
-                rotary is not None and rotary.interleaved, L.ptr(positions),
-                0 if positions is None else positions.element_size(), axes, L.ptr(out), L.stream_of(k))
+                k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, L.ptr(q), qt, qh, Hq, kind, codes, scales, n, page, H, D,
+                table.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), B, width, T, L.ptr(freqs), L.ptr(axis), pairs,
+                interleaved, L.ptr(positions), bytes_, axes, L.ptr(out), L.stream_on(gpu))
         if rc:
             L.check(rc, f"kv_pages.append({T} tokens, {H} heads of {D})")
         return out
@@ -325,11 +335,13 @@ class kv_pages:
         Codes are used as they are, q to 16 bits of its row's largest element
         (24 where it is float32), probabilities to 11 bits (22), sums in float32.
         Nothing is differentiable."""
-        if q.dtype not in _FLOATS:
+        kind = _FLOATS.get(q.dtype)
+        if kind is None:
             raise TypeError(f"kv_pages.attend: float32, float16 or bfloat16 expected, got {q.dtype}")
-        q = self._queries("kv_pages.attend", q)
+        codes, scales, n, page, H, D = self._pool()
+        q = self._rows("kv_pages.attend", "q", q, H, D)
         _check_batch("kv_pages.attend", batch)
-        T, Hq, D = q.shape
+        T, Hq, _ = q.shape
         words = 0
         if mask is not None:
             if mask.dtype != torch.int64:
@@ -342,18 +354,16 @@ class kv_pages:
         if not (scale > 0.0 and math.isfinite(scale)):
             raise ValueError(f"kv_pages.attend: a positive scale expected, got {scale}")
         table, lengths, offsets = batch
-        dev = L.require_gpu(self.codes, q, mask, *batch)
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-        codes, scales, n, page, H, _ = self._pool()
+        gpu = _together(self.codes, q, mask, table, lengths, offsets)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lib = L.lib()
-        B, width = table.shape
-        nbytes = lib.mxk_kv_pages_attend_workspace(_FLOATS[q.dtype], T, B, width, page, H, Hq, D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with L.on_device(dev):
-            rc = lib.mxk_kv_pages_attend(q.data_ptr(), _FLOATS[q.dtype], q.stride(0), q.stride(1), Hq, codes, scales, n,
-                                         page, H, D, table.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), B, width,
-                                         T, L.ptr(mask), words, scale, out.data_ptr(), L.ptr(ws), nbytes,
-                                         L.stream_of(out))
+        (qt, qh, _), (B, width) = q.stride(), table.shape
+        nbytes = lib.mxk_kv_pages_attend_workspace(kind, T, B, width, page, H, Hq, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        with L.on_gpu(gpu):
+            rc = lib.mxk_kv_pages_attend(q.data_ptr(), kind, qt, qh, Hq, codes, scales, n, page, H, D, table.data_ptr(),
+                                         lengths.data_ptr(), offsets.data_ptr(), B, width, T, L.ptr(mask), words, scale,
+                                         out.data_ptr(), L.ptr(ws), nbytes, L.stream_on(gpu))
         if rc:
             L.check(rc, f"kv_pages.attend({T} tokens, {Hq} heads of {D})")
         return out
@@ -371,12 +381,12 @@ class kv_pages:
         if path.dim() != 2 or path.shape[0] != table.shape[0]:
             raise ValueError(f"kv_pages.keep: a path [{table.shape[0]}, steps] expected, got {tuple(path.shape)}")
         path = path.contiguous()
-        dev = L.require_gpu(self.codes, path, *batch)
+        gpu = _together(self.codes, path, table, lengths, offsets)
         codes, scales, n, page, H, D = self._pool()
-        with L.on_device(dev):
+        with L.on_gpu(gpu):
             rc = L.lib().mxk_kv_pages_keep(codes, scales, n, page, H, D, table.data_ptr(), lengths.data_ptr(),
                                            offsets.data_ptr(), table.shape[0], table.shape[1], _MANY, path.data_ptr(),
-                                           path.shape[1], L.stream_of(path))
+                                           path.shape[1], L.stream_on(gpu))
         if rc:
             L.check(rc, f"kv_pages.keep({tuple(path.shape)})")
 
@@ -388,15 +398,15 @@ class kv_pages:
         if tokens < 0:
             raise ValueError(f"kv_pages.read: a number of tokens expected, got {tokens}")
         kind = L.elem_type(dtype)
-        dev = L.require_gpu(self.codes, *batch)
-        codes, scales, n, page, H, D = self._pool()
         table, lengths, offsets = batch
-        k = torch.empty((tokens, H, D), dtype=dtype, device=dev)
-        v = torch.empty((tokens, H, D), dtype=dtype, device=dev)
-        with L.on_device(dev):
+        gpu = _together(self.codes, table, lengths, offsets)
+        codes, scales, n, page, H, D = self._pool()
+        k = torch.empty((tokens, H, D), dtype=dtype, device=self.codes.device)
+        v = torch.empty_like(k)
+        with L.on_gpu(gpu):
             rc = L.lib().mxk_kv_pages_read(codes, scales, n, page, H, D, table.data_ptr(), lengths.data_ptr(),
                                            offsets.data_ptr(), table.shape[0], table.shape[1], tokens, kind,
-                                           k.data_ptr(), v.data_ptr(), L.stream_of(k))
+                                           k.data_ptr(), v.data_ptr(), L.stream_on(gpu))
         if rc:
             L.check(rc, f"kv_pages.read({tokens} tokens)")
         return k, v
