@@ -117,40 +117,52 @@ __global__ __launch_bounds__(256) void k_rotary(const T* __restrict__ x, int64_t
 }
 
 // ---------------------------------------------------------------- append
-// Eight elements e..e+7 of a row, rotated.  Half a head apart, the partners
-// of a whole chunk are a chunk too where R/2 is a multiple of 8 (their second
-// read is served by the L1); other R take them one by one.
+// A lane's eight elements e..e+7 of the rotated rows of one token: y[i] = x[i] * c[i] + x[partner(i)] * s[i].
+// The partners are eight in a row too where pairs lie half a head apart and R/2 is a multiple of 8 (they are read
+// with a load of their own, which the L1 serves), or within the eight where pairs are neighbours; else
+// they are read one by one.
+struct Turn8 {
+  float c[8], s[8];
+  int first;  // of the partners in a row; -1: within the eight, -2: one by one, -3: nothing is rotated
+};
+
+__device__ __forceinline__ Turn8 turn8(const Rotation& r, int e, const float2* __restrict__ cs) {
+  Turn8 t;
+  const int R = 2 * r.pairs;
+  t.first = e >= R ? -3 : r.interleaved ? (e + 8 <= R ? -1 : -2) : r.pairs % 8 ? -2 : e < r.pairs ? e + r.pairs : e - r.pairs;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int k = e + i;
+    const bool low = r.interleaved ? (i & 1) == 0 : k < r.pairs;  // the pair's first element
+    const float2 a = k >= R ? make_float2(1.0f, 0.0f) : cs[r.interleaved ? k >> 1 : low ? k : k - r.pairs];
+    t.c[i] = a.x;
+    t.s[i] = low ? -a.y : a.y;
+  }
+  return t;
+}
+
+// turn: this lane's row is rotated
 template <typename T>
-__device__ __forceinline__ void row_rotated(const T* __restrict__ row, int e, const Rotation& r,
-                                            const float2* __restrict__ cs, float (&v)[8]) {
-  row_load<T, 8>(row + e, v);
-  const int R = 2 * r.pairs, half = r.pairs;
-  if (e >= R) return;
-  if (r.interleaved && e + 8 <= R) {
+__device__ __forceinline__ void row_values(const T* __restrict__ row, int e, const Rotation& r, bool turn, const Turn8& t,
+                                           float (&x)[8]) {
+  row_load<T, 8>(row + e, x);
+  if (!turn || t.first == -3) return;
+  float w[8];
+  if (t.first >= 0) {
+    row_load<T, 8>(row + t.first, w);
+  } else if (t.first == -1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 a = cs[e / 2 + i];
-      const float u = v[2 * i], w = v[2 * i + 1];
-      v[2 * i] = __builtin_fmaf(u, a.x, -(w * a.y));
-      v[2 * i + 1] = __builtin_fmaf(w, a.x, u * a.y);
-    }
-  } else if (!r.interleaved && half % 8 == 0) {
-    const bool first = e < half;
-    float w[8];
-    row_load<T, 8>(row + (first ? e + half : e - half), w);
-    const float2* a = cs + (first ? e : e - half);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(v[i], a[i].x, first ? -(w[i] * a[i].y) : w[i] * a[i].y);
+    for (int i = 0; i < 8; ++i) w[i] = x[i ^ 1];
   } else {
-    for (int i = 0; i < 8 && e + i < R; ++i) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
       const int k = e + i;
-      const bool first = r.interleaved ? (k & 1) == 0 : k < half;
-      const int other = r.interleaved ? k ^ 1 : first ? k + half : k - half;
-      const float2 a = cs[r.interleaved ? k >> 1 : first ? k : k - half];
-      const float w = ElemT<T>::cvt(row[other]);
-      v[i] = __builtin_fmaf(v[i], a.x, first ? -(w * a.y) : w * a.y);
+      const int other = r.interleaved ? k ^ 1 : k < r.pairs ? k + r.pairs : k - r.pairs;
+      w[i] = k < 2 * r.pairs ? ElemT<T>::cvt(row[other]) : 0.0f;
     }
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf(x[i], t.c[i], w[i] * t.s[i]);
 }
 
 // Keys, values and queries of new tokens: keys and queries rotated, keys and
@@ -159,54 +171,45 @@ __device__ __forceinline__ void row_rotated(const T* __restrict__ row, int e, co
 // with a NaN or an infinity has a scale of NaN and codes of zero.  A rotated
 // key goes to its codes unrounded.
 //
-// Four tokens a workgroup of four waves (each wave finds one token's place
-// and angles), or one where that leaves CUs idle, its rows then in parts over
-// blockIdx.y.  D / 8 lanes a row.
-template <typename T, int D, int TB>
+// A wave a token: it finds the token's place and angles (which pass through LDS of its own: no barrier) and takes
+// its rows, or blockIdx.y's part of them.  D / 8 lanes a row, so that a lane has the same elements of all of the
+// rows and keeps their angles in registers.  10400 tokens of 32 + 8 + 8 heads of 128 in bfloat16: 62 us, 4.1 TB/s, at 74
+// registers; bound by the latency of a step's reads at the waves that fit (two or three steps' rows requested at
+// once: 66 to 68 us at 90 to 104 registers; four tokens shared by a workgroup's waves: 69).
+template <typename T, int D>
 __global__ __launch_bounds__(256) void k_kv_append_pages(
     const T* __restrict__ k, int64_t k_token, int64_t k_head, const T* __restrict__ v, int64_t v_token, int64_t v_head,
     const T* __restrict__ q, int64_t q_token, int64_t q_head, int Hq, Rotation r, KvBatch s, KvPool p,
     T* __restrict__ q_out) {
   constexpr int LPR = D / 8, RPW = 64 / LPR;  // lanes a row, rows a wave and step
-  extern __shared__ float2 cs[];              // [TB][pairs]
-  __shared__ int place[TB][2];                // page and position in it, page -1: nowhere; -2: token of no sequence
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t0 = blockIdx.x * TB;
-  if (wave < TB && t0 + wave < s.T) {
-    const int t = t0 + wave, b = kv_sequence(s, t);
-    const int64_t at = b < 0 ? 0 : (int64_t)s.lengths[b] + (t - s.offsets[b]);
-    if (lane == 0) {
-      place[wave][0] = b < 0 ? -2 : at < 0 ? -1 : kv_page(s, p, b, at >> p.shift);
-      place[wave][1] = (int)(at & ((1 << p.shift) - 1));
-    }
-    for (int i = lane; i < r.pairs; i += 64) cs[wave * r.pairs + i] = rot_turn(r, at, t, i);
-  }
-  __syncthreads();
-  const int rows = 2 * p.H + Hq, tn = min(TB, s.T - t0);
-  const int li = lane % LPR, e = li * 8;
+  __shared__ float2 angles[4][D / 2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x * 4 + wave;
+  if (t >= s.T) return;
+  const int b = kv_sequence(s, t);
+  const int64_t place = b < 0 ? 0 : (int64_t)s.lengths[b] + (t - s.offsets[b]);
+  for (int i = lane; i < r.pairs; i += 64) angles[wave][i] = rot_turn(r, place, t, i);
+  const int page = b < 0 || place < 0 ? -1 : kv_page(s, p, b, place >> p.shift);
+  const int rows = 2 * p.H + Hq, li = lane % LPR, e = li * 8, sub = lane / LPR;
+  const Turn8 turn = turn8(r, e, angles[wave]);
+  const T *kt = k + (int64_t)t * k_token, *vt = v + (int64_t)t * v_token, *qt = q + (int64_t)t * q_token;
+  T* qo = q_out + (int64_t)t * Hq * D;
+  const int64_t values = (int64_t)p.H << p.shift;
+  const int64_t key0 = kv_row(p, max(page, 0), 0, 0, (int)(place & ((1 << p.shift) - 1)));
   // every lane of a wave takes part in the reductions: a row past the end is the last one again, not stored
-  for (int base = (blockIdx.y * 4 + wave) * RPW; base < tn * rows; base += gridDim.y * 4 * RPW) {
-    const int at = base + lane / LPR, it = min(at, tn * rows - 1);
-    const int tl = it / rows, row = it - tl * rows, t = t0 + tl;
-    const int page = place[tl][0], pos = place[tl][1];
-    const float2* a = cs + tl * r.pairs;
+  for (int first = blockIdx.y * RPW; first < rows; first += gridDim.y * RPW) {
+    const int row = min(first + sub, rows - 1);
+    const bool is_q = row >= 2 * p.H, is_v = !is_q && row >= p.H, live = first + sub < rows;
     float x[8];
-    if (row >= 2 * p.H) {
-      const int h = row - 2 * p.H;
-      row_rotated<T>(q + (int64_t)t * q_token + (int64_t)h * q_head, e, r, a, x);
-      if (page == -2) {
+    row_values<T>(is_q ? qt + (row - 2 * p.H) * q_head : is_v ? vt + (row - p.H) * v_head : kt + row * k_head, e, r, !is_v,
+                  turn, x);
+    if (is_q && live) {
+      float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-      }
-      if (at == it) row_store<T, 8>(q_out + ((int64_t)t * Hq + h) * D + e, x);
+      for (int i = 0; i < 8; ++i) y[i] = b < 0 ? 0.0f : x[i];
+      row_store<T, 8>(qo + (row - 2 * p.H) * D + e, y);
     }
-    if (__ballot(row < 2 * p.H) == 0) continue;  // queries alone
-    if (row >= 2 * p.H) {
-    } else if (row < p.H) {
-      row_rotated<T>(k + (int64_t)t * k_token + (int64_t)row * k_head, e, r, a, x);
-    } else {
-      row_load<T, 8>(v + (int64_t)t * v_token + (int64_t)(row - p.H) * v_head + e, x);
-    }
+    if (first >= 2 * p.H) continue;  // queries alone
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, mag_bits(x[i]));
@@ -217,8 +220,8 @@ __global__ __launch_bounds__(256) void k_kv_append_pages(
     uint32_t w[2] = {0u, 0u};
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)encode_vec_q(x[i], 127.0f) & 255u) << (8 * (i & 3));
-    if (row < 2 * p.H && page >= 0 && at == it) {
-      const int64_t dst = kv_row(p, page, row >= p.H, row >= p.H ? row - p.H : row, pos);
+    if (!is_q && page >= 0 && live) {
+      const int64_t dst = key0 + (is_v ? values : 0) + ((int64_t)(is_v ? row - p.H : row) << p.shift);
       *reinterpret_cast<u32x2*>(p.codes + dst * D + e) = whole ? u32x2{w[0], w[1]} : u32x2{0u, 0u};
       if (li == 0) p.scales[dst] = whole ? scale : __uint_as_float(0x7FC00000u);
     }
@@ -237,21 +240,32 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch s, KvPool p, T* __restr
   const int64_t at = b < 0 ? -1 : (int64_t)s.lengths[b] + (t - s.offsets[b]);
   const int page = at < 0 ? -1 : kv_page(s, p, b, at >> p.shift);
   const int pos = (int)(at & ((1 << p.shift) - 1));
-  const int step = gridDim.y * 64;
-  for (int it = blockIdx.y * 64 + lane; it < 2 * p.H * LPR; it += step) {
-    const int row = it / LPR, e = (it - row * LPR) * 8;
-    const int which = row >= p.H, h = which ? row - p.H : row;
-    float x[8];
-    u32x2 c = {0u, 0u};
-    float scale = 0.0f;
-    if (page >= 0) {
-      const int64_t src = kv_row(p, page, which, h, pos);
-      c = *reinterpret_cast<const u32x2*>(p.codes + src * D + e);
-      scale = p.scales[src];
+  const int step = gridDim.y * 64, items = 2 * p.H * LPR;
+  for (int first = blockIdx.y * 64 + lane; first < items; first += 4 * step) {
+    u32x2 c[4];
+    float scale[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {  // four requests in flight
+      const int row = min(first + u * step, items - 1) / LPR, e = (first + u * step) % LPR * 8;
+      const int which = row >= p.H, h = which ? row - p.H : row;
+      c[u] = u32x2{0u, 0u};
+      scale[u] = 0.0f;
+      if (page >= 0) {
+        const int64_t src = kv_row(p, page, which, h, pos);
+        c[u] = *reinterpret_cast<const u32x2*>(p.codes + src * D + e);
+        scale[u] = p.scales[src];
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)((int)(c[i >> 2] << (24 - 8 * (i & 3))) >> 24) * scale;
-    row_store<T, 8>((which ? v : k) + ((int64_t)t * p.H + h) * D + e, x);
+    for (int u = 0; u < 4; ++u) {
+      const int it = first + u * step, row = it / LPR, e = it % LPR * 8;
+      if (it >= items) break;
+      const int which = row >= p.H, h = which ? row - p.H : row;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)((int)(c[u][i >> 2] << (24 - 8 * (i & 3))) >> 24) * scale[u];
+      row_store<T, 8>((which ? v : k) + ((int64_t)t * p.H + h) * D + e, x);
+    }
   }
 }
 
@@ -376,20 +390,14 @@ template <typename T, int D>
 static int launch_append(const void* k, int64_t kt, int64_t kh, const void* v, int64_t vt, int64_t vh, const void* q,
                          int64_t qt, int64_t qh, int Hq, const Rotation& r, const KvBatch& s, const KvPool& p,
                          void* q_out, hipStream_t st) {
-  const int rows = 2 * p.H + Hq, rpb = 4 * (64 / (D / 8));
-  const bool four = s.T >= 8 * num_cus();  // four tokens a workgroup, two workgroups a CU
-  const int64_t blocks = ceil_div(s.T, four ? 4 : 1);
-  const int64_t parts = four ? 1 : std::min<int64_t>(ceil_div(rows, rpb),
-                                                     std::max<int64_t>(1, 4 * num_cus() / blocks));
-  const size_t lds = (size_t)(four ? 4 : 1) * r.pairs * sizeof(float2);
+  const int steps = (int)ceil_div(2 * p.H + Hq, 64 / (D / 8));
+  const int64_t blocks = ceil_div(s.T, 4);
+  // few tokens: a wave takes a part of a token's rows, down to one step of them
+  const int64_t parts = std::min<int64_t>(steps, std::max<int64_t>(1, 4 * num_cus() / blocks));
   const dim3 grid((unsigned)blocks, (unsigned)parts);
-#define MXK_A(TB_)                                                                                                  \
-  hipLaunchKernelGGL((k_kv_append_pages<T, D, TB_>), grid, dim3(256), lds, st, reinterpret_cast<const T*>(k), kt, kh, \
-                     reinterpret_cast<const T*>(v), vt, vh, reinterpret_cast<const T*>(q), qt, qh, Hq, r, s, p,     \
-                     reinterpret_cast<T*>(q_out))
-  if (four) MXK_A(4);
-  else MXK_A(1);
-#undef MXK_A
+  hipLaunchKernelGGL((k_kv_append_pages<T, D>), grid, dim3(256), 0, st, reinterpret_cast<const T*>(k), kt, kh,
+                     reinterpret_cast<const T*>(v), vt, vh, reinterpret_cast<const T*>(q), qt, qh, Hq, r, s, p,
+                     reinterpret_cast<T*>(q_out));
   return check_launch("kv_append");
 }
 
