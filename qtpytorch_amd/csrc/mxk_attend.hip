@@ -1047,12 +1047,13 @@ __global__ __launch_bounds__(64 * NW, D == 256 || (NW == 4 && sizeof(T) == 4) ? 
 
 // A tile that share s begins and does not end: its parts are share s's second
 // one and the first ones of the shares after it, up to the one with its last
-// block.  A wave a row, 64 parts at a time: a lane finds a part's weight, then
-// all lanes add the parts' sums in their order.
-template <typename T, int D>
+// block.  LANES lanes a row: all 64 where a tile has few rows and maybe many parts, 16 where it has many rows and few
+// parts (255 tiles of 256 rows in two or three parts: 35 us with 64).  A lane finds the weight of
+// every LANES-th part, then all lanes of the row add the parts' sums in their order.
+template <typename T, int D, int LANES>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs A) {
-  constexpr int E = D / 64;
-  const int s = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int E = D / LANES, RPB = 256 / LANES, U = LANES == 64 ? 8 : 2;  // parts in flight
+  const int s = blockIdx.x, lane = threadIdx.x & (LANES - 1), base = threadIdx.x & 63 & ~(LANES - 1);
   const PartTile t = A.part_t[s];
   if (t.last < 0) return;
   SeqWork w;
@@ -1062,42 +1063,49 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs A) {
   p.h = t.h;
   p.x = t.x;
   const int parts = t.last - s + 1;
-  for (int r = blockIdx.y * 4 + wave; r < A.rows; r += gridDim.y * 4) {
+  for (int r0 = blockIdx.y * RPB; r0 < A.rows; r0 += gridDim.y * RPB) {
+    const int r = r0 + threadIdx.x / LANES;  // RPB divides the rows
     int tok, head;
-    if (!tile_row(A, w, p, r, tok, head)) continue;
-    auto slot = [&](int i) { return ((int64_t)(s + i) * 2 + (i == 0)) * A.rows + r; };
+    const bool live = tile_row(A, w, p, r, tok, head);
+    if (__ballot(live) == 0) continue;
+    // rows that do not exist take part in the exchanges with what another row has: a part of theirs may not be written
+    auto slot = [&](int i) { return ((int64_t)(s + i) * 2 + (i == 0)) * A.rows + (live ? r : 0); };
     float m = -__builtin_inff();
-    for (int i = lane; i < parts; i += 64) m = fmaxf(m, A.part_s[slot(i)].x);
+    for (int i = lane; i < parts; i += LANES) m = fmaxf(m, A.part_s[slot(i)].x);
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
+    for (int i = 1; i < LANES; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
     float sum = 0.0f, acc[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) acc[j] = 0.0f;
-    for (int i0 = 0; i0 < parts; i0 += 64) {
-      const int n = min(64, parts - i0);
+    for (int i0 = 0; i0 < parts; i0 += LANES) {
+      const int n = min(LANES, parts - i0);
       const float2 ms = A.part_s[slot(i0 + min(lane, n - 1))];
       const float f = lane >= n ? 0.0f : ms.x == m ? 1.0f : __builtin_amdgcn_exp2f(ms.x - m);
       if (lane < n) sum += f * ms.y;
-      for (int i = 0; i < n; i += 8) {
-        float v[8][E];
+      for (int i = 0; i < n; i += U) {
+        float v[U][E];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)  // past the last part: it again, with a weight of zero
+        for (int u = 0; u < U; ++u)  // past the last part: it again, not added
           __builtin_memcpy(v[u], A.part_o + slot(i0 + min(i + u, n - 1)) * D + lane * E, sizeof(v[u]));
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float g = __uint_as_float(lane_of(__float_as_uint(f), min(i + u, 63)));
+        for (int u = 0; u < U; ++u) {
+          const float g = __shfl(f, base + min(i + u, LANES - 1));
+          if (i + u < n) {
 #pragma unroll
-          for (int j = 0; j < E; ++j) acc[j] = __builtin_fmaf(i + u < n ? g : 0.0f, v[u][j], acc[j]);
+            for (int j = 0; j < E; ++j) acc[j] = __builtin_fmaf(g, v[u][j], acc[j]);
+          }
         }
       }
     }
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T e[E];
+    for (int i = 1; i < LANES; i <<= 1) sum += __shfl_xor(sum, i);
+    if (live) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      T e[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) e[j] = out_cvt<T>(acc[j] * inv);
-    __builtin_memcpy(reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D + lane * E, e, sizeof(e));
+      for (int j = 0; j < E; ++j) e[j] = out_cvt<T>(acc[j] * inv);
+      __builtin_memcpy(reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D + lane * E, e, sizeof(e));
+    }
   }
 }
 
@@ -1136,17 +1144,19 @@ static size_t attend_bytes(const AttendPlan& a, int D) {
 
 template <typename T, int D, int QT, int PT>
 static int launch_attend(const AttendArgs& A, const AttendPlan& a, hipStream_t st) {
-  constexpr int QH = sizeof(T) == 4 ? 2 : 1;  // float16 terms of a query
+  constexpr int QH = sizeof(T) == 4 ? 2 : 1;  // float16 terms of a query and of the probabilities in the tile kernel
   if (a.rows == 16) {
     hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A);
   } else if (a.rows == 128) {
-    hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 4>), dim3(a.shares), dim3(256), 0, st, A);
+    hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 4>), dim3(a.shares), dim3(256), 0, st, A);
   } else {
     if constexpr (D < 256 && sizeof(T) == 2)
-      hipLaunchKernelGGL((k_attend_tile<T, D, QH, PT, 8>), dim3(a.shares), dim3(512), 0, st, A);
+      hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 8>), dim3(a.shares), dim3(512), 0, st, A);
   }
-  if (a.cut && a.shares > 1)
-    hipLaunchKernelGGL((k_attend_join<T, D>), dim3(a.shares - 1, a.rows == 16 ? 4 : 16), dim3(256), 0, st, A);
+  if (a.cut && a.shares > 1) {
+    if (a.rows == 16) hipLaunchKernelGGL((k_attend_join<T, D, 64>), dim3(a.shares - 1, 4), dim3(256), 0, st, A);
+    else hipLaunchKernelGGL((k_attend_join<T, D, 16>), dim3(a.shares - 1, a.rows / 16), dim3(256), 0, st, A);
+  }
   return check_launch("kv_attend");
 }
 
@@ -1227,7 +1237,7 @@ int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_he
   A.part_s = need ? reinterpret_cast<float2*>(A.part_o + part * D) : nullptr;
   A.part_t = need ? reinterpret_cast<PartTile*>(A.part_s + part) : nullptr;
   if (q_type == MXK_IN_F32) return launch_attend_d<float, 3, 2>(D, A, a, st);
-  if (q_type == MXK_IN_F16) return launch_attend_d<__half, 2, 1>(D, A, a, st);
+  if (q_type == MXK_IN_F16) return launch_attend_d<__half, 2, 2>(D, A, a, st);
   return launch_attend_d<hip_bfloat16, 2, 1>(D, A, a, st);
 }
 
