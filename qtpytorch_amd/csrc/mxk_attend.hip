@@ -912,7 +912,7 @@ __device__ __forceinline__ uint64_t row_sees(const AttendArgs& A, const uint64_t
 }
 
 template <typename T, int D, int QT, int PT, int NW>
-__global__ __launch_bounds__(64 * NW, D == 256 || (NW == 4 && sizeof(T) == 4) ? 1 : 2) void k_attend_tile(AttendArgs A) {
+__global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
   constexpr int K = tile_keys<D>(), RUNS = K / 16, BATCH = 64 / RUNS;  // runs of a step, steps of a batch of pages
   __shared__ TileLds<D, NW> S;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1120,7 +1120,11 @@ static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int
   AttendPlan a;
   // rows of a sequence and key head, on average
   const double each = B > 0 ? (double)T * G / (double)std::min(B, T) : 0.0;
-  a.rows = each <= 32 ? 16 : each <= 128 || D == 256 || wide ? 128 : 256;
+  // Up to 64 rows (128 of 256 elements) tiles of 16, whose waves need no barrier: several of them read the same keys, but
+  // from the L2.  16 sequences of 4000 keys, 8 heads of 128, bfloat16, us by tiles of 16 / 256: 32 rows 41 / 62, 64 rows
+  // 58 / 72, 128 rows 93 / 62; 2 sequences of 60000: 64 rows 104 / 121, 128 rows 188 / 132; float32 by 16 / 128: 64 rows
+  // 58 / 86, 128 rows 93 / 80; heads of 256: 128 rows 82 / 87, 256 rows 125 / 110.
+  a.rows = each <= (D == 256 ? 128 : 64) ? 16 : D == 256 || wide ? 128 : 256;
   a.keys = a.rows == 16 ? 128 : 256;
   a.GC = std::min(G, a.rows);
   a.chunks = (int)ceil_div(G, a.GC);
@@ -1132,7 +1136,7 @@ static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int
   a.most = std::max(1, (a.cap + a.keys - 1) / a.keys);
   a.cut = a.most > 1 && B > 0;
   a.fits = tiles * a.most < 2147483648.0;
-  const double most = (a.rows == 256 || D == 256 || (a.rows == 128 && wide) ? 1.0 : 2.0) * num_cus();  // workgroups that run at once
+  const double most = (a.rows > 16 || D == 256 ? 1.0 : 2.0) * num_cus();  // workgroups that run at once
   a.shares = (int)std::max(1.0, std::min(most, tiles * a.most));
   return a;
 }
@@ -1145,14 +1149,9 @@ static size_t attend_bytes(const AttendPlan& a, int D) {
 template <typename T, int D, int QT, int PT>
 static int launch_attend(const AttendArgs& A, const AttendPlan& a, hipStream_t st) {
   constexpr int QH = sizeof(T) == 4 ? 2 : 1;  // float16 terms of a query and of the probabilities in the tile kernel
-  if (a.rows == 16) {
-    hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A);
-  } else if (a.rows == 128) {
-    hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 4>), dim3(a.shares), dim3(256), 0, st, A);
-  } else {
-    if constexpr (D < 256 && sizeof(T) == 2)
-      hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 8>), dim3(a.shares), dim3(512), 0, st, A);
-  }
+  constexpr int NW = D == 256 || QH == 2 ? 4 : 8;
+  if (a.rows == 16) hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A);
+  else hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, NW>), dim3(a.shares), dim3(64 * NW), 0, st, A);
   if (a.cut && a.shares > 1) {
     if (a.rows == 16) hipLaunchKernelGGL((k_attend_join<T, D, 64>), dim3(a.shares - 1, 4), dim3(256), 0, st, A);
     else hipLaunchKernelGGL((k_attend_join<T, D, 16>), dim3(a.shares - 1, a.rows / 16), dim3(256), 0, st, A);
