@@ -596,37 +596,44 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
 // meets itself in a bank.
 #define MXK_TILE 64
 
-template <typename T, int D, int QT>
-__device__ __forceinline__ void query_halves(const T* __restrict__ row, int h, f16x8a (&q)[QT][D / 16], float& unit,
-                                             bool& nan) {
-  float x[D / 16][8];
+// A lane's elements i*16 + h*8 + 0..7 of a query row (null: zeros), and the exponent of the row's largest; rows below
+// 2^-100 count as zeros, and so do, at first, those with a NaN or an infinity.
+template <typename T, int D>
+struct QueryHalf {
+  T x[D / 16][8];
+  int e;
+  bool some, nan;
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void query_load(const T* __restrict__ row, int h, QueryHalf<T, D>& q) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    T e[8];
-    if (row) __builtin_memcpy(e, row + i * 16 + h * 8, sizeof(e));
+    __builtin_memset(q.x[i], 0, sizeof(q.x[i]));
+    if (row) __builtin_memcpy(q.x[i], row + i * 16 + h * 8, sizeof(q.x[i]));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[i][j] = row ? ElemT<T>::cvt(e[j]) : 0.0f;
-      m = max(m, mag_bits(x[i][j]));
-    }
+    for (int j = 0; j < 8; ++j) m = max(m, mag_bits(ElemT<T>::cvt(q.x[i][j])));
   }
   m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-  // a power of two takes the largest to 2^14 .. 2^15; rows below 2^-100 count as zeros, and so do, at first, those
-  // with a NaN or an infinity
-  const bool some = m >= 0x0D800000u && m < 0x7F800000u;
-  const int e = some ? (int)(m >> 23) - 127 : 0;
-  const float up = some ? scale_of_exp(14 - e) : 0.0f;
-  unit = scale_of_exp(e - 14 + 9);
-  nan = m >= 0x7F800000u;
+  q.some = m >= 0x0D800000u && m < 0x7F800000u;
+  q.nan = m >= 0x7F800000u;
+  q.e = q.some ? (int)(m >> 23) - 127 : -100;
+}
+
+// The row times 2^(14 - e), e the exponent of the largest element of the workgroup's rows: float16 has 11 bits of it (22
+// in two terms) down to 2^-28 of that element.
+template <typename T, int D, int QT>
+__device__ __forceinline__ void query_terms16(const QueryHalf<T, D>& q, int e, f16x8a (&term)[QT][D / 16]) {
+  const float up = q.some ? scale_of_exp(14 - e) : 0.0f;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float v = some ? x[i][j] * up : 0.0f;
+      float v = q.some ? ElemT<T>::cvt(q.x[i][j]) * up : 0.0f;
       if constexpr (QT == 2) asm("" : "+v"(v));  // one rounding for both terms, as for the probabilities
-      q[0][i][j] = (_Float16)v;
-      if constexpr (QT == 2) q[1][i][j] = (_Float16)(v - (float)q[0][i][j]);
+      term[0][i][j] = (_Float16)v;
+      if constexpr (QT == 2) term[1][i][j] = (_Float16)(v - (float)term[0][i][j]);
     }
 }
 
@@ -652,8 +659,10 @@ struct TileLds {
   static constexpr int K = tile_keys<D>();
   u32x4 k[2][K * D / 8];  // [key][D] float16, pieces of 8 swizzled
   u32x4 v[3][K * D / 8];  // [row][K keys] float16, pieces of 8 swizzled
-  float ks[3][K], vs[3][K];  // vs times 2^(10 - e)
+  float ks[3][K];    // times the queries' unit
+  float vs[3][K];    // times 2^(10 - e); coarse: float16, times 2^-e, in the order of a lane's weights
   int e[3];
+  int top[NW];     // exponents of the waves' largest query elements
   uint32_t ok[3];  // bits of the step's runs of 16 keys that have a page; bit 31: a value's scale is not finite
 };
 
@@ -705,8 +714,8 @@ __device__ __forceinline__ void tile_fetch(const AttendArgs& A, int h, int key, 
   }
 }
 
-template <int D, int NW>
-__device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>& S, int step, int& e_run) {
+template <int D, int NW, bool COARSE>
+__device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>& S, int step, float unit, int& e_run) {
   using F = Fetched<D, NW>;
   constexpr int K = tile_keys<D>(), RUNS = K / 16;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -741,14 +750,22 @@ __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>
       reinterpret_cast<u32x2*>(&S.v[buf][row * (K / 8) + (run ^ value_swizzle<D>(row))])[b] = two;
     }
   }
-  if (wave == 0 && lane < K) S.ks[buf][lane] = f.scale;
+  if (wave == 0 && lane < K) S.ks[buf][lane] = f.scale * unit;
   if (wave == 1) {
     const uint32_t bb = mag_bits(f.scale);
     int top = (int)((bb < 0x7F800000u ? bb : 0u) >> 23) - 127;
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) top = max(top, __shfl_xor(top, i));
     e_run = max(e_run, top);
-    if (lane < K) S.vs[buf][lane] = f.scale * scale_of_exp(10 - e_run);
+    if (lane < K) {
+      if constexpr (COARSE) {
+        // key 32 kt + 8 a + 4 h + r is weight 4 a + r of half h
+        const int to = (lane & 32) + (lane >> 2 & 1) * 16 + (lane >> 3 & 3) * 4 + (lane & 3);
+        reinterpret_cast<_Float16*>(S.vs[buf])[to] = (_Float16)(f.scale * scale_of_exp(-e_run));
+      } else {
+        S.vs[buf][lane] = f.scale * scale_of_exp(10 - e_run);
+      }
+    }
     const uint64_t there = __ballot(f.page >= 0);
     uint32_t ok = 0;
 #pragma unroll
@@ -775,13 +792,12 @@ template <int D, int QT, int NW>
 __device__ __forceinline__ void tile_scores(const TileLds<D, NW>& S, int step, const f16x8a (&q)[QT][D / 16],
                                             f32x16a (&t)[tile_keys<D>() / 32]) {
   constexpr int KT = tile_keys<D>() / 32, N = D / 16;
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, buf = step % 3;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   auto key = [&](int kt, int i) {
     const int row = kt * 32 + l32;
     return __builtin_bit_cast(f16x8a, S.k[step & 1][row * (D / 8) + ((2 * i + h) ^ key_swizzle<D>(row))]);
   };
   f16x8a a[N], b[N];
-  f32x4a ks[KT][4];
 #pragma unroll
   for (int i = 0; i < N; ++i) a[i] = key(0, i);
   __builtin_amdgcn_sched_barrier(0);
@@ -794,10 +810,6 @@ __device__ __forceinline__ void tile_scores(const TileLds<D, NW>& S, int step, c
     for (int n = 0; n < QT; ++n) t[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i], q[n][i], t[0], 0, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
   }
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) ks[kt][x] = *reinterpret_cast<const f32x4a*>(&S.ks[buf][kt * 32 + x * 8 + h * 4]);
   if constexpr (KT == 2) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) t[1][i] = 0.0f;
@@ -806,21 +818,33 @@ __device__ __forceinline__ void tile_scores(const TileLds<D, NW>& S, int step, c
 #pragma unroll
       for (int n = 0; n < QT; ++n) t[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[i], q[n][i], t[1], 0, 0, 0);
   }
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t[kt][i] *= ks[kt][i >> 2][i & 3];
   __builtin_amdgcn_sched_barrier(0);
 }
 
 // Scores to probabilities and their product with the step's values.  see: a bit for each key that the
 // row sees (shifted down by the lane's 4h), used where not `all` of the rows see all keys.
-template <int D, int PT, int NW>
-__device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f32x16a (&t)[tile_keys<D>() / 32], float unit,
-                                            bool all, bool finite, uint64_t see, RowState<D>& st) {
+//
+// VALU work bounds the kernel (it does not overlap with MFMAs here), so that its instructions per score
+// are counted: one fma takes the product with the key's scale and from the maximum; then the
+// maximum (half), exponential, conversion (half).  COARSE (bfloat16 results): the probability itself goes to
+// float16, the value's scale is applied to pairs, and the weight is a dot product of pairs with ones, 1.5 where the
+// exact form takes 2.5 with products and sums in float32.
+template <int D, int PT, int NW, bool COARSE>
+__device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f32x16a (&t)[tile_keys<D>() / 32], bool all,
+                                            bool finite, uint64_t see, RowState<D>& st) {
   constexpr int K = tile_keys<D>(), KT = K / 32, N = D / 16;  // N fragments of values for 32 keys
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, buf = step % 3;
   const int e_new = __builtin_amdgcn_readfirstlane(S.e[buf]);
+  constexpr float UP = COARSE ? 10.0f : 0.0f;  // log2 of the factor that the exact form has in the values' scales
+  const float from = st.m == -__builtin_inff() ? 0.0f : st.m;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const f32x4a ks = *reinterpret_cast<const f32x4a*>(&S.ks[buf][kt * 32 + a * 8 + h * 4]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[kt][4 * a + r] = __builtin_fmaf(t[kt][4 * a + r], ks[r], UP - from);
+    }
   if (!all) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
@@ -833,29 +857,38 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, t[kt][i]);
-  top *= unit;
-  // the running maximum follows the largest score by steps of at least 2^4, as in step32
-  if (__ballot(top > st.m + 4.0f) || e_new != st.e) {
+  // the running maximum follows the largest score by steps of at least 2^4, as in step32; a row's first score sets it
+  if (__ballot(top > UP + 4.0f || (st.m == -__builtin_inff() && top > -__builtin_inff())) || e_new != st.e) {
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float m = fmaxf(st.m, top);
-    const float shrink = m == st.m ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
+    const bool first = st.m == -__builtin_inff();
+    const float rise = first ? (top > -__builtin_inff() ? top - UP : 0.0f) : fmaxf(top - UP, 0.0f);
+    const float shrink = first ? 1.0f : __builtin_amdgcn_exp2f(-rise);
     const float both = shrink * scale_of_exp(st.e - e_new);
     st.l *= shrink;
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
       for (int i = 0; i < 16; ++i) st.o[j][i] *= both;
-    st.m = m;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t[kt][i] -= rise;
+    if (!first || top > -__builtin_inff()) st.m = from + rise;
     st.e = e_new;
   }
-  const float m = st.m == -__builtin_inff() ? 0.0f : st.m;
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
     __builtin_amdgcn_sched_barrier(0);
-    f16x8a vf[N];
+    f16x8a vf[N], sc[2];
     f32x4a vs[4];
+    if constexpr (COARSE) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) vs[x] = *reinterpret_cast<const f32x4a*>(&S.vs[buf][kt * 32 + x * 8 + h * 4]);
+      for (int x = 0; x < 2; ++x)
+        sc[x] = *reinterpret_cast<const f16x8a*>(reinterpret_cast<const _Float16*>(S.vs[buf]) + kt * 32 + h * 16 + x * 8);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) vs[x] = *reinterpret_cast<const f32x4a*>(&S.vs[buf][kt * 32 + x * 8 + h * 4]);
+    }
 #pragma unroll
     for (int x = 0; x < N; ++x) {
       const int s = x / (N / 2), row = x % (N / 2) * 32 + l32, run = (kt * 2 + s) * 2 + h;
@@ -863,14 +896,25 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
     }
     __builtin_amdgcn_sched_barrier(0);
     f16x8a p[PT][2];
+    if constexpr (COARSE) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t[kt][i], unit, -m));
-      float c = x * vs[i >> 2][i & 3];
-      st.l += x;
-      if constexpr (PT == 2) asm("" : "+v"(c));
-      p[0][i >> 3][i & 7] = (_Float16)c;
-      if constexpr (PT == 2) p[1][i >> 3][i & 7] = (_Float16)(c - (float)p[0][i >> 3][i & 7]);
+      for (int i = 0; i < 16; i += 2) {
+        const f16x2a x = {(_Float16)__builtin_amdgcn_exp2f(t[kt][i]), (_Float16)__builtin_amdgcn_exp2f(t[kt][i + 1])};
+        st.l = __builtin_amdgcn_fdot2(x, f16x2a{(_Float16)1.0f, (_Float16)1.0f}, st.l, false);
+        const f16x2a c = x * f16x2a{sc[i >> 3][i & 7], sc[i >> 3][(i & 7) + 1]};
+        p[0][i >> 3][i & 7] = c[0];
+        p[0][i >> 3][(i & 7) + 1] = c[1];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = __builtin_amdgcn_exp2f(t[kt][i]);
+        float c = x * vs[i >> 2][i & 3];
+        st.l += x;
+        if constexpr (PT == 2) asm("" : "+v"(c));
+        p[0][i >> 3][i & 7] = (_Float16)c;
+        if constexpr (PT == 2) p[1][i >> 3][i & 7] = (_Float16)(c - (float)p[0][i >> 3][i & 7]);
+      }
     }
     if (!finite) {  // zero times such a scale: what a row does not see adds nothing to it all the same
 #pragma unroll
@@ -914,6 +958,7 @@ __device__ __forceinline__ uint64_t row_sees(const AttendArgs& A, const uint64_t
 template <typename T, int D, int QT, int PT, int NW>
 __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
   constexpr int K = tile_keys<D>(), RUNS = K / 16, BATCH = 64 / RUNS;  // runs of a step, steps of a batch of pages
+  constexpr bool COARSE = __is_same(T, hip_bfloat16);
   __shared__ TileLds<D, NW> S;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
@@ -939,14 +984,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
     int tok, head;
     const bool row_ok = tile_row(A, w, p, wave * 32 + l32, tok, head);
     const bool busy = __ballot(row_ok) != 0;
-    f16x8a q[QT][D / 16];
-    float unit;
-    bool nan;
-    query_halves<T, D, QT>(row_ok ? reinterpret_cast<const T*>(A.q) + (int64_t)(w.first + tok) * A.q_token +
-                                        (int64_t)head * A.q_head
-                                  : nullptr,
-                           h, q, unit, nan);
-    unit *= A.scale;
+    QueryHalf<T, D> raw;
+    query_load<T, D>(row_ok ? reinterpret_cast<const T*>(A.q) + (int64_t)(w.first + tok) * A.q_token + (int64_t)head * A.q_head
+                            : nullptr,
+                     h, raw);
+    int e_q = raw.e;
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) e_q = max(e_q, __shfl_xor(e_q, i));
     const uint64_t* bits = A.mask && row_ok ? A.mask + (int64_t)(w.first + tok) * A.words : A.mask;
     // the wave's first token: it sees all keys up to it, and a causal step past it needs its mask
     int lo_tok = row_ok ? tok : 0x7FFFFFFF;
@@ -972,14 +1016,22 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
     };
     fetch(0);
     __syncthreads();  // the tile before is read
-    if (steps) tile_put<D, NW>(f, S, 0, e_run);
+    if (lane == 0) S.top[wave] = e_q;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) e_q = max(e_q, S.top[i]);
+    e_q = __builtin_amdgcn_readfirstlane(e_q);
+    f16x8a q[QT][D / 16];
+    query_terms16<T, D, QT>(raw, e_q, q);
+    const float unit = scale_of_exp(e_q - 14 + 9) * A.scale;  // of a product of a query's terms and a key's code * 2^-9
+    if (steps) tile_put<D, NW, COARSE>(f, S, 0, unit, e_run);
     __syncthreads();
     fetch(1);
     // Between two barriers the first half of the waves takes a step's scores and then its values, the second half the
     // values of the step before and then the scores: on a SIMD one wave's MFMAs meet the other's exponentials.
     // Values stay in LDS for one step more than keys.
     auto pass_on = [&](int n) {
-      if (n + 1 < steps) tile_put<D, NW>(f, S, n + 1, e_run);
+      if (n + 1 < steps) tile_put<D, NW, COARSE>(f, S, n + 1, unit, e_run);
       __syncthreads();
       fetch(n + 2);
     };
@@ -994,7 +1046,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
                          (j0 + K <= 0 || (!A.mask && j0 + K - 1 <= lo_tok));
         uint64_t see = ~0ull;
         if (!all) see = row_sees<K>(A, bits, key, w.ctx, end, tok, ok) >> (4 * h);
-        tile_values<D, PT, NW>(S, n, t, unit, all, ok >> 31 == 0, see, st);
+        tile_values<D, PT, NW, COARSE>(S, n, t, all, ok >> 31 == 0, see, st);
         if constexpr (!decltype(late)::value) pass_on(n);
       }
     };
@@ -1009,7 +1061,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
     // a lane has its row's elements 4c .. 4c+3 for every c with bit 2 of c equal to h
     float l = st.l;
     l += __shfl_xor(l, 32);
-    if (nan && l != 0.0f) l = __uint_as_float(0x7FC00000u);  // of a row that sees a key
+    if constexpr (COARSE) l *= 0x1p-10f;
+    if (raw.nan && l != 0.0f) l = __uint_as_float(0x7FC00000u);  // of a row that sees a key
     if (row_ok) {
       const float down = scale_of_exp(st.e - 1), inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t slot = ((int64_t)share * 2 + (p.k == 0 ? 1 : 0)) * (32 * NW) + wave * 32 + l32;
