@@ -797,28 +797,30 @@ __device__ __forceinline__ void tile_scores(const TileLds<D, NW>& S, int step, c
     const int row = kt * 32 + l32;
     return __builtin_bit_cast(f16x8a, S.k[step & 1][row * (D / 8) + ((2 * i + h) ^ key_swizzle<D>(row))]);
   };
-  f16x8a a[N], b[N];
+  constexpr int AHEAD = 4;  // reads in front of their MFMAs
+  f16x8a f[N][KT];
 #pragma unroll
-  for (int i = 0; i < N; ++i) a[i] = key(0, i);
+  for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) f[i][kt] = key(kt, i);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) t[0][i] = 0.0f;
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[kt][i] = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if constexpr (KT == 2) b[i] = key(1, i);
+    if (i + AHEAD < N) {
 #pragma unroll
-    for (int n = 0; n < QT; ++n) t[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i], q[n][i], t[0], 0, 0, 0);
+      for (int kt = 0; kt < KT; ++kt) f[i + AHEAD][kt] = key(kt, i + AHEAD);
+    }
+#pragma unroll
+    for (int n = 0; n < QT; ++n)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+        t[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i][kt], q[n][i], t[kt], 0, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
   }
-  if constexpr (KT == 2) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t[1][i] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int n = 0; n < QT; ++n) t[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[i], q[n][i], t[1], 0, 0, 0);
-  }
-  __builtin_amdgcn_sched_barrier(0);
 }
 
 // Scores to probabilities and their product with the step's values.  see: a bit for each key that the
