@@ -31,7 +31,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 namespace mxk {
 
@@ -658,12 +657,12 @@ template <int D, int NW>
 struct TileLds {
   static constexpr int K = tile_keys<D>();
   u32x4 k[2][K * D / 8];  // [key][D] float16, pieces of 8 swizzled
-  u32x4 v[3][K * D / 8];  // [row][K keys] float16, pieces of 8 swizzled
-  float ks[3][K];    // times the queries' unit
-  float vs[3][K];    // times 2^(10 - e); coarse: float16, times 2^-e, in the order of a lane's weights
-  int e[3];
+  u32x4 v[2][K * D / 8];  // [row][K keys] float16, pieces of 8 swizzled
+  float ks[2][K];    // times the queries' unit
+  float vs[2][K];    // times 2^(10 - e); coarse: float16, times 2^-e, in the order of a lane's weights
+  int e[2];
   int top[NW];     // exponents of the waves' largest query elements
-  uint32_t ok[3];  // bits of the step's runs of 16 keys that have a page; bit 31: a value's scale is not finite
+  uint32_t ok[2];  // bits of the step's runs of 16 keys that have a page; bit 31: a value's scale is not finite
 };
 
 // Swizzle of the 16-byte pieces of a value row (K * 2 bytes)
@@ -719,7 +718,7 @@ __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>
   using F = Fetched<D, NW>;
   constexpr int K = tile_keys<D>(), RUNS = K / 16;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int buf = step % 3;
+  const int buf = step & 1;
 #pragma unroll
   for (int i = 0; i < F::N; ++i) {
     const uint32_t first = (wave + i * NW) * 64, piece = first + lane;
@@ -734,7 +733,7 @@ __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>
         half[x >> 1][2 * (x & 1) + 1] = codes_f16(__builtin_amdgcn_perm(0u, u, 0x0C030C02u));
       }
 #pragma unroll
-      for (int x = 0; x < 2; ++x) S.k[step & 1][row * (D / 8) + ((2 * c + x) ^ key_swizzle<D>(row))] = half[x];
+      for (int x = 0; x < 2; ++x) S.k[buf][row * (D / 8) + ((2 * c + x) ^ key_swizzle<D>(row))] = half[x];
     }
     // keys 16s + 8b + 4h': run s*2 + h', its half b
     const uint32_t four = piece / (D / 4), c = piece % (D / 4);
@@ -835,7 +834,7 @@ template <int D, int PT, int NW, bool COARSE>
 __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f32x16a (&t)[tile_keys<D>() / 32], bool all,
                                             bool finite, uint64_t see, RowState<D>& st) {
   constexpr int K = tile_keys<D>(), KT = K / 32, N = D / 16;  // N fragments of values for 32 keys
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, buf = step % 3;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, buf = step & 1;
   const int e_new = __builtin_amdgcn_readfirstlane(S.e[buf]);
   constexpr float UP = COARSE ? 10.0f : 0.0f;  // log2 of the factor that the exact form has in the values' scales
   const float from = st.m == -__builtin_inff() ? 0.0f : st.m;
@@ -1029,35 +1028,21 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
     if (steps) tile_put<D, NW, COARSE>(f, S, 0, unit, e_run);
     __syncthreads();
     fetch(1);
-    // Between two barriers the first half of the waves takes a step's scores and then its values, the second half the
-    // values of the step before and then the scores: on a SIMD one wave's MFMAs meet the other's exponentials.
-    // Values stay in LDS for one step more than keys.
-    auto pass_on = [&](int n) {
-      if (n + 1 < steps) tile_put<D, NW, COARSE>(f, S, n + 1, unit, e_run);
-      __syncthreads();
-      fetch(n + 2);
-    };
-    auto loop = [&](auto late) {
-      for (int n = 0; n < steps; ++n) {
+    for (int n = 0; n < steps; ++n) {
+      if (busy) {
         const int key = key0 + n * K, j0 = key - w.ctx;
         f32x16a t[K / 32];
         tile_scores<D, QT, NW>(S, n, q, t);
-        const uint32_t ok = __builtin_amdgcn_readfirstlane(S.ok[n % 3]);
-        if constexpr (decltype(late)::value) pass_on(n);
+        const uint32_t ok = __builtin_amdgcn_readfirstlane(S.ok[n & 1]);
         const bool all = key + K <= end && (ok & 0xFFFFu) == (1u << RUNS) - 1 &&
                          (j0 + K <= 0 || (!A.mask && j0 + K - 1 <= lo_tok));
         uint64_t see = ~0ull;
         if (!all) see = row_sees<K>(A, bits, key, w.ctx, end, tok, ok) >> (4 * h);
         tile_values<D, PT, NW, COARSE>(S, n, t, all, ok >> 31 == 0, see, st);
-        if constexpr (!decltype(late)::value) pass_on(n);
       }
-    };
-    if (!busy) {
-      for (int n = 0; n < steps; ++n) pass_on(n);
-    } else if (wave >= NW / 2) {
-      loop(std::true_type{});
-    } else {
-      loop(std::false_type{});
+      if (n + 1 < steps) tile_put<D, NW, COARSE>(f, S, n + 1, unit, e_run);
+      __syncthreads();
+      fetch(n + 2);
     }
 
     // a lane has its row's elements 4c .. 4c+3 for every c with bit 2 of c equal to h
