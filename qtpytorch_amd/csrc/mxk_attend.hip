@@ -877,10 +877,10 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
     if (!first || top > -__builtin_inff()) st.m = from + rise;
     st.e = e_new;
   }
+  f16x8a p[KT][PT][2];
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
-    __builtin_amdgcn_sched_barrier(0);
-    f16x8a vf[N], sc[2];
+    f16x8a sc[2];
     f32x4a vs[4];
     if constexpr (COARSE) {
 #pragma unroll
@@ -890,21 +890,14 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
 #pragma unroll
       for (int x = 0; x < 4; ++x) vs[x] = *reinterpret_cast<const f32x4a*>(&S.vs[buf][kt * 32 + x * 8 + h * 4]);
     }
-#pragma unroll
-    for (int x = 0; x < N; ++x) {
-      const int s = x / (N / 2), row = x % (N / 2) * 32 + l32, run = (kt * 2 + s) * 2 + h;
-      vf[x] = __builtin_bit_cast(f16x8a, S.v[buf][row * (K / 8) + (run ^ value_swizzle<D>(row))]);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    f16x8a p[PT][2];
     if constexpr (COARSE) {
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
         const f16x2a x = {(_Float16)__builtin_amdgcn_exp2f(t[kt][i]), (_Float16)__builtin_amdgcn_exp2f(t[kt][i + 1])};
         st.l = __builtin_amdgcn_fdot2(x, f16x2a{(_Float16)1.0f, (_Float16)1.0f}, st.l, false);
         const f16x2a c = x * f16x2a{sc[i >> 3][i & 7], sc[i >> 3][(i & 7) + 1]};
-        p[0][i >> 3][i & 7] = c[0];
-        p[0][i >> 3][(i & 7) + 1] = c[1];
+        p[kt][0][i >> 3][i & 7] = c[0];
+        p[kt][0][i >> 3][(i & 7) + 1] = c[1];
       }
     } else {
 #pragma unroll
@@ -913,8 +906,8 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
         float c = x * vs[i >> 2][i & 3];
         st.l += x;
         if constexpr (PT == 2) asm("" : "+v"(c));
-        p[0][i >> 3][i & 7] = (_Float16)c;
-        if constexpr (PT == 2) p[1][i >> 3][i & 7] = (_Float16)(c - (float)p[0][i >> 3][i & 7]);
+        p[kt][0][i >> 3][i & 7] = (_Float16)c;
+        if constexpr (PT == 2) p[kt][1][i >> 3][i & 7] = (_Float16)(c - (float)p[kt][0][i >> 3][i & 7]);
       }
     }
     if (!finite) {  // zero times such a scale: what a row does not see adds nothing to it all the same
@@ -922,13 +915,25 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
       for (int n = 0; n < PT; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (!((uint32_t)(see >> (32 * kt)) >> (8 * (i >> 2) + (i & 3)) & 1)) p[n][i >> 3][i & 7] = (_Float16)0.0f;
+          if (!((uint32_t)(see >> (32 * kt)) >> (8 * (i >> 2) + (i & 3)) & 1)) p[kt][n][i >> 3][i & 7] = (_Float16)0.0f;
     }
+  }
+  auto value = [&](int x) {  // fragment x: keys x / (N / 2) * 16 on, elements x % (N / 2) * 32 on
+    const int row = x % (N / 2) * 32 + l32, run = x / (N / 2) * 2 + h;
+    return __builtin_bit_cast(f16x8a, S.v[buf][row * (K / 8) + (run ^ value_swizzle<D>(row))]);
+  };
+  constexpr int F = KT * N, AHEAD = 8 < F ? 8 : F;
+  f16x8a vf[F];
 #pragma unroll
-    for (int x = 0; x < N; ++x)
+  for (int x = 0; x < AHEAD; ++x) vf[x] = value(x);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int n = 0; n < PT; ++n)
-        st.o[x % (N / 2)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x], p[n][x / (N / 2)], st.o[x % (N / 2)], 0, 0, 0);
+  for (int x = 0; x < F; ++x) {
+    if (x + AHEAD < F) vf[x + AHEAD] = value(x + AHEAD);
+#pragma unroll
+    for (int n = 0; n < PT; ++n)
+      st.o[x % (N / 2)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x], p[x / N][n][x / (N / 2) % 2], st.o[x % (N / 2)], 0, 0, 0);
+    if (x & 1) __builtin_amdgcn_sched_barrier(0);
   }
   __builtin_amdgcn_sched_barrier(0);
 }
