@@ -542,7 +542,7 @@ int mxk_expert_combine_grad(const void* dy, const void* h, int h_type, int64_t r
  * angles, the gradient).  x: x_type, tokens token_stride and heads head_stride
  * elements apart.  freqs float64 [pairs], axis int32 [pairs] (NULL: axis 0; an
  * axis outside [0, axes) has position 0), pos [tokens][axes] of pos_bytes 4 or
- * 8 (signed). */
+ * 8 (signed); with one axis all pairs turn by it.  At most 2^30 tokens. */
 int mxk_rotary(const void* x, int x_type, int64_t tokens, int heads, int64_t D, int64_t token_stride,
                int64_t head_stride, const double* freqs, const int32_t* axis, int pairs, int interleaved,
                const void* pos, int pos_bytes, int axes, int backward, void* y, void* stream);

@@ -4,9 +4,11 @@
 //
 // over the keys j that a token sees: those held before the call, and of the
 // call's own tokens the ones up to itself, or those whose bit its mask has.
-// One pass over the keys with a running maximum m.
+// One pass over the keys with a running maximum m.  Few rows a sequence and
+// head take tiles of 16 rows (k_attend), which are bound by the cache's bytes;
+// more take tiles of up to 256 (k_attend_tile), bound by their arithmetic.
 //
-// Keys.  The codes go to the int8 MFMA as they are stored.  A query row is
+// Tiles of 16 rows, keys.  The codes go to the int8 MFMA as they are stored.  A query row is
 // taken to integers of 16 bits (24 for float32 queries) against its largest
 // element, as two (three) int8 terms, so that <q, k> is an exact integer:
 // the only error is the query's, 2^-16 (2^-24) of its largest element, and a
@@ -19,7 +21,7 @@
 // (code + 128) * 2^-24; one packed fma makes it code * 2^-9, exact.  The
 // probabilities carry the values' scales: p_j * scale_j * 2^(10 - e), e the
 // exponent of the largest scale so far, is at most 2^15, and keeps 11 bits (22
-// for float32 queries: a second term) down to 2^-24 of the largest.
+// for float32 and float16 queries: a second term) down to 2^-24 of the largest.
 //
 // Work.  The blocks of 128 keys of all sequences, heads and tiles of rows
 // lie on one line, which is cut into equal shares, one a workgroup: uneven
@@ -39,7 +41,6 @@ typedef float f32x4a __attribute__((ext_vector_type(4)));
 typedef float f32x16a __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x2a __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8a __attribute__((ext_vector_type(8)));
-
 
 struct AttendArgs {
   const void* q;
@@ -106,9 +107,9 @@ __device__ __forceinline__ uint32_t blocks_below(const AttendArgs& A, const Line
 
 __device__ __forceinline__ SeqWork seq_work(const AttendArgs& A, const Line& L, int b) {
   SeqWork w;
-  const int held = A.batch.lengths[b], o0 = A.batch.offsets[b], o1 = A.batch.offsets[b + 1];
-  w.first = min(max(o0, 0), A.batch.T);
-  w.n = max(0, min(o1, A.batch.T) - max(o0, 0));
+  const int held = A.batch.lengths[b];
+  w.first = kv_offset(A.batch, b);
+  w.n = kv_count(A.batch, b);
   w.ctx = min(max(held, 0), A.cap);
   w.tiles = (w.n + A.TT - 1) >> L.ts;
   w.a = (w.ctx + A.TT + A.keys - 1) >> L.ts;
@@ -166,9 +167,10 @@ __device__ __forceinline__ bool line_share(const AttendArgs& A, const Line& L, i
   if (from >= to) return false;
   uint32_t at = from;
   int b0 = 0;
-  while (at >= lane_of(upto, 63)) {  // below the total: it ends
+  while (at >= lane_of(upto, 63)) {
     at -= lane_of(upto, 63);
     b0 += 64;
+    if (b0 >= B) return false;  // offsets that do not ascend, and so many tokens that the sum has wrapped
     mine = seq_work(A, L, min(b0 + lane, B - 1));
     own = b0 + lane < B ? mine.head * (uint32_t)A.pool.H : 0;
     upto = wave_scan(own);
@@ -201,18 +203,21 @@ __device__ __forceinline__ bool line_share(const AttendArgs& A, const Line& L, i
   return true;
 }
 
-// The next tile on the line (there is one)
-__device__ __forceinline__ void next_tile(const AttendArgs& A, const Line& L, SeqWork& w, Place& p) {
+// The next tile on the line; false: none, which ascending offsets do not come to
+__device__ __forceinline__ bool next_tile(const AttendArgs& A, const Line& L, SeqWork& w, Place& p) {
   p.k = 0;
   if (++p.x == w.tiles * A.chunks) {
     p.x = 0;
     if (++p.h == A.pool.H) {
       p.h = 0;
-      do ++p.b, w = seq_work(A, L, p.b);
-      while (w.head == 0);
+      do {
+        if (++p.b >= A.batch.B) return false;
+        w = seq_work(A, L, p.b);
+      } while (w.head == 0);
     }
   }
   p.blocks = tile_blocks(A, L, w, p.x / A.chunks);
+  return true;
 }
 
 // The tile that a share ends in and does not end, if it begins there too
@@ -221,7 +226,7 @@ __device__ __forceinline__ void leave_part(const AttendArgs& A, int share, bool 
   if (!A.part_t || threadIdx.x != 0) return;
   PartTile t = {};
   t.last = -1;
-  if (some) t = PartTile{w.first, w.n, p.h, p.x, (int)((end - 1) / per), {0, 0, 0}};
+  if (some) t = PartTile{w.first, w.n, p.h, p.x, min((int)((end - 1) / per), A.shares - 1), {0, 0, 0}};
   A.part_t[share] = t;
 }
 
@@ -454,15 +459,19 @@ __device__ __forceinline__ bool tile_row(const AttendArgs& A, const SeqWork& w, 
 template <typename T, int D, int THREADS>
 __device__ __forceinline__ void zero_padding(const AttendArgs& A) {
   const int B = A.batch.B;
-  const int lo = B ? min(max(A.batch.offsets[0], 0), A.batch.T) : 0;
-  const int hi = B ? min(max(A.batch.offsets[B], 0), A.batch.T) : 0;
+  const int64_t lo = B ? kv_offset(A.batch, 0) : 0, hi = B ? kv_offset(A.batch, B) : 0;
   const int64_t row = (int64_t)A.Hq * D, n = (lo + (A.batch.T - hi)) * row;
   T* out = reinterpret_cast<T*>(A.out);
   for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)A.shares * THREADS)
     out[i < lo * row ? i : i - lo * row + hi * row] = out_cvt<T>(0.0f);
 }
 
-// Tiles of 16 rows
+// Tiles of 16 rows, four waves that take 32 keys of each block of 128 and are
+// joined in LDS; two workgroups a CU.  Bound by memory: 64 sequences of up to
+// 8192 keys, 8 heads of 128 with 4 of queries each, bfloat16, 598 MB of cache:
+// 126 us, 4.75 TB/s of the 5.0 that a large copy reaches; 2 sequences of up to 130003, 447 MB:
+// 88 us, 5.1 TB/s.  A wave asks for the next block's keys and values before it
+// computes the present one's; pages come a batch of 32 blocks ahead.
 template <typename T, int D, int QT, int PT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) {
   constexpr int LD = D + 4;
@@ -576,7 +585,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
       break;
     }
     __syncthreads();
-    next_tile(A, L, w, p);
+    if (!next_tile(A, L, w, p)) {
+      leave_part(A, share, false, 0, 1, w, p);
+      break;
+    }
   }
 }
 
@@ -593,7 +605,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
 // four elements of four keys, and its writes, like the MFMA's reads, take
 // rows that follow each other.  16-byte pieces are swizzled so that neither
 // meets itself in a bank.
-#define MXK_TILE 64
+//
+// Roundings: a query is one float16 term (two for float32), which holds
+// float16 and bfloat16 queries whole as far as the tile's largest element allows;
+// probabilities times the values' scales are one float16 term (two for
+// float32), 2^-11 of a weight.  For bfloat16 the probability and the scale go to
+// float16 before their product (three roundings of 2^-11 against the result's 2^-8), and a
+// scale keeps 11 bits down to 2^-14 of the largest one so far, one less for each power of two
+// below; the other forms' do down to 2^-24.
+//
+// Bound by issue: matrix and vector instructions of a SIMD's two waves
+// hardly overlap (matrix 31 % of the cycles, vector 45 %).  2 sequences with up to 2000 new
+// tokens behind up to 6000 keys, 8 heads of 128 with 4 of queries each, bfloat16: 281 GFLOP in
+// 361 us, 0.78 PFLOP/s of the 1.20 that a large bfloat16 product reaches.
 
 // A lane's elements i*16 + h*8 + 0..7 of a query row (null: zeros), and the exponent of the row's largest; rows below
 // 2^-100 count as zeros, and so do, at first, those with a NaN or an infinity.
@@ -777,7 +801,7 @@ __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>
   }
 }
 
-// Sums of a lane's row; of its elements those that query_halves' half h names
+// Sums of a lane's row: o[j][i] is row j * 32 + (i / 4) * 8 + h * 4 + i % 4 of the values in LDS
 template <int D>
 struct RowState {
   f32x16a o[D / 32];
@@ -945,8 +969,8 @@ __device__ __forceinline__ uint64_t row_sees(const AttendArgs& A, const uint64_t
   const int j0 = key - ctx;  // the first key among the new tokens
   uint64_t see = ~0ull;
   if (!A.mask) {
-    const int last = tok - j0;  // the last key of the step that the row sees
-    see = last < 0 ? 0 : last >= 63 ? ~0ull : (2ull << last) - 1;
+    const int64_t last = (int64_t)tok - j0;  // the last key of the step that the row sees
+    see = last < 0 ? 0 : last >= 63 ? ~0ull : (2ull << (int)last) - 1;
   } else if (j0 >= 0) {
     const int word = j0 >> 6, sh = j0 & 63;
     const uint64_t one = word < A.words ? bits[word] : 0, two = word + 1 < A.words ? bits[word + 1] : 0;
@@ -1086,14 +1110,17 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
       leave_part(A, share, p.k == 0 && k1 < p.blocks, at + (uint32_t)(p.blocks - k1), per, w, p);
       break;
     }
-    next_tile(A, L, w, p);
+    if (!next_tile(A, L, w, p)) {
+      leave_part(A, share, false, 0, 1, w, p);
+      break;
+    }
   }
 }
 
 // A tile that share s begins and does not end: its parts are share s's second
 // one and the first ones of the shares after it, up to the one with its last
 // block.  LANES lanes a row: all 64 where a tile has few rows and maybe many parts, 16 where it has many rows and few
-// parts (255 tiles of 256 rows in two or three parts: 35 us with 64).  A lane finds the weight of
+// parts (255 tiles of 256 rows in two or three parts: 35 us with 64, 14 with 16).  A lane finds the weight of
 // every LANES-th part, then all lanes of the row add the parts' sums in their order.
 template <typename T, int D, int LANES>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs A) {
@@ -1237,9 +1264,10 @@ int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_he
   if (q_heads < heads || q_heads % heads || q_heads > 65536)
     return fail(MXK_EINVAL, "kv_attend: query heads are a multiple of the cache's, at most 65536");
   if (B < 0 || width < 0 || tokens < 0 || B >= ((int64_t)1 << 24) || width >= ((int64_t)1 << 31) ||
-      tokens >= ((int64_t)1 << 31) - 64)
-    return fail(MXK_EINVAL, "kv_attend: bad sizes (sequences below 2^24, pages of one and tokens below 2^31)");
-  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(MXK_EINVAL, "kv_attend: the scale is a positive number");
+      tokens > (int64_t)1 << 30)
+    return fail(MXK_EINVAL, "kv_attend: bad sizes (sequences below 2^24, pages of one below 2^31, at most 2^30 tokens)");
+  if (!(scale > 0.0f) || !std::isfinite(scale * 1.4426950408889634f))
+    return fail(MXK_EINVAL, "kv_attend: the scale is a positive number");
   if (q_type != MXK_IN_F32 && q_type != MXK_IN_F16 && q_type != MXK_IN_BF16)
     return fail(MXK_EINVAL, "kv_attend: unknown q_type");
   if (mask && (words < 1 || words > (1 << 20))) return fail(MXK_EINVAL, "kv_attend: 1 to 2^20 words of mask a token");

@@ -37,11 +37,22 @@ __device__ __forceinline__ int kv_page(const KvBatch& s, const KvPool& p, int b,
   return (uint32_t)page < p.pages ? page : -1;
 }
 
-// New tokens of sequence b: first one and how many, inside [0, T]
-__device__ __forceinline__ int kv_first(const KvBatch& s, int b) { return min(max(s.offsets[b], 0), s.T); }
-__device__ __forceinline__ int kv_count(const KvBatch& s, int b) {
-  return max(0, min(s.offsets[b + 1], s.T) - max(s.offsets[b], 0));
+// New tokens of sequences: offset i taken into [0, T], and how many tokens sequence b has (with its first one inside [0, T])
+__device__ __forceinline__ int kv_offset(const KvBatch& s, int i) { return min(max(s.offsets[i], 0), s.T); }
+__device__ __forceinline__ int kv_count(const KvBatch& s, int b) { return max(0, kv_offset(s, b + 1) - kv_offset(s, b)); }
+
+// Position of token t in sequence b
+__device__ __forceinline__ int64_t kv_place(const KvBatch& s, int b, int t) {
+  return (int64_t)s.lengths[b] + ((int64_t)t - s.offsets[b]);
 }
+
+// Blocks of a launch over tokens: x and z, since the threads of one dimension stay below 2^32.  Up to 2^22 - 1 of them lie
+// past the last: their kernels end at once.
+inline dim3 kv_grid(int64_t blocks, int64_t parts) {
+  const int64_t x = blocks < ((int64_t)1 << 22) ? blocks : (int64_t)1 << 22;
+  return dim3((unsigned)x, (unsigned)parts, (unsigned)ceil_div(blocks, x));
+}
+__device__ __forceinline__ int kv_block() { return (int)(blockIdx.z * gridDim.x + blockIdx.x); }
 
 // Sequence of token t, found by a whole wave: the number of sequences that
 // end at or before t; -1 for a token of none.  64 ends at a time, one load

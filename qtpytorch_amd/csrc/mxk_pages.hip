@@ -14,7 +14,7 @@ namespace mxk {
 struct Rotation {
   const double* __restrict__ freqs;  // radians per position
   const int* __restrict__ axis;      // null: axis 0
-  const void* __restrict__ pos;      // [T][axes]; null: the token's own place
+  const void* __restrict__ pos;      // [T][axes], one axis: for all pairs; null: the token's own place
   int wide;                          // int64 positions
   int pairs, axes, interleaved;
   float sign;
@@ -26,7 +26,7 @@ struct Rotation {
 __device__ __forceinline__ float2 rot_turn(const Rotation& r, int64_t at, int t, int i) {
   int64_t p = at;
   if (r.pos) {
-    const int ax = r.axis ? r.axis[i] : 0;
+    const int ax = r.axis && r.axes > 1 ? r.axis[i] : 0;
     const int64_t e = (int64_t)t * r.axes + ax;
     p = (uint32_t)ax >= (uint32_t)r.axes ? 0
         : r.wide ? reinterpret_cast<const int64_t*>(r.pos)[e] : (int64_t) reinterpret_cast<const int*>(r.pos)[e];
@@ -62,14 +62,16 @@ __device__ __forceinline__ void row_store(T* p, const float (&v)[V]) {
 
 // ---------------------------------------------------------------- rotary
 // TB tokens a workgroup: their angles once into LDS, then V pairs (or V
-// elements that are not rotated) a thread and step.  Bound by memory; the
-// angles, ~100 instructions each, are shared by all heads of a token.
+// elements that are not rotated) a thread and step.  The angles, ~100
+// instructions each, are shared by all heads of a token.  Bound by memory: 8190
+// tokens of 32 heads of 128 in bfloat16, 134 MB in 24.8 us, 5.4 TB/s.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_rotary(const T* __restrict__ x, int64_t token_stride, int64_t head_stride,
                                                 Rotation r, int T_, int D, int TB, uint32_t per_token, DivU32 by_token,
                                                 uint32_t per_head, DivU32 by_head, int H, T* __restrict__ y) {
   extern __shared__ float2 cs[];  // [TB][pairs]
-  const int t0 = blockIdx.x * TB, tn = min(TB, T_ - t0);
+  const int t0 = kv_block() * TB, tn = min(TB, T_ - t0);
+  if (tn <= 0) return;  // blocks past the last
   for (int i = threadIdx.x; i < tn * r.pairs; i += 256) {
     const int t = i / r.pairs;
     cs[i] = rot_turn(r, t0 + t, t0 + t, i - t * r.pairs);
@@ -184,11 +186,14 @@ __global__ __launch_bounds__(256) void k_kv_append_pages(
   constexpr int LPR = D / 8, RPW = 64 / LPR;  // lanes a row, rows a wave and step
   __shared__ float2 angles[4][D / 2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = blockIdx.x * 4 + wave;
+  const int t = kv_block() * 4 + wave;
   if (t >= s.T) return;
   const int b = kv_sequence(s, t);
-  const int64_t place = b < 0 ? 0 : (int64_t)s.lengths[b] + (t - s.offsets[b]);
+  const int64_t place = b < 0 ? 0 : kv_place(s, b, t);
   for (int i = lane; i < r.pairs; i += 64) angles[wave][i] = rot_turn(r, place, t, i);
+  // the wave's lanes read each other's angles
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
   const int page = b < 0 || place < 0 ? -1 : kv_page(s, p, b, place >> p.shift);
   const int rows = 2 * p.H + Hq, li = lane % LPR, e = li * 8, sub = lane / LPR;
   const Turn8 turn = turn8(r, e, angles[wave]);
@@ -234,10 +239,10 @@ __global__ __launch_bounds__(256) void k_kv_append_pages(
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_kv_read(KvBatch s, KvPool p, T* __restrict__ k, T* __restrict__ v) {
   constexpr int LPR = D / 8;
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int t = kv_block() * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (t >= s.T) return;
   const int b = kv_sequence(s, t);
-  const int64_t at = b < 0 ? -1 : (int64_t)s.lengths[b] + (t - s.offsets[b]);
+  const int64_t at = b < 0 ? -1 : kv_place(s, b, t);
   const int page = at < 0 ? -1 : kv_page(s, p, b, at >> p.shift);
   const int pos = (int)(at & ((1 << p.shift) - 1));
   const int step = gridDim.y * 64, items = 2 * p.H * LPR;
@@ -329,8 +334,8 @@ static int check_batch(const char* who, const int32_t* table, const int32_t* len
                        int64_t B, int64_t width, int64_t T) {
   const std::string w(who);
   if (B < 0 || width < 0 || T < 0 || B >= ((int64_t)1 << 24) || width >= ((int64_t)1 << 31) ||
-      T >= ((int64_t)1 << 31) - 64)
-    return fail(MXK_EINVAL, w + ": bad sizes (sequences below 2^24, pages of one and tokens below 2^31)");
+      T > (int64_t)1 << 30)
+    return fail(MXK_EINVAL, w + ": bad sizes (sequences below 2^24, pages of one below 2^31, at most 2^30 tokens)");
   if (!offsets || (B > 0 && (!lengths || (width > 0 && !table)))) return fail(MXK_EINVAL, w + ": null pointer");
   return MXK_OK;
 }
@@ -370,7 +375,7 @@ static int launch_rotary(const void* x, int64_t ts, int64_t hs, const Rotation& 
   // few tokens of many heads: a workgroup takes a part of a token's items
   const int64_t parts = std::min<int64_t>(ceil_div((int64_t)per_token * TB, 256),
                                           std::max<int64_t>(1, (2 * num_cus()) / std::max<int64_t>(1, blocks)));
-  const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(parts, 65535));
+  const dim3 grid = kv_grid(blocks, std::min<int64_t>(parts, 65535));
   const size_t lds = (size_t)TB * r.pairs * sizeof(float2);
   const T* xp = reinterpret_cast<const T*>(x);
   T* yp = reinterpret_cast<T*>(y);
@@ -394,7 +399,7 @@ static int launch_append(const void* k, int64_t kt, int64_t kh, const void* v, i
   const int64_t blocks = ceil_div(s.T, 4);
   // few tokens: a wave takes a part of a token's rows, down to one step of them
   const int64_t parts = std::min<int64_t>(steps, std::max<int64_t>(1, 4 * num_cus() / blocks));
-  const dim3 grid((unsigned)blocks, (unsigned)parts);
+  const dim3 grid = kv_grid(blocks, parts);
   hipLaunchKernelGGL((k_kv_append_pages<T, D>), grid, dim3(256), 0, st, reinterpret_cast<const T*>(k), kt, kh,
                      reinterpret_cast<const T*>(v), vt, vh, reinterpret_cast<const T*>(q), qt, qh, Hq, r, s, p,
                      reinterpret_cast<T*>(q_out));
@@ -415,7 +420,7 @@ static int launch_read(int D, const KvBatch& s, const KvPool& p, void* k, void* 
   const int64_t blocks = ceil_div(s.T, 4);
   const int64_t parts = std::min<int64_t>(ceil_div((int64_t)2 * p.H * D / 8, 64),
                                           std::max<int64_t>(1, 2 * num_cus() / blocks));
-  const dim3 grid((unsigned)blocks, (unsigned)parts);
+  const dim3 grid = kv_grid(blocks, parts);
   T *kp = reinterpret_cast<T*>(k), *vp = reinterpret_cast<T*>(v);
   if (D == 64) hipLaunchKernelGGL((k_kv_read<T, 64>), grid, dim3(256), 0, st, s, p, kp, vp);
   else if (D == 128) hipLaunchKernelGGL((k_kv_read<T, 128>), grid, dim3(256), 0, st, s, p, kp, vp);
@@ -433,9 +438,9 @@ int mxk_rotary(const void* x, int x_type, int64_t tokens, int heads, int64_t D, 
                int64_t head_stride, const double* freqs, const int32_t* axis, int pairs, int interleaved,
                const void* pos, int pos_bytes, int axes, int backward, void* y, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (tokens < 0 || heads < 0 || D < 0 || tokens >= ((int64_t)1 << 31) - 64 || heads > 65536 || D > 4096 ||
+  if (tokens < 0 || heads < 0 || D < 0 || tokens > (int64_t)1 << 30 || heads > 65536 || D > 4096 ||
       (int64_t)heads * D >= ((int64_t)1 << 28))
-    return fail(MXK_EINVAL, "rotary: bad sizes (tokens below 2^31, at most 65536 heads of 4096, below 2^28 elements)");
+    return fail(MXK_EINVAL, "rotary: bad sizes (at most 2^30 tokens, at most 65536 heads of 4096, below 2^28 elements)");
   if (tokens == 0 || heads == 0 || D == 0) return MXK_OK;
   if (const int rc = check_rotation("rotary", freqs, pairs, axes, pos_bytes, pos, D, false)) return rc;
   if (!x || !y) return fail(MXK_EINVAL, "rotary: null pointer");

@@ -21,15 +21,15 @@ import math
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .microscale import _FLOATS, _no_tangents
+from .tensor import mx_tensor
 
 Tensor = torch.Tensor
 
 _HEADS = (64, 128, 256)
-_MANY = (1 << 31) - 65  # more tokens than a batch has
+_MANY = 1 << 30  # more tokens than a batch has
 
 
 def _together(first: Tensor, *rest: Optional[Tensor]) -> int:
@@ -41,6 +41,16 @@ def _together(first: Tensor, *rest: Optional[Tensor]) -> int:
     if index < 0:
         L.require_gpu(first)
     return index
+
+
+def _values(name: str, x: Tensor) -> Tensor:
+    """A packed tensor's values; a tensor that would need a gradient or a tangent is refused."""
+    if isinstance(x, mx_tensor):
+        x = x.dequantize()
+    if x.requires_grad and torch.is_grad_enabled():
+        raise L.MXKError(f"{name} has no gradient: call it under torch.no_grad(), or with detached tensors")
+    _no_tangents(name, x)
+    return x
 
 
 # ---------------------------------------------------------------- rotary positions
@@ -131,26 +141,34 @@ def _rotary(x: Tensor, positions: Tensor, axes: int, table: rotary_table, backwa
 
 
 class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, positions, axes, table):
-        ctx.save_for_backward(positions)
-        ctx.axes, ctx.table = axes, table
-        return _rotary(x, positions, axes, table, False)
+    """Linear in x: its gradient is the opposite rotation, to any order."""
 
     @staticmethod
-    @once_differentiable
+    def forward(ctx, x, positions, axes, table, backward):
+        ctx.save_for_backward(positions)
+        ctx.how = axes, table, backward
+        return _rotary(x, positions, axes, table, backward)
+
+    @staticmethod
     def backward(ctx, dy):
         (positions,) = ctx.saved_tensors
-        return _rotary(dy, positions, ctx.axes, ctx.table, True), None, None, None
+        axes, table, backward = ctx.how
+        if torch.is_grad_enabled() and dy.requires_grad:
+            return _Rotary.apply(dy, positions, axes, table, not backward), None, None, None, None
+        return _rotary(dy, positions, axes, table, not backward), None, None, None, None
 
 
 def rotary(x: Tensor, positions: Tensor, table: rotary_table) -> Tensor:
     """Heads x [..., heads, D] (float32, float16 or bfloat16, any strides)
-    rotated by their tokens' positions [...] or [..., axes] (int32 or int64).
+    rotated by their tokens' positions [...] or [..., axes] (int32 or int64; an
+    axis of the table that they lack is at position 0).
 
     Angles are reduced in float64, so that far positions keep them; products
     and sums are float32, rounded once.  The gradient is the opposite rotation
-    of the output's."""
+    of the output's, itself differentiable.  Positions without axes, or with one,
+    are the same for all pairs."""
+    if isinstance(x, mx_tensor):
+        x = x.dequantize()
     if x.dtype not in _FLOATS:
         raise TypeError(f"rotary: float32, float16 or bfloat16 expected, got {x.dtype}")
     if x.dim() < 2:
@@ -160,7 +178,7 @@ def rotary(x: Tensor, positions: Tensor, table: rotary_table) -> Tensor:
     if 2 * table.freqs.numel() > x.shape[-1]:
         raise ValueError(f"rotary: the table rotates {2 * table.freqs.numel()} elements, a head has {x.shape[-1]}")
     if x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, positions, axes, table)
+        return _Rotary.apply(x, positions, axes, table, False)
     return _rotary(x, positions, axes, table, False)
 
 
@@ -261,6 +279,7 @@ class kv_pages:
 
     def _rows(self, name: str, what: str, x: Tensor, H: int, D: int) -> Tensor:
         """x [tokens, heads, D] with D contiguous; H: heads of keys and values, whose multiple queries have."""
+        x = _values(name, x)
         shape = x.shape
         if len(shape) != 3 or shape[2] != D or (what != "q" and shape[1] != H):
             raise ValueError(f"{name}: {what} [tokens, {'heads' if what == 'q' else H}, {D}] expected, got {tuple(shape)}")
@@ -277,16 +296,17 @@ class kv_pages:
         [tokens, axes] (None: each token's position in its sequence, on every
         axis); they are packed from the unrounded rotation.  q [tokens, q_heads,
         head_dim] is rotated along and returned.  A head's row with a NaN or an
-        infinity reads as NaN.  Nothing is differentiable."""
+        infinity reads as NaN.  Nothing is differentiable: tensors that require a
+        gradient are refused where gradients are recorded."""
+        codes, scales, n, page, H, D = self._pool()
+        k, v = self._rows("kv_pages.append", "k", k, H, D), self._rows("kv_pages.append", "v", v, H, D)
+        if q is not None:
+            q = self._rows("kv_pages.append", "q", q, H, D)
         kind = _FLOATS.get(k.dtype)
         if kind is None or v.dtype != k.dtype or q is not None and q.dtype != k.dtype:
             raise TypeError(f"kv_pages.append: keys, values and queries of one type (float32, float16 or bfloat16) "
                             f"expected, got {k.dtype}, {v.dtype}{'' if q is None else f' and {q.dtype}'}")
-        codes, scales, n, page, H, D = self._pool()
-        k, v = self._rows("kv_pages.append", "k", k, H, D), self._rows("kv_pages.append", "v", v, H, D)
         T = k.shape[0]
-        if q is not None:
-            q = self._rows("kv_pages.append", "q", q, H, D)
         if v.shape[0] != T or q is not None and q.shape[0] != T:
             raise ValueError(f"kv_pages.append: one row for each of {T} tokens expected, got {v.shape[0]} of v"
                              f"{'' if q is None else f' and {q.shape[0]} of q'}")
@@ -332,14 +352,18 @@ class kv_pages:
         is new token j of the same sequence.  scale: of the scores, 1 /
         sqrt(head_dim) unless given.  A row that sees nothing is zeros.
 
-        Codes are used as they are, q to 16 bits of its row's largest element
-        (24 where it is float32), probabilities to 11 bits (22), sums in float32.
-        Nothing is differentiable."""
+        Codes are used as they are and sums are float32.  Where a sequence has
+        few rows a head (64 on average; 128 at heads of 256 elements), q keeps 16
+        bits of its row's largest element (24 in float32), and a probability times
+        its value's scale 11 bits (22 in float32 and float16) down to 2^-24 of
+        the largest.  Else q's elements keep 11 bits (22 in float32) down to 2^-28 of
+        the largest of 128 or 256 rows, and those products 11 (22 in float32), in bfloat16 with two
+        roundings more and down to 2^-14.  Nothing is differentiable, as in append."""
+        codes, scales, n, page, H, D = self._pool()
+        q = self._rows("kv_pages.attend", "q", q, H, D)
         kind = _FLOATS.get(q.dtype)
         if kind is None:
             raise TypeError(f"kv_pages.attend: float32, float16 or bfloat16 expected, got {q.dtype}")
-        codes, scales, n, page, H, D = self._pool()
-        q = self._rows("kv_pages.attend", "q", q, H, D)
         _check_batch("kv_pages.attend", batch)
         T, Hq, _ = q.shape
         words = 0

@@ -57,6 +57,9 @@ def _attend(**kw):
     (_attend, dict(q_heads=0), b"multiple"), (_attend, dict(scale=0.0), b"positive"),
     (_attend, dict(scale=float("nan")), b"positive"), (_attend, dict(scale=float("inf")), b"positive"),
     (_attend, dict(q_type=7), b"q_type"), (_attend, dict(mask=SOME, words=0), b"words"), (_attend, dict(pages=0), b"without pages"),
+    (_attend, dict(tokens=(1 << 30) + 1), b"bad sizes"), (_append, dict(tokens=(1 << 30) + 1), b"bad sizes"),
+    (_rotary, dict(tokens=(1 << 30) + 1), b"bad sizes"), (_attend, dict(tokens=30000, width=1 << 30), b"2^31 blocks"),
+    (_attend, dict(scale=3e38), b"positive"),
     (_attend, dict(width=400, ws=0), b"workspace"), (_attend, dict(width=400, ws_bytes=100), b"workspace"),
     (_attend, dict(width=400, ws=SOME + 4), b"workspace"),
 ])

@@ -371,6 +371,18 @@ def test_attend_values_of_far_apart_scales(dtype, group):
     R.near(_pages(codes, scales).attend(q.cuda(), batch.gpu()), want, error)
 
 
+@pytest.mark.parametrize("group", [3, 20, 80])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_attend_rows_of_far_apart_sizes(dtype, group):
+    """Rows of one tile whose queries differ by 2^15: each keeps its own precision."""
+    batch = R.Batch([300, 40], [2, 3], 16)
+    codes, scales = R.pool(batch, 1, 64)
+    size = torch.tensor([1e-3, 1.0, 30.0])[torch.randint(0, 3, (5, group, 1), generator=R.gen(2))]
+    q = (size * _rand((5, group, 64), 1)).to(dtype)
+    want, error = R.attend(batch, codes, scales, q)
+    R.near(_pages(codes, scales).attend(q.cuda(), batch.gpu()), want, error)
+
+
 @pytest.mark.parametrize("group", [2, 64])
 @pytest.mark.parametrize("factor", [1e-30, 1e20])
 def test_attend_scales_at_both_ends(factor, group):
@@ -404,6 +416,49 @@ def test_attend_more_positions_than_the_table(group):
     R.near(_pages(codes, scales).attend(q.cuda(), batch.gpu()), want, error)
     batch.table, batch.width = batch.table[:, :0].contiguous(), 0
     assert (_pages(codes, scales).attend(q.cuda(), batch.gpu()).cpu() == 0).all()
+
+
+@pytest.mark.parametrize("group", [2, 80])
+def test_attend_sequences_whose_offsets_do_not_ascend(group):
+    """A sequence that would end before it begins has no tokens, whatever the distance."""
+    batch = R.Batch([100], [5], 16)
+    codes, scales = R.pool(batch, 1, 64)
+    q = _rand((5, group, 64), 1)
+    want, error = R.attend(batch, codes, scales, q)
+    one = batch.gpu()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    least = -(1 << 31)
+    three = one._replace(table=one.table.repeat(3, 1), lengths=one.lengths.repeat(3), offsets=torch.tensor([0, 5, least, 5], **i32))
+    pages = _pages(codes, scales)
+    R.near(pages.attend(q.cuda(), three), want, error)
+    before = pages.codes.clone()
+    second = one._replace(offsets=torch.tensor([5, least], **i32))
+    pages.keep(second, torch.tensor([[3, 1, 4]], **i32))
+    assert torch.equal(before, pages.codes)
+
+
+def test_more_blocks_than_one_dimension_has():
+    """More than 2^24 tokens: the last ones are rotated, stored and read as they are alone."""
+    import qtpytorch_amd as qa
+    n, D = (1 << 24) + 3, 64
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = qa.rotary_table.make(D)
+    x = torch.zeros(n, 1, D, dtype=torch.bfloat16, device="cuda")
+    x[-20:] = _rand((20, 1, D), 1, torch.bfloat16).cuda()
+    # the last 20 tokens are a sequence's, those in front of them padding
+    batch = qa.kv_batch(torch.tensor([[1, 0]], **i32), torch.tensor([7], **i32), torch.tensor([n - 20, n], **i32))
+    alone = batch._replace(offsets=torch.tensor([0, 20], **i32))
+    big, small = qa.kv_pages.empty(2, 16, 1, D), qa.kv_pages.empty(2, 16, 1, D)
+    for p in (big, small):
+        p.codes.zero_()
+        p.scales.zero_()
+    got = big.append(x, x, batch, rotary=table, q=x)
+    want = small.append(x[-20:], x[-20:], alone, rotary=table, q=x[-20:])
+    assert torch.equal(got[-20:], want) and not got[:-20].any()
+    assert torch.equal(big.codes, small.codes) and torch.equal(big.scales, small.scales) and big.codes.any()
+    k, v = big.read(batch, n)
+    k1, v1 = small.read(alone, 20)
+    assert torch.equal(k[-20:], k1) and torch.equal(v[-20:], v1) and not k[:-20].any()
 
 
 def test_attend_many_sequences():
@@ -626,5 +681,15 @@ def test_refusals():
         pages.read(gb, 2, torch.float64)
     with pytest.raises(ValueError, match="number"):
         pages.read(gb, -1)
+    leaf = x.clone().requires_grad_()
+    for call in (lambda t: pages.append(t, x, gb), lambda t: pages.append(x, t, gb), lambda t: pages.attend(t, gb),
+                 lambda t: pages.append(x, x, gb, rotary=table, q=t)):
+        with pytest.raises(qa._lib.MXKError, match="no gradient"):
+            call(leaf)
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(qa._lib.MXKError, match="forward-mode"):
+                call(torch.autograd.forward_ad.make_dual(x, x))
+        with torch.no_grad():
+            call(leaf)
     with pytest.raises(qa._lib.MXKError, match="without pages"):
         qa.kv_pages.empty(0, 16, 2, 64).attend(x, gb)

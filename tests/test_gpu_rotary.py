@@ -102,6 +102,23 @@ def test_gradient_of_a_broadcast_input_and_of_a_shared_one():
                                            + 2.0 ** -23 * want.abs()).sum(1, keepdim=True))
 
 
+def test_gradient_of_the_gradient():
+    """dx is linear in dy: its gradient towards dy is the rotation of the vector that it is weighted with."""
+    import qtpytorch_amd as qa
+    _, _, table = _table(32, 1, False)
+    pos = _positions(6, 1, 0, True, 2).cuda()
+    x, dy, v = (torch.randn(6, 3, 64, generator=R.gen(i)).cuda().requires_grad_() for i in range(3))
+    (dx,) = torch.autograd.grad(qa.rotary(x, pos, table), x, dy, create_graph=True)
+    assert dx.requires_grad
+    (back,) = torch.autograd.grad(dx, dy, v.detach())
+    assert torch.equal(back, qa.rotary(v.detach(), pos, table))
+    # and it adds up along two uses of one leaf
+    y = qa.rotary(x, pos, table) * qa.rotary(x, pos + 1, table).detach()
+    (one,) = torch.autograd.grad(y.sum(), x)
+    want = qa.rotary(qa.rotary(x, pos + 1, table).detach(), -pos, table)
+    assert (one - want).abs().max() < 2.0 ** -19 * 2 * want.abs().max()  # the opposite angles, rounded apart
+
+
 @pytest.mark.parametrize("shape", [(0, 4, 64), (5, 0, 64), (2, 0, 3, 64)])
 def test_nothing_to_rotate(shape):
     import qtpytorch_amd as qa
@@ -131,6 +148,38 @@ def test_an_axis_without_positions_turns_nothing():
     y = qa.rotary(x, torch.full((3, 2), 7).cuda(), table)
     assert torch.equal(y[..., [1, 2, 5, 6]], x[..., [1, 2, 5, 6]])
     assert not torch.equal(y[..., [0, 3]], x[..., [0, 3]])
+
+
+def test_one_axis_of_positions_turns_all_pairs():
+    import qtpytorch_amd as qa
+    freqs, axis, table = _table(32, 3, False)
+    x, pos = torch.randn(5, 2, 64, generator=R.gen(1)).cuda(), torch.arange(5).cuda() + 3
+    want = qa.rotary(x, pos[:, None].repeat(1, 3), table)
+    for p in (pos, pos[:, None], pos.int()):
+        assert torch.equal(qa.rotary(x, p, table), want)
+    one = qa.rotary_table(freqs.cuda())
+    assert torch.equal(qa.rotary(x, pos, one), want)
+
+
+def test_more_blocks_than_one_dimension_has():
+    """2^22 workgroups and more: the last tokens get what they get alone."""
+    import qtpytorch_amd as qa
+    _, _, table = _table(129, 1, False)
+    n = (1 << 22) + 5
+    x = torch.zeros(n, 1, 258, dtype=torch.float16, device="cuda")
+    at = torch.tensor([0, 1, (1 << 22) - 1, 1 << 22, n - 1], device="cuda")
+    x[at] = torch.randn(5, 1, 258, generator=R.gen(1)).half().cuda()
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    got = qa.rotary(x, pos, table)
+    assert torch.equal(got[at], qa.rotary(x[at], pos[at], table))
+
+
+def test_packed_heads_are_their_values():
+    import qtpytorch_amd as qa
+    _, _, table = _table(32, 1, False)
+    x = qa.mx_tensor.quantize(torch.randn(3, 4, 64, generator=R.gen(1)).cuda(), "int8d")
+    pos = torch.arange(3).cuda()
+    assert torch.equal(qa.rotary(x, pos, table), qa.rotary(x.dequantize(), pos, table))
 
 
 def test_nan_and_infinity_stay_in_their_pair():
