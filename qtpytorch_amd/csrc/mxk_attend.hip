@@ -580,15 +580,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
       }
     }
     at += (uint32_t)(k1 - p.k);
-    if (at >= to) {
-      leave_part(A, share, p.k == 0 && k1 < p.blocks, at + (uint32_t)(p.blocks - k1), per, w, p);
+    const bool some = p.k == 0 && k1 < p.blocks;  // then at >= to
+    const uint32_t last = at + (uint32_t)(p.blocks - k1);
+    if (at >= to || !next_tile(A, L, w, p)) {
+      leave_part(A, share, some, last, per, w, p);
       break;
     }
     __syncthreads();
-    if (!next_tile(A, L, w, p)) {
-      leave_part(A, share, false, 0, 1, w, p);
-      break;
-    }
   }
 }
 
@@ -617,7 +615,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
 // Bound by issue: matrix and vector instructions of a SIMD's two waves
 // hardly overlap (matrix 31 % of the cycles, vector 45 %).  2 sequences with up to 2000 new
 // tokens behind up to 6000 keys, 8 heads of 128 with 4 of queries each, bfloat16: 281 GFLOP in
-// 361 us, 0.78 PFLOP/s of the 1.20 that a large bfloat16 product reaches.
+// 356 us with the join, 0.79 PFLOP/s of the 1.20 that a large bfloat16 product reaches.
 
 // A lane's elements i*16 + h*8 + 0..7 of a query row (null: zeros), and the exponent of the row's largest; rows below
 // 2^-100 count as zeros, and so do, at first, those with a NaN or an infinity.
@@ -985,6 +983,11 @@ __device__ __forceinline__ uint64_t row_sees(const AttendArgs& A, const uint64_t
   return see;
 }
 
+// Place in a part of the four elements 32 a + 16 h + 4 r .. of row `wave` * 32 + lane % 32 (a lane's 4 r follow by 256): a
+// wave writes and reads 1 KB in a row.
+template <int D>
+__device__ __forceinline__ int tile_part(int wave, int a, int lane) { return ((wave * (D / 32) + a) * 256 + lane) * 4; }
+
 template <typename T, int D, int QT, int PT, int NW>
 __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
   constexpr int K = tile_keys<D>(), RUNS = K / 16, BATCH = 64 / RUNS;  // runs of a step, steps of a batch of pages
@@ -1081,10 +1084,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
     if (raw.nan && l != 0.0f) l = __uint_as_float(0x7FC00000u);  // of a row that sees a key
     if (row_ok) {
       const float down = scale_of_exp(st.e - 1), inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int64_t slot = ((int64_t)share * 2 + (p.k == 0 ? 1 : 0)) * (32 * NW) + wave * 32 + l32;
+      const int64_t slot = (int64_t)share * 2 + (p.k == 0 ? 1 : 0);
       T* dst = reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D;
+      float* part = A.part_o + slot * (32 * NW * D) + tile_part<D>(wave, 0, lane);
 #pragma unroll
-      for (int a = 0; a < D / 32; ++a)
+      for (int a = 0; a < D / 32; ++a) {  // 16 elements in a row
+        T y[16];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           f32x4a x;
@@ -1093,25 +1098,19 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
             const int row = j * (D / 4) + 8 * a + r;
             x[j] = st.o[row / 32][(row % 32 / 8) * 4 + row % 4] * down;
           }
-          const int d = 4 * (8 * a + 4 * h + r);
-          if (whole) {
-            T y[4];
+          if (!whole) *reinterpret_cast<f32x4a*>(part + a * 1024 + r * 256) = x;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = out_cvt<T>(x[j] * inv);
-            __builtin_memcpy(dst + d, y, sizeof(y));
-          } else {
-            *reinterpret_cast<f32x4a*>(A.part_o + slot * D + d) = x;
-          }
+          for (int j = 0; j < 4; ++j) y[4 * r + j] = out_cvt<T>(x[j] * inv);
         }
-      if (!whole && h == 0) A.part_s[slot] = make_float2(st.m, l);
+        if (whole) __builtin_memcpy(dst + 32 * a + 16 * h, y, sizeof(y));
+      }
+      if (!whole && h == 0) A.part_s[slot * (32 * NW) + wave * 32 + l32] = make_float2(st.m, l);
     }
     at += (uint32_t)(k1 - p.k);
-    if (at >= to) {
-      leave_part(A, share, p.k == 0 && k1 < p.blocks, at + (uint32_t)(p.blocks - k1), per, w, p);
-      break;
-    }
-    if (!next_tile(A, L, w, p)) {
-      leave_part(A, share, false, 0, 1, w, p);
+    const bool some = p.k == 0 && k1 < p.blocks;  // then at >= to
+    const uint32_t last = at + (uint32_t)(p.blocks - k1);
+    if (at >= to || !next_tile(A, L, w, p)) {
+      leave_part(A, share, some, last, per, w, p);
       break;
     }
   }
@@ -1119,13 +1118,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
 
 // A tile that share s begins and does not end: its parts are share s's second
 // one and the first ones of the shares after it, up to the one with its last
-// block.  LANES lanes a row: all 64 where a tile has few rows and maybe many parts, 16 where it has many rows and few
-// parts (255 tiles of 256 rows in two or three parts: 35 us with 64, 14 with 16).  A lane finds the weight of
-// every LANES-th part, then all lanes of the row add the parts' sums in their order.
-template <typename T, int D, int LANES>
+// block.  Tiles of 16 rows, which may have many parts: a wave a row; a lane finds the weight of
+// every 64th part, then all lanes add the parts' sums in their order.
+template <typename T, int D>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs A) {
-  constexpr int E = D / LANES, RPB = 256 / LANES, U = LANES == 64 ? 8 : 2;  // parts in flight
-  const int s = blockIdx.x, lane = threadIdx.x & (LANES - 1), base = threadIdx.x & 63 & ~(LANES - 1);
+  constexpr int E = D / 64, U = 8;  // elements of a lane, parts in flight
+  const int s = blockIdx.x, lane = threadIdx.x & 63, r = blockIdx.y * 4 + (threadIdx.x >> 6);
   const PartTile t = A.part_t[s];
   if (t.last < 0) return;
   SeqWork w;
@@ -1134,51 +1132,91 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs A) {
   Place p;
   p.h = t.h;
   p.x = t.x;
+  int tok, head;
+  if (!tile_row(A, w, p, r, tok, head)) return;
   const int parts = t.last - s + 1;
-  for (int r0 = blockIdx.y * RPB; r0 < A.rows; r0 += gridDim.y * RPB) {
-    const int r = r0 + threadIdx.x / LANES;  // RPB divides the rows
-    int tok, head;
-    const bool live = tile_row(A, w, p, r, tok, head);
-    if (__ballot(live) == 0) continue;
-    // rows that do not exist take part in the exchanges with what another row has: a part of theirs may not be written
-    auto slot = [&](int i) { return ((int64_t)(s + i) * 2 + (i == 0)) * A.rows + (live ? r : 0); };
-    float m = -__builtin_inff();
-    for (int i = lane; i < parts; i += LANES) m = fmaxf(m, A.part_s[slot(i)].x);
+  auto slot = [&](int i) { return ((int64_t)(s + i) * 2 + (i == 0)) * A.rows + r; };
+  float m = -__builtin_inff();
+  for (int i = lane; i < parts; i += 64) m = fmaxf(m, A.part_s[slot(i)].x);
 #pragma unroll
-    for (int i = 1; i < LANES; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
-    float sum = 0.0f, acc[E];
+  for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
+  float sum = 0.0f, acc[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) acc[j] = 0.0f;
-    for (int i0 = 0; i0 < parts; i0 += LANES) {
-      const int n = min(LANES, parts - i0);
-      const float2 ms = A.part_s[slot(i0 + min(lane, n - 1))];
-      const float f = lane >= n ? 0.0f : ms.x == m ? 1.0f : __builtin_amdgcn_exp2f(ms.x - m);
-      if (lane < n) sum += f * ms.y;
-      for (int i = 0; i < n; i += U) {
-        float v[U][E];
+  for (int j = 0; j < E; ++j) acc[j] = 0.0f;
+  for (int i0 = 0; i0 < parts; i0 += 64) {
+    const int n = min(64, parts - i0);
+    const float2 ms = A.part_s[slot(i0 + min(lane, n - 1))];
+    const float f = lane >= n ? 0.0f : ms.x == m ? 1.0f : __builtin_amdgcn_exp2f(ms.x - m);
+    if (lane < n) sum += f * ms.y;
+    for (int i = 0; i < n; i += U) {
+      float v[U][E];
 #pragma unroll
-        for (int u = 0; u < U; ++u)  // past the last part: it again, not added
-          __builtin_memcpy(v[u], A.part_o + slot(i0 + min(i + u, n - 1)) * D + lane * E, sizeof(v[u]));
+      for (int u = 0; u < U; ++u)  // past the last part: it again, not added
+        __builtin_memcpy(v[u], A.part_o + slot(i0 + min(i + u, n - 1)) * D + lane * E, sizeof(v[u]));
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float g = __shfl(f, base + min(i + u, LANES - 1));
-          if (i + u < n) {
+      for (int u = 0; u < U; ++u) {
+        const float g = __shfl(f, min(i + u, 63));
+        if (i + u < n) {
 #pragma unroll
-            for (int j = 0; j < E; ++j) acc[j] = __builtin_fmaf(g, v[u][j], acc[j]);
-          }
+          for (int j = 0; j < E; ++j) acc[j] = __builtin_fmaf(g, v[u][j], acc[j]);
         }
       }
     }
-#pragma unroll
-    for (int i = 1; i < LANES; i <<= 1) sum += __shfl_xor(sum, i);
-    if (live) {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      T e[E];
-#pragma unroll
-      for (int j = 0; j < E; ++j) e[j] = out_cvt<T>(acc[j] * inv);
-      __builtin_memcpy(reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D + lane * E, e, sizeof(e));
-    }
   }
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T e[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) e[j] = out_cvt<T>(acc[j] * inv);
+  __builtin_memcpy(reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D + lane * E, e, sizeof(e));
+}
+
+// The same for tiles of many rows, which have few parts: a lane has 16 elements of a row as in k_attend_tile and finds the
+// parts' weights itself.  Bound by the parts' bytes: 256 shares of 256 rows of 128, 7.5 to 13.5 us at 5 to 6 TB/s.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attend_join_tile(AttendArgs A) {
+  const int s = blockIdx.x, lane = threadIdx.x & 63, unit = blockIdx.y * 4 + (threadIdx.x >> 6);
+  const int wave = unit / (D / 32), a = unit % (D / 32), r = wave * 32 + (lane & 31);
+  const PartTile t = A.part_t[s];
+  if (t.last < 0) return;
+  SeqWork w;
+  w.first = t.first;
+  w.n = t.n;
+  Place p;
+  p.h = t.h;
+  p.x = t.x;
+  int tok, head;
+  if (!tile_row(A, w, p, r, tok, head)) return;
+  const int parts = t.last - s + 1;
+  auto slot = [&](int i) { return (int64_t)(s + i) * 2 + (i == 0); };
+  float m = -__builtin_inff(), sum = 0.0f;
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, A.part_s[slot(i) * A.rows + r].x);
+  f32x4a acc[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) acc[x] = f32x4a{0, 0, 0, 0};
+#pragma unroll 2
+  for (int i = 0; i < parts; ++i) {
+    const float2 ms = A.part_s[slot(i) * A.rows + r];
+    const float* part = A.part_o + slot(i) * A.rows * D + tile_part<D>(wave, a, lane);
+    f32x4a v[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const f32x4a*>(part + x * 256);
+    const float f = ms.x == m ? 1.0f : __builtin_amdgcn_exp2f(ms.x - m);
+    sum += f * ms.y;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[x][j] = __builtin_fmaf(f, v[x][j], acc[x][j]);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T e[16];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[4 * x + j] = out_cvt<T>(acc[x][j] * inv);
+  __builtin_memcpy(reinterpret_cast<T*>(A.out) + ((int64_t)(w.first + tok) * A.Hq + head) * D + 32 * a + 16 * (lane >> 5), e,
+                   sizeof(e));
 }
 
 // ---------------------------------------------------------------- host
@@ -1225,8 +1263,8 @@ static int launch_attend(const AttendArgs& A, const AttendPlan& a, hipStream_t s
   if (a.rows == 16) hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A);
   else hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, NW>), dim3(a.shares), dim3(64 * NW), 0, st, A);
   if (a.cut && a.shares > 1) {
-    if (a.rows == 16) hipLaunchKernelGGL((k_attend_join<T, D, 64>), dim3(a.shares - 1, 4), dim3(256), 0, st, A);
-    else hipLaunchKernelGGL((k_attend_join<T, D, 16>), dim3(a.shares - 1, a.rows / 16), dim3(256), 0, st, A);
+    if (a.rows == 16) hipLaunchKernelGGL((k_attend_join<T, D>), dim3(a.shares - 1, 4), dim3(256), 0, st, A);
+    else hipLaunchKernelGGL((k_attend_join_tile<T, D>), dim3(a.shares - 1, a.rows * D / 4096), dim3(256), 0, st, A);
   }
   return check_launch("kv_attend");
 }
