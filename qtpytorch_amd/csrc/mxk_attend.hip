@@ -1119,10 +1119,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
 // A tile that share s begins and does not end: its parts are share s's second
 // one and the first ones of the shares after it, up to the one with its last
 // block.  Tiles of 16 rows, which may have many parts: a wave a row; a lane finds the weight of
-// every 64th part, then all lanes add the parts' sums in their order.
+// every 64th part, all lanes add the parts' sums in their order.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs A) {
-  constexpr int E = D / 64, U = 8;  // elements of a lane, parts in flight
+  constexpr int E = D / 64, U = 16;  // elements of a lane, parts in flight
   const int s = blockIdx.x, lane = threadIdx.x & 63, r = blockIdx.y * 4 + (threadIdx.x >> 6);
   const PartTile t = A.part_t[s];
   if (t.last < 0) return;
@@ -1136,23 +1136,30 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs A) {
   if (!tile_row(A, w, p, r, tok, head)) return;
   const int parts = t.last - s + 1;
   auto slot = [&](int i) { return ((int64_t)(s + i) * 2 + (i == 0)) * A.rows + r; };
-  float m = -__builtin_inff();
-  for (int i = lane; i < parts; i += 64) m = fmaxf(m, A.part_s[slot(i)].x);
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
-  float sum = 0.0f, acc[E];
+  float m = -__builtin_inff(), sum = 0.0f, acc[E];
 #pragma unroll
   for (int j = 0; j < E; ++j) acc[j] = 0.0f;
   for (int i0 = 0; i0 < parts; i0 += 64) {
     const int n = min(64, parts - i0);
-    const float2 ms = A.part_s[slot(i0 + min(lane, n - 1))];
-    const float f = lane >= n ? 0.0f : ms.x == m ? 1.0f : __builtin_amdgcn_exp2f(ms.x - m);
-    if (lane < n) sum += f * ms.y;
-    for (int i = 0; i < n; i += U) {
-      float v[U][E];
+    float v[U][E];
+    auto load = [&](int i) {  // past the last part: it again, not added
 #pragma unroll
-      for (int u = 0; u < U; ++u)  // past the last part: it again, not added
+      for (int u = 0; u < U; ++u)
         __builtin_memcpy(v[u], A.part_o + slot(i0 + min(i + u, n - 1)) * D + lane * E, sizeof(v[u]));
+    };
+    const float2 ms = A.part_s[slot(i0 + min(lane, n - 1))];
+    load(0);  // on its way while the weights are found
+    float top = fmaxf(m, ms.x);
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
+    const float shrink = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    const float f = lane >= n ? 0.0f : ms.x == m ? 1.0f : __builtin_amdgcn_exp2f(ms.x - m);
+    sum *= shrink;
+    if (lane < n) sum += f * ms.y;
+#pragma unroll
+    for (int j = 0; j < E; ++j) acc[j] *= shrink;
+    for (int i = 0;;) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const float g = __shfl(f, min(i + u, 63));
@@ -1161,6 +1168,8 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs A) {
           for (int j = 0; j < E; ++j) acc[j] = __builtin_fmaf(g, v[u][j], acc[j]);
         }
       }
+      if ((i += U) >= n) break;
+      load(i);
     }
   }
 #pragma unroll
@@ -1190,24 +1199,42 @@ __global__ __launch_bounds__(256) void k_attend_join_tile(AttendArgs A) {
   if (!tile_row(A, w, p, r, tok, head)) return;
   const int parts = t.last - s + 1;
   auto slot = [&](int i) { return (int64_t)(s + i) * 2 + (i == 0); };
+  constexpr int U = 4;  // parts in flight
   float m = -__builtin_inff(), sum = 0.0f;
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, A.part_s[slot(i) * A.rows + r].x);
   f32x4a acc[4];
 #pragma unroll
   for (int x = 0; x < 4; ++x) acc[x] = f32x4a{0, 0, 0, 0};
-#pragma unroll 2
-  for (int i = 0; i < parts; ++i) {
-    const float2 ms = A.part_s[slot(i) * A.rows + r];
-    const float* part = A.part_o + slot(i) * A.rows * D + tile_part<D>(wave, a, lane);
-    f32x4a v[4];
+  for (int i = 0; i < parts; i += U) {
+    float2 ms[U];
+    f32x4a v[U][4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const f32x4a*>(part + x * 256);
-    const float f = ms.x == m ? 1.0f : __builtin_amdgcn_exp2f(ms.x - m);
-    sum += f * ms.y;
+    for (int u = 0; u < U; ++u) {
+      ms[u].x = -__builtin_inff();
+      if (i + u < parts) {
+        ms[u] = A.part_s[slot(i + u) * A.rows + r];
+        const float* part = A.part_o + slot(i + u) * A.rows * D + tile_part<D>(wave, a, lane);
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < 4; ++x) v[u][x] = *reinterpret_cast<const f32x4a*>(part + x * 256);
+      }
+    }
+    float top = m;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[x][j] = __builtin_fmaf(f, v[x][j], acc[x][j]);
+    for (int u = 0; u < U; ++u) top = fmaxf(top, ms[u].x);
+    const float shrink = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    sum *= shrink;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) acc[x] *= shrink;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u < parts) {
+        const float f = ms[u].x == m ? 1.0f : __builtin_amdgcn_exp2f(ms[u].x - m);
+        sum += f * ms[u].y;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[x][j] = __builtin_fmaf(f, v[u][x][j], acc[x][j]);
+      }
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   T e[16];
