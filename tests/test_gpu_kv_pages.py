@@ -233,6 +233,23 @@ def test_keep_of_the_longest_path_and_of_absent_pages():
     assert torch.equal(pages.codes.cpu(), want)
 
 
+def test_keep_moves_scales_along():
+    batch = R.Batch([30, 5], [40, 20], 16)
+    codes, scales = R.pool(batch, 2, 64)
+    pages = _pages(codes, scales)
+    path = torch.tensor([[3, 3, 39, 0, 1], [-1, 19, 20, 2, 2]], dtype=torch.int32)  # twice the same, none, past the last
+    pages.keep(batch.gpu(), path.cuda())
+    want_c, want_s = codes.clone(), scales.clone()
+    for b in range(2):
+        for j, pick in enumerate(path[b].tolist()):
+            if 0 <= pick < batch.new[b]:
+                to, at = batch.place(b, batch.held[b] + j), batch.place(b, batch.held[b] + pick)
+                want_c[to[0], :, :, to[1]] = codes[at[0], :, :, at[1]]
+                want_s[to[0], :, :, to[1]] = scales[at[0], :, :, at[1]]
+    assert torch.equal(pages.codes.cpu(), want_c)
+    assert torch.equal(pages.scales.cpu().nan_to_num(-1.0), want_s.nan_to_num(-1.0))
+
+
 # ---------------------------------------------------------------- attend
 def _check_attend(batch, heads, group, dim, dtype, mask=None, scale=None, seed=0, qscale=1.5):
     codes, scales = R.pool(batch, heads, dim, seed)
@@ -484,6 +501,61 @@ def test_attend_layouts(layout, dtype):
         y = torch.zeros(5 * 4 * 64 + 1, dtype=dtype, device="cuda")[1:].view(5, 4, 64)
     y.copy_(x)
     assert torch.equal(pages.attend(x, batch.gpu()), pages.attend(y, batch.gpu()))
+
+
+@pytest.mark.parametrize("layout", ["apart", "heads first", "odd address", "broadcast"])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_attend_layouts_of_large_tiles(layout, dtype):
+    batch = R.Batch([30, 5], [2, 3], 16)
+    pages = _pages(*R.pool(batch, 1, 128))
+    x = _rand((5, 90, 128), 1, dtype).cuda()
+    if layout == "apart":
+        y = torch.zeros(5, 97, 150, dtype=dtype, device="cuda")[:, 2:92, 3:131]
+    elif layout == "heads first":
+        y = torch.zeros(90, 5, 128, dtype=dtype, device="cuda").transpose(0, 1)
+    elif layout == "odd address":
+        y = torch.zeros(5 * 90 * 128 + 1, dtype=dtype, device="cuda")[1:].view(5, 90, 128)
+    else:
+        x = x[:, :1].repeat(1, 90, 1)
+        y = x[:, :1].clone().expand(5, 90, 128)
+    if layout != "broadcast":
+        y.copy_(x)
+    assert torch.equal(pages.attend(x, batch.gpu()), pages.attend(y, batch.gpu()))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("group", [300, 513])
+def test_attend_groups_larger_than_a_tile(group, dtype):
+    _check_attend(R.Batch([70, 0, 9], [1, 2, 0], 16), 2, group, 64, dtype)
+
+
+@pytest.mark.parametrize("group", [2, 40])
+def test_attend_large_pages(group):
+    batch = R.Batch([1500, 10], [3, 3], 1024)
+    _check_attend(batch, 2, group, 64, torch.bfloat16)
+    _check_attend(batch, 2, group, 64, torch.bfloat16, mask=_tree(batch))
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_pool_of_more_than_4_gib(new):
+    """The same step in pages in front and behind 4 GiB of codes: bit for bit the same."""
+    import qtpytorch_amd as qa
+    H, G, D, n = 2, 4, 128, 1 << 20
+    pages = qa.kv_pages.empty(n, 16, H, D)
+    assert pages.codes.numel() > 1 << 32
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = qa.rotary_table.make(D)
+    got = []
+    for base in (0, n - 8):
+        batch = qa.kv_batch(torch.arange(base, base + 8, **i32)[None].flip(1).contiguous(), torch.tensor([0], **i32),
+                            torch.tensor([0, 60], **i32))
+        q, k, v = (_rand((60, h, D), 7 + h, torch.bfloat16).cuda() for h in (H * G, H, H))
+        q = pages.append(k, v, batch, rotary=table, q=q)
+        step = batch._replace(lengths=torch.tensor([60 - new], **i32), offsets=torch.tensor([0, new], **i32))
+        o = pages.attend(q[60 - new:], step)
+        pages.keep(batch, torch.tensor([[5, 50, 20]], **i32))
+        got.append((q, o, *pages.read(batch, 60)))
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and torch.isfinite(got[0][1]).all()
 
 
 def test_repeats_bit_for_bit():
