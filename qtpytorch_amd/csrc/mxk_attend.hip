@@ -146,20 +146,36 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return __bui
 __device__ __forceinline__ int lane_of(int v, int lane) { return (int)__builtin_amdgcn_readlane((uint32_t)v, lane); }
 
 // Share `share` of the line, [from, to), and the place it begins at.  Found by
-// a whole wave, which holds a sequence a lane: for up to 64 of them one round of loads.
+// every wave for itself, which holds a sequence a lane: for up to 64 of them one round of loads.
+// More are first summed by the workgroup's THREADS threads, a run of sequences each (1024 sequences of 256 keys, one head: 30 us,
+// and 39 where each wave walks them 64 at a time; 4096 of 64: 57 and 106).
 // false: an empty share.
+template <int THREADS>
 __device__ __forceinline__ bool line_share(const AttendArgs& A, const Line& L, int share, uint32_t& from, uint32_t& to,
                                            uint32_t& per, SeqWork& w, Place& p) {
   const int lane = threadIdx.x & 63, B = A.batch.B;
+  __shared__ uint32_t sums[THREADS];
   if (B == 0) return false;
-  SeqWork mine = seq_work(A, L, min(lane, B - 1));
-  uint32_t own = lane < B ? mine.head * (uint32_t)A.pool.H : 0;
-  uint32_t upto = wave_scan(own);
-  uint32_t total = lane_of(upto, 63);
-  if (B > 64) {
+  uint32_t total, upto4 = 0, four = 0;
+  const int run = (B + THREADS - 1) / THREADS;
+  SeqWork mine;
+  uint32_t own = 0, upto = 0;
+  if (B <= 64) {
+    mine = seq_work(A, L, min(lane, B - 1));
+    own = lane < B ? mine.head * (uint32_t)A.pool.H : 0;
+    upto = wave_scan(own);
+    total = lane_of(upto, 63);
+  } else {
     uint32_t sum = 0;
-    for (int b = 64 + lane; b < B; b += 64) sum += seq_work(A, L, b).head * (uint32_t)A.pool.H;
-    total += lane_of(wave_scan(sum), 63);
+    const int first = (int)threadIdx.x * run, end = min(first + run, B);
+#pragma unroll 4
+    for (int b = first; b < end; ++b) sum += seq_work(A, L, b).head * (uint32_t)A.pool.H;
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) four += sums[lane * (THREADS / 64) + i];
+    upto4 = wave_scan(four);
+    total = lane_of(upto4, 63);
   }
   per = (total + (uint32_t)A.shares - 1) / (uint32_t)A.shares;
   from = (uint32_t)share * per;
@@ -167,6 +183,18 @@ __device__ __forceinline__ bool line_share(const AttendArgs& A, const Line& L, i
   if (from >= to) return false;
   uint32_t at = from;
   int b0 = 0;
+  if (B > 64) {
+    const int l = __builtin_ctzll(__ballot(upto4 > at));
+    at -= lane_of(upto4 - four, l);
+    int i = l * (THREADS / 64);
+    while (i < THREADS - 1 && at >= sums[i]) at -= sums[i++];
+    b0 = __builtin_amdgcn_readfirstlane(i) * run;
+    at = __builtin_amdgcn_readfirstlane(at);
+    if (b0 >= B) return false;  // of sums that have wrapped, as below
+    mine = seq_work(A, L, min(b0 + lane, B - 1));
+    own = b0 + lane < B ? mine.head * (uint32_t)A.pool.H : 0;
+    upto = wave_scan(own);
+  }
   while (at >= lane_of(upto, 63)) {
     at -= lane_of(upto, 63);
     b0 += 64;
@@ -484,7 +512,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
   uint32_t from, to, per;
   SeqWork w;
   Place p;
-  if (!line_share(A, L, share, from, to, per, w, p)) {
+  if (!line_share<256>(A, L, share, from, to, per, w, p)) {
     leave_part(A, share, false, 0, 1, w, p);
     return;
   }
@@ -1002,7 +1030,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
   uint32_t from, to, per;
   SeqWork w;
   Place p;
-  if (!line_share(A, L, share, from, to, per, w, p)) {
+  if (!line_share<64 * NW>(A, L, share, from, to, per, w, p)) {
     leave_part(A, share, false, 0, 1, w, p);
     return;
   }

@@ -483,6 +483,33 @@ def test_attend_many_sequences():
     _check_attend(R.Batch(held, [(i * 7) % 3 for i in range(200)], 16), 1, 2, 64, torch.bfloat16)
 
 
+@pytest.mark.parametrize("count,group", [(65, 2), (70, 90), (1500, 2), (600, 90), (1100, 70)])
+def test_attend_more_sequences_than_threads(count, group):
+    held = [(i * 37) % 45 for i in range(count)]
+    _check_attend(R.Batch(held, [(i * 7) % 5 // 2 for i in range(count)], 16, front=2, back=3), 1, group, 64, torch.float16)
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 4095, 4097, 9000])
+def test_every_token_finds_its_sequence(count):
+    """Each sequence stores a value of its own in its page; idle ones store nothing."""
+    import qtpytorch_amd as qa
+    i32 = dict(dtype=torch.int32)
+    new = torch.randint(0, 3, (count,), generator=R.gen(count), **i32)
+    offsets = torch.cat([torch.zeros(1, **i32), new.cumsum(0).int()]) + 2
+    T = int(offsets[-1]) + 3
+    owner = torch.full((T,), -1)
+    owner[2:T - 3] = torch.repeat_interleave(torch.arange(count), new.long())
+    batch = qa.kv_batch(torch.arange(count, **i32)[:, None].cuda(), (torch.arange(count, **i32) % 13).cuda(), offsets.cuda())
+    pages = qa.kv_pages.empty(count, 16, 1, 64)
+    pages.scales.zero_()
+    x = (owner + 1).clamp(min=0).float()[:, None, None].expand(T, 1, 64).contiguous().cuda()
+    pages.append(x, -x, batch)
+    k, v = pages.read(batch, T, torch.float32)
+    assert torch.allclose(k, x, rtol=2.0 ** -22, atol=0) and torch.allclose(v, -x, rtol=2.0 ** -22, atol=0)
+    rows = (pages.scales[:, 0, 0] != 0).sum(1).cpu()
+    assert torch.equal(rows, new.long())
+
+
 def test_attend_long_context_in_parts():
     _check_attend(R.Batch([20011, 3], [1, 1], 64), 1, 4, 64, torch.float32)
 
