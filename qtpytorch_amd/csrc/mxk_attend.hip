@@ -248,6 +248,12 @@ __device__ __forceinline__ bool next_tile(const AttendArgs& A, const Line& L, Se
   return true;
 }
 
+// The workgroup's share.  Neighbours on the line may read the same keys: they go to one XCD.  Tiles of 16 rows, 16 trees of 64
+// tokens on 4000 keys of 8 heads: 65 us, 91 in the order of the blocks.
+__device__ __forceinline__ int share_of_block(const AttendArgs& A) {
+  return A.shares % 8 == 0 ? (blockIdx.x & 7) * (A.shares >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+}
+
 // The tile that a share ends in and does not end, if it begins there too
 __device__ __forceinline__ void leave_part(const AttendArgs& A, int share, bool some, uint32_t end, uint32_t per,
                                            const SeqWork& w, const Place& p) {
@@ -506,7 +512,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
   __shared__ float so[4][16][LD];
   __shared__ float sm[4][16], sl[4][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int l16 = lane & 15, g = lane >> 4, share = blockIdx.x;
+  const int l16 = lane & 15, g = lane >> 4, share = share_of_block(A);
   const Line L = make_line(A);
   zero_padding<T, D, 256>(A);
   uint32_t from, to, per;
@@ -619,7 +625,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
 }
 
 // ---------------------------------------------------------------- tiles of many rows
-// NW waves of 32 rows each share the keys, 64 at a time: their codes are
+// NW waves of 32 rows each (4 or 8) share the keys, 64 at a time: their codes are
 // made float16 (code * 2^-9, exact) once for the workgroup on the way into LDS,
 // values transposed, and both products run on the 32x32x16 MFMA.  As above S^T
 // leaves a lane with one row's keys, which are the second product's operand as
@@ -1017,14 +1023,13 @@ template <int D>
 __device__ __forceinline__ int tile_part(int wave, int a, int lane) { return ((wave * (D / 32) + a) * 256 + lane) * 4; }
 
 template <typename T, int D, int QT, int PT, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void k_attend_tile(AttendArgs A) {
+__global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend_tile(AttendArgs A) {
   constexpr int K = tile_keys<D>(), RUNS = K / 16, BATCH = 64 / RUNS;  // runs of a step, steps of a batch of pages
   constexpr bool COARSE = __is_same(T, hip_bfloat16);
   __shared__ TileLds<D, NW> S;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
-  // neighbours on the line read the same keys: they go to one XCD
-  const int share = A.shares % 8 == 0 ? (blockIdx.x & 7) * (A.shares >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+  const int share = share_of_block(A);
   const Line L = make_line(A);
   zero_padding<T, D, 64 * NW>(A);
   uint32_t from, to, per;
@@ -1285,11 +1290,12 @@ static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int
   AttendPlan a;
   // rows of a sequence and key head, on average
   const double each = B > 0 ? (double)T * G / (double)std::min(B, T) : 0.0;
-  // Up to 64 rows (128 of 256 elements) tiles of 16, whose waves need no barrier: several of them read the same keys, but
-  // from the L2.  16 sequences of 4000 keys, 8 heads of 128, bfloat16, us by tiles of 16 / 256: 32 rows 41 / 62, 64 rows
-  // 58 / 72, 128 rows 93 / 62; 2 sequences of 60000: 64 rows 104 / 121, 128 rows 188 / 132; float32 by 16 / 128: 64 rows
-  // 58 / 86, 128 rows 93 / 80; heads of 256: 128 rows 82 / 87, 256 rows 125 / 110.
-  a.rows = each <= (D == 256 ? 128 : 64) ? 16 : D == 256 || wide ? 128 : 256;
+  // Tiles of 16 rows, whose waves need no barrier, though several of them read the same keys from the L2, then of 128 (two
+  // workgroups a CU but for float32 and heads of 256), then of 256.  16 sequences of 4000 keys, 8 heads of 128, bfloat16,
+  // us by tiles of 16 / 128 / 256: 64 rows 66 / - / 84, 96 rows 102 / 69 / 85, 128 rows 122 / 70 / 86, 192 rows 181 / - / 97;
+  // 2 sequences of 60000: 64 rows 118 / - / 152, 128 rows 229 / 128 / 151; 16 of 300: 96 rows 33 / 30 / 25.  float32 by 16 /
+  // 128: 96 rows of 4000 keys 113 / 122, of 60000 180 / 220, 128 rows 136 / 132; heads of 256: 64 rows 141 / 189, 96 rows 208 / 190.
+  a.rows = each <= (wide ? 96 : 64) ? 16 : D == 256 || wide || each <= 128 ? 128 : 256;
   a.keys = a.rows == 16 ? 128 : 256;
   a.GC = std::min(G, a.rows);
   a.chunks = (int)ceil_div(G, a.GC);
@@ -1301,7 +1307,7 @@ static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int
   a.most = std::max(1, (a.cap + a.keys - 1) / a.keys);
   a.cut = a.most > 1 && B > 0;
   a.fits = tiles * a.most < 2147483648.0;
-  const double most = (a.rows > 16 || D == 256 ? 1.0 : 2.0) * num_cus();  // workgroups that run at once
+  const double most = (a.rows == 256 || D == 256 || (a.rows == 128 && wide) ? 1.0 : 2.0) * num_cus();  // workgroups that run at once
   a.shares = (int)std::max(1.0, std::min(most, tiles * a.most));
   return a;
 }
@@ -1314,9 +1320,14 @@ static size_t attend_bytes(const AttendPlan& a, int D) {
 template <typename T, int D, int QT, int PT>
 static int launch_attend(const AttendArgs& A, const AttendPlan& a, hipStream_t st) {
   constexpr int QH = sizeof(T) == 4 ? 2 : 1;  // float16 terms of a query and of the probabilities in the tile kernel
-  constexpr int NW = D == 256 || QH == 2 ? 4 : 8;
-  if (a.rows == 16) hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A);
-  else hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, NW>), dim3(a.shares), dim3(64 * NW), 0, st, A);
+  if (a.rows == 16) {
+    hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A);
+  } else if (a.rows == 128) {
+    hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 4>), dim3(a.shares), dim3(256), 0, st, A);
+  } else {
+    if constexpr (D < 256 && QH == 1)
+      hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 8>), dim3(a.shares), dim3(512), 0, st, A);
+  }
   if (a.cut && a.shares > 1) {
     if (a.rows == 16) hipLaunchKernelGGL((k_attend_join<T, D>), dim3(a.shares - 1, 4), dim3(256), 0, st, A);
     else hipLaunchKernelGGL((k_attend_join_tile<T, D>), dim3(a.shares - 1, a.rows * D / 4096), dim3(256), 0, st, A);

@@ -353,7 +353,7 @@ class kv_pages:
         sqrt(head_dim) unless given.  A row that sees nothing is zeros.
 
         Codes are used as they are and sums are float32.  Where a sequence has
-        few rows a head (64 on average; 128 at heads of 256 elements), q keeps 16
+        few rows a head (64 on average; 96 in float32), q keeps 16
         bits of its row's largest element (24 in float32), and a probability times
         its value's scale 11 bits (22 in float32 and float16) down to 2^-24 of
         the largest.  Else q's elements keep 11 bits (22 in float32) down to 2^-28 of
