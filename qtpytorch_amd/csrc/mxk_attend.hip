@@ -504,7 +504,7 @@ __device__ __forceinline__ void zero_padding(const AttendArgs& A) {
 // joined in LDS; two workgroups a CU.  Bound by memory: 64 sequences of up to
 // 8192 keys, 8 heads of 128 with 4 of queries each, bfloat16, 598 MB of cache:
 // 126 us, 4.75 TB/s of the 5.0 that a large copy reaches; 2 sequences of up to 130003, 447 MB:
-// 88 us, 5.1 TB/s.  A wave asks for the next block's keys and values before it
+// 84 us, 5.3 TB/s.  A wave asks for the next block's keys and values before it
 // computes the present one's; pages come a batch of 32 blocks ahead.
 template <typename T, int D, int QT, int PT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) {
@@ -665,7 +665,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
 // Bound by issue: matrix and vector instructions of a SIMD's two waves
 // hardly overlap (matrix 31 % of the cycles, vector 45 %).  2 sequences with up to 2000 new
 // tokens behind up to 6000 keys, 8 heads of 128 with 4 of queries each, bfloat16: 281 GFLOP in
-// 356 us with the join, 0.79 PFLOP/s of the 1.20 that a large bfloat16 product reaches.
+// 353 us with the join, 0.80 PFLOP/s of the 1.20 that a large bfloat16 product reaches.
 
 // A lane's elements i*16 + h*8 + 0..7 of a query row (null: zeros), and the exponent of the row's largest; rows below
 // 2^-100 count as zeros, and so do, at first, those with a NaN or an infinity.
