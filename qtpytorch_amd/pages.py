@@ -43,13 +43,18 @@ def _together(first: Tensor, *rest: Optional[Tensor]) -> int:
     return index
 
 
+def _no_gradients(name: str, x: Tensor) -> None:
+    """Refuse a tensor that would need a gradient or a tangent."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise L.MXKError(f"{name} has no gradient: call it under torch.no_grad(), or with detached tensors")
+    _no_tangents(name, x)
+
+
 def _values(name: str, x: Tensor) -> Tensor:
     """A packed tensor's values; a tensor that would need a gradient or a tangent is refused."""
     if isinstance(x, mx_tensor):
         x = x.dequantize()
-    if x.requires_grad and torch.is_grad_enabled():
-        raise L.MXKError(f"{name} has no gradient: call it under torch.no_grad(), or with detached tensors")
-    _no_tangents(name, x)
+    _no_gradients(name, x)
     return x
 
 
@@ -238,7 +243,8 @@ class kv_pages:
 
     page_size is a power of two from 16 on, head_dim 64, 128 or 256.  Which
     sequence has which page is the caller's: pages are named by a kv_batch alone.
-    A page may stand in several tables (a shared prefix) while nobody writes to it."""
+    A page may stand in several tables (a shared prefix) while nobody writes to it.
+    Scales that require a gradient are refused by the calls where gradients are recorded."""
 
     __slots__ = ("codes", "scales")
 
@@ -273,7 +279,9 @@ class kv_pages:
     def nbytes(self) -> int:
         return self.codes.numel() + 4 * self.scales.numel()
 
-    def _pool(self):
+    def _pool(self, name: str):
+        """Addresses and sizes for a call; scales that need a gradient or a tangent are refused as its tensors are."""
+        _no_gradients(name, self.scales)
         n, _, H, page, D = self.codes.shape
         return self.codes.data_ptr(), self.scales.data_ptr(), n, page, H, D
 
@@ -298,7 +306,7 @@ class kv_pages:
         head_dim] is rotated along and returned.  A head's row with a NaN or an
         infinity reads as NaN.  Nothing is differentiable: tensors that require a
         gradient are refused where gradients are recorded."""
-        codes, scales, n, page, H, D = self._pool()
+        codes, scales, n, page, H, D = self._pool("kv_pages.append")
         k, v = self._rows("kv_pages.append", "k", k, H, D), self._rows("kv_pages.append", "v", v, H, D)
         if q is not None:
             q = self._rows("kv_pages.append", "q", q, H, D)
@@ -359,7 +367,7 @@ class kv_pages:
         the largest.  Else q's elements keep 11 bits (22 in float32) down to 2^-28 of
         the largest of 128 or 256 rows, and those products 11 (22 in float32), in bfloat16 with two
         roundings more and down to 2^-14.  Nothing is differentiable, as in append."""
-        codes, scales, n, page, H, D = self._pool()
+        codes, scales, n, page, H, D = self._pool("kv_pages.attend")
         q = self._rows("kv_pages.attend", "q", q, H, D)
         kind = _FLOATS.get(q.dtype)
         if kind is None:
@@ -406,7 +414,7 @@ class kv_pages:
             raise ValueError(f"kv_pages.keep: a path [{table.shape[0]}, steps] expected, got {tuple(path.shape)}")
         path = path.contiguous()
         gpu = _together(self.codes, path, table, lengths, offsets)
-        codes, scales, n, page, H, D = self._pool()
+        codes, scales, n, page, H, D = self._pool("kv_pages.keep")
         with L.on_gpu(gpu):
             rc = L.lib().mxk_kv_pages_keep(codes, scales, n, page, H, D, table.data_ptr(), lengths.data_ptr(),
                                            offsets.data_ptr(), table.shape[0], table.shape[1], _MANY, path.data_ptr(),
@@ -424,7 +432,7 @@ class kv_pages:
         kind = L.elem_type(dtype)
         table, lengths, offsets = batch
         gpu = _together(self.codes, table, lengths, offsets)
-        codes, scales, n, page, H, D = self._pool()
+        codes, scales, n, page, H, D = self._pool("kv_pages.read")
         k = torch.empty((tokens, H, D), dtype=dtype, device=self.codes.device)
         v = torch.empty_like(k)
         with L.on_gpu(gpu):
