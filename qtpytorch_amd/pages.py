@@ -63,9 +63,11 @@ class rotary_table:
     """Angles of rotary positions: pair i of a head turns by ``freqs[i]`` radians
     for each position on axis ``axis[i]``.
 
-    freqs float64 [pairs] and axis int32 [pairs] (None: one axis) on the GPU.
-    Pair i is elements (i, i + pairs), or (2i, 2i + 1) where ``interleaved``;
-    a head's elements from 2 * pairs on are not rotated."""
+    freqs float64 [pairs] and axis int32 [pairs] (None: one axis) on the GPU, used as
+    they are: a change in place counts for the calls after it, and a gradient of a call
+    before it is refused as torch refuses its own.  Pair i is elements (i, i + pairs), or
+    (2i, 2i + 1) where ``interleaved``; a head's elements from 2 * pairs on are not rotated.
+    Nothing is differentiable towards freqs: calls refuse them where they would need a gradient."""
 
     __slots__ = ("freqs", "axis", "interleaved")
 
@@ -129,8 +131,8 @@ def _token_rows(x: Tensor) -> Tensor:
     return x if x.stride(2) == 1 or x.shape[2] <= 1 else x.contiguous()
 
 
-def _rotary(x: Tensor, positions: Tensor, axes: int, table: rotary_table, backward: bool) -> Tensor:
-    freqs, axis = table.freqs, table.axis
+def _rotary(x: Tensor, positions: Tensor, axes: int, freqs: Tensor, axis: Optional[Tensor], interleaved: bool,
+            backward: bool) -> Tensor:
     gpu = _together(x, positions, freqs, axis)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     rows = _token_rows(x)
@@ -138,7 +140,7 @@ def _rotary(x: Tensor, positions: Tensor, axes: int, table: rotary_table, backwa
     token, head, _ = rows.stride()
     with L.on_gpu(gpu):
         rc = L.lib().mxk_rotary(rows.data_ptr(), _FLOATS[x.dtype], tokens, H, D, token, head, freqs.data_ptr(),
-                                L.ptr(axis), freqs.numel(), table.interleaved, positions.data_ptr(),
+                                L.ptr(axis), freqs.numel(), interleaved, positions.data_ptr(),
                                 positions.element_size(), axes, backward, y.data_ptr(), L.stream_on(gpu))
     if rc:
         L.check(rc, f"rotary({tokens}x{H}x{D})")
@@ -149,18 +151,17 @@ class _Rotary(torch.autograd.Function):
     """Linear in x: its gradient is the opposite rotation, to any order."""
 
     @staticmethod
-    def forward(ctx, x, positions, axes, table, backward):
-        ctx.save_for_backward(positions)
-        ctx.how = axes, table, backward
-        return _rotary(x, positions, axes, table, backward)
+    def forward(ctx, x, positions, axes, freqs, axis, interleaved, backward):
+        ctx.save_for_backward(positions, freqs, axis)
+        ctx.how = axes, interleaved, backward
+        return _rotary(x, positions, axes, freqs, axis, interleaved, backward)
 
     @staticmethod
     def backward(ctx, dy):
-        (positions,) = ctx.saved_tensors
-        axes, table, backward = ctx.how
-        if torch.is_grad_enabled() and dy.requires_grad:
-            return _Rotary.apply(dy, positions, axes, table, not backward), None, None, None, None
-        return _rotary(dy, positions, axes, table, not backward), None, None, None, None
+        positions, freqs, axis = ctx.saved_tensors
+        axes, interleaved, backward = ctx.how
+        turn = _Rotary.apply if torch.is_grad_enabled() and dy.requires_grad else _rotary
+        return turn(dy, positions, axes, freqs, axis, interleaved, not backward), None, None, None, None, None, None
 
 
 def rotary(x: Tensor, positions: Tensor, table: rotary_table) -> Tensor:
@@ -182,9 +183,9 @@ def rotary(x: Tensor, positions: Tensor, table: rotary_table) -> Tensor:
     positions, axes = _positions("rotary", positions, x.shape[:-2])
     if 2 * table.freqs.numel() > x.shape[-1]:
         raise ValueError(f"rotary: the table rotates {2 * table.freqs.numel()} elements, a head has {x.shape[-1]}")
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, positions, axes, table, False)
-    return _rotary(x, positions, axes, table, False)
+    _no_gradients("rotary towards a table's frequencies", table.freqs)
+    turn = _Rotary.apply if x.requires_grad and torch.is_grad_enabled() else _rotary
+    return turn(x, positions, axes, table.freqs, table.axis, table.interleaved, False)
 
 
 # ---------------------------------------------------------------- the paged cache
@@ -324,6 +325,7 @@ class kv_pages:
         pairs = axes = bytes_ = interleaved = 0
         if rotary is not None:
             freqs, axis, interleaved = rotary.freqs, rotary.axis, rotary.interleaved
+            _no_gradients("kv_pages.append towards a table's frequencies", freqs)
             pairs = freqs.numel()
             if 2 * pairs > D:
                 raise ValueError(f"kv_pages.append: the table rotates {2 * pairs} elements, a head has {D}")

@@ -43,3 +43,57 @@ def test_scales_that_need_a_gradient_are_refused(call):
         dual = torch.autograd.forward_ad.make_dual(scales, scales.clone())
         with pytest.raises(qa._lib.MXKError, match=f"kv_pages.{call} has no forward-mode"):
             _calls(qa, qa.kv_pages(codes, dual), batch)[call]()
+
+
+# ---------------------------------------------------------------- a rotary table's tensors
+def _turned(qa, freqs, axis, seed=1):
+    x = torch.randn(5, 3, 64, generator=R.gen(seed)).cuda().requires_grad_()
+    pos = torch.arange(10).view(5, 2).cuda()
+    return x, qa.rotary(x, pos, qa.rotary_table(freqs, axis))
+
+
+@pytest.mark.parametrize("which", ["freqs", "axis"])
+def test_a_table_changed_before_the_gradient_is_an_error(which):
+    import qtpytorch_amd as qa
+    table = {"freqs": torch.rand(32, dtype=torch.float64).cuda(), "axis": (torch.arange(32) % 2).int().cuda()}
+    x, y = _turned(qa, **table)
+    table[which].mul_(0)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.sum().backward()
+    # the change counts for what is called after it
+    x, y = _turned(qa, **table)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    if which == "freqs":
+        assert torch.equal(y, x) and torch.equal(dx, torch.ones_like(x))
+
+
+def test_a_table_whose_pairing_changes_before_the_gradient():
+    import qtpytorch_amd as qa
+    table = qa.rotary_table.make(64)
+    x = torch.randn(5, 3, 64, generator=R.gen(1)).cuda().requires_grad_()
+    pos = torch.arange(5).cuda()
+    y = qa.rotary(x, pos, table)
+    want = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)[0]
+    table.interleaved = True
+    assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], want)
+
+
+def test_frequencies_that_need_a_gradient_are_refused():
+    import qtpytorch_amd as qa
+    freqs = torch.rand(32, dtype=torch.float64).cuda()
+    leaf = freqs.clone().requires_grad_()
+    table = qa.rotary_table(leaf)
+    batch = R.Batch([5], [2], 16)
+    pages = qa.kv_pages(*(t.cuda() for t in R.pool(batch, 2, 64, poison=False)))
+    x, pos = torch.ones(2, 2, 64).cuda(), torch.arange(2).cuda()
+    for name, call in (("rotary", lambda t: qa.rotary(x, pos, t)),
+                       ("rotary", lambda t: qa.rotary(x.clone().requires_grad_(), pos, t)),
+                       ("kv_pages.append", lambda t: pages.append(x, x, batch.gpu(), rotary=t, q=x))):
+        with pytest.raises(qa._lib.MXKError, match=f"{name} towards a table's frequencies has no gradient"):
+            call(table)
+        with torch.no_grad():
+            call(table)
+        with torch.autograd.forward_ad.dual_level():
+            dual = qa.rotary_table(torch.autograd.forward_ad.make_dual(freqs, freqs.clone()))
+            with pytest.raises(qa._lib.MXKError, match=f"{name} towards a table's frequencies has no forward-mode"):
+                call(dual)
