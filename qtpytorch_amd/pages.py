@@ -286,6 +286,10 @@ class kv_pages:
         n, _, H, page, D = self.codes.shape
         return self.codes.data_ptr(), self.scales.data_ptr(), n, page, H, D
 
+    def _written(self) -> None:
+        """The pool's tensors count as changed in place, for what autograd has saved of them."""
+        torch.autograd.graph.increment_version((self.codes, self.scales))
+
     def _rows(self, name: str, what: str, x: Tensor, H: int, D: int) -> Tensor:
         """x [tokens, heads, D] with D contiguous; H: heads of keys and values, whose multiple queries have."""
         x = _values(name, x)
@@ -347,6 +351,7 @@ class kv_pages:
                 interleaved, L.ptr(positions), bytes_, axes, L.ptr(out), L.stream_on(gpu))
         if rc:
             L.check(rc, f"kv_pages.append({T} tokens, {H} heads of {D})")
+        self._written()
         return out
 
     def attend(self, q: Tensor, batch: kv_batch, *, mask: Optional[Tensor] = None,
@@ -423,6 +428,7 @@ class kv_pages:
                                            path.shape[1], L.stream_on(gpu))
         if rc:
             L.check(rc, f"kv_pages.keep({tuple(path.shape)})")
+        self._written()
 
     def read(self, batch: kv_batch, tokens: int, dtype: torch.dtype = torch.bfloat16) -> Tuple[Tensor, Tensor]:
         """Keys and values [tokens, heads, head_dim] at positions lengths[b] + i,

@@ -45,6 +45,25 @@ def test_scales_that_need_a_gradient_are_refused(call):
             _calls(qa, qa.kv_pages(codes, dual), batch)[call]()
 
 
+@pytest.mark.parametrize("call", ["append", "keep"])
+def test_a_pool_that_autograd_has_saved_counts_as_changed(call):
+    import qtpytorch_amd as qa
+    batch = R.Batch([5, 20], [2, 1], 16)
+    pages = qa.kv_pages(*(t.cuda() for t in R.pool(batch, 2, 64, poison=False)))
+    w = torch.ones((), device="cuda", requires_grad=True)
+    loss = (w * pages.scales).sum()
+    _calls(qa, pages, batch)[call]()
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    for other in ("attend", "read"):
+        loss = (w * pages.scales).sum()
+        _calls(qa, pages, batch)[other]()
+        loss.backward()
+    with torch.inference_mode():  # tensors without versions
+        pages = qa.kv_pages.empty(4, 16, 2, 64)
+        _calls(qa, pages, batch)[call]()
+
+
 # ---------------------------------------------------------------- a rotary table's tensors
 def _turned(qa, freqs, axis, seed=1):
     x = torch.randn(5, 3, 64, generator=R.gen(seed)).cuda().requires_grad_()
