@@ -268,9 +268,10 @@ class kv_pages:
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_heads: int, head_dim: int, device="cuda") -> "kv_pages":
-        """A pool of its own; what its pages hold before they are written is never attended."""
+        """A pool of its own.  Positions that nothing was stored for read as zeros: a step that is run or recorded
+        ahead of its tokens attends what the pool defines, not what its memory held before."""
         return cls(torch.empty(n_pages, 2, n_heads, page_size, head_dim, dtype=torch.int8, device=device),
-                   torch.empty(n_pages, 2, n_heads, page_size, dtype=torch.float32, device=device))
+                   torch.zeros(n_pages, 2, n_heads, page_size, dtype=torch.float32, device=device))
 
     @property
     def device(self) -> torch.device:

@@ -116,3 +116,63 @@ def test_frequencies_that_need_a_gradient_are_refused():
             dual = qa.rotary_table(torch.autograd.forward_ad.make_dual(freqs, freqs.clone()))
             with pytest.raises(qa._lib.MXKError, match=f"{name} towards a table's frequencies has no forward-mode"):
                 call(dual)
+
+
+# ---------------------------------------------------------------- pools made by empty
+def test_an_empty_pool_reads_as_zeros_whatever_its_memory_held():
+    import qtpytorch_amd as qa
+    n, D = 20000, 64
+    torch.cuda.empty_cache()
+    # blocks of the sizes of the pool's tensors, as the allocator gives them out again
+    before = [torch.full((m,), math.nan, device="cuda") for m in (n * 2 * 16 * D // 4, n * 2 * 16)]
+    del before
+    pages = qa.kv_pages.empty(n, 16, 1, D)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    batch = qa.kv_batch(torch.arange(n, **i32)[None], torch.tensor([0], **i32), torch.tensor([0, 16 * n], **i32))
+    k, v = pages.read(batch, 16 * n, torch.float32)
+    assert not k.any() and not v.any()
+    one = batch._replace(lengths=torch.tensor([16 * n - 1], **i32), offsets=torch.tensor([0, 1], **i32))
+    assert not pages.attend(torch.ones(1, 4, D, device="cuda"), one).any()
+
+
+def test_a_step_in_a_graph_on_pools_with_values():
+    """Recorded once and replayed with other lengths, pages and values over contexts that hold values, eager work between."""
+    import qtpytorch_amd as qa
+    H, G, D, page, B = 2, 2, 128, 16, 3
+    table = qa.rotary_table.make(D)
+    g = R.gen(11)
+    codes = (40 * torch.randn(40, 2, H, page, D, generator=g)).round().clamp(-127, 127).to(torch.int8)
+    scales = (torch.rand(40, 2, H, page, generator=g) + 0.5) / 40
+    pages, other = qa.kv_pages(codes.cuda(), scales.cuda()), qa.kv_pages(codes.cuda(), scales.cuda())
+    batch = qa.kv_batch(torch.zeros(B, 9, **I32).cuda(), torch.zeros(B, **I32).cuda(), torch.arange(B + 1, **I32).cuda())
+    q, k, v = (torch.zeros(B, h, D, dtype=torch.bfloat16).cuda() for h in (H * G, H, H))
+
+    def step(pages):
+        return pages.attend(pages.append(k, v, batch, rotary=table, q=q), batch)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(pages)
+    torch.cuda.current_stream().wait_stream(side)
+    step(other)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(pages)
+    batch.table.copy_(torch.randperm(40, generator=g)[:27].int().view(B, 9))
+    last = None
+    for n in range(6):
+        for t, h in ((q, H * G), (k, H), (v, H)):
+            t.copy_(torch.randn(B, h, D, generator=g).bfloat16())
+        batch.offsets.copy_(torch.tensor([[0, 1, 2, 3], [0, 0, 1, 2], [0, 1, 1, 3]][n % 3], **I32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = held.clone()
+        want = step(other)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(pages.codes, other.codes) and torch.equal(pages.scales, other.scales)
+        rows = int(batch.offsets[-1])
+        assert torch.isfinite(got).all() and (got[:rows] != 0).any(-1).all() and not got[rows:].any()
+        assert last is None or not torch.equal(got, last)
+        last = got
+        batch.lengths.add_(torch.tensor([20, 1, 25], **I32).cuda())
