@@ -20,7 +20,7 @@
 // keys transposes them.  code + 128 in the low byte of a float16 is
 // (code + 128) * 2^-24; one packed fma makes it code * 2^-9, exact.  The
 // probabilities carry the values' scales: p_j * scale_j * 2^(10 - e), e the
-// exponent of the largest scale so far, is at most 2^15, and keeps 11 bits (22
+// exponent of the largest scale that the row has seen so far, is at most 2^15, and keeps 11 bits (22
 // for float32 and float16 queries: a second term) down to 2^-24 of the largest.
 //
 // Work.  The blocks of 128 keys of all sequences, heads and tiles of rows
@@ -373,7 +373,7 @@ template <typename T, int D, int QT, int PT>
 struct TileState {
   f32x4a o[D / 16];  // row lane%16, elements (g*4 + r) * (D/16) + j in o[j][r], times 2^(1 - e)
   float m, l;        // maximum (log2 units), the lane's own sum
-  int e;             // exponent of the largest value scale, wave-uniform
+  int e;             // exponent of the largest value scale that the row sees
 };
 
 template <typename T, int D, int QT, int PT>
@@ -425,10 +425,10 @@ __device__ __forceinline__ void step32(const AttendArgs& A, const i32x4a (&q)[QT
   if (__ballot(top > st.m + 4.0f || eb > st.e)) {
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    int e = eb;
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) e = max(e, __shfl_xor(e, i));
-    e = max(e, st.e);
+    // of the row's own keys: a scale that only other rows see would take its bits from the row's
+    int e = max(eb, st.e);
+    e = max(e, __shfl_xor(e, 16));
+    e = max(e, __shfl_xor(e, 32));
     const float m = fmaxf(st.m, top);
     const float shrink = m == st.m ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
     const float both = shrink * scale_of_exp(st.e - e);
