@@ -61,6 +61,9 @@ struct AttendArgs {
   float* part_o;
   float2* part_s;
   struct PartTile* part_t;
+  // of tiles of many rows, [shares]: bit i (31: any from there on) of the share's tile i whose value scales are too far apart
+  // for a common largest one
+  uint32_t* apart;
 };
 
 struct PartTile {
@@ -366,6 +369,17 @@ __device__ __forceinline__ void load_keys(const KvPool& p, int h, int key, int p
 
 __device__ __forceinline__ float scale_of_exp(int e) {  // 2^e, zero below the normal range
   return e < -126 ? 0.0f : __uint_as_float((uint32_t)(min(e, 127) + 127) << 23);
+}
+
+// Exponent of a scale, -127 of one that is not finite
+__device__ __forceinline__ int scale_exp(float s) {
+  const uint32_t b = mag_bits(s);
+  return (int)((b < 0x7F800000u ? b : 0u) >> 23) - 127;
+}
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) v = max(v, __shfl_xor(v, i));
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
 // One tile over blocks [k0, k1): four waves, 32 keys of a block each
@@ -731,7 +745,7 @@ struct TileLds {
   u32x4 k[2][K * D / 8];  // [key][D] float16, pieces of 8 swizzled
   u32x4 v[2][K * D / 8];  // [row][K keys] float16, pieces of 8 swizzled
   float ks[2][K];    // times the queries' unit
-  float vs[2][K];    // times 2^(10 - e); coarse: float16, times 2^-e, in the order of a lane's weights
+  float vs[2][K];    // times 2^(10 - e); coarse: float16, times 2^-e, in the order of a lane's weights; own: as they are
   int e[2];
   int top[NW];     // exponents of the waves' largest query elements
   uint32_t ok[2];  // bits of the step's runs of 16 keys that have a page; bit 31: a value's scale is not finite
@@ -785,8 +799,16 @@ __device__ __forceinline__ void tile_fetch(const AttendArgs& A, int h, int key, 
   }
 }
 
-template <int D, int NW, bool COARSE>
-__device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>& S, int step, float unit, int& e_run) {
+// Of wave 1, which finds it for all: the exponent of the largest value scale of the tile's keys so far, and one that no
+// row's own largest is below (of the keys that all rows see; if there are none, of the smallest)
+struct ScaleRange {
+  int top, low;
+};
+
+// key: the step's first, bound: the first that not all rows see
+template <int D, int NW, bool COARSE, bool OWN>
+__device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>& S, int step, float unit, int key, int bound,
+                                         ScaleRange& range) {
   using F = Fetched<D, NW>;
   constexpr int K = tile_keys<D>(), RUNS = K / 16;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -824,12 +846,20 @@ __device__ __forceinline__ void tile_put(const Fetched<D, NW>& f, TileLds<D, NW>
   if (wave == 0 && lane < K) S.ks[buf][lane] = f.scale * unit;
   if (wave == 1) {
     const uint32_t bb = mag_bits(f.scale);
-    int top = (int)((bb < 0x7F800000u ? bb : 0u) >> 23) - 127;
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) top = max(top, __shfl_xor(top, i));
-    e_run = max(e_run, top);
+    if constexpr (!OWN) {
+      const int e = scale_exp(f.scale), top = wave_max(e), shared = bound - key;
+      if (shared < K) {
+        if (shared > 0) range.low = max(range.top, wave_max((int)lane < shared ? e : -127));
+        else if (shared + step * K <= 0) range.low = min(range.low, -wave_max(e > -127 ? -e : -127));
+      }
+      range.top = max(range.top, top);
+      if (shared >= K) range.low = range.top;
+    }
+    const int e_run = range.top;
     if (lane < K) {
-      if constexpr (COARSE) {
+      if constexpr (OWN) {
+        S.vs[buf][lane] = f.scale;
+      } else if constexpr (COARSE) {
         // key 32 kt + 8 a + 4 h + r is weight 4 a + r of half h
         const int to = (lane & 32) + (lane >> 2 & 1) * 16 + (lane >> 3 & 3) * 4 + (lane & 3);
         reinterpret_cast<_Float16*>(S.vs[buf])[to] = (_Float16)(f.scale * scale_of_exp(-e_run));
@@ -854,7 +884,7 @@ template <int D>
 struct RowState {
   f32x16a o[D / 32];
   float m, l;
-  int e;
+  int e;  // exponent of the largest value scale: of the tile's keys so far, own: of those that the row sees
 };
 
 // Scores of a wave's 32 rows against a step's keys, but for the row's unit.  The stages' LDS reads are issued
@@ -902,12 +932,21 @@ __device__ __forceinline__ void tile_scores(const TileLds<D, NW>& S, int step, c
 // maximum (half), exponential, conversion (half).  COARSE (bfloat16 results): the probability itself goes to
 // float16, the value's scale is applied to pairs, and the weight is a dot product of pairs with ones, 1.5 where the
 // exact form takes 2.5 with products and sums in float32.
-template <int D, int PT, int NW, bool COARSE>
+// OWN: value scales relative to the largest that the row sees.
+template <int D, int PT, int NW, bool COARSE, bool OWN>
 __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f32x16a (&t)[tile_keys<D>() / 32], bool all,
                                             bool finite, uint64_t see, RowState<D>& st) {
   constexpr int K = tile_keys<D>(), KT = K / 32, N = D / 16;  // N fragments of values for 32 keys
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, buf = step & 1;
-  const int e_new = __builtin_amdgcn_readfirstlane(S.e[buf]);
+  int e_new = OWN ? st.e : __builtin_amdgcn_readfirstlane(S.e[buf]);
+  if constexpr (OWN) {
+#pragma unroll
+    for (int i = 0; i < 16 * KT; ++i) {
+      const int k = (i >> 2) * 8 + (i & 3);
+      if (see >> k & 1) e_new = max(e_new, scale_exp(S.vs[buf][k + h * 4]));
+    }
+    e_new = max(e_new, __shfl_xor(e_new, 32));
+  }
   constexpr float UP = COARSE ? 10.0f : 0.0f;  // log2 of the factor that the exact form has in the values' scales
   const float from = st.m == -__builtin_inff() ? 0.0f : st.m;
 #pragma unroll
@@ -931,7 +970,8 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, t[kt][i]);
   // the running maximum follows the largest score by steps of at least 2^4, as in step32; a row's first score sets it
-  if (__ballot(top > UP + 4.0f || (st.m == -__builtin_inff() && top > -__builtin_inff())) || e_new != st.e) {
+  if (__ballot(top > UP + 4.0f || (st.m == -__builtin_inff() && top > -__builtin_inff())) ||
+      (OWN ? __ballot(e_new != st.e) != 0 : e_new != st.e)) {
     top = fmaxf(top, __shfl_xor(top, 32));
     const bool first = st.m == -__builtin_inff();
     const float rise = first ? (top > -__builtin_inff() ? top - UP : 0.0f) : fmaxf(top - UP, 0.0f);
@@ -962,6 +1002,12 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
 #pragma unroll
       for (int x = 0; x < 4; ++x) vs[x] = *reinterpret_cast<const f32x4a*>(&S.vs[buf][kt * 32 + x * 8 + h * 4]);
     }
+    if constexpr (OWN) {
+      const float up = scale_of_exp(10 - st.e);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)  // what the row does not see may be past its own
+        vs[i >> 2][i & 3] = (uint32_t)(see >> (32 * kt)) >> (8 * (i >> 2) + (i & 3)) & 1 ? vs[i >> 2][i & 3] * up : 0.0f;
+    }
     if constexpr (COARSE) {
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
@@ -982,7 +1028,7 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
         if constexpr (PT == 2) p[kt][1][i >> 3][i & 7] = (_Float16)(c - (float)p[kt][0][i >> 3][i & 7]);
       }
     }
-    if (!finite) {  // zero times such a scale: what a row does not see adds nothing to it all the same
+    if (!OWN && !finite) {  // zero times such a scale: what a row does not see adds nothing to it all the same
 #pragma unroll
       for (int n = 0; n < PT; ++n)
 #pragma unroll
@@ -1038,29 +1084,48 @@ __device__ __forceinline__ uint64_t row_sees(const AttendArgs& A, const uint64_t
 template <int D>
 __device__ __forceinline__ int tile_part(int wave, int a, int lane) { return ((wave * (D / 32) + a) * 256 + lane) * 4; }
 
-template <typename T, int D, int QT, int PT, int NW>
+// The value scales of a tile's keys are taken relative to one exponent, which costs a row bits where its own largest scale is
+// far below it: keys that it does not see must not do that.  The first launch (not OWN) notes tiles where a row's own may be
+// below 2^-4 of the largest; a second one computes these again with an exponent for each row, in the exact form for
+// bfloat16 too, and ends at once where there are none.  Both forms in one kernel cost it registers: 16 trees of 16 tokens with 8
+// queries a head behind 4000 keys 71 us without, 73 in two launches, 77 in one; 4 of 64 tokens behind 30000 180, 189, 195.
+template <typename T, int D, int QT, int PT, int NW, bool OWN>
 __global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend_tile(AttendArgs A) {
   constexpr int K = tile_keys<D>(), RUNS = K / 16, BATCH = 64 / RUNS;  // runs of a step, steps of a batch of pages
-  constexpr bool COARSE = __is_same(T, hip_bfloat16);
+  constexpr bool COARSE = __is_same(T, hip_bfloat16) && !OWN;
   __shared__ TileLds<D, NW> S;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
   const int share = share_of_block(A);
   const Line L = make_line(A);
-  zero_padding<T, D, 64 * NW>(A);
+  uint32_t apart = 0;  // OWN: the share's tiles to compute; else found by wave 1
+  if constexpr (OWN) {
+    apart = A.apart[share];
+    if (apart == 0) return;
+  } else {
+    zero_padding<T, D, 64 * NW>(A);
+  }
   uint32_t from, to, per;
   SeqWork w;
   Place p;
   if (!line_share<64 * NW>(A, L, share, from, to, per, w, p)) {
-    leave_part(A, share, false, 0, 1, w, p);
+    if constexpr (!OWN) {
+      leave_part(A, share, false, 0, 1, w, p);
+      if (threadIdx.x == 0) A.apart[share] = 0;
+    }
     return;
   }
   uint32_t at = from;
-  while (true) {
+  for (int tile = 0;; tile = min(tile + 1, 31)) {
     const int k1 = (int)min((uint32_t)p.blocks, (uint32_t)p.k + (to - at));
     const bool whole = p.k == 0 && k1 == p.blocks;
     const int end = tile_end(A, w, p);
     const int key0 = p.k * A.keys, stop = (int)min((int64_t)end, (int64_t)k1 * A.keys);
+    if (OWN && !(apart >> tile & 1)) {
+      at += (uint32_t)(k1 - p.k);
+      if (at >= to || !next_tile(A, L, w, p)) break;
+      continue;
+    }
     RunPages pages;
     pages.start(A, p.b, key0 >> 4);
     int tok, head;
@@ -1088,7 +1153,9 @@ __global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend
     st.m = -__builtin_inff();
     st.l = 0.0f;
     st.e = -100;
-    int e_run = -100;  // of wave 1, which finds the exponent for all
+    // keys in front of this one are seen by all rows: the ones held, causal also those up to the tile's first token
+    const int bound = A.mask ? w.ctx : w.ctx + min(end - w.ctx, p.x / A.chunks * A.TT + 1);
+    ScaleRange range = {-100, 127};
     Fetched<D, NW> f;
     const int steps = stop > key0 ? (stop - key0 + K - 1) / K : 0;
     auto fetch = [&](int n) {
@@ -1106,7 +1173,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend
     f16x8a q[QT][D / 16];
     query_terms16<T, D, QT>(raw, e_q, q);
     const float unit = scale_of_exp(e_q - 14 + 9) * A.scale;  // of a product of a query's terms and a key's code * 2^-9
-    if (steps) tile_put<D, NW, COARSE>(f, S, 0, unit, e_run);
+    if (steps) tile_put<D, NW, COARSE, OWN>(f, S, 0, unit, key0, bound, range);
     __syncthreads();
     fetch(1);
     for (int n = 0; n < steps; ++n) {
@@ -1119,9 +1186,9 @@ __global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend
                          (j0 + K <= 0 || (!A.mask && j0 + K - 1 <= lo_tok));
         uint64_t see = ~0ull;
         if (!all) see = row_sees<K>(A, bits, key, w.ctx, end, tok, ok) >> (4 * h);
-        tile_values<D, PT, NW, COARSE>(S, n, t, all, ok >> 31 == 0, see, st);
+        tile_values<D, PT, NW, COARSE, OWN>(S, n, t, all, ok >> 31 == 0, see, st);
       }
-      if (n + 1 < steps) tile_put<D, NW, COARSE>(f, S, n + 1, unit, e_run);
+      if (n + 1 < steps) tile_put<D, NW, COARSE, OWN>(f, S, n + 1, unit, key0 + (n + 1) * K, bound, range);
       __syncthreads();
       fetch(n + 2);
     }
@@ -1155,11 +1222,15 @@ __global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend
       }
       if (!whole && h == 0) A.part_s[slot * (32 * NW) + wave * 32 + l32] = make_float2(st.m, l);
     }
+    if (!OWN && wave == 1 && range.top > range.low + 4) apart |= 1u << tile;
     at += (uint32_t)(k1 - p.k);
     const bool some = p.k == 0 && k1 < p.blocks;  // then at >= to
     const uint32_t last = at + (uint32_t)(p.blocks - k1);
     if (at >= to || !next_tile(A, L, w, p)) {
-      leave_part(A, share, some, last, per, w, p);
+      if constexpr (!OWN) {
+        leave_part(A, share, some, last, per, w, p);
+        if (threadIdx.x == 64) A.apart[share] = apart;
+      }
       break;
     }
   }
@@ -1328,9 +1399,11 @@ static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int
   return a;
 }
 
+static bool has_parts(const AttendPlan& a) { return a.cut && a.shares > 1; }
+
 static size_t attend_bytes(const AttendPlan& a, int D) {
-  if (!a.cut || a.shares == 1) return 0;
-  return (size_t)a.shares * (2 * (size_t)a.rows * ((size_t)D * 4 + sizeof(float2)) + sizeof(PartTile));
+  return (size_t)a.shares * ((has_parts(a) ? 2 * (size_t)a.rows * ((size_t)D * 4 + sizeof(float2)) + sizeof(PartTile) : 0) +
+                             (a.rows > 16 ? sizeof(uint32_t) : 0));
 }
 
 template <typename T, int D, int QT, int PT>
@@ -1339,12 +1412,15 @@ static int launch_attend(const AttendArgs& A, const AttendPlan& a, hipStream_t s
   if (a.rows == 16) {
     hipLaunchKernelGGL((k_attend<T, D, QT, PT>), dim3(a.shares), dim3(256), 0, st, A);
   } else if (a.rows == 128) {
-    hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 4>), dim3(a.shares), dim3(256), 0, st, A);
+    hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 4, false>), dim3(a.shares), dim3(256), 0, st, A);
+    hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 4, true>), dim3(a.shares), dim3(256), 0, st, A);
   } else {
-    if constexpr (D < 256 && QH == 1)
-      hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 8>), dim3(a.shares), dim3(512), 0, st, A);
+    if constexpr (D < 256 && QH == 1) {
+      hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 8, false>), dim3(a.shares), dim3(512), 0, st, A);
+      hipLaunchKernelGGL((k_attend_tile<T, D, QH, QH, 8, true>), dim3(a.shares), dim3(512), 0, st, A);
+    }
   }
-  if (a.cut && a.shares > 1) {
+  if (has_parts(a)) {
     if (a.rows == 16) hipLaunchKernelGGL((k_attend_join<T, D>), dim3(a.shares - 1, 4), dim3(256), 0, st, A);
     else hipLaunchKernelGGL((k_attend_join_tile<T, D>), dim3(a.shares - 1, a.rows * D / 4096), dim3(256), 0, st, A);
   }
@@ -1425,9 +1501,11 @@ int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_he
   A.most = a.most;
   A.rows = a.rows;
   A.shares = a.shares;
-  A.part_o = need ? reinterpret_cast<float*>(workspace) : nullptr;
-  A.part_s = need ? reinterpret_cast<float2*>(A.part_o + part * D) : nullptr;
-  A.part_t = need ? reinterpret_cast<PartTile*>(A.part_s + part) : nullptr;
+  const bool parts = has_parts(a);
+  A.part_o = parts ? reinterpret_cast<float*>(workspace) : nullptr;
+  A.part_s = parts ? reinterpret_cast<float2*>(A.part_o + part * D) : nullptr;
+  A.part_t = parts ? reinterpret_cast<PartTile*>(A.part_s + part) : nullptr;
+  A.apart = reinterpret_cast<uint32_t*>(parts ? static_cast<void*>(A.part_t + a.shares) : workspace);
   if (q_type == MXK_IN_F32) return launch_attend_d<float, 3, 2>(D, A, a, st);
   if (q_type == MXK_IN_F16) return launch_attend_d<__half, 2, 2>(D, A, a, st);
   return launch_attend_d<hip_bfloat16, 2, 1>(D, A, a, st);

@@ -56,7 +56,19 @@ def test_probabilities_of_few_rows_keep_22_bits(group, dtype):
 
 
 # ---------------------------------------------------------------- large scales of keys that a row does not see
-def _check_unseen(group, masked, factor, dim, dtype):
+def _coarse(batch, scales, mask, head=0):
+    """What bfloat16 rows of large tiles may be off beside R.attend's error: a value's scale is a float16 there, relative
+    to 2^e, e up to 4 above the exponent of the largest that the row sees: half a step of the smallest ones is 2^-25 * 2^e,
+    at most 2^-21 of that largest scale, times a code of 127; the weights sum to 1."""
+    out = torch.zeros(batch.tokens, 1, 1, dtype=torch.float64)
+    for b, (h, n) in enumerate(zip(batch.held, batch.new)):
+        where = [batch.place(b, at) for at in range(h + n)]
+        vs = torch.tensor([float(scales[page, 1, head, off]) for page, off in where], dtype=torch.float64)
+        out[batch.first[b]:batch.first[b] + n, 0, 0] = torch.where(R.seen(batch, b, mask), vs, 0.0).amax(1)
+    return 127 * 2.0 ** -21 * out
+
+
+def _check_unseen(group, masked, factor, dim, dtype, large=False):
     """A new token's values are larger than all others by a factor: the rows that do not see it, before it or on
     other branches of a tree, keep what they have without it, and the other rows are within their own bounds."""
     import qtpytorch_amd as qa
@@ -71,6 +83,8 @@ def _check_unseen(group, masked, factor, dim, dtype):
     q = torch.randn(batch.tokens, group, dim, generator=R.gen(7)).to(dtype)
     got = _pages(codes, scales).attend(q.cuda(), batch.gpu(), mask=None if mask is None else mask.cuda())
     want, error = R.attend(batch, codes, scales, q, mask)
+    if large and dtype == torch.bfloat16:
+        error = error + _coarse(batch, scales, mask)
     sees = torch.zeros(batch.tokens, dtype=torch.bool)
     for b, i in ((0, 2), (1, 1)):
         sees[batch.first[b]:batch.first[b] + batch.new[b]] = R.seen(batch, b, mask)[:, batch.held[b] + i]
@@ -90,3 +104,110 @@ def _check_unseen(group, masked, factor, dim, dtype):
 def test_values_that_a_row_does_not_see_take_no_bits_from_it(group, masked, factor, dim, dtype):
     """Tiles of 16 rows."""
     _check_unseen(group, masked, factor, dim, dtype)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("factor", [6.0, 32.0, 1e6, 1e12, 1e36])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("group", [16, 26, 60])
+def test_values_that_a_row_of_a_large_tile_does_not_see_take_no_bits_from_it(group, masked, factor, dim, dtype):
+    """Tiles of 128 and of 256 rows."""
+    _check_unseen(group, masked, factor, dim, dtype, large=True)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 4), (256, 2)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_values_of_growing_sizes(masked, dim, group, dtype):
+    """A prompt whose tokens' values grow by steps from 2^-60 to 2^60, the sequence's own or a tree's: every row is
+    within the bounds of what it sees itself, over several steps and tiles."""
+    batch = R.Batch([0, 30], [150, 90], 16)
+    codes, scales = R.pool(batch, 1, dim, 1)
+    for b, n in enumerate(batch.new):
+        for i in range(n):
+            page, off = batch.place(b, batch.held[b] + i)
+            scales[page, 1, :, off] *= 2.0 ** (12 * (i // 15) - 60)
+    mask = None
+    if masked:
+        mask = torch.zeros(batch.tokens, 3, dtype=torch.int64)
+        for b, n in enumerate(batch.new):
+            for i in range(n):
+                for j in {i, i // 2, i // 3, max(0, i - 40), (7 * i) % n}:  # also tokens behind it
+                    mask[batch.first[b] + i, j // 64] |= (1 << (j % 64)) if j % 64 < 63 else -(1 << 63)
+    q = torch.randn(batch.tokens, group, dim, generator=R.gen(7)).to(dtype)
+    if dtype == torch.float16:
+        scales[:, 1] *= 2.0 ** -50  # below its largest
+    want, error = R.attend(batch, codes, scales, q, mask)
+    if dtype == torch.bfloat16:
+        error = error + _coarse(batch, scales, mask)
+    got = _pages(codes, scales).attend(q.cuda(), batch.gpu(), mask=None if mask is None else mask.cuda())
+    R.near(got, want, error)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("group", [3, 12])
+def test_values_far_apart_in_tiles_that_are_cut(group, masked, dtype):
+    """Several tiles a workgroup and several workgroups a tile, some of whose tiles have such a token."""
+    batch = R.Batch([1100, 300, 0], [90, 40, 70], 16, front=2, back=3)
+    codes, scales = R.pool(batch, 2, 64, 1)
+    for b, i, size in ((0, 50, 1e7), (0, 77, 1e15), (1, 20, 1e5), (2, 3, 1e20)):
+        page, off = batch.place(b, batch.held[b] + i)
+        scales[page, 1, 1, off] *= size if dtype != torch.float16 else size ** 0.1
+    mask = None
+    if masked:
+        mask = torch.randint(-(1 << 62), 1 << 62, (batch.tokens, 2), generator=R.gen(3))
+    q = torch.randn(batch.tokens, 2 * group, 64, generator=R.gen(7)).to(dtype)
+    want, error = R.attend(batch, codes, scales, q, mask)
+    if dtype == torch.bfloat16:
+        for head in range(2):
+            error[:, head * group:(head + 1) * group] += _coarse(batch, scales, mask, head)
+    got = _pages(codes, scales).attend(q.cuda(), batch.gpu(), mask=None if mask is None else mask.cuda())
+    R.near(got, want, error)
+
+
+def test_values_far_apart_in_many_tiles_of_a_workgroup():
+    """More tiles a workgroup than it has bits for: the first of two new tokens sees itself alone, and so gives its value."""
+    import qtpytorch_amd as qa
+    n, G, D = 9000, 50, 64
+    i32 = dict(dtype=torch.int32, device="cuda")
+    pages = qa.kv_pages.empty(n, 16, 1, D)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pages.codes.copy_(torch.randint(-127, 128, pages.codes.shape, generator=g, device="cuda", dtype=torch.int8))
+    pages.scales.copy_(torch.rand(pages.scales.shape, generator=g, device="cuda") + 0.5)
+    pages.scales[::3, 1, :, 1] *= 1e12
+    batch = qa.kv_batch(torch.arange(n, **i32)[:, None].contiguous(), torch.zeros(n, **i32), torch.arange(0, 2 * n + 1, 2, **i32))
+    q = torch.randn(2 * n, G, D, generator=g, device="cuda")
+    got = pages.attend(q, batch)[::2]
+    want = (pages.codes[:, 1, 0, 0].float() * pages.scales[:, 1, 0, :1])[:, None]
+    # one probability of 1 in two terms of 11 bits, and the division
+    assert ((got - want).abs() <= 2.0 ** -20 * want.abs()).all()
+
+
+def test_values_far_apart_come_and_go_in_a_graph():
+    """A recorded call replayed where its tokens' values are far apart and where they are not."""
+    import qtpytorch_amd as qa
+    batch = R.Batch([70, 20], [30, 25], 16)
+    codes, scales = R.pool(batch, 1, 64, 1)
+    pages, gb = _pages(codes, scales), batch.gpu()
+    q = torch.randn(batch.tokens, 8, 64, generator=R.gen(7)).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        pages.attend(q, gb)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = pages.attend(q, gb)
+    page, off = batch.place(0, 70 + 11)
+    for factor in (1.0, 1e9, 1.0, 1e-9, 1e18, 1.0):
+        now = scales.clone()
+        now[page, 1, 0, off] *= factor
+        pages.scales.copy_(now)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = held.clone()
+        assert torch.equal(got, pages.attend(q, gb))
+        want, error = R.attend(batch, codes, now, q.cpu())
+        R.near(got, want, error)
