@@ -61,8 +61,8 @@ struct AttendArgs {
   float* part_o;
   float2* part_s;
   struct PartTile* part_t;
-  // of tiles of many rows, [shares]: bit i (31: any from there on) of the share's tile i whose value scales are too far apart
-  // for a common largest one
+  // of tiles of many rows, [shares]: bit i (31: any from there on) of the share's tile i whose value scales or queries are
+  // too far apart for a common largest one
   uint32_t* apart;
 };
 
@@ -669,7 +669,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
 // meets itself in a bank.
 //
 // Roundings: a query is one float16 term (two for float32), which holds
-// float16 and bfloat16 queries whole as far as the tile's largest element allows;
+// float16 and bfloat16 queries whole as far as the tile's largest element allows (a row of less than 2^-8 of
+// it is computed by its own, k_attend_tile);
 // probabilities times the values' scales are one float16 term (two for
 // float32), 2^-11 of a weight.  For bfloat16 the probability and the scale go to
 // float16 before their product (three roundings of 2^-11 against the result's 2^-8), and a
@@ -744,10 +745,10 @@ struct TileLds {
   static constexpr int K = tile_keys<D>();
   u32x4 k[2][K * D / 8];  // [key][D] float16, pieces of 8 swizzled
   u32x4 v[2][K * D / 8];  // [row][K keys] float16, pieces of 8 swizzled
-  float ks[2][K];    // times the queries' unit
+  float ks[2][K];    // times the queries' unit (own: but for the row's exponent)
   float vs[2][K];    // times 2^(10 - e); coarse: float16, times 2^-e, in the order of a lane's weights; own: as they are
   int e[2];
-  int top[NW];     // exponents of the waves' largest query elements
+  int top[NW], low[NW];  // exponents of the waves' largest query elements: of all rows, the smallest of a row's own
   uint32_t ok[2];  // bits of the step's runs of 16 keys that have a page; bit 31: a value's scale is not finite
 };
 
@@ -932,10 +933,10 @@ __device__ __forceinline__ void tile_scores(const TileLds<D, NW>& S, int step, c
 // maximum (half), exponential, conversion (half).  COARSE (bfloat16 results): the probability itself goes to
 // float16, the value's scale is applied to pairs, and the weight is a dot product of pairs with ones, 1.5 where the
 // exact form takes 2.5 with products and sums in float32.
-// OWN: value scales relative to the largest that the row sees.
+// OWN: value scales relative to the largest that the row sees, scores times the row's own unit.
 template <int D, int PT, int NW, bool COARSE, bool OWN>
 __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f32x16a (&t)[tile_keys<D>() / 32], bool all,
-                                            bool finite, uint64_t see, RowState<D>& st) {
+                                            bool finite, uint64_t see, float own_unit, RowState<D>& st) {
   constexpr int K = tile_keys<D>(), KT = K / 32, N = D / 16;  // N fragments of values for 32 keys
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5, buf = step & 1;
   int e_new = OWN ? st.e : __builtin_amdgcn_readfirstlane(S.e[buf]);
@@ -955,7 +956,9 @@ __device__ __forceinline__ void tile_values(const TileLds<D, NW>& S, int step, f
     for (int a = 0; a < 4; ++a) {
       const f32x4a ks = *reinterpret_cast<const f32x4a*>(&S.ks[buf][kt * 32 + a * 8 + h * 4]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t[kt][4 * a + r] = __builtin_fmaf(t[kt][4 * a + r], ks[r], UP - from);
+      for (int r = 0; r < 4; ++r)
+        t[kt][4 * a + r] = OWN ? __builtin_fmaf(t[kt][4 * a + r] * ks[r], own_unit, UP - from)
+                               : __builtin_fmaf(t[kt][4 * a + r], ks[r], UP - from);
     }
   if (!all) {
 #pragma unroll
@@ -1085,8 +1088,8 @@ template <int D>
 __device__ __forceinline__ int tile_part(int wave, int a, int lane) { return ((wave * (D / 32) + a) * 256 + lane) * 4; }
 
 // The value scales of a tile's keys are taken relative to one exponent, which costs a row bits where its own largest scale is
-// far below it: keys that it does not see must not do that.  The first launch (not OWN) notes tiles where a row's own may be
-// below 2^-4 of the largest; a second one computes these again with an exponent for each row, in the exact form for
+// far below it: keys that it does not see must not do that.  So are the queries of a tile's rows.  The first launch (not OWN)
+// notes tiles where a row's own may be below 2^-4 of the largest scale, or its query below 2^-8 of the largest; a second one computes these again with an exponent for each row, in the exact form for
 // bfloat16 too, and ends at once where there are none.  Both forms in one kernel cost it registers: 16 trees of 16 tokens with 8
 // queries a head behind 4000 keys 71 us without, 73 in two launches, 77 in one; 4 of 64 tokens behind 30000 180, 189, 195.
 template <typename T, int D, int QT, int PT, int NW, bool OWN>
@@ -1138,6 +1141,11 @@ __global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend
     int e_q = raw.e;
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) e_q = max(e_q, __shfl_xor(e_q, i));
+    int e_low = raw.some ? raw.e : 127;
+    if constexpr (!OWN) {
+#pragma unroll
+      for (int i = 1; i < 32; i <<= 1) e_low = min(e_low, __shfl_xor(e_low, i));
+    }
     const uint64_t* bits = A.mask && row_ok ? A.mask + (int64_t)(w.first + tok) * A.words : A.mask;
     // the wave's first token: it sees all keys up to it, and a causal step past it needs its mask
     int lo_tok = row_ok ? tok : 0x7FFFFFFF;
@@ -1165,14 +1173,16 @@ __global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend
     };
     fetch(0);
     __syncthreads();  // the tile before is read
-    if (lane == 0) S.top[wave] = e_q;
+    if (lane == 0) S.top[wave] = e_q, S.low[wave] = e_low;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NW; ++i) e_q = max(e_q, S.top[i]);
+    for (int i = 0; i < NW; ++i) e_q = max(e_q, S.top[i]), e_low = min(e_low, S.low[i]);
     e_q = __builtin_amdgcn_readfirstlane(e_q);
+    if (!OWN && __builtin_amdgcn_readfirstlane(e_low) < e_q - 8) apart |= 1u << tile;
     f16x8a q[QT][D / 16];
-    query_terms16<T, D, QT>(raw, e_q, q);
-    const float unit = scale_of_exp(e_q - 14 + 9) * A.scale;  // of a product of a query's terms and a key's code * 2^-9
+    query_terms16<T, D, QT>(raw, OWN ? raw.e : e_q, q);
+    // of a product of a query's terms and a key's code * 2^-9
+    const float unit = OWN ? 0x1p-5f * A.scale : scale_of_exp(e_q - 14 + 9) * A.scale, own_unit = OWN ? scale_of_exp(raw.e) : 0.0f;
     if (steps) tile_put<D, NW, COARSE, OWN>(f, S, 0, unit, key0, bound, range);
     __syncthreads();
     fetch(1);
@@ -1186,7 +1196,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend
                          (j0 + K <= 0 || (!A.mask && j0 + K - 1 <= lo_tok));
         uint64_t see = ~0ull;
         if (!all) see = row_sees<K>(A, bits, key, w.ctx, end, tok, ok) >> (4 * h);
-        tile_values<D, PT, NW, COARSE, OWN>(S, n, t, all, ok >> 31 == 0, see, st);
+        tile_values<D, PT, NW, COARSE, OWN>(S, n, t, all, ok >> 31 == 0, see, own_unit, st);
       }
       if (n + 1 < steps) tile_put<D, NW, COARSE, OWN>(f, S, n + 1, unit, key0 + (n + 1) * K, bound, range);
       __syncthreads();

@@ -372,8 +372,8 @@ class kv_pages:
         few rows a head (64 on average; 96 in float32), q keeps 16
         bits of its row's largest element (24 in float32), and a probability times
         its value's scale 11 bits (22 in float32 and float16) down to 2^-24 of
-        the largest that the row sees.  Else q's elements keep 11 bits (22 in float32) down to 2^-28 of
-        the largest of 128 or 256 rows, and those products 11 (22 in float32) down to 2^-20, in bfloat16 with two
+        the largest that the row sees.  Else q's elements keep 11 bits (22 in float32) down to 2^-20 of
+        their row's largest, and those products 11 (22 in float32) down to 2^-20, in bfloat16 with two
         roundings more and down to 2^-10.  Nothing is differentiable, as in append."""
         codes, scales, n, page, H, D = self._pool("kv_pages.attend")
         q = self._rows("kv_pages.attend", "q", q, H, D)

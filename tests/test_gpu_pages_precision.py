@@ -211,3 +211,24 @@ def test_values_far_apart_come_and_go_in_a_graph():
         assert torch.equal(got, pages.attend(q, gb))
         want, error = R.attend(batch, codes, now, q.cpu())
         R.near(got, want, error)
+
+
+# ---------------------------------------------------------------- large queries in other rows
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group", [3, 40, 80])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("size", [1e5, 1e12, 1e30])
+def test_queries_of_other_rows_take_no_bits_from_a_row(size, dim, group, dtype):
+    """One row's query is larger than the others' by far: theirs keep their own precision."""
+    batch = R.Batch([300, 40], [2, 3], 16)
+    codes, scales = R.pool(batch, 1, dim)
+    q = torch.randn(5, group, dim, generator=R.gen(1))
+    q[0, 1] *= size
+    q[4, 0] *= size
+    q = q.to(dtype)
+    want, error = R.attend(batch, codes, scales, q)
+    rows = torch.ones(5, group, dtype=torch.bool)
+    rows[0, 1] = rows[4, 0] = False
+    got = _pages(codes, scales).attend(q.cuda(), batch.gpu())
+    R.near(got[rows.cuda()], want[rows], error[rows])
+    assert torch.isfinite(got).all()
