@@ -1388,11 +1388,16 @@ static AttendPlan plan_attend(int64_t T, int64_t B, int64_t width, int page, int
   // rows of a sequence and key head, on average
   const double each = B > 0 ? (double)T * G / (double)std::min(B, T) : 0.0;
   // Tiles of 16 rows, whose waves need no barrier, though several of them read the same keys from the L2, then of 128 (two
-  // workgroups a CU but for float32 and heads of 256), then of 256.  16 sequences of 4000 keys, 8 heads of 128, bfloat16,
-  // us by tiles of 16 / 128 / 256: 64 rows 66 / - / 84, 96 rows 102 / 69 / 85, 128 rows 122 / 70 / 86, 192 rows 181 / - / 97;
-  // 2 sequences of 60000: 64 rows 118 / - / 152, 128 rows 229 / 128 / 151; 16 of 300: 96 rows 33 / 30 / 25.  float32 by 16 /
-  // 128: 96 rows of 4000 keys 113 / 122, of 60000 180 / 220, 128 rows 136 / 132; heads of 256: 64 rows 141 / 189, 96 rows 208 / 190.
-  a.rows = each <= (wide ? 96 : 64) ? 16 : D == 256 || wide || each <= 128 ? 128 : 256;
+  // workgroups a CU but for float32 and heads of 256), then of 256.  us by tiles of 16 / 128 / 256, 8 heads with 4 queries each:
+  // heads of 128, bfloat16, 16 sequences of 4000 keys: 48 rows 75 / 66 / 88, 64 rows 70 / 66 / 89, 80 rows 109 / 71 / 88, 128 rows
+  // 127 / 74 / 89, 160 rows 161 / 113 / 93, 192 rows 178 / 112 / 98; 2 of 60000: 64 rows 128 / 114 / 157, 80 rows 147 / 124 / 158, 128
+  // rows 224 / 129 / 156, 160 rows 265 / 199 / 163; 16 of 300: 48 rows 17 / 28 / 24, 64 rows 18 / 30 / 26, 80 rows 31 / 32 / 27, 128 rows
+  // 29 / 35 / 30.  float32 by 16 / 128, 4000 keys: 80 rows 110 / 124, 96 rows 104 / 126, 112 rows 148 / 126, 128 rows 125 / 129; 60000: 96
+  // rows 174 / 220, 112 rows 254 / 225.  Heads of 256, bfloat16 by 16 / 128, 4000 keys: 64 rows 125 / 197, 80 rows 199 / 198, 96 rows
+  // 182 / 199, 112 rows 272 / 201; 60000: 80 rows 420 / 360, 96 rows 334 / 360, 112 rows 559 / 363; float32, 4000 keys: 80 rows 201 / 249, 96
+  // rows 204 / 248, 112 rows 275 / 251.
+  // (Up to 64 rows short contexts would lose more by 128 than long ones win.)
+  a.rows = each <= (wide || D == 256 ? 96 : 64) ? 16 : D == 256 || wide || each <= 128 ? 128 : 256;
   a.keys = a.rows == 16 ? 128 : 256;
   a.GC = std::min(G, a.rows);
   a.chunks = (int)ceil_div(G, a.GC);
