@@ -379,7 +379,7 @@ __device__ __forceinline__ int scale_exp(float s) {
 __device__ __forceinline__ int wave_max(int v) {
 #pragma unroll
   for (int i = 1; i < 64; i <<= 1) v = max(v, __shfl_xor(v, i));
-  return __builtin_amdgcn_readfirstlane(v);
+  return v;
 }
 
 // One tile over blocks [k0, k1): four waves, 32 keys of a block each
