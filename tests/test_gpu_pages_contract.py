@@ -176,3 +176,71 @@ def test_a_step_in_a_graph_on_pools_with_values():
         assert last is None or not torch.equal(got, last)
         last = got
         batch.lengths.add_(torch.tensor([20, 1, 25], **I32).cuda())
+
+
+# ---------------------------------------------------------------- calls that the documentation allows
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_page_in_several_tables(new):
+    """Two sequences that share a prefix's pages read and attend as two with pages of their own."""
+    import qtpytorch_amd as qa
+    own = R.Batch([96, 96], [new, new], 16)
+    codes, scales = R.pool(own, 2, 64, poison=False)
+    for i in range(6):  # the prefix's six pages have the same contents in both
+        codes[own.table[1, i]], scales[own.table[1, i]] = codes[own.table[0, i]], scales[own.table[0, i]]
+    pages = qa.kv_pages(codes.cuda(), scales.cuda())
+    q = torch.randn(2 * new, 6, 64, generator=R.gen(1)).cuda()
+    batch = own.gpu()
+    shared = batch.table.clone()
+    shared[1, :6] = shared[0, :6]
+    both = batch._replace(table=shared)
+    assert torch.equal(pages.attend(q, batch), pages.attend(q, both))
+    whole = dict(lengths=torch.zeros(2, **I32).cuda(), offsets=torch.tensor([0, 96 + new, 2 * (96 + new)], **I32).cuda())
+    one, two = (pages.read(b._replace(**whole), 2 * (96 + new)) for b in (batch, both))
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+def test_packed_keys_values_and_queries_are_their_values():
+    import qtpytorch_amd as qa
+    batch = R.Batch([5, 20], [2, 3], 16)
+    k, v, q = (qa.mx_tensor.quantize(torch.randn(5, h, 64, generator=R.gen(h)).cuda(), "int8d") for h in (2, 2, 6))
+    table = qa.rotary_table.make(64)
+    one, two = (qa.kv_pages(*(t.cuda() for t in R.pool(batch, 2, 64, poison=False))) for _ in range(2))
+    a = one.append(k, v, batch.gpu(), rotary=table, q=q)
+    b = two.append(k.dequantize(), v.dequantize(), batch.gpu(), rotary=table, q=q.dequantize())
+    assert torch.equal(a, b) and torch.equal(one.codes, two.codes) and torch.equal(one.scales, two.scales)
+    assert torch.equal(one.attend(q, batch.gpu()), one.attend(q.dequantize(), batch.gpu()))
+
+
+@pytest.mark.parametrize("group", [2, 40])
+def test_masks_of_any_strides(group):
+    import qtpytorch_amd as qa
+    batch = R.Batch([30, 7], [9, 9], 16)
+    pages = qa.kv_pages(*(t.cuda() for t in R.pool(batch, 1, 64)))
+    q = torch.randn(18, group, 64, generator=R.gen(1)).cuda()
+    mask = torch.randint(-(1 << 62), 1 << 62, (18, 2), generator=R.gen(2)).cuda()
+    wide = torch.zeros(18, 5, dtype=torch.int64).cuda()
+    wide[:, 1::2] = mask
+    want = pages.attend(q, batch.gpu(), mask=mask)
+    assert torch.equal(pages.attend(q, batch.gpu(), mask=wide[:, 1::2]), want)
+    assert torch.equal(pages.attend(q, batch.gpu(), mask=mask.t().contiguous().t()), want)
+    row = mask[:1]
+    assert torch.equal(pages.attend(q, batch.gpu(), mask=row.expand(18, 2)), pages.attend(q, batch.gpu(), mask=row.repeat(18, 1)))
+
+
+@pytest.mark.parametrize("group", [2, 40])
+def test_two_streams_at_once_over_one_pool(group):
+    import qtpytorch_amd as qa
+    batch = R.Batch([3000, 40, 700], [5, 1, 3], 16)
+    pages = qa.kv_pages(*(t.cuda() for t in R.pool(batch, 2, 64)))
+    gb = batch.gpu()
+    q = [torch.randn(9, 2 * group, 64, generator=R.gen(i)).cuda() for i in range(2)]
+    want = [pages.attend(x, gb) for x in q]
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in q]
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(side):
+            with torch.cuda.stream(s):
+                got[i].append(pages.attend(q[i], gb))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for many, w in zip(got, want) for g in many)
