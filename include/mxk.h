@@ -578,7 +578,8 @@ int mxk_kv_pages_read(const void* codes, const float* scales, int64_t pages, int
                       const int32_t* table, const int32_t* lengths, const int32_t* offsets, int64_t B, int64_t width,
                       int64_t tokens, int y_type, void* k, void* v, void* stream);
 
-/* Workspace bytes (16-byte aligned) mxk_kv_pages_attend needs (0 if none). */
+/* Workspace bytes (16-byte aligned) mxk_kv_pages_attend needs (0 if none).  A
+ * call's own: nothing is kept in it from one call for the next. */
 size_t mxk_kv_pages_attend_workspace(int q_type, int64_t tokens, int64_t B, int64_t width, int page, int heads,
                                      int q_heads, int D);
 
@@ -587,8 +588,15 @@ size_t mxk_kv_pages_attend_workspace(int q_type, int64_t tokens, int64_t B, int6
  * are in the pages already) those up to itself, or with mask (uint64
  * [tokens][words]) those whose bit j its words have.  Query head i reads head
  * i / (q_heads / heads).  Rows that see nothing, and tokens of no sequence, are
- * zeros; a row of q with a NaN or an infinity that sees a key is NaN.  Scores
- * and sums float32, probabilities 11 significant bits (22 for float32 q). */
+ * zeros; a row of q with a NaN or an infinity that sees a key is NaN.
+ * Scores, maxima and sums are float32.  Significant bits of what enters the
+ * products, where tokens * q_heads / heads is at most 64 for each of min(B, tokens)
+ * sequences (96 for float32 q and D of 256): q 16 (float32 24) of its row's largest
+ * element, a probability times its value's scale 11 for bfloat16, else 22.
+ * Where it is more: q 11 (float32 22) an element down to 2^-20 of its row's largest;
+ * a probability times its scale 11 (float32 22), for bfloat16 each of the two 11
+ * before that, and the probability so in the sum that divides.  Keys and rows that a row does not
+ * see, and other rows, take none of these bits. */
 int mxk_kv_pages_attend(const void* q, int q_type, int64_t q_token, int64_t q_head, int q_heads, const void* codes,
                         const float* scales, int64_t pages, int page, int heads, int D, const int32_t* table,
                         const int32_t* lengths, const int32_t* offsets, int64_t B, int64_t width, int64_t tokens,

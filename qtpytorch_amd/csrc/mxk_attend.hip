@@ -672,15 +672,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend(AttendArgs A) 
 // float16 and bfloat16 queries whole as far as the tile's largest element allows (a row of less than 2^-8 of
 // it is computed by its own, k_attend_tile);
 // probabilities times the values' scales are one float16 term (two for
-// float32), 2^-11 of a weight.  For bfloat16 the probability and the scale go to
-// float16 before their product (three roundings of 2^-11 against the result's 2^-8), and a
+// float32), 2^-11 of a weight: half the matrix work of two, against results of 8 and 11 bits (the float16 cases' error
+// grows from 2.1e-4, the result's own rounding, to 3.0e-4).  For bfloat16 the probability and the scale go to
+// float16 before their product (three roundings of 2^-11 against the result's 2^-8), the row's weight is the float32 sum of
+// these float16 probabilities, whose roundings so are in both parts of the quotient, and a
 // scale keeps 11 bits down to 2^-14 of the largest one so far, one less for each power of two
 // below; the other forms' do down to 2^-24.
 //
 // Bound by issue: matrix and vector instructions of a SIMD's two waves
-// hardly overlap (matrix 31 % of the cycles, vector 45 %).  2 sequences with up to 2000 new
+// hardly overlap (matrix 35 % of the cycles, vector 45 %).  2 sequences with up to 2000 new
 // tokens behind up to 6000 keys, 8 heads of 128 with 4 of queries each, bfloat16: 281 GFLOP in
-// 353 us with the join, 0.80 PFLOP/s of the 1.20 that a large bfloat16 product reaches.
+// 355 us with the join, 0.79 PFLOP/s of the 1.20 that a large bfloat16 product reaches.
+//
+// Registers: the sums of a wave's rows (D / 2), the queries (D / 4, float32 twice) and a step's keys on their way fill 256.  Heads
+// of 128 spill two, outside the loop over the steps; float32 and heads of 256 take accumulation registers too, so that a
+// SIMD has one wave, which nothing runs beside; both together also spill 16, some in the loop.
 
 // A lane's elements i*16 + h*8 + 0..7 of a query row (null: zeros), and the exponent of the row's largest; rows below
 // 2^-100 count as zeros, and so do, at first, those with a NaN or an infinity.

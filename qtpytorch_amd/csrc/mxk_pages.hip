@@ -64,7 +64,7 @@ __device__ __forceinline__ void row_store(T* p, const float (&v)[V]) {
 // TB tokens a workgroup: their angles once into LDS, then V pairs (or V
 // elements that are not rotated) a thread and step.  The angles, ~100
 // instructions each, are shared by all heads of a token.  Bound by memory: 8190
-// tokens of 32 heads of 128 in bfloat16, 134 MB in 24.8 us, 5.4 TB/s.
+// tokens of 32 heads of 128 in bfloat16, 134 MB in 24.3 us, 5.5 TB/s.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_rotary(const T* __restrict__ x, int64_t token_stride, int64_t head_stride,
                                                 Rotation r, int T_, int D, int TB, uint32_t per_token, DivU32 by_token,
@@ -279,8 +279,8 @@ __global__ __launch_bounds__(256) void k_kv_read(KvBatch s, KvPool p, T* __restr
 // Position lengths[b] + j takes the row of new token path[b][j], for every
 // entry inside [0, its sequence's new tokens).  One workgroup a sequence and
 // head holds all the rows in LDS before it writes any, so that a row may be
-// read by one entry and written by another, in any order.  250 paths of 16 in 16
-// heads of 128: 9 us for 34 MB, bound by the latency of look-up, reads and writes one after the other.
+// read by one entry and written by another, in any order.  250 paths of 1 to 16, 8.5 on average, in 16
+// heads of 128: 8.5 us for 18 MB, bound by the latency of look-up, reads and writes one after the other.
 #define MXK_KEEP_MOST 64
 template <int D>
 __global__ __launch_bounds__(256) void k_kv_keep(KvBatch s, KvPool p, const int* __restrict__ path, int L) {

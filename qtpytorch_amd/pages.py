@@ -308,7 +308,7 @@ class kv_pages:
 
         With a rotary table keys are rotated on the way, by positions [tokens] or
         [tokens, axes] (None: each token's position in its sequence, on every
-        axis); they are packed from the unrounded rotation.  q [tokens, q_heads,
+        axis); they are packed from the unrounded float32 rotation.  q [tokens, q_heads,
         head_dim] is rotated along and returned.  A head's row with a NaN or an
         infinity reads as NaN.  Nothing is differentiable: tensors that require a
         gradient are refused where gradients are recorded."""
@@ -369,7 +369,7 @@ class kv_pages:
         sqrt(head_dim) unless given.  A row that sees nothing is zeros.
 
         Codes are used as they are and sums are float32.  Where a sequence has
-        few rows a head (64 on average; 96 in float32), q keeps 16
+        few rows a head (64 on average; 96 in float32 and with heads of 256), q keeps 16
         bits of its row's largest element (24 in float32), and a probability times
         its value's scale 11 bits (22 in float32 and float16) down to 2^-24 of
         the largest that the row sees.  Else q's elements keep 11 bits (22 in float32) down to 2^-20 of
