@@ -244,3 +244,18 @@ def test_two_streams_at_once_over_one_pool(group):
                 got[i].append(pages.attend(q[i], gb))
     torch.cuda.synchronize()
     assert all(torch.equal(g, w) for many, w in zip(got, want) for g in many)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("name,held,new", [("tokens beside a chunk", [(7 * i) % 90 for i in range(30)] + [50], [1] * 30 + [140]),
+                                           ("a chunk beside many tokens", [(11 * i) % 60 for i in range(90)] + [0], [1] * 90 + [70]),
+                                           ("a chunk among idle slots", [0] * 40 + [90] + [17] * 60, [0] * 40 + [130] + [0] * 60),
+                                           ("a tree-sized step among idle slots", [3] * 70 + [200], [0] * 70 + [9])])
+def test_steps_of_several_kinds_at_once(name, held, new, dtype):
+    """Single tokens, chunks and idle slots of one call: every row is within its own bounds, whichever tiles it takes."""
+    import qtpytorch_amd as qa
+    batch = R.Batch(held, new, 16, front=1, back=2)
+    codes, scales = R.pool(batch, 1, 64)
+    q = torch.randn(batch.tokens, 4, 64, generator=R.gen(5)).to(dtype)
+    want, error = R.attend(batch, codes, scales, q)
+    R.near(qa.kv_pages(codes.cuda(), scales.cuda()).attend(q.cuda(), batch.gpu()), want, error)

@@ -232,3 +232,20 @@ def test_queries_of_other_rows_take_no_bits_from_a_row(size, dim, group, dtype):
     got = _pages(codes, scales).attend(q.cuda(), batch.gpu())
     R.near(got[rows.cuda()], want[rows], error[rows])
     assert torch.isfinite(got).all()
+
+
+def test_values_far_apart_among_many_sequences_in_tiles_of_256_rows():
+    """The same in bfloat16: more sequences than a wave holds, tiles of 256 rows."""
+    import qtpytorch_amd as qa
+    n, G, D = 3000, 80, 64
+    i32 = dict(dtype=torch.int32, device="cuda")
+    pages = qa.kv_pages.empty(n, 16, 1, D)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pages.codes.copy_(torch.randint(-127, 128, pages.codes.shape, generator=g, device="cuda", dtype=torch.int8))
+    pages.scales.copy_(torch.rand(pages.scales.shape, generator=g, device="cuda") + 0.5)
+    pages.scales[1::3, 1, :, 1] *= 1e12
+    batch = qa.kv_batch(torch.arange(n, **i32)[:, None].contiguous(), torch.zeros(n, **i32), torch.arange(0, 2 * n + 1, 2, **i32))
+    got = pages.attend(torch.randn(2 * n, G, D, generator=g, device="cuda").bfloat16(), batch)[::2].float()
+    want = (pages.codes[:, 1, 0, 0].float() * pages.scales[:, 1, 0, :1])[:, None]
+    # the scale, the probability and their product in float16, half a step of bfloat16
+    assert ((got - want).abs() <= (2.0 ** -8 + 3 * 2.0 ** -11) * want.abs()).all()
