@@ -1095,9 +1095,10 @@ __device__ __forceinline__ int tile_part(int wave, int a, int lane) { return ((w
 
 // The value scales of a tile's keys are taken relative to one exponent, which costs a row bits where its own largest scale is
 // far below it: keys that it does not see must not do that.  So are the queries of a tile's rows.  The first launch (not OWN)
-// notes tiles where a row's own may be below 2^-4 of the largest scale, or its query below 2^-8 of the largest; a second one computes these again with an exponent for each row, in the exact form for
-// bfloat16 too, and ends at once where there are none.  Both forms in one kernel cost it registers: 16 trees of 16 tokens with 8
-// queries a head behind 4000 keys 71 us without, 73 in two launches, 77 in one; 4 of 64 tokens behind 30000 180, 189, 195.
+// notes tiles where a row's own may be below 2^-4 of the largest scale, or its query below 2^-8 of the largest; a second one
+// computes these again with exponents of each row's own, in the exact form for bfloat16 too, and ends at once where there are
+// none.  Both forms in one kernel cost it registers: 16 trees of 16 tokens with 8 queries a head behind 4000 keys 71 us without,
+// 73 in two launches, 77 in one; 4 of 64 tokens behind 30000 180, 189, 195.
 template <typename T, int D, int QT, int PT, int NW, bool OWN>
 __global__ __launch_bounds__(64 * NW, D == 256 || QT == 2 ? 1 : 2) void k_attend_tile(AttendArgs A) {
   constexpr int K = tile_keys<D>(), RUNS = K / 16, BATCH = 64 / RUNS;  // runs of a step, steps of a batch of pages
